@@ -1,6 +1,6 @@
 """ctypes binding of libclarus_hip.so (declarations: include/clarus_hip.h).
 
-The structures below mirror ClarusGemmArgs / ClarusConvArgs field by field; `load()` checks
+The structures below mirror ClarusGemmArgs / ClarusConvArgs / ClarusCrossArgs field by field; `load()` checks
 their sizes against the library's own sizeof and the ABI version before handing it out.
 torch is imported first so that the process's HIP runtime is torch's (the library links the
 same soname, libamdhip64.so.7, and binds to the already-loaded copy).
@@ -22,7 +22,8 @@ PRO_NONE, PRO_LN, PRO_MUL, PRO_RMS, PRO_LNMUL = 0, 1, 2, 3, 5
 PRO_ROUND = 0x100  # or-ed into pro: the prologue output may be rounded once to bf16
 A_ROWS, A_S2D = 0, 1
 C_ROWS, C_SHUFFLE, C_NCHW = 0, 1, 2
-ACT_NONE, ACT_GELU, ACT_LRELU = 0, 1, 2
+ACT_NONE, ACT_GELU, ACT_LRELU, ACT_SILU = 0, 1, 2, 3
+MASK_NONE, MASK_KEYS, MASK_PAIRS = 0, 1, 2  # mask_mode of clarus_hip_cross_attention
 CHANNEL_ATTENTION_SCRATCH_MAX = 16 << 20  # bytes of clarus_hip_channel_attention_noalloc's static scratch
 
 _vp, _i64, _i32, _f32 = ctypes.c_void_p, ctypes.c_int64, ctypes.c_int32, ctypes.c_float
@@ -54,6 +55,17 @@ class ConvArgs(ctypes.Structure):
         ("act", _i32), ("up2", _i32), ("c_mode", _i32),
         ("out_scale", _f32), ("slope", _f32),
         ("tile", _i32),
+    ]
+
+
+class CrossArgs(ctypes.Structure):
+    _fields_ = [
+        ("q", _vp), ("k", _vp), ("v", _vp), ("out", _vp), ("mask", _vp),
+        ("n", _i64), ("lq", _i64), ("lk", _i64), ("heads", _i64), ("kv_heads", _i64), ("d", _i64),
+        ("q_bstride", _i64), ("ldq", _i64), ("k_bstride", _i64), ("ldk", _i64), ("v_bstride", _i64), ("ldv", _i64),
+        ("mask_bstride", _i64), ("mask_qstride", _i64),
+        ("dtype", _i32), ("o_dtype", _i32), ("mask_mode", _i32),
+        ("scale", _f32),
     ]
 
 
@@ -91,9 +103,15 @@ SIGNATURES = {
     "clarus_hip_selective_scan_workspace": (ctypes.c_size_t, [_i64, _i64, _i64]),
     "clarus_hip_selective_scan": (_i32, [_vp, _i32, _vp, _i64, _vp, _i64, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _vp,
                                          ctypes.c_size_t, _vp]),
+    "clarus_hip_group_norm_workspace": (ctypes.c_size_t, [_i64, _i64, _i64, _i64]),
+    "clarus_hip_group_norm": (_i32, [_vp, _i32, _i64, _i64, _vp, _i64, _vp, _i64, _vp, _i32, _i64, _i64, _i64, _i64,
+                                     _f32, _i32, _vp, ctypes.c_size_t, _vp]),
+    "clarus_hip_cross_attention_workspace": (ctypes.c_size_t, [_i32, _i64, _i64, _i64, _i64, _i64, _i64]),
+    "clarus_hip_cross_attention": (_i32, [ctypes.POINTER(CrossArgs), _vp, ctypes.c_size_t, _vp]),
     "clarus_hip_abi_version": (_i32, []),
     "clarus_hip_sizeof_gemm_args": (ctypes.c_size_t, []),
     "clarus_hip_sizeof_conv_args": (ctypes.c_size_t, []),
+    "clarus_hip_sizeof_cross_args": (ctypes.c_size_t, []),
     "clarus_hip_last_error": (ctypes.c_char_p, []),
     "clarus_hip_last_kernel": (ctypes.c_char_p, []),
 }
@@ -124,6 +142,8 @@ def load(path: str = LIB_PATH):
         raise RuntimeError("ClarusGemmArgs layout differs between the library and the binding")
     if lib.clarus_hip_sizeof_conv_args() != ctypes.sizeof(ConvArgs):
         raise RuntimeError("ClarusConvArgs layout differs between the library and the binding")
+    if lib.clarus_hip_sizeof_cross_args() != ctypes.sizeof(CrossArgs):
+        raise RuntimeError("ClarusCrossArgs layout differs between the library and the binding")
     _LIB = lib
     return lib
 

@@ -49,6 +49,8 @@ size_t clarus_hip_sizeof_gemm_args(void) { return sizeof(ClarusGemmArgs); }
 
 size_t clarus_hip_sizeof_conv_args(void) { return sizeof(ClarusConvArgs); }
 
+size_t clarus_hip_sizeof_cross_args(void) { return sizeof(ClarusCrossArgs); }
+
 const char* clarus_hip_last_error(void) { return clarus::g_err; }
 
 const char* clarus_hip_last_kernel(void) { return clarus::g_kernel; }

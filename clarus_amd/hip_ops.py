@@ -10,8 +10,9 @@ adapter (python/clarus/ops/triton_cuda.py): arguments the kernels do not handle 
 Ops served: linear, down, up, intro, ending, conv3x3, channel_attention, linear_per_image,
 patch_filter, linear_patch_filter, patch_corr, ln_mul_linear (the GEMM family), plus dwconv
 (depthwise 3x3 + gates) and boxmean (the other ops of the NAFNet forward), selective_scan
-(EVSSM's state-space scan), attention_apply (MDTA attn . V) and linear_ln_linear (a residual
-GEMM and the LayerNorm GEMM on its output).
+(EVSSM's state-space scan), attention_apply (MDTA attn . V), linear_ln_linear (a residual
+GEMM and the LayerNorm GEMM on its output), group_norm (with its activation) and cross_attention
+(positions over an encoder's states).
 
 Capture safety: kernels launch on torch's current stream, scratch comes from torch's
 allocator, weight re-layouts are computed once through `Backend.cached` (in the eager warm-up
@@ -19,7 +20,9 @@ pass), and no call synchronises.
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes
+import math
 
 import torch
 
@@ -59,6 +62,26 @@ def _vec16(t: torch.Tensor, *strides: int) -> bool:
     """Base pointer and the given element strides keep 16-byte alignment."""
     es = t.element_size()
     return t.data_ptr() % 16 == 0 and all((s * es) % 16 == 0 for s in strides)
+
+
+def _rows(t: torch.Tensor):
+    """(rows per image, row stride, image stride) of t [N, ..., C] addressable as image, row, channel
+    with a unit channel stride (any number of inner dimensions, one row stride over all of them; a
+    channel slice qualifies), else None."""
+    if t.dim() < 2 or (t.stride(-1) != 1 and t.shape[-1] > 1):
+        return None
+    ld = nxt = None
+    rows = 1
+    for size, stride in zip(reversed(t.shape[1:-1]), reversed(t.stride()[1:-1])):
+        rows *= size
+        if size == 1:
+            continue
+        if ld is None:
+            ld = stride
+        elif stride != nxt:
+            return None
+        nxt = stride * size
+    return rows, t.shape[-1] if ld is None else ld, t.stride(0) if t.shape[0] > 1 else 0
 
 
 @register_backend("hip")
@@ -190,6 +213,23 @@ class HipOps(Backend):
 
     def _stream(self, t: torch.Tensor) -> int:
         return torch.cuda.current_stream(t.device).cuda_stream
+
+    def _forward_only(self, what, *ts):
+        """Declines what a forward-only op of this device cannot answer: operands elsewhere, and operands
+        whose gradient autograd would lose."""
+        for t in ts:
+            if t is None:
+                continue
+            if t.device != self.dev:
+                raise Unsupported(f"{what}: operands on {self.dev}, got {t.device}")
+            if t.requires_grad and torch.is_grad_enabled():
+                raise Unsupported(f"{what}: forward only, an operand requires its gradient")
+
+    def _current(self):
+        """Launches go to this backend's device whatever device is current."""
+        if torch.cuda.current_device() == self.dev.index:
+            return contextlib.nullcontext()
+        return torch.cuda.device(self.dev)
 
     def _bias(self, b):
         """fp32 contiguous copy of a (weight-like) vector, once per tensor."""
@@ -768,7 +808,104 @@ class HipOps(Backend):
             self._stream(x)), "dwconv")
         return out
 
+    def group_norm(self, x, groups, weight=None, bias=None, eps=1e-5, act=None, out_dtype=None):
+        """act(group_norm(x) * weight + bias) of x [N, ..., C], channels last: per image and group of
+        C / groups channels the mean and biased variance over all pixels of the group's channels, in
+        fp32, rounded once. weight, bias: [C], or [N, C] for a scale and shift of each image's own. act
+        None, "silu" or "gelu". x may be a channel slice (one pixel stride); the result is contiguous."""
+        if x.dim() < 2 or act not in (None, "silu", "gelu") or not isinstance(groups, int) or groups < 1:
+            raise Unsupported(f"group_norm: x [N, ..., C], groups >= 1, act none / silu / gelu, got {groups!r} {act!r}")
+        n, c = x.shape[0], x.shape[-1]
+        odt = out_dtype or self.dtype
+        self._forward_only("group_norm", x, weight, bias)
+        if not (_kdt(x) and odt in _KDT and c % 8 == 0 and c % groups == 0 and c > 0
+                and (c // groups) * 8 // math.gcd(8, c // groups) <= 2048):
+            raise Unsupported("group_norm: bf16 / fp32, channels a multiple of 8 and of the groups, "
+                              "lcm(8, channels per group) at most 2048")
+        if any(t is not None and (tuple(t.shape) not in ((c,), (n, c)) or not t.is_floating_point()) for t in (weight, bias)):
+            raise Unsupported("group_norm: weight and bias [C] or [N, C]")
+        out = torch.empty(x.shape, device=x.device, dtype=odt)
+        if out.numel() == 0:
+            return out
+        at = _rows(x)
+        if at is None or at[1] < c or not _vec16(x, at[1], at[2]):
+            raise Unsupported("group_norm: unit channel stride, one pixel stride, 16-byte aligned rows")
+        p, ldx, xbs = at
+        if p >= 1 << 31 or n >= 65536:
+            raise Unsupported("group_norm: fewer than 2^31 pixels of an image and 65536 images")
+        with self._current():
+            # an image's own scale and shift are new with every call: converted, not kept; nor is what a graph's
+            # pool holds, which is written by the replay only
+            keep = not torch.cuda.is_current_stream_capturing()
+            wf, bf = (t if t is None else self._bias(t) if t.dim() == 1 and keep else t.float().contiguous()
+                      for t in (weight, bias))
+            need = self.lib.clarus_hip_group_norm_workspace(n, p, c, groups)
+            scratch = torch.empty(need, device=x.device, dtype=torch.uint8)
+            _lib.check(self.lib.clarus_hip_group_norm(
+                x.data_ptr(), _lib.dtype_code(x.dtype), xbs, ldx, _lib.ptr(wf), c if wf is not None and wf.dim() == 2 else 0,
+                _lib.ptr(bf), c if bf is not None and bf.dim() == 2 else 0, out.data_ptr(), _lib.dtype_code(odt), n, p, c,
+                groups, float(eps), {None: _lib.ACT_NONE, "silu": _lib.ACT_SILU, "gelu": _lib.ACT_GELU}[act],
+                scratch.data_ptr(), need, self._stream(x)), "group_norm")
+        return out
+
     # ------------------------------------------------------------------ attention
+    def cross_attention(self, q, k, v, heads, kv_heads=None, mask=None, scale=None, out_dtype=None):
+        """Every position of q attends the states of another sequence: q [N, ..., heads * d] (NHWC pixels or
+        tokens), k and v [N, ..., kv_heads * d] of any other length (their inner dimensions are their keys, in
+        order; slices of one wider buffer qualify). Head h reads kv head h // (heads // kv_heads). Per head
+        softmax(scale q k^T) v over the keys that `mask` keeps, scale 1 / sqrt(d) by default; 0 for a query that
+        keeps none, or without keys. mask: bool [N, Lk] (a masked key counts for nothing whatever k and v hold)
+        or [N, Lq, Lk] (v has to be finite: a masked pair weighs 0). fp32 scores, softmax and sums; bf16 weights
+        enter the product with v rounded to bf16. Returns a contiguous tensor of q's shape."""
+        if q.dim() < 2 or k.dim() < 2 or v.dim() < 2:
+            raise Unsupported("cross_attention: q, k, v [N, ..., C]")
+        kv_heads = heads if kv_heads is None else kv_heads
+        n, c, ck = q.shape[0], q.shape[-1], k.shape[-1]
+        if not (isinstance(heads, int) and isinstance(kv_heads, int) and heads > 0 and kv_heads > 0
+                and heads % kv_heads == 0 and c % heads == 0 and tuple(k.shape) == tuple(v.shape) and k.shape[0] == n
+                and ck * heads == c * kv_heads):
+            raise Unsupported("cross_attention: q [N, ..., heads d], k and v [N, ..., kv_heads d] of one shape, "
+                              "heads a multiple of kv_heads")
+        d = c // heads
+        odt = out_dtype or self.dtype
+        lq, lk = math.prod(q.shape[1:-1]), math.prod(k.shape[1:-1])
+        scale = d ** -0.5 if scale is None and d else scale
+        self._forward_only("cross_attention", q, k, v, mask)
+        if not (_kdt(q) and q.dtype == k.dtype == v.dtype and odt in _KDT and 8 <= d <= 128 and d % 8 == 0
+                and 0.0 < scale < math.inf):
+            raise Unsupported("cross_attention: bf16 / fp32 q, k, v of one type, head width a multiple of 8 up to 128, "
+                              "scale positive and finite")
+        mode, mbs, mqs = _lib.MASK_NONE, 0, 0
+        if mask is not None:
+            if mask.dtype != torch.bool or tuple(mask.shape) not in ((n, lk), (n, lq, lk)):
+                raise Unsupported("cross_attention: mask bool [N, Lk] or [N, Lq, Lk]")
+            if mask.stride(-1) != 1 and lk > 1 or any(s < 0 for s in mask.stride()):
+                raise Unsupported("cross_attention: mask with unit key stride")
+            # [N, Lk] where Lq is absent: a 2-D mask never stands for [Lq, Lk]
+            mode = _lib.MASK_KEYS if mask.dim() == 2 else _lib.MASK_PAIRS
+            mbs, mqs = mask.stride(0), mask.stride(1) if mask.dim() == 3 else 0
+        out = torch.empty(q.shape, device=q.device, dtype=odt)
+        if out.numel() == 0:
+            return out
+        if lk == 0:
+            return out.zero_()
+        qa, ka, va = _rows(q), _rows(k), _rows(v)
+        if None in (qa, ka, va) or not (_vec16(q, *qa[1:]) and _vec16(k, *ka[1:]) and _vec16(v, *va[1:])):
+            raise Unsupported("cross_attention: unit channel stride, one row stride, 16-byte aligned rows")
+        if max(lk, lq * (heads // kv_heads)) >= 1 << 31 or n * kv_heads >= 65536:
+            raise Unsupported("cross_attention: fewer than 2^31 keys and rows, fewer than 65536 (image, kv head) pairs")
+        args = _lib.CrossArgs(
+            q=q.data_ptr(), k=k.data_ptr(), v=v.data_ptr(), out=out.data_ptr(), mask=_lib.ptr(mask), n=n, lq=lq, lk=lk,
+            heads=heads, kv_heads=kv_heads, d=d, q_bstride=qa[2], ldq=qa[1], k_bstride=ka[2], ldk=ka[1], v_bstride=va[2],
+            ldv=va[1], mask_bstride=mbs, mask_qstride=mqs, dtype=_lib.dtype_code(q.dtype), o_dtype=_lib.dtype_code(odt),
+            mask_mode=mode, scale=scale)
+        with self._current():
+            need = self.lib.clarus_hip_cross_attention_workspace(args.dtype, n, lq, lk, heads, kv_heads, d)
+            scratch = torch.empty(need, device=q.device, dtype=torch.uint8) if need else None
+            _lib.check(self.lib.clarus_hip_cross_attention(ctypes.byref(args), _lib.ptr(scratch), need, self._stream(q)),
+                       "cross_attention")
+        return out
+
     def channel_attention(self, qkv, heads, temperature):
         if not qkv.is_contiguous():
             raise Unsupported("channel_attention: contiguous qkv only")

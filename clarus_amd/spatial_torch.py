@@ -1,5 +1,5 @@
 """PyTorch backend for the NON-GEMM ops the NAFNet harness needs (depthwise conv, TLC local
-mean, scaled add, pixel (un)shuffle), run on the device with torch.
+mean, scaled add, pixel (un)shuffle) and group norm, run on the device with torch.
 
 These ops are outside the HIP hot path; in clarus they fall through to the reference torch
 backend (python/clarus/ops/torch_ref.py:133-218), whose semantics this follows. Registered as
@@ -8,6 +8,8 @@ backend (python/clarus/ops/torch_ref.py:133-218), whose semantics this follows. 
 backend declines raises `Unsupported` instead of silently running on torch.
 """
 from __future__ import annotations
+
+import math
 
 import torch
 import torch.nn.functional as F
@@ -41,6 +43,21 @@ class TorchSpatialOps(Backend):
         if act == "gelu":
             y = F.gelu(y)
         return y.contiguous().to(self.dtype)
+
+    def group_norm(self, x, groups, weight=None, bias=None, eps=1e-5, act=None, out_dtype=None):
+        """Group norm of x [N, ..., C], channels last, in fp32 (weight and bias [C] or [N, C]), then
+        SiLU / GELU."""
+        n, c = x.shape[0], x.shape[-1]
+        p = math.prod(x.shape[1:-1])
+        y = x.float().reshape(n, p, groups, c // groups)
+        var, mean = torch.var_mean(y, (1, 3), correction=0, keepdim=True)
+        y = ((y - mean) * torch.rsqrt(var + eps)).reshape(n, p, c)
+        if weight is not None:
+            y = y * weight.float().reshape(-1, 1, c)
+        if bias is not None:
+            y = y + bias.float().reshape(-1, 1, c)
+        y = F.silu(y) if act == "silu" else F.gelu(y) if act == "gelu" else y
+        return y.reshape(x.shape).to(out_dtype or self.dtype)
 
     def add_scaled(self, a, b, alpha, out_dtype=None, out=None):
         """a * alpha + b (torch_ref.py:201-207)."""

@@ -63,6 +63,7 @@ extern "C" {
 #define CLARUS_ACT_NONE 0
 #define CLARUS_ACT_GELU 1  /* exact erf GELU                                        */
 #define CLARUS_ACT_LRELU 2 /* LeakyReLU(slope)                                      */
+#define CLARUS_ACT_SILU 3  /* y / (1 + e^-y) (group_norm only)                      */
 
 /*
  * Fused NHWC GEMM:  out[p, n] = epilogue( prologue(A)[p, :] . W[:, n] ), fp32 accumulation.
@@ -464,10 +465,62 @@ int clarus_hip_selective_scan(const void* u, int32_t u_dtype, const float* dbl, 
                               int64_t t, int64_t l, int64_t d, void* scratch, size_t scratch_bytes,
                               void* stream);
 
+/*
+ * Group norm with its activation, NHWC: for image n and group g of c / groups channels, mean and
+ * biased variance over the p pixels and the group's channels, then
+ *   out = act((x - mean) * rsqrt(var + eps) * w[ch] + b[ch]).
+ * x: pixel rows at x + n * x_bstride + pixel * ldx (a channel slice of a wider buffer, or an image
+ * stride of its own; x_dtype), 16-byte aligned rows; w, b fp32 [c] (stride 0) or one row per image
+ * (w_bstride, b_bstride >= c), or NULL for 1 / 0. out [n, p, c] contiguous (o_dtype), not overlapping x
+ * unless it is x itself, contiguous and of one dtype. act: CLARUS_ACT_NONE, CLARUS_ACT_GELU or
+ * CLARUS_ACT_SILU. c a multiple of 8 and of groups, lcm(8, c / groups) at most 2048. Statistics and the
+ * affine in fp32, rounded once. scratch holds clarus_hip_group_norm_workspace(...) bytes (the partial
+ * statistics), 8-byte aligned. Deterministic.
+ * No counterpart in the reference (its norms are the LayerNorm / RMS prologues of linear).
+ */
+size_t clarus_hip_group_norm_workspace(int64_t n, int64_t p, int64_t c, int64_t groups);
+int clarus_hip_group_norm(const void* x, int32_t x_dtype, int64_t x_bstride, int64_t ldx, const float* w,
+                          int64_t w_bstride, const float* b, int64_t b_bstride, void* out, int32_t o_dtype,
+                          int64_t n, int64_t p, int64_t c, int64_t groups, float eps, int32_t act,
+                          void* scratch, size_t scratch_bytes, void* stream);
+
+/*
+ * Attention of lq positions over lk states of another sequence, per image and head:
+ *   out[n, i, h] = sum_j p_j v[n, j, g],  p = softmax_j(scale q[n, i, h] . k[n, j, g]),  g = h / (heads / kv_heads)
+ * over the keys j that the mask keeps; 0 where it keeps none. q rows at q + n * q_bstride + i * ldq, head h
+ * at column h * d; k, v likewise with head g (strides in elements, multiples of 16 bytes; slices of wider
+ * rows, shared rows with stride 0). out [n, lq, heads * d] contiguous, overlapping no input.
+ * mask (bytes, 0 = masked): mask_mode 1: key j of image n kept where mask[n * mask_bstride + j]; such a
+ * masked key counts for nothing, whatever k and v hold. mask_mode 2: kept for query i where
+ * mask[n * mask_bstride + i * mask_qstride + j]; k and v of the masked pairs enter no score and weigh 0,
+ * so v has to be finite. dtype bf16 or fp32 (of q, k and v), o_dtype either; d a multiple of 8, at most
+ * 128; scale > 0. Scores, softmax and output are accumulated in fp32; with bf16 the weights p are rounded
+ * once to bf16 for the product with v. scratch holds clarus_hip_cross_attention_workspace(...) bytes
+ * (partial results where few rows ask many keys; may be 0), 16-byte aligned. Deterministic.
+ * No counterpart in the reference (its attention is over channels: clarus_hip_channel_attention).
+ */
+typedef struct ClarusCrossArgs {
+  const void* q;
+  const void* k;
+  const void* v;
+  void* out;
+  const void* mask; /* NULL with mask_mode 0 */
+  int64_t n, lq, lk, heads, kv_heads, d;
+  int64_t q_bstride, ldq, k_bstride, ldk, v_bstride, ldv;
+  int64_t mask_bstride, mask_qstride; /* bytes */
+  int32_t dtype, o_dtype, mask_mode;
+  float scale;
+} ClarusCrossArgs;
+
+size_t clarus_hip_cross_attention_workspace(int32_t dtype, int64_t n, int64_t lq, int64_t lk, int64_t heads,
+                                            int64_t kv_heads, int64_t d);
+int clarus_hip_cross_attention(const ClarusCrossArgs* args, void* scratch, size_t scratch_bytes, void* stream);
+
 /* ABI version (CLARUS_HIP_ABI_VERSION) and struct sizes, for binding checks. */
 int clarus_hip_abi_version(void);
 size_t clarus_hip_sizeof_gemm_args(void);
 size_t clarus_hip_sizeof_conv_args(void);
+size_t clarus_hip_sizeof_cross_args(void);
 
 /* Text of the calling thread's last failure ("" if none). */
 const char* clarus_hip_last_error(void);

@@ -144,6 +144,36 @@ class TorchRef:
             return out
         return y.contiguous().to(self._odt(out_dtype))
 
+    def group_norm(self, x, groups, weight=None, bias=None, eps=1e-5, act=None, out_dtype=None):
+        """No reference op: torch's group norm (biased variance, eps inside the root) of x [N, ..., C]
+        channels last, weight and bias [C] or [N, C], then SiLU / GELU."""
+        n, c = x.shape[0], x.shape[-1]
+        y = x.float().reshape(n, -1, groups, c // groups)
+        y = y - y.mean((1, 3), keepdim=True)
+        y = (y * torch.rsqrt(y.square().mean((1, 3), keepdim=True) + eps)).reshape(n, -1, c)
+        if weight is not None:
+            y = y * weight.float().reshape(-1, 1, c)
+        if bias is not None:
+            y = y + bias.float().reshape(-1, 1, c)
+        y = F.silu(y) if act == "silu" else F.gelu(y) if act == "gelu" else y
+        return y.reshape(x.shape).to(self._odt(out_dtype))
+
+    def cross_attention(self, q, k, v, heads, kv_heads=None, mask=None, scale=None, out_dtype=None):
+        """No reference op: softmax(scale q k^T) v per head over the kept keys, 0 where none is kept; a key
+        that a [N, Lk] mask drops counts for nothing whatever it holds."""
+        kv_heads = kv_heads or heads
+        n, d, rep = q.shape[0], q.shape[-1] // heads, heads // kv_heads
+        qh = q.float().reshape(n, -1, heads, d).permute(0, 2, 1, 3)
+        kh, vh = (t.float().reshape(n, -1, kv_heads, d).permute(0, 2, 1, 3).repeat_interleave(rep, 1) for t in (k, v))
+        s = (qh @ kh.transpose(-1, -2).contiguous()) * (d ** -0.5 if scale is None else scale)
+        if mask is not None:
+            if mask.dim() == 2:
+                vh = vh.masked_fill(~mask[:, None, :, None], 0)
+            s = s.masked_fill(~(mask[:, None, None] if mask.dim() == 2 else mask[:, None]), float("-inf"))
+        none = torch.isneginf(s).all(-1, keepdim=True)
+        p = torch.softmax(s.masked_fill(none, 0), -1).masked_fill(none, 0)
+        return (p @ vh).permute(0, 2, 1, 3).reshape(q.shape).to(self._odt(out_dtype))
+
     def channel_attention(self, qkv, heads, temperature):
         """torch_ref.py:220-235: softmax((q/|q|)(k/|k|)^T * t) per image and head, fp32."""
         n, h, w, c3 = qkv.shape
