@@ -30,6 +30,8 @@ constexpr int XA_T = 256;    // threads
 constexpr int XA_ROWS = 128; // rows of a workgroup
 constexpr float XA_FLOOR = -3e38f;  // running maximum before any key: exp2(-inf - XA_FLOOR) = 0, no inf - inf
 
+constexpr float XA_SLACK = 8.f;
+
 enum : int { MASK_NONE = 0, MASK_KEYS = 1, MASK_PAIRS = 2 };
 
 struct CrossP {
@@ -53,36 +55,42 @@ __device__ __forceinline__ float xor32(float v) {
 template <int DT, int D>
 struct XaTile {
   static constexpr int ES = DT == DT_BF16 ? 2 : 4;
-  static constexpr int KT = DT == DT_BF16 ? 64 : 32;       // keys per tile
-  static constexpr int CPR = D * ES / 16;                  // 16-byte chunks per row
-  static constexpr int NCH = KT * CPR / XA_T;              // chunks per thread and operand
-  static constexpr int ROWB = DT == DT_BF16 ? D * 2 : D * 4 + 16;  // LDS row: swizzled, or padded
+  static constexpr int KT = DT == DT_BF16 ? 64 : 32;  // keys per tile
+  static constexpr int ROWB = D * ES;                 // bytes of a row in LDS
+  static constexpr int CPR = ROWB / 16;               // 16-byte chunks per row
   static constexpr int BYTES = KT * ROWB;
-  // position of chunk c of row r. bf16 rows are a multiple of 64 bytes: the XOR spreads K's reads (32
-  // consecutive rows, one chunk) and V's transposing reads (8 rows, 4 chunks) over all banks.
-  static __device__ __forceinline__ int at_k(int r, int c) {
-    if constexpr (DT != DT_BF16) return r * ROWB + c * 16;
-    else if constexpr (D == 32) return r * ROWB + (c ^ ((r >> 2) & 3)) * 16;
-    else if constexpr (D == 64) return r * ROWB + (c ^ ((r >> 1) & 7)) * 16;
-    else if constexpr (D == 96) return r * ROWB + (c ^ ((r >> 2) & 3)) * 16;
-    else return r * ROWB + (c ^ (r & 15)) * 16;
+  static constexpr int NI = BYTES / 1024 / (XA_T / 64);  // 1 KiB copies per wave and operand
+  // chunk c of row r sits at position c ^ swz(r). K: 16 lanes read one chunk of 16 consecutive rows; V: bf16
+  // 8 rows x 4 chunks (transposing), fp32 two rows 4 apart x 8 chunks: each over all banks (fp32 V of 32 and
+  // 96 columns excepted, whose rows r and r + 4 meet)
+  static __device__ __forceinline__ int swz_k(int r) {
+    return ROWB == 64 ? (r >> 2) & 3 : ROWB == 128 || ROWB == 384 ? (r >> 1) & 7 : ROWB == 192 ? (r >> 2) & 3 : r & 15;
   }
-  static __device__ __forceinline__ int at_v(int r, int c) {
-    if constexpr (DT != DT_BF16) return r * ROWB + c * 16;
-    else if constexpr (D == 64) return r * ROWB + (c ^ (((r >> 1) & 1) * 4)) * 16;
-    else if constexpr (D == 128) return r * ROWB + (c ^ ((r & 3) * 4)) * 16;
-    else return r * ROWB + c * 16;
+  static __device__ __forceinline__ int swz_v(int r) {
+    if constexpr (DT == DT_BF16) return D == 64 ? ((r >> 1) & 1) * 4 : D == 128 ? (r & 3) * 4 : 0;
+    return D == 64 || D == 128 ? ((r >> 2) & 1) * 8 : 0;
   }
+  static __device__ __forceinline__ int at_k(int r, int c) { return r * ROWB + (c ^ swz_k(r)) * 16; }
+  static __device__ __forceinline__ int at_v(int r, int c) { return r * ROWB + (c ^ swz_v(r)) * 16; }
 };
 
-template <int DT, int D, int MASK>
-__global__ void __launch_bounds__(XA_T, 2) xa_kernel(const CrossP p) {
-  using T = XaTile<DT, D>;
-  constexpr int KT = T::KT, KB = KT / 32, DB = D / 32, ES = T::ES;
-  __shared__ __align__(16) unsigned char tiles[2][2 * T::BYTES];
-  __shared__ __align__(16) float lims[2][KT];
+// what a masked, padding or absent piece of K or V is copied from
+__device__ const u32x4 xa_zeros[1] = {u32x4{0, 0, 0, 0}};
 
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+// keep ? v : -inf, keep = bit `bit` of w (v may be NaN)
+__device__ __forceinline__ float keep_bit(float v, unsigned w, int bit) {
+  const unsigned k = (unsigned)__builtin_amdgcn_sbfe((int)w, bit, 1);
+  return __uint_as_float((__float_as_uint(v) & k) | (0xff800000u & ~k));
+}
+
+template <int DT, int D, int MASK>
+__global__ void __launch_bounds__(XA_T, D <= 64 ? 4 : 2) xa_kernel(const CrossP p) {
+  using T = XaTile<DT, D>;
+  constexpr int KT = T::KT, KB = KT / 32, DB = D / 32, ES = T::ES, NI = T::NI;
+  constexpr uint64_t ALL = KT == 64 ? ~0ull : 0xffffffffull;
+  __shared__ __align__(16) unsigned char tiles[2][2 * T::BYTES];
+
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int col = lane & 31, hl = lane >> 5;
   // row blocks of one (image, kv head) run on one XCD, whose L2 then holds that head's K and V
   const int64_t total = p.nblk * p.nk * p.splits, span = (total + 7) >> 3;
@@ -105,6 +113,57 @@ __global__ void __launch_bounds__(XA_T, 2) xa_kernel(const CrossP p) {
   const unsigned char* mrow = MASK == MASK_PAIRS ? p.mask + n * p.mbs + qi * p.mqs : nullptr;
   const unsigned char* mkey = MASK == MASK_KEYS ? p.mask + n * p.mbs : nullptr;
 
+  const int64_t k0 = (int64_t)split * p.split_len, k1 = k0 + p.split_len < p.lk ? k0 + p.split_len : p.lk;
+  const int ntile = (int)((k1 - k0 + KT - 1) / KT);
+
+  // this lane's piece of each copy: row and chunk of the tile, and its offset from the tile's first row
+  uint32_t koff[NI], voff[NI];
+  int rowc[NI];      // row
+  bool have_k[NI], have_v[NI];  // the chunk lies within the head
+#pragma unroll
+  for (int j = 0; j < NI; ++j) {
+    const int at = (wave + (XA_T / 64) * j) * 1024 + lane * 16;
+    const int r = at / T::ROWB, cpos = (at % T::ROWB) / 16;
+    const int ck = cpos ^ T::swz_k(r), cv = cpos ^ T::swz_v(r);
+    rowc[j] = r;
+    koff[j] = (uint32_t)(r * p.ldk * ES) + ck * 16;
+    voff[j] = (uint32_t)(r * p.ldv * ES) + cv * 16;
+    have_k[j] = ck * 16 < p.d * ES;
+    have_v[j] = cv * 16 < p.d * ES;
+  }
+  // the kept keys of a tile, one bit each. MASK_KEYS: the byte is loaded a tile ahead of its use
+  auto key_byte = [&](int t) __attribute__((always_inline)) -> int {
+    const int64_t key = k0 + (int64_t)t * KT + lane;
+    const bool in = lane < KT && key < k1;
+    if constexpr (MASK == MASK_KEYS) return in ? mkey[key] : 0;
+    return in;
+  };
+  auto copy = [&](int t, uint64_t bits) __attribute__((always_inline)) {
+    const int64_t base = k0 + (int64_t)t * KT;
+    const unsigned char* kt = kp + base * p.ldk * ES;
+    const unsigned char* vt = vp + base * p.ldv * ES;
+    unsigned char* dst = tiles[t & 1] + wave * 1024;
+#define XA_COPY(src, to)                                                                                   \
+  __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(src),                  \
+                                   (__attribute__((address_space(3))) void*)(to), 16, 0, 0)
+    if (bits == ALL && p.d == D) {
+#pragma unroll
+      for (int j = 0; j < NI; ++j) {
+        XA_COPY(kt + koff[j], dst + j * (XA_T / 64) * 1024);
+        XA_COPY(vt + voff[j], dst + T::BYTES + j * (XA_T / 64) * 1024);
+      }
+    } else {
+      const unsigned char* zero = (const unsigned char*)xa_zeros;
+#pragma unroll
+      for (int j = 0; j < NI; ++j) {
+        const bool in = (bits >> rowc[j]) & 1;
+        XA_COPY(in && have_k[j] ? kt + koff[j] : zero, dst + j * (XA_T / 64) * 1024);
+        XA_COPY(in && have_v[j] ? vt + voff[j] : zero, dst + T::BYTES + j * (XA_T / 64) * 1024);
+      }
+    }
+#undef XA_COPY
+  };
+
   // Q^T fragments
   constexpr int QN = DT == DT_BF16 ? D / 16 : D / 8;  // 16-byte chunks per lane
   u32x4 qf[QN];
@@ -125,148 +184,134 @@ __global__ void __launch_bounds__(XA_T, 2) xa_kernel(const CrossP p) {
     for (int j = 0; j < 16; ++j) o[b][j] = 0.f;
   float m = XA_FLOOR, l = 0.f;
 
-  const int64_t k0 = (int64_t)split * p.split_len, k1 = k0 + p.split_len < p.lk ? k0 + p.split_len : p.lk;
-  const int ntile = (int)((k1 - k0 + KT - 1) / KT);
-
-  u32x4 kr[T::NCH], vr[T::NCH];
-  float lim = 0.f;
-  auto load = [&](int t) __attribute__((always_inline)) {
-    const int64_t base = k0 + (int64_t)t * KT;
-    const int left = (int)(k1 - base);
-#pragma unroll
-    for (int j = 0; j < T::NCH; ++j) {
-      const int e = tid + XA_T * j, r = e / T::CPR, c = e - r * T::CPR;
-      const bool in = r < left && c * 16 < p.d * ES;
-      kr[j] = vr[j] = u32x4{0, 0, 0, 0};
-      if (in) kr[j] = *reinterpret_cast<const u32x4*>(kp + ((base + r) * p.ldk) * ES + c * 16);
-      if (in && (MASK != MASK_KEYS || mkey[base + r])) vr[j] = *reinterpret_cast<const u32x4*>(vp + ((base + r) * p.ldv) * ES + c * 16);
-    }
-    if (tid < KT) lim = tid < left && (MASK != MASK_KEYS || mkey[base + tid]) ? INFINITY : -INFINITY;
-  };
-  auto put = [&](int buf) __attribute__((always_inline)) {
-#pragma unroll
-    for (int j = 0; j < T::NCH; ++j) {
-      const int e = tid + XA_T * j, r = e / T::CPR, c = e - r * T::CPR;
-      *reinterpret_cast<u32x4*>(tiles[buf] + T::at_k(r, c)) = kr[j];
-      *reinterpret_cast<u32x4*>(tiles[buf] + T::BYTES + T::at_v(r, c)) = vr[j];
-    }
-    if (tid < KT) lims[buf][tid] = lim;
-  };
-
+  uint64_t bits = 0;
+  int byte = 0;
   if (ntile > 0) {
-    load(0);
-    put(0);
+    bits = __ballot(key_byte(0));
+    if (ntile > 1) byte = key_byte(1);
+    if (bits) copy(0, bits);
   }
   for (int t = 0; t < ntile; ++t) {
-    const int buf = t & 1;
-    __syncthreads();
-    if (t + 1 < ntile) load(t + 1);
-    if (busy) {
-      const unsigned char* ks = tiles[buf];
-      const unsigned char* vs = tiles[buf] + T::BYTES;
+    const uint64_t now = bits;
+    __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0): this wave's copies of tile t have landed
+    barrier_keep_vm();                   // everybody's have, and tile t - 1 has been read
+    if (t + 1 < ntile) {
+      bits = __ballot(byte);
+      if (t + 2 < ntile) byte = key_byte(t + 2);
+      if (bits) copy(t + 1, bits);
+    }
+    if (!busy || !now) continue;
+    const unsigned char* ks = tiles[t & 1];
+    const unsigned char* vs = tiles[t & 1] + T::BYTES;
+    unsigned pair[KB][4];
+    if constexpr (MASK == MASK_PAIRS) {
       const int64_t base = k0 + (int64_t)t * KT;
-      f32x16 s[KB];
-#pragma unroll
-      for (int b = 0; b < KB; ++b) {
-#pragma unroll
-        for (int j = 0; j < 16; ++j) s[b][j] = 0.f;
-#pragma unroll
-        for (int i = 0; i < QN; ++i) {
-          const u32x4 a = *reinterpret_cast<const u32x4*>(ks + T::at_k(32 * b + col, 2 * i + hl));
-          if constexpr (DT == DT_BF16) {
-            s[b] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, qf[i]), s[b], 0, 0, 0);
-          } else {
-#pragma unroll
-            for (int e = 0; e < 4; ++e)
-              s[b] = __builtin_amdgcn_mfma_f32_32x32x2f32(__uint_as_float(a[e]), __uint_as_float(qf[i][e]), s[b], 0, 0, 0);
-          }
-        }
-      }
-      // masked and padding keys: fminf(NaN, -inf) = -inf
-      const bool whole = k1 - base >= KT;
-      if (MASK == MASK_KEYS || !whole) {
-#pragma unroll
-        for (int b = 0; b < KB; ++b)
-#pragma unroll
-          for (int j4 = 0; j4 < 4; ++j4) {
-            const f32x4 lv = *reinterpret_cast<const f32x4*>(&lims[buf][32 * b + 8 * j4 + 4 * hl]);
-#pragma unroll
-            for (int j = 0; j < 4; ++j) s[b][4 * j4 + j] = fminf(s[b][4 * j4 + j], lv[j]);
-          }
-      }
-      if constexpr (MASK == MASK_PAIRS) {
-#pragma unroll
-        for (int b = 0; b < KB; ++b)
-#pragma unroll
-          for (int j4 = 0; j4 < 4; ++j4) {
-            const int64_t key = base + 32 * b + 8 * j4 + 4 * hl;
-            unsigned char by[4];
-            if (whole) {
-              __builtin_memcpy(by, mrow + key, 4);
-            } else {
-#pragma unroll
-              for (int j = 0; j < 4; ++j) by[j] = key + j < k1 ? mrow[key + j] : 0;
-            }
-#pragma unroll
-            for (int j = 0; j < 4; ++j) s[b][4 * j4 + j] = by[j] ? s[b][4 * j4 + j] : -INFINITY;
-          }
-      }
-      float mx = -INFINITY;
+      unsigned any = 0;
 #pragma unroll
       for (int b = 0; b < KB; ++b)
 #pragma unroll
-        for (int j = 0; j < 16; ++j) mx = fmaxf(mx, s[b][j]);
+        for (int j4 = 0; j4 < 4; ++j4) {
+          const int64_t key = base + 32 * b + 8 * j4 + 4 * hl;
+          unsigned w = 0;
+          if (now == ALL) {
+            __builtin_memcpy(&w, mrow + key, 4);
+          } else {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) w |= (key + j < k1 ? (unsigned)mrow[key + j] : 0u) << (8 * j);
+          }
+          pair[b][j4] = w;
+          any |= w;
+        }
+      if (!__any(any)) continue;
+    }
+    f32x16 s[KB];
+#pragma unroll
+    for (int b = 0; b < KB; ++b) {
+#pragma unroll
+      for (int j = 0; j < 16; ++j) s[b][j] = 0.f;
+#pragma unroll
+      for (int i = 0; i < QN; ++i) {
+        const u32x4 a = *reinterpret_cast<const u32x4*>(ks + T::at_k(32 * b + col, 2 * i + hl));
+        if constexpr (DT == DT_BF16) {
+          s[b] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, qf[i]), s[b], 0, 0, 0);
+        } else {
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            s[b] = __builtin_amdgcn_mfma_f32_32x32x2f32(__uint_as_float(a[e]), __uint_as_float(qf[i][e]), s[b], 0, 0, 0);
+        }
+      }
+    }
+    // masked and padding keys weigh nothing, whatever their scores
+    if constexpr (MASK == MASK_PAIRS) {
+#pragma unroll
+      for (int b = 0; b < KB; ++b)
+#pragma unroll
+        for (int j = 0; j < 16; ++j) s[b][j] = keep_bit(s[b][j], pair[b][j >> 2], 8 * (j & 3));
+    } else if (now != ALL) {
+#pragma unroll
+      for (int b = 0; b < KB; ++b) {
+        const unsigned w = (unsigned)(now >> (32 * b)) >> (4 * hl);
+#pragma unroll
+        for (int j = 0; j < 16; ++j) s[b][j] = keep_bit(s[b][j], w, 8 * (j >> 2) + (j & 3));
+      }
+    }
+    // the running maximum moves only when a score passes it by XA_SLACK (weights then stay below 2^XA_SLACK,
+    // and fp32 sums keep their digits): the accumulators are rescaled in few tiles instead of all
+    float mx = -INFINITY;
+#pragma unroll
+    for (int b = 0; b < KB; ++b)
+#pragma unroll
+      for (int j = 0; j < 16; ++j) mx = fmaxf(mx, s[b][j]);
+    if (__any(mx * p.c > m + XA_SLACK)) {
       mx = fmaxf(mx, xor32(mx));
       const float mn = fmaxf(m, mx * p.c);
       const float alpha = __builtin_amdgcn_exp2f(m - mn);
       m = mn;
-      float sum = 0.f;
-#pragma unroll
-      for (int b = 0; b < KB; ++b)
-#pragma unroll
-        for (int j = 0; j < 16; ++j) {
-          s[b][j] = __builtin_amdgcn_exp2f(fmaf(s[b][j], p.c, -m));
-          sum += s[b][j];
-        }
-      l = fmaf(l, alpha, sum);
+      l *= alpha;
 #pragma unroll
       for (int b = 0; b < DB; ++b)
 #pragma unroll
         for (int j = 0; j < 16; ++j) o[b][j] *= alpha;
-      if constexpr (DT == DT_BF16) {
-#pragma unroll
-        for (int ks2 = 0; ks2 < KT / 16; ++ks2) {
-          f32x8 pv;
-#pragma unroll
-          for (int i = 0; i < 8; ++i) pv.v[i] = s[ks2 >> 1][8 * (ks2 & 1) + i];
-          const bf16x8 pb = pack_bf16(pv);
-#pragma unroll
-          for (int b = 0; b < DB; ++b) {
-            const int i = lane & 15;
-            const int r = 16 * ks2 + 4 * hl + (i >> 2), cc = 4 * b + 2 * ((lane >> 4) & 1) + ((i & 3) >> 1);
-            const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-                (__attribute__((address_space(3))) s16x4*)(vs + T::at_v(r, cc) + (i & 1) * 8));
-            const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-                (__attribute__((address_space(3))) s16x4*)(vs + T::at_v(r + 8, cc) + (i & 1) * 8));
-            typedef __attribute__((ext_vector_type(8))) short s16x8;
-            const s16x8 a = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
-            o[b] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), pb, o[b], 0, 0, 0);
-          }
-        }
-      } else {
-#pragma unroll
-        for (int b = 0; b < DB; ++b)
-#pragma unroll
-          for (int kb = 0; kb < KB; ++kb)
-#pragma unroll
-            for (int j = 0; j < 16; ++j) {
-              const int r = 32 * kb + 8 * (j >> 2) + 4 * hl + (j & 3);
-              const float a = *reinterpret_cast<const float*>(vs + r * T::ROWB + (32 * b + col) * 4);
-              o[b] = __builtin_amdgcn_mfma_f32_32x32x2f32(a, s[kb][j], o[b], 0, 0, 0);
-            }
-      }
     }
-    if (t + 1 < ntile) put(buf ^ 1);
+#pragma unroll
+    for (int b = 0; b < KB; ++b)
+#pragma unroll
+      for (int j = 0; j < 16; ++j) {
+        s[b][j] = __builtin_amdgcn_exp2f(fmaf(s[b][j], p.c, -m));
+        l += s[b][j];
+      }
+    if constexpr (DT == DT_BF16) {
+      const int i = lane & 15;
+      const int vr = 4 * hl + (i >> 2), vc = 2 * ((lane >> 4) & 1) + ((i & 3) >> 1);
+#pragma unroll
+      for (int ks2 = 0; ks2 < KT / 16; ++ks2) {
+        f32x8 pv;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) pv.v[e] = s[ks2 >> 1][8 * (ks2 & 1) + e];
+        const bf16x8 pb = pack_bf16(pv);
+#pragma unroll
+        for (int b = 0; b < DB; ++b) {
+          typedef __attribute__((ext_vector_type(8))) short s16x8;
+          const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+              (__attribute__((address_space(3))) s16x4*)(vs + T::at_v(16 * ks2 + vr, 4 * b + vc) + (i & 1) * 8));
+          const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+              (__attribute__((address_space(3))) s16x4*)(vs + T::at_v(16 * ks2 + vr + 8, 4 * b + vc) + (i & 1) * 8));
+          const s16x8 a = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+          o[b] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), pb, o[b], 0, 0, 0);
+        }
+      }
+    } else {
+#pragma unroll
+      for (int b = 0; b < DB; ++b)
+#pragma unroll
+        for (int kb = 0; kb < KB; ++kb)
+#pragma unroll
+          for (int j = 0; j < 16; ++j) {
+            const int r = 32 * kb + 8 * (j >> 2) + 4 * hl + (j & 3);
+            const float a = *reinterpret_cast<const float*>(vs + T::at_v(r, 8 * b + (col >> 2)) + (col & 3) * 4);
+            o[b] = __builtin_amdgcn_mfma_f32_32x32x2f32(a, s[kb][j], o[b], 0, 0, 0);
+          }
+    }
   }
   if (!busy || wrow + col >= p.rows) return;
   l += xor32(l);
@@ -381,6 +426,7 @@ extern "C" int clarus_hip_cross_attention(const ClarusCrossArgs* a, void* scratc
                      a->ldk * es % 16 == 0 && a->ldv * es % 16 == 0 && a->q_bstride * es % 16 == 0 &&
                      a->k_bstride * es % 16 == 0 && a->v_bstride * es % 16 == 0,
                  "cross_attention: 16-byte aligned rows");
+  CLARUS_REQUIRE(a->ldk < (1 << 24) && a->ldv < (1 << 24), "cross_attention: rows of k and v less than 2^24 elements apart");
   CLARUS_REQUIRE(a->ldq >= 0 && a->ldk >= 0 && a->ldv >= 0 && a->q_bstride >= 0 && a->k_bstride >= 0 && a->v_bstride >= 0,
                  "cross_attention: strides");
   CLARUS_REQUIRE(a->mask_mode >= MASK_NONE && a->mask_mode <= MASK_PAIRS && (a->mask_mode == MASK_NONE || a->mask),
