@@ -9,9 +9,11 @@
 //   mean = sum(cnt mean) / sum(cnt),  M2 = sum(M2 + cnt (mean_i - mean)^2)
 // in a fixed order, all in fp32: no sum of squares of uncentred values occurs, so a mean far from
 // zero or a single large value costs no digits, and the result is deterministic.
-//   1. gn_stats_kernel: per (image, chunk of pixels) the groups' mean and M2
-//   2. gn_join_kernel:  per (image, group) the chunks joined: mean, rstd
-//   3. gn_apply_kernel: y, one read of x and one write
+//   gn_stats_kernel  per (image, chunk of pixels) the groups' mean and M2: one read of x
+//   gn_join_kernel   per (image, group) the chunks joined: mean, rstd
+//   gn_apply_kernel  y: one read of x, one write
+//   gn_small_kernel  all in one launch, x held in registers between them, where the pixels of a few
+//                    whole groups fit one workgroup
 #include "capi.hpp"
 #include "common.hpp"
 
@@ -19,22 +21,31 @@ namespace clarus {
 
 namespace {
 
-constexpr int GN_T = 256;   // threads of a workgroup
-constexpr int UR = 8;       // rows in flight per thread
-constexpr int GN_SILU = 3;  // CLARUS_ACT_SILU
+constexpr int GN_T = 256;    // threads of an apply workgroup
+constexpr int GN_TS = 512;   // threads of a stats or small workgroup
+constexpr int UR = 8;        // rows in flight per thread (stats)
+constexpr int UA = 4;        // rows in flight per thread (apply)
+constexpr int NRMAX = 16;    // rows held per thread (small)
+constexpr int GN_JOIN = 8;   // partial statistics in flight per thread (join)
+constexpr int GN_UNIT = 2048;  // channels that a workgroup has to hold together, at most
+constexpr int GN_SILU = CLARUS_ACT_SILU;
 
 struct GroupNormP {
   const void* x;
   void* out;
   const float* w;    // [C] or [N][C] (wbs = C), or null
   const float* b;
-  float2* part;      // [n][chunk][G] mean, M2
+  float2* part;      // [n][G][chunk] mean, M2
   float2* stat;      // [n][G] mean, rstd
   int64_t xbs, ldx;  // image and pixel stride of x (elements)
-  int64_t p, chunk;  // pixels, pixels per chunk
+  int64_t p;         // pixels
+  int64_t chunk;     // pixels per workgroup of this launch
+  int64_t schunk;    // pixels per statistics chunk
   int64_t wbs, bbs;
   int c, groups, cg, nchunk;
   int tr, rpb;       // threads per row (octets of a strip), rows per pass of a workgroup
+  int lpg;           // lanes that join a group: a power of two <= 64
+  int act;
   float eps;
 };
 
@@ -43,14 +54,35 @@ __device__ __forceinline__ f32x8 gn_load(const void* x, int64_t i) {
   return load8<DT>((const unsigned char*)x + i * (DT == DT_BF16 ? 2 : 4));
 }
 
-__device__ __forceinline__ float wave_sum(float v) { return group_sum<64>(v); }
+// 8 values as they lie in memory, and widened
+template <int DT> struct GnRaw { typedef u32x4 T; };
+template <> struct GnRaw<DT_F32> { struct T { f32x4 a, b; }; };
+template <int DT>
+__device__ __forceinline__ typename GnRaw<DT>::T gn_raw(const void* x, int64_t i) {
+  return *reinterpret_cast<const typename GnRaw<DT>::T*>((const unsigned char*)x + i * (DT == DT_BF16 ? 2 : 4));
+}
+template <int DT>
+__device__ __forceinline__ f32x8 gn_widen(const typename GnRaw<DT>::T& v) { return load8<DT>(&v); }
+
+// sum over the lpg consecutive lanes of a group (lpg a power of two <= 64)
+__device__ __forceinline__ float lanes_sum(float v, int lpg) {
+  for (int o = 1; o < lpg; o <<= 1) v += __shfl_xor(v, o, 64);
+  return v;
+}
+
+// f(group) on the lpg consecutive threads of each of ng groups at a time, every lane of a wave in step
+template <int T, class F>
+__device__ __forceinline__ void for_groups(int ng, int lpg, F&& f) {
+  const int per = T / lpg, mine = threadIdx.x / lpg;
+  for (int g0 = 0; g0 < ng; g0 += per) f(g0 + mine < ng ? g0 + mine : ng - 1, g0 + mine < ng);
+}
 
 // WHOLE: cg % 8 == 0, an octet lies in one group and is one set of 8 values per row
 template <int DT, bool WHOLE>
-__global__ void __launch_bounds__(GN_T) gn_stats_kernel(const GroupNormP p) {
+__global__ void __launch_bounds__(GN_TS) gn_stats_kernel(const GroupNormP p) {
   constexpr int NA = WHOLE ? 1 : 8;  // (mean, M2) pairs per thread
   constexpr int PER = WHOLE ? 8 : 1;
-  __shared__ float sm[GN_T * NA], s2[GN_T * NA];
+  __shared__ float sm[GN_TS * NA], s2[GN_TS * NA];
   const int tid = threadIdx.x;
   const int rl = tid / p.tr, oct = tid - rl * p.tr;
   const int64_t n = blockIdx.z, r0 = (int64_t)blockIdx.x * p.chunk;
@@ -64,11 +96,18 @@ __global__ void __launch_bounds__(GN_T) gn_stats_kernel(const GroupNormP p) {
   if (act) {
     const int64_t base = n * p.xbs + r0 * p.ldx + c0 + oct * 8;
     int r = rl;
+    typename GnRaw<DT>::T w[UR];  // the next batch
+    auto fetch = [&](int at) __attribute__((always_inline)) {
+#pragma unroll
+      for (int k = 0; k < UR; ++k) w[k] = gn_raw<DT>(p.x, base + (int64_t)(at + k * p.rpb) * p.ldx);
+    };
+    if (r + (UR - 1) * p.rpb < rows) fetch(r);
     for (; r + (UR - 1) * p.rpb < rows; r += UR * p.rpb) {
       f32x8 v[UR];
 #pragma unroll
-      for (int k = 0; k < UR; ++k) v[k] = gn_load<DT>(p.x, base + (int64_t)(r + k * p.rpb) * p.ldx);
-      const float join = (float)cnt / (float)(cnt + UR), part = (float)UR / (float)(cnt + UR);
+      for (int k = 0; k < UR; ++k) v[k] = gn_widen<DT>(w[k]);
+      if (r + (2 * UR - 1) * p.rpb < rows) fetch(r + UR * p.rpb);
+      const float part = (float)UR * __builtin_amdgcn_rcpf((float)(cnt + UR)), join = (float)cnt * part * PER;
 #pragma unroll
       for (int a = 0; a < NA; ++a) {
         float s = 0.f, q = 0.f;
@@ -86,13 +125,13 @@ __global__ void __launch_bounds__(GN_T) gn_stats_kernel(const GroupNormP p) {
           }
         const float d = m - mean[a];
         mean[a] = fmaf(d, part, mean[a]);
-        m2[a] += q + d * d * (join * (UR * PER));
+        m2[a] += fmaf(d * d, join, q);
       }
       cnt += UR;
     }
     for (; r < rows; r += p.rpb) {
       const f32x8 v = gn_load<DT>(p.x, base + (int64_t)r * p.ldx);
-      const float join = (float)cnt / (float)(cnt + 1), part = 1.f / (float)(cnt + 1);
+      const float part = __builtin_amdgcn_rcpf((float)(cnt + 1)), join = (float)cnt * part * PER;
 #pragma unroll
       for (int a = 0; a < NA; ++a) {
         float s = 0.f, q = 0.f;
@@ -106,7 +145,7 @@ __global__ void __launch_bounds__(GN_T) gn_stats_kernel(const GroupNormP p) {
         }
         const float d = m - mean[a];
         mean[a] = fmaf(d, part, mean[a]);
-        m2[a] += q + d * d * (join * PER);
+        m2[a] += fmaf(d * d, join, q);
       }
       ++cnt;
     }
@@ -117,122 +156,278 @@ __global__ void __launch_bounds__(GN_T) gn_stats_kernel(const GroupNormP p) {
     s2[tid * NA + a] = m2[a];
   }
   __syncthreads();
-  // a wave joins one group at a time: entries (row lane, unit), unit = an octet or a channel
-  const int wave = tid >> 6, lane = tid & 63;
-  const int units = p.cg / PER;                 // entries of a group per row lane
+  // entries of a group: row lanes (over the group's lanes) x its octets or channels of a row
+  const int units = p.cg / PER, sub = tid & (p.lpg - 1);
   const int sgroups = min(p.tr * 8, p.c - c0) / p.cg;  // groups of the strip
-  for (int g = wave; g < sgroups; g += GN_T / 64) {
-    float cs = 0.f, ms = 0.f;
-    for (int e = lane; e < units * p.rpb; e += 64) {
-      const int el = e / units, u = e - el * units;
-      const float k = (float)(PER * ((rows - el + p.rpb - 1) / p.rpb));  // el < rpb: 0 where el >= rows
-      cs += k;
-      ms = fmaf(k, sm[el * p.tr * NA + g * units + u], ms);
+  const int full = rows / p.rpb, rem = rows - full * p.rpb;
+  const float total = (float)rows * (float)p.cg;
+  for_groups<GN_TS>(sgroups, p.lpg, [&](int g, bool mine) {
+    float ms = 0.f;
+    for (int el = sub; el < p.rpb; el += p.lpg) {
+      const float k = (float)(PER * (full + (el < rem)));
+      for (int u = 0; u < units; ++u) ms = fmaf(k, sm[el * p.tr * NA + g * units + u], ms);
     }
-    cs = wave_sum(cs);
-    const float mu = wave_sum(ms) / cs;
+    const float mu = lanes_sum(ms, p.lpg) / total;  // divided: the mean of equal values is that value
     float q = 0.f;
-    for (int e = lane; e < units * p.rpb; e += 64) {
-      const int el = e / units, u = e - el * units;
-      const float k = (float)(PER * ((rows - el + p.rpb - 1) / p.rpb));
-      const int at = el * p.tr * NA + g * units + u;
-      const float d = sm[at] - mu;
-      q += fmaf(d * d, k, s2[at]);
+    for (int el = sub; el < p.rpb; el += p.lpg) {
+      const float k = (float)(PER * (full + (el < rem)));
+      if (k == 0.f) continue;
+      for (int u = 0; u < units; ++u) {
+        const int at = el * p.tr * NA + g * units + u;
+        const float d = sm[at] - mu;
+        q += fmaf(d * d, k, s2[at]);
+      }
     }
-    q = wave_sum(q);
-    if (lane == 0) p.part[((int64_t)n * p.nchunk + blockIdx.x) * p.groups + c0 / p.cg + g] = float2{mu, q};
-  }
+    q = lanes_sum(q, p.lpg);
+    if (mine && sub == 0) p.part[(n * p.groups + c0 / p.cg + g) * p.nchunk + blockIdx.x] = float2{mu, q};
+  });
 }
 
-__global__ void __launch_bounds__(64) gn_join_kernel(const GroupNormP p) {
-  const int g = blockIdx.x, lane = threadIdx.x;
-  const int64_t n = blockIdx.y;
-  const float2* part = p.part + n * p.nchunk * p.groups + g;
-  const float last = (float)(p.p - (p.nchunk - 1) * p.chunk) * (float)p.cg, full = (float)p.chunk * (float)p.cg;
-  float ms = 0.f;
-  for (int e = lane; e < p.nchunk; e += 64) ms = fmaf(e == p.nchunk - 1 ? last : full, part[(int64_t)e * p.groups].x, ms);
-  const float total = (float)p.p * (float)p.cg;
-  const float mu = wave_sum(ms) / total;
-  float q = 0.f;
-  for (int e = lane; e < p.nchunk; e += 64) {
-    const float2 v = part[(int64_t)e * p.groups];
-    const float d = v.x - mu;
-    q += fmaf(d * d, e == p.nchunk - 1 ? last : full, v.y);
-  }
-  q = wave_sum(q);
-  if (lane == 0) p.stat[n * p.groups + g] = float2{mu, rsqrtf(q / total + p.eps)};
-}
-
-template <int ACT>
-__device__ __forceinline__ float gn_act(float y) {
-  if constexpr (ACT == ACT_GELU) return gelu_erf(y);
-  if constexpr (ACT == GN_SILU) return y * __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(y * -1.4426950408889634f));
+__device__ __forceinline__ float gn_act(float y, int act) {
+  if (act == ACT_GELU) return gelu_erf(y);
+  if (act == GN_SILU) return y * __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(y * -1.4426950408889634f));
   return y;
 }
 
-template <int DT, int ODT, int ACT>
-__global__ void __launch_bounds__(GN_T) gn_apply_kernel(const GroupNormP p) {
-  const int tid = threadIdx.x;
-  const int rl = tid / p.tr, oct = tid - rl * p.tr;
-  const int c0 = (blockIdx.y * p.tr + oct) * 8;
-  if (rl >= p.rpb || c0 >= p.c) return;
-  const int64_t n = blockIdx.z, r0 = (int64_t)blockIdx.x * p.chunk;
-  const int rows = (int)((r0 + p.chunk < p.p ? r0 + p.chunk : p.p) - r0);
-  float mean[8], a[8], b[8];
-#pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const float2 s = p.stat[n * p.groups + (c0 + i) / p.cg];
-    mean[i] = s.x;
-    a[i] = s.y * (p.w ? p.w[n * p.wbs + c0 + i] : 1.f);
-    b[i] = p.b ? p.b[n * p.bbs + c0 + i] : 0.f;
+template <int ODT>
+__device__ __forceinline__ void gn_store(void* out, int64_t at, const f32x8& y) {
+  if constexpr (ODT == DT_BF16) {
+    *reinterpret_cast<bf16x8*>((unsigned short*)out + at) = pack_bf16(y);
+  } else {
+    f32x4* o = reinterpret_cast<f32x4*>((float*)out + at);
+    o[0] = f32x4{y.v[0], y.v[1], y.v[2], y.v[3]};
+    o[1] = f32x4{y.v[4], y.v[5], y.v[6], y.v[7]};
   }
-  const int64_t xb = n * p.xbs + r0 * p.ldx + c0, ob = (n * p.p + r0) * p.c + c0;
-  auto put = [&](const f32x8& v, int r) __attribute__((always_inline)) {
-    f32x8 y;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) y.v[i] = gn_act<ACT>(fmaf(v.v[i] - mean[i], a[i], b[i]));
-    const int64_t at = ob + (int64_t)r * p.c;
-    if constexpr (ODT == DT_BF16) {
-      *reinterpret_cast<bf16x8*>((unsigned short*)p.out + at) = pack_bf16(y);
-    } else {
-      f32x4* o = reinterpret_cast<f32x4*>((float*)p.out + at);
-      o[0] = f32x4{y.v[0], y.v[1], y.v[2], y.v[3]};
-      o[1] = f32x4{y.v[4], y.v[5], y.v[6], y.v[7]};
-    }
-  };
-  constexpr int UA = 4;
-  int r = rl;
-  for (; r + (UA - 1) * p.rpb < rows; r += UA * p.rpb) {
-    f32x8 v[UA];
-#pragma unroll
-    for (int k = 0; k < UA; ++k) v[k] = gn_load<DT>(p.x, xb + (int64_t)(r + k * p.rpb) * p.ldx);
-#pragma unroll
-    for (int k = 0; k < UA; ++k) put(v[k], r + k * p.rpb);
-  }
-  for (; r < rows; r += p.rpb) put(gn_load<DT>(p.x, xb + (int64_t)r * p.ldx), r);
 }
 
-struct GnPlan {
-  int tr, rpb, strips, nchunk;
-  int64_t chunk;
-};
+// One workgroup per (group, image): each thread takes GN_JOIN chunks at a time, all in flight, in two passes
+__global__ void __launch_bounds__(64) gn_join_kernel(const GroupNormP p) {
+  const int64_t n = blockIdx.y;
+  const float full = (float)p.schunk * (float)p.cg, last = (float)(p.p - (p.nchunk - 1) * p.schunk) * (float)p.cg;
+  const float2* part = p.part + (n * p.groups + blockIdx.x) * p.nchunk;
+  float cnt = 0.f, mu = 0.f, q = 0.f;
+  auto join = [&](float k, const float2& v) __attribute__((always_inline)) {
+    const float d = v.x - mu, f = k * __builtin_amdgcn_rcpf(fmaxf(cnt + k, 1.f));
+    mu = fmaf(d, f, mu);
+    q += fmaf(d * d, cnt * f, v.y);
+    cnt += k;
+  };
+  for (int e0 = threadIdx.x; e0 < p.nchunk; e0 += 64 * GN_JOIN) {
+    float2 t[GN_JOIN];
+#pragma unroll
+    for (int j = 0; j < GN_JOIN; ++j) t[j] = e0 + j * 64 < p.nchunk ? part[e0 + j * 64] : float2{0.f, 0.f};
+    float ks = 0.f, ms = 0.f, qs = 0.f;
+#pragma unroll
+    for (int j = 0; j < GN_JOIN; ++j) {
+      const int e = e0 + j * 64;
+      const float k = e < p.nchunk - 1 ? full : e == p.nchunk - 1 ? last : 0.f;
+      ks += k;
+      ms = fmaf(k, t[j].x, ms);
+    }
+    const float m = ms / ks;
+#pragma unroll
+    for (int j = 0; j < GN_JOIN; ++j) {
+      const int e = e0 + j * 64;
+      const float k = e < p.nchunk - 1 ? full : e == p.nchunk - 1 ? last : 0.f, d = t[j].x - m;
+      if (e < p.nchunk) qs += fmaf(d * d, k, t[j].y);
+    }
+    join(ks, float2{m, qs});
+  }
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) {
+    const float k = __shfl_xor(cnt, o, 64);
+    const float2 v = float2{__shfl_xor(mu, o, 64), __shfl_xor(q, o, 64)};
+    join(k, v);
+  }
+  if (threadIdx.x == 0) p.stat[n * p.groups + blockIdx.x] = float2{mu, rsqrtf(q / ((float)p.p * (float)p.cg) + p.eps)};
+}
+
+// the affine of 8 channels, all loads in flight together (4-byte aligned: a slice of a vector qualifies)
+__device__ __forceinline__ void gn_affine(const GroupNormP& p, int64_t n, int c, float (&a)[8], float (&b)[8]) {
+  struct __attribute__((packed, aligned(4))) Vec { float v[8]; };
+  if (p.w) {
+    const Vec t = *reinterpret_cast<const Vec*>(p.w + n * p.wbs + c);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) a[i] = t.v[i];
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) a[i] = 1.f;
+  }
+  if (p.b) {
+    const Vec t = *reinterpret_cast<const Vec*>(p.b + n * p.bbs + c);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) b[i] = t.v[i];
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) b[i] = 0.f;
+  }
+}
+
+template <int DT, int ODT, int ACT, bool WHOLE>
+__global__ void __launch_bounds__(GN_T) gn_apply_kernel(const GroupNormP p) {
+  const int tid = threadIdx.x;
+  const int64_t n = blockIdx.z;
+  const int rl = tid / p.tr, oct = tid - rl * p.tr, c0 = (blockIdx.y * p.tr + oct) * 8;
+  const bool act = rl < p.rpb && c0 < p.c;
+  const int64_t r0 = (int64_t)blockIdx.x * p.chunk;
+  const int rows = (int)((r0 + p.chunk < p.p ? r0 + p.chunk : p.p) - r0);
+  const int64_t xb = n * p.xbs + r0 * p.ldx + c0, ob = (n * p.p + r0) * p.c + c0;
+  // the first rows are on their way before the statistics and the affine are asked for
+  typename GnRaw<DT>::T v[UA];
+  auto fetch = [&](int at) __attribute__((always_inline)) {
+#pragma unroll
+    for (int k = 0; k < UA; ++k) {  // rows past the end repeat the last one
+      const int r = at + k * p.rpb < rows ? at + k * p.rpb : rows - 1;
+      v[k] = gn_raw<DT>(p.x, xb + (int64_t)r * p.ldx);
+    }
+  };
+  if (!act) return;
+  fetch(rl);
+  float a[8], b[8];
+  gn_affine(p, n, c0, a, b);
+  const float2* stat = p.stat + n * p.groups;
+  float mean[8];
+  int g = c0 / p.cg, gc = c0 - g * p.cg;
+  float2 t = stat[g];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    if (!WHOLE && i) {
+      if (++gc == p.cg) gc = 0, ++g;
+      t = stat[g];
+    }
+    mean[i] = t.x;
+    a[i] *= t.y;
+  }
+  for (int r = rl; r < rows; r += UA * p.rpb) {
+    typename GnRaw<DT>::T u[UA];
+#pragma unroll
+    for (int k = 0; k < UA; ++k) u[k] = v[k];
+    if (r + UA * p.rpb < rows) fetch(r + UA * p.rpb);
+#pragma unroll
+    for (int k = 0; k < UA; ++k) {
+      if (r + k * p.rpb >= rows) break;
+      const f32x8 x = gn_widen<DT>(u[k]);
+      f32x8 y;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) y.v[i] = gn_act(fmaf(x.v[i] - mean[i], a[i], b[i]), ACT);
+      gn_store<ODT>(p.out, ob + (int64_t)(r + k * p.rpb) * p.c, y);
+    }
+  }
+}
+
+// One workgroup per (image, strip of whole groups): x in registers (at most NR rows per thread), two exact passes
+template <int DT, int ODT, bool WHOLE, int NR>
+__global__ void __launch_bounds__(GN_TS) gn_small_kernel(const GroupNormP p) {
+  constexpr int NA = WHOLE ? 1 : 8, PER = WHOLE ? 8 : 1;
+  __shared__ float sm[GN_TS * NA];
+  __shared__ float stat[2][GN_UNIT];
+  const int tid = threadIdx.x, sub = tid & (p.lpg - 1);
+  const int rl = tid / p.tr, oct = tid - rl * p.tr;
+  const int64_t n = blockIdx.z;
+  const int s0 = blockIdx.y * p.tr * 8, c0 = s0 + oct * 8, P = (int)p.p;
+  const bool act = rl < p.rpb && c0 < p.c;
+  const int sgroups = min(p.tr * 8, p.c - s0) / p.cg;
+  const int units = p.cg / PER;
+  const float total = (float)P * (float)p.cg;
+  const int64_t xb = n * p.xbs + (act ? c0 : s0);
+  f32x8 v[NR];
+#pragma unroll
+  for (int k = 0; k < NR; ++k) {
+    const int r = rl + k * p.rpb < P ? rl + k * p.rpb : P - 1;  // rows past the end repeat the last one and count nothing
+    v[k] = gn_load<DT>(p.x, xb + (int64_t)r * p.ldx);
+  }
+  float a[8], b[8];
+  gn_affine(p, n, act ? c0 : 0, a, b);
+  float mean[NA], rstd[NA];
+#pragma unroll
+  for (int i = 0; i < NA; ++i) mean[i] = 0.f;
+#pragma unroll
+  for (int pass = 0; pass < 2; ++pass) {
+#pragma unroll
+    for (int a = 0; a < NA; ++a) {
+      float s = 0.f;
+#pragma unroll
+      for (int k = 0; k < NR; ++k) {
+        float t = 0.f;
+#pragma unroll
+        for (int i = 0; i < PER; ++i) {
+          const float d = v[k].v[a * PER + i] - mean[a];
+          t = pass ? fmaf(d, d, t) : t + d;
+        }
+        if (act && rl + k * p.rpb < P) s += t;
+      }
+      sm[tid * NA + a] = s;
+    }
+    __syncthreads();
+    for_groups<GN_TS>(sgroups, p.lpg, [&](int g, bool mine) {
+      float s = 0.f;
+      for (int el = sub; el < p.rpb; el += p.lpg)
+        for (int u = 0; u < units; ++u) s += sm[el * p.tr * NA + g * units + u];
+      s = lanes_sum(s, p.lpg) / total;
+      if (mine && sub == 0) stat[pass][g] = pass ? rsqrtf(s + p.eps) : s;
+    });
+    __syncthreads();
+    int g = oct * 8 / p.cg, gc = oct * 8 - g * p.cg;
+#pragma unroll
+    for (int a = 0; a < NA; ++a) {
+      const float t = act ? stat[pass][g] : 0.f;
+      if (++gc == p.cg) gc = 0, ++g;
+      if (pass) rstd[a] = t;
+      else mean[a] = t;
+    }
+  }
+  if (!act) return;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) a[i] *= rstd[i / PER];
+  const int64_t ob = n * p.p * p.c + c0;
+#pragma unroll
+  for (int k = 0; k < NR; ++k) {
+    if (rl + k * p.rpb >= P) continue;
+    f32x8 y;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) y.v[i] = gn_act(fmaf(v[k].v[i] - mean[i / PER], a[i], b[i]), p.act);
+    gn_store<ODT>(p.out, ob + (int64_t)(rl + k * p.rpb) * p.c, y);
+  }
+}
 
 // least common multiple of 8 and cg
 int64_t gn_unit(int64_t cg) { return cg % 8 == 0 ? cg : cg % 4 == 0 ? 2 * cg : cg % 2 == 0 ? 4 * cg : 8 * cg; }
 
+// lanes that join one of `groups` groups of `ents` rows of entries in a workgroup of t threads
+int gn_lanes(int64_t groups, int64_t ents, int t) {
+  int l = 1;
+  while (l < 64 && 2 * l * groups <= t && l < ents) l *= 2;
+  return l;
+}
+
+struct GnPlan {
+  bool small;
+  int tr, strips;     // octets per row of a workgroup, strips of them
+  int nchunk;         // statistics chunks of an image
+  int64_t schunk, achunk;
+};
+
 GnPlan gn_plan(int64_t n, int64_t p, int64_t c, int64_t groups) {
-  GnPlan g;
+  GnPlan g{};
   const int64_t u = gn_unit(c / groups) / 8;  // octets a workgroup has to hold together
+  // One launch where a unit's pixels fit the registers of one workgroup
+  g.small = p * u <= (int64_t)(GN_TS / u) * u * NRMAX && p <= (int64_t)(GN_TS / u) * NRMAX;
+  if (g.small) {
+    g.tr = (int)u;
+    g.strips = (int)(c / 8 / u);
+    g.nchunk = 1;
+    return g;
+  }
   g.tr = (int)(c / 8 <= GN_T ? c / 8 : u * (GN_T / u));
   g.strips = (int)cdiv(c / 8, g.tr);
-  g.rpb = GN_T / g.tr;
-  // about four workgroups per CU, each at least UR rows per thread
-  int64_t want = cdiv(4LL * device_cus(), n * g.strips);
-  int64_t chunk = cdiv(p, want < 1 ? 1 : want);
-  const int64_t least = (int64_t)UR * g.rpb;
-  chunk = cdiv(chunk < least ? least : chunk, g.rpb) * g.rpb;
-  g.chunk = chunk < p ? chunk : p;
-  g.nchunk = (int)cdiv(p, g.chunk);
+  // statistics: one workgroup per CU; apply: four. Each at least UR (UA) rows per thread
+  auto split = [&](int64_t blocks, int64_t least) {
+    const int64_t want = cdiv(blocks, n * g.strips), len = cdiv(p, want);
+    return len < least ? least : len;
+  };
+  g.schunk = split(device_cus(), (int64_t)UR * (GN_TS / g.tr));
+  g.achunk = split(4LL * device_cus(), (int64_t)UA * (GN_T / g.tr));
+  g.nchunk = (int)cdiv(p, g.schunk);
   return g;
 }
 
@@ -243,9 +438,9 @@ GnPlan gn_plan(int64_t n, int64_t p, int64_t c, int64_t groups) {
 using namespace clarus;
 
 extern "C" size_t clarus_hip_group_norm_workspace(int64_t n, int64_t p, int64_t c, int64_t groups) {
-  if (n <= 0 || p <= 0 || c <= 0 || groups <= 0 || c % groups || c % 8 || gn_unit(c / groups) > 8 * GN_T) return 0;
+  if (n <= 0 || p <= 0 || c <= 0 || groups <= 0 || c % groups || c % 8 || gn_unit(c / groups) > GN_UNIT) return 0;
   const GnPlan g = gn_plan(n, p, c, groups);
-  return (size_t)(n * groups * (g.nchunk + 1)) * sizeof(float2);
+  return g.small ? 8 : (size_t)(n * groups * (g.nchunk + 1)) * sizeof(float2);
 }
 
 extern "C" int clarus_hip_group_norm(const void* x, int32_t x_dtype, int64_t x_bstride, int64_t ldx, const float* w,
@@ -258,7 +453,7 @@ extern "C" int clarus_hip_group_norm(const void* x, int32_t x_dtype, int64_t x_b
   CLARUS_REQUIRE((x_dtype == DT_BF16 || x_dtype == DT_F32) && (o_dtype == DT_BF16 || o_dtype == DT_F32),
                  "group_norm: bf16 or fp32");
   CLARUS_REQUIRE(c % 8 == 0 && c % groups == 0, "group_norm: channels a multiple of 8 and of the groups");
-  CLARUS_REQUIRE(gn_unit(c / groups) <= 8 * GN_T, "group_norm: lcm(8, channels per group) at most %d", 8 * GN_T);
+  CLARUS_REQUIRE(gn_unit(c / groups) <= GN_UNIT, "group_norm: lcm(8, channels per group) at most %d", GN_UNIT);
   CLARUS_REQUIRE(act == ACT_NONE || act == ACT_GELU || act == CLARUS_ACT_SILU, "group_norm: act none, GELU or SiLU");
   const int64_t es = x_dtype == DT_BF16 ? 2 : 4;
   CLARUS_REQUIRE(ldx >= c && (n == 1 || x_bstride >= 0), "group_norm: strides");
@@ -274,27 +469,64 @@ extern "C" int clarus_hip_group_norm(const void* x, int32_t x_dtype, int64_t x_b
   k.x = x; k.out = out; k.w = w; k.b = b;
   k.stat = (float2*)scratch;
   k.part = k.stat + n * groups;
-  k.xbs = x_bstride; k.ldx = ldx; k.p = p; k.chunk = g.chunk;
+  k.xbs = x_bstride; k.ldx = ldx; k.p = p; k.schunk = g.schunk;
   k.wbs = w_bstride; k.bbs = b_bstride;
   k.c = (int)c; k.groups = (int)groups; k.cg = (int)(c / groups); k.nchunk = g.nchunk;
-  k.tr = g.tr; k.rpb = g.rpb; k.eps = eps;
+  k.tr = g.tr; k.eps = eps; k.act = act;
   hipStream_t st = (hipStream_t)stream;
-  const dim3 grid((unsigned)g.nchunk, (unsigned)g.strips, (unsigned)n);
-  note_kernel("gn_stats_kernel + gn_apply_kernel nchunk=%d strips=%d", g.nchunk, g.strips);
   const bool whole = k.cg % 8 == 0;
+  const int64_t sgroups = (c < 8 * g.tr ? c : 8 * g.tr) / k.cg;
+  k.rpb = GN_TS / g.tr;
+  k.lpg = gn_lanes(sgroups, k.rpb, GN_TS);
+  if (g.small) {
+    const int nr = (int)cdiv(p, k.rpb);
+    const dim3 grid(1, (unsigned)g.strips, (unsigned)n);
+    note_kernel("gn_small_kernel strips=%d rows=%d", g.strips, nr);
+#define CLARUS_GN_S(DT, ODT, W)                                                                                  \
+  do {                                                                                                           \
+    if (nr <= 4) hipLaunchKernelGGL((gn_small_kernel<DT, ODT, W, 4>), grid, dim3(GN_TS), 0, st, k);              \
+    else hipLaunchKernelGGL((gn_small_kernel<DT, ODT, W, NRMAX>), grid, dim3(GN_TS), 0, st, k);                  \
+  } while (0)
+#define CLARUS_GN(DT, ODT)                \
+  do {                                    \
+    if (whole) CLARUS_GN_S(DT, ODT, true); \
+    else CLARUS_GN_S(DT, ODT, false);     \
+  } while (0)
+    if (x_dtype == DT_BF16) {
+      if (o_dtype == DT_BF16) CLARUS_GN(DT_BF16, DT_BF16);
+      else CLARUS_GN(DT_BF16, DT_F32);
+    } else {
+      if (o_dtype == DT_BF16) CLARUS_GN(DT_F32, DT_BF16);
+      else CLARUS_GN(DT_F32, DT_F32);
+    }
+#undef CLARUS_GN
+#undef CLARUS_GN_S
+    return check_launch("group_norm");
+  }
+  k.chunk = g.schunk;
+  const dim3 sgrid((unsigned)g.nchunk, (unsigned)g.strips, (unsigned)n);
+  note_kernel("gn_stats_kernel + gn_apply_kernel nchunk=%d strips=%d", g.nchunk, g.strips);
   if (x_dtype == DT_BF16) {
-    if (whole) hipLaunchKernelGGL((gn_stats_kernel<DT_BF16, true>), grid, dim3(GN_T), 0, st, k);
-    else hipLaunchKernelGGL((gn_stats_kernel<DT_BF16, false>), grid, dim3(GN_T), 0, st, k);
+    if (whole) hipLaunchKernelGGL((gn_stats_kernel<DT_BF16, true>), sgrid, dim3(GN_TS), 0, st, k);
+    else hipLaunchKernelGGL((gn_stats_kernel<DT_BF16, false>), sgrid, dim3(GN_TS), 0, st, k);
   } else {
-    if (whole) hipLaunchKernelGGL((gn_stats_kernel<DT_F32, true>), grid, dim3(GN_T), 0, st, k);
-    else hipLaunchKernelGGL((gn_stats_kernel<DT_F32, false>), grid, dim3(GN_T), 0, st, k);
+    if (whole) hipLaunchKernelGGL((gn_stats_kernel<DT_F32, true>), sgrid, dim3(GN_TS), 0, st, k);
+    else hipLaunchKernelGGL((gn_stats_kernel<DT_F32, false>), sgrid, dim3(GN_TS), 0, st, k);
   }
   hipLaunchKernelGGL(gn_join_kernel, dim3((unsigned)groups, (unsigned)n), dim3(64), 0, st, k);
-#define CLARUS_GN(DT, ODT)                                                                               \
-  do {                                                                                                   \
-    if (act == ACT_NONE) hipLaunchKernelGGL((gn_apply_kernel<DT, ODT, ACT_NONE>), grid, dim3(GN_T), 0, st, k);       \
-    else if (act == ACT_GELU) hipLaunchKernelGGL((gn_apply_kernel<DT, ODT, ACT_GELU>), grid, dim3(GN_T), 0, st, k);  \
-    else hipLaunchKernelGGL((gn_apply_kernel<DT, ODT, GN_SILU>), grid, dim3(GN_T), 0, st, k);                        \
+  k.chunk = g.achunk;
+  k.rpb = GN_T / g.tr;
+  const dim3 grid((unsigned)cdiv(p, g.achunk), (unsigned)g.strips, (unsigned)n);
+#define CLARUS_GN_A(DT, ODT, ACT)                                                                      \
+  do {                                                                                                 \
+    if (whole) hipLaunchKernelGGL((gn_apply_kernel<DT, ODT, ACT, true>), grid, dim3(GN_T), 0, st, k);  \
+    else hipLaunchKernelGGL((gn_apply_kernel<DT, ODT, ACT, false>), grid, dim3(GN_T), 0, st, k);       \
+  } while (0)
+#define CLARUS_GN(DT, ODT)                                  \
+  do {                                                      \
+    if (act == ACT_NONE) CLARUS_GN_A(DT, ODT, ACT_NONE);    \
+    else if (act == ACT_GELU) CLARUS_GN_A(DT, ODT, ACT_GELU); \
+    else CLARUS_GN_A(DT, ODT, GN_SILU);                     \
   } while (0)
   if (x_dtype == DT_BF16) {
     if (o_dtype == DT_BF16) CLARUS_GN(DT_BF16, DT_BF16);
@@ -304,5 +536,6 @@ extern "C" int clarus_hip_group_norm(const void* x, int32_t x_dtype, int64_t x_b
     else CLARUS_GN(DT_F32, DT_F32);
   }
 #undef CLARUS_GN
+#undef CLARUS_GN_A
   return check_launch("group_norm");
 }
