@@ -38,18 +38,33 @@ struct CrossP {
   const void *q, *k, *v;
   void* out;
   const unsigned char* mask;
-  float* part;               // [split][nk][rows][D] O, then [split][nk][rows] m, then l
+  float* part;               // [split][nk][rows][D] O, then [split][nk][rows] (m, l)
   int64_t qbs, ldq, kbs, ldk, vbs, ldv, mbs, mqs;
   int64_t rows;              // lq * rep
   int64_t lk, split_len, nk; // nk = n * kv_heads
-  int64_t nblk;              // row blocks
+  int64_t nblk;              // row blocks (resident: workgroups) of an (image, kv head)
   int lq, rep, kv_heads, d, splits, o_dt;
   float c;                   // scale log2(e)
 };
 
+// a and b of lanes l and l ^ 32: the low half keeps a's low and gets a's high lanes in b, the high half gets b's low
+// lanes in a and keeps b's high
+__device__ __forceinline__ void swap32(unsigned& a, unsigned& b) {
+  const auto r = __builtin_amdgcn_permlane32_swap(a, b, false, false);
+  a = r[0];
+  b = r[1];
+}
+
 // max / sum with lane ^ 32
-__device__ __forceinline__ float xor32(float v) {
-  return __shfl_xor(v, 32, 64);
+__device__ __forceinline__ float max32(float v) {
+  unsigned a = __float_as_uint(v), b = a;
+  swap32(a, b);
+  return fmaxf(__uint_as_float(a), __uint_as_float(b));
+}
+__device__ __forceinline__ float sum32(float v) {
+  unsigned a = __float_as_uint(v), b = a;
+  swap32(a, b);
+  return __uint_as_float(a) + __uint_as_float(b);
 }
 
 template <int DT, int D>
@@ -59,7 +74,8 @@ struct XaTile {
   static constexpr int ROWB = D * ES;                 // bytes of a row in LDS
   static constexpr int CPR = ROWB / 16;               // 16-byte chunks per row
   static constexpr int BYTES = KT * ROWB;
-  static constexpr int NI = BYTES / 1024 / (XA_T / 64);  // 1 KiB copies per wave and operand
+  static constexpr int QN = DT == DT_BF16 ? D / 16 : D / 8;  // 16-byte chunks of a row of Q per lane
+  static constexpr uint64_t ALL = KT == 64 ? ~0ull : 0xffffffffull;
   // chunk c of row r sits at position c ^ swz(r). K: 16 lanes read one chunk of 16 consecutive rows; V: bf16
   // 8 rows x 4 chunks (transposing), fp32 two rows 4 apart x 8 chunks: each over all banks (fp32 V of 32 and
   // 96 columns excepted, whose rows r and r + 4 meet)
@@ -83,100 +99,371 @@ __device__ __forceinline__ float keep_bit(float v, unsigned w, int bit) {
   return __uint_as_float((__float_as_uint(v) & k) | (0xff800000u & ~k));
 }
 
-template <int DT, int D, int MASK>
-__global__ void __launch_bounds__(XA_T, D <= 64 ? 4 : 2) xa_kernel(const CrossP p) {
+// one row of a wave: its query, head and mask row
+struct XaRow {
+  int64_t qi;
+  int head;
+};
+
+__device__ __forceinline__ XaRow xa_row(const CrossP& p, int kvh, int64_t row) {
+  // 32-bit division: rows < 2^31
+  const int qi = p.rep == 1 ? (int)row : (int)((unsigned)row / (unsigned)p.rep);
+  return XaRow{qi, kvh * p.rep + (int)row - qi * p.rep};
+}
+
+// Q^T fragments of a row
+template <int DT, int D>
+__device__ __forceinline__ void xa_load_q(const CrossP& p, int64_t n, const XaRow& r, int hl, u32x4 (&qf)[XaTile<DT, D>::QN]) {
   using T = XaTile<DT, D>;
-  constexpr int KT = T::KT, KB = KT / 32, DB = D / 32, ES = T::ES, NI = T::NI;
-  constexpr uint64_t ALL = KT == 64 ? ~0ull : 0xffffffffull;
-  __shared__ __align__(16) unsigned char tiles[2][2 * T::BYTES];
-
-  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int col = lane & 31, hl = lane >> 5;
-  // row blocks of one (image, kv head) run on one XCD, whose L2 then holds that head's K and V
-  const int64_t total = p.nblk * p.nk * p.splits, span = (total + 7) >> 3;
-  const int64_t id = (int64_t)(blockIdx.x & 7) * span + (blockIdx.x >> 3);
-  if ((blockIdx.x >> 3) >= span || id >= total) return;
-  const int64_t rb = id % p.nblk, hs = id / p.nblk;
-  const int split = (int)(hs % p.splits);
-  const int64_t nk = hs / p.splits;
-  const int64_t n = nk / p.kv_heads;
-  const int kvh = (int)(nk - n * p.kv_heads);
-
-  const int64_t wrow = rb * XA_ROWS + wave * 32;  // the wave's first row
-  const bool busy = wrow < p.rows;
-  const int64_t row = wrow + col < p.rows ? wrow + col : p.rows - 1;  // rows past the end repeat the last one
-  const int64_t qi = row / p.rep;
-  const int head = kvh * p.rep + (int)(row - qi * p.rep);
-
-  const unsigned char* kp = (const unsigned char*)p.k + (n * p.kbs + (int64_t)kvh * p.d) * ES;
-  const unsigned char* vp = (const unsigned char*)p.v + (n * p.vbs + (int64_t)kvh * p.d) * ES;
-  const unsigned char* mrow = MASK == MASK_PAIRS ? p.mask + n * p.mbs + qi * p.mqs : nullptr;
-  const unsigned char* mkey = MASK == MASK_KEYS ? p.mask + n * p.mbs : nullptr;
-
-  const int64_t k0 = (int64_t)split * p.split_len, k1 = k0 + p.split_len < p.lk ? k0 + p.split_len : p.lk;
-  const int ntile = (int)((k1 - k0 + KT - 1) / KT);
-
-  // this lane's piece of each copy: row and chunk of the tile, and its offset from the tile's first row
-  uint32_t koff[NI], voff[NI];
-  int rowc[NI];      // row
-  bool have_k[NI], have_v[NI];  // the chunk lies within the head
+  constexpr int E = 16 / T::ES;
+  const unsigned char* qp = (const unsigned char*)p.q + (n * p.qbs + r.qi * p.ldq + (int64_t)r.head * p.d) * T::ES;
 #pragma unroll
-  for (int j = 0; j < NI; ++j) {
-    const int at = (wave + (XA_T / 64) * j) * 1024 + lane * 16;
-    const int r = at / T::ROWB, cpos = (at % T::ROWB) / 16;
-    const int ck = cpos ^ T::swz_k(r), cv = cpos ^ T::swz_v(r);
-    rowc[j] = r;
-    koff[j] = (uint32_t)(r * p.ldk * ES) + ck * 16;
-    voff[j] = (uint32_t)(r * p.ldv * ES) + cv * 16;
-    have_k[j] = ck * 16 < p.d * ES;
-    have_v[j] = cv * 16 < p.d * ES;
+  for (int s = 0; s < T::QN; ++s) {
+    const int at = (2 * s + hl) * E;
+    qf[s] = *reinterpret_cast<const u32x4*>(qp + (at < p.d ? at : 0) * T::ES);
+    if (at >= p.d) qf[s] = u32x4{0, 0, 0, 0};
   }
-  // the kept keys of a tile, one bit each. MASK_KEYS: the byte is loaded a tile ahead of its use
-  auto key_byte = [&](int t) __attribute__((always_inline)) -> int {
-    const int64_t key = k0 + (int64_t)t * KT + lane;
-    const bool in = lane < KT && key < k1;
-    if constexpr (MASK == MASK_KEYS) return in ? mkey[key] : 0;
-    return in;
-  };
-  auto copy = [&](int t, uint64_t bits) __attribute__((always_inline)) {
-    const int64_t base = k0 + (int64_t)t * KT;
-    const unsigned char* kt = kp + base * p.ldk * ES;
-    const unsigned char* vt = vp + base * p.ldv * ES;
-    unsigned char* dst = tiles[t & 1] + wave * 1024;
+}
+
+// the mask bytes of a lane's keys of a tile that starts at key `base` and ends at k1
+template <int KB>
+__device__ __forceinline__ void xa_load_pairs(const unsigned char* mrow, int64_t base, int64_t k1, int hl, unsigned (&w)[KB][4]) {
+  const bool whole = k1 - base >= 32 * KB;
+#pragma unroll
+  for (int b = 0; b < KB; ++b)
+#pragma unroll
+    for (int j4 = 0; j4 < 4; ++j4) {
+      const int64_t key = base + 32 * b + 8 * j4 + 4 * hl;
+      if (whole) {
+        __builtin_memcpy(&w[b][j4], mrow + key, 4);
+      } else {
+        w[b][j4] = 0;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) w[b][j4] |= (key + j < k1 ? (unsigned)mrow[key + j] : 0u) << (8 * j);
+      }
+    }
+}
+
+// One tile of NB x 32 keys for a wave's 32 rows: S^T = K Q^T, the softmax's step, O^T += V^T P^T. bits: the keys that
+// count (MASK_PAIRS: pair instead).
+template <int DT, int D, int MASK, int NB, bool ANEW>
+__device__ __forceinline__ void xa_tile(const unsigned char* ks, const unsigned char* vs, const u32x4 (&qf)[XaTile<DT, D>::QN],
+                                        f32x16 (&o)[D / 32], float& m, float& l, float c, uint64_t bits, bool whole,
+                                        const unsigned (*pair)[4]) {
+  using T = XaTile<DT, D>;
+  constexpr int DB = D / 32, QN = T::QN;
+  // ANEW: the lane's LDS offsets are worked out for each tile instead of kept over the loop, where they spill
+  int lane = threadIdx.x & 63;
+  if constexpr (ANEW) asm volatile("" : "+v"(lane));
+  const int col = lane & 31, hl = lane >> 5;
+  f32x16 s[NB];
+#pragma unroll
+  for (int b = 0; b < NB; ++b) {
+#pragma unroll
+    for (int j = 0; j < 16; ++j) s[b][j] = 0.f;
+#pragma unroll
+    for (int i = 0; i < QN; ++i) {
+      const u32x4 a = *reinterpret_cast<const u32x4*>(ks + T::at_k(32 * b + col, 2 * i + hl));
+      if constexpr (DT == DT_BF16) {
+        s[b] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, qf[i]), s[b], 0, 0, 0);
+      } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          s[b] = __builtin_amdgcn_mfma_f32_32x32x2f32(__uint_as_float(a[e]), __uint_as_float(qf[i][e]), s[b], 0, 0, 0);
+      }
+    }
+  }
+  // masked and padding keys weigh nothing, whatever their scores
+  if constexpr (MASK == MASK_PAIRS) {
+#pragma unroll
+    for (int b = 0; b < NB; ++b)
+#pragma unroll
+      for (int j = 0; j < 16; ++j) s[b][j] = keep_bit(s[b][j], pair[b][j >> 2], 8 * (j & 3));
+  } else if (!whole) {
+#pragma unroll
+    for (int b = 0; b < NB; ++b) {
+      const unsigned w = (unsigned)(bits >> (32 * b)) >> (4 * hl);
+#pragma unroll
+      for (int j = 0; j < 16; ++j) s[b][j] = keep_bit(s[b][j], w, 8 * (j >> 2) + (j & 3));
+    }
+  }
+  // the running maximum moves only when a score passes it by XA_SLACK (weights then stay below 2^XA_SLACK,
+  // and fp32 sums keep their digits): the accumulators are rescaled in few tiles instead of all
+  float mx = -INFINITY;
+#pragma unroll
+  for (int b = 0; b < NB; ++b)
+#pragma unroll
+    for (int j = 0; j < 16; ++j) mx = fmaxf(mx, s[b][j]);
+  if (__any(mx * c > m + XA_SLACK)) {
+    mx = max32(mx);
+    const float mn = fmaxf(m, mx * c);
+    const float alpha = __builtin_amdgcn_exp2f(m - mn);
+    m = mn;
+    l *= alpha;
+#pragma unroll
+    for (int b = 0; b < DB; ++b)
+#pragma unroll
+      for (int j = 0; j < 16; ++j) o[b][j] *= alpha;
+  }
+#pragma unroll
+  for (int b = 0; b < NB; ++b)
+#pragma unroll
+    for (int j = 0; j < 16; ++j) {
+      s[b][j] = __builtin_amdgcn_exp2f(fmaf(s[b][j], c, -m));
+      l += s[b][j];
+    }
+  if constexpr (DT == DT_BF16) {
+    const int i = lane & 15;
+    const int vr = 4 * hl + (i >> 2), vc = 2 * ((lane >> 4) & 1) + ((i & 3) >> 1);
+#pragma unroll
+    for (int ks2 = 0; ks2 < 2 * NB; ++ks2) {
+      f32x8 pv;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) pv.v[e] = s[ks2 >> 1][8 * (ks2 & 1) + e];
+      const bf16x8 pb = pack_bf16(pv);
+#pragma unroll
+      for (int b = 0; b < DB; ++b) {
+        typedef __attribute__((ext_vector_type(8))) short s16x8;
+        const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+            (__attribute__((address_space(3))) s16x4*)(vs + T::at_v(16 * ks2 + vr, 4 * b + vc) + (i & 1) * 8));
+        const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+            (__attribute__((address_space(3))) s16x4*)(vs + T::at_v(16 * ks2 + vr + 8, 4 * b + vc) + (i & 1) * 8));
+        const s16x8 a = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+        o[b] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), pb, o[b], 0, 0, 0);
+      }
+    }
+  } else {
+#pragma unroll
+    for (int b = 0; b < DB; ++b)
+#pragma unroll
+      for (int kb = 0; kb < NB; ++kb)
+#pragma unroll
+        for (int j = 0; j < 16; ++j) {
+          const int r = 32 * kb + 8 * (j >> 2) + 4 * hl + (j & 3);
+          const float a = *reinterpret_cast<const float*>(vs + T::at_v(r, 8 * b + (col >> 2)) + (col & 3) * 4);
+          o[b] = __builtin_amdgcn_mfma_f32_32x32x2f32(a, s[kb][j], o[b], 0, 0, 0);
+        }
+  }
+}
+
+// a finished row: O / l (every lane takes part; live: the row is there)
+template <int D>
+__device__ __forceinline__ void xa_store(const CrossP& p, int64_t n, const XaRow& r, const f32x16 (&o)[D / 32], float l, bool live) {
+  const int hl = (threadIdx.x >> 5) & 1;
+  const float inv = l == 0.f ? 0.f : 1.f / l;
+  const int64_t at = ((n * p.lq + r.qi) * (int64_t)(p.kv_heads * p.rep) + r.head) * p.d;
+#pragma unroll
+  for (int b = 0; b < D / 32; ++b)
+#pragma unroll
+    for (int j = 0; j < 16; j += 8) {
+      f32x4 y[2];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) y[i >> 2][i & 3] = o[b][j + i] * inv;
+      if (p.o_dt == DT_BF16) {
+        // columns 8 (j / 4) + 4 hl .. + 3 of two j / 4: exchanged so that each lane stores 8 columns
+        u32x4 w = {pack2_bf16(y[0][0], y[0][1]), pack2_bf16(y[0][2], y[0][3]), pack2_bf16(y[1][0], y[1][1]), pack2_bf16(y[1][2], y[1][3])};
+        unsigned a0 = w[0], a1 = w[1], b0 = w[2], b1 = w[3];
+        swap32(a0, b0);
+        swap32(a1, b1);
+        const int dd = 32 * b + 2 * j + 8 * hl;
+        if (dd < p.d && live) *reinterpret_cast<u32x4*>((unsigned short*)p.out + at + dd) = u32x4{a0, a1, b0, b1};
+      } else {
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const int dd = 32 * b + 2 * j + 8 * i + 4 * hl;
+          if (dd < p.d && live) *reinterpret_cast<f32x4*>((float*)p.out + at + dd) = y[i];
+        }
+      }
+    }
+}
+
+// The copies of a tile's K and V to LDS: this lane's piece of each of a wave's 1 KiB copies (W waves share a tile)
+template <int DT, int D, int W>
+struct XaCopy {
+  using T = XaTile<DT, D>;
+  static constexpr int NI = (T::BYTES / 1024 + W - 1) / W;  // copies per wave and operand
+  static constexpr bool EVEN = T::BYTES / 1024 % W == 0;
+  uint32_t koff[NI], voff[NI];  // from the tile's first row
+  int row[NI];
+  bool have_k[NI], have_v[NI];  // the chunk lies within the head
+  int wave;
+
+  __device__ __forceinline__ XaCopy(const CrossP& p, int wave_, int lane) : wave(wave_) {
+#pragma unroll
+    for (int j = 0; j < NI; ++j) {
+      const int at = (wave + W * j) * 1024 + lane * 16;
+      const int r = at / T::ROWB, cpos = (at % T::ROWB) / 16;
+      const int ck = cpos ^ T::swz_k(r), cv = cpos ^ T::swz_v(r);
+      row[j] = r;
+      koff[j] = (uint32_t)(r * p.ldk * T::ES) + ck * 16;
+      voff[j] = (uint32_t)(r * p.ldv * T::ES) + cv * 16;
+      have_k[j] = ck * 16 < p.d * T::ES;
+      have_v[j] = cv * 16 < p.d * T::ES;
+    }
+  }
+  __device__ __forceinline__ void operator()(const CrossP& p, const unsigned char* kt, const unsigned char* vt, unsigned char* tile,
+                                             uint64_t bits) const {
+    unsigned char* dst = tile + wave * 1024;
 #define XA_COPY(src, to)                                                                                   \
   __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(src),                  \
                                    (__attribute__((address_space(3))) void*)(to), 16, 0, 0)
-    if (bits == ALL && p.d == D) {
+    if (bits == T::ALL && p.d == D) {
 #pragma unroll
       for (int j = 0; j < NI; ++j) {
-        XA_COPY(kt + koff[j], dst + j * (XA_T / 64) * 1024);
-        XA_COPY(vt + voff[j], dst + T::BYTES + j * (XA_T / 64) * 1024);
+        if (!EVEN && wave + W * j >= T::BYTES / 1024) break;
+        XA_COPY(kt + koff[j], dst + j * W * 1024);
+        XA_COPY(vt + voff[j], dst + T::BYTES + j * W * 1024);
       }
     } else {
       const unsigned char* zero = (const unsigned char*)xa_zeros;
 #pragma unroll
       for (int j = 0; j < NI; ++j) {
-        const bool in = (bits >> rowc[j]) & 1;
-        XA_COPY(in && have_k[j] ? kt + koff[j] : zero, dst + j * (XA_T / 64) * 1024);
-        XA_COPY(in && have_v[j] ? vt + voff[j] : zero, dst + T::BYTES + j * (XA_T / 64) * 1024);
+        if (!EVEN && wave + W * j >= T::BYTES / 1024) break;
+        const bool in = (bits >> row[j]) & 1;
+        XA_COPY(in && have_k[j] ? kt + koff[j] : zero, dst + j * W * 1024);
+        XA_COPY(in && have_v[j] ? vt + voff[j] : zero, dst + T::BYTES + j * W * 1024);
       }
     }
 #undef XA_COPY
-  };
+  }
+};
 
-  // Q^T fragments
-  constexpr int QN = DT == DT_BF16 ? D / 16 : D / 8;  // 16-byte chunks per lane
-  u32x4 qf[QN];
+// this lane's key of a tile counts (MASK_KEYS: the mask's byte)
+template <int KT, int MASK>
+__device__ __forceinline__ int xa_key_byte(const unsigned char* mkey, int64_t base, int64_t k1, int lane) {
+  const int64_t key = base + lane;
+  const bool in = lane < KT && key < k1;
+  if constexpr (MASK == MASK_KEYS) return in ? mkey[key] : 0;
+  return in;
+}
+
+// ---------------------------------------------------------------- keys that fit LDS
+// All keys of an (image, kv head) stay in a workgroup's LDS: copied once, one barrier, then its 8 waves take 32 rows
+// each, chunk after chunk, the next chunk's queries in flight. Workgroups of the same rows and other heads run on one
+// XCD, whose L2 then reads and writes each line of q and out once.
+constexpr int XR_T = 512;
+__host__ __device__ constexpr int xr_tiles(int d, int tile_bytes) { return (d <= 64 ? 80 : 160) * 1024 / (2 * tile_bytes); }
+
+template <int DT, int D, int MASK>
+__global__ void __launch_bounds__(XR_T, D <= 64 ? 4 : 2) xa_resident_kernel(const CrossP p) {
+  using T = XaTile<DT, D>;
+  constexpr int KT = T::KT, W = XR_T / 64;
+  extern __shared__ __attribute__((aligned(16))) unsigned char tiles[];
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int col = lane & 31, hl = lane >> 5;
+  const unsigned total = (unsigned)(p.nblk * p.nk), span = (total + 7) >> 3;
+  const unsigned id = (blockIdx.x & 7) * span + (blockIdx.x >> 3);
+  if ((blockIdx.x >> 3) >= span || id >= total) return;
+  const int part = (int)(id / (unsigned)p.nk);
+  const int nk = (int)(id - part * (unsigned)p.nk);
+  const int n = nk / p.kv_heads, kvh = nk - n * p.kv_heads;
+  const unsigned char* kp = (const unsigned char*)p.k + (n * p.kbs + (int64_t)kvh * p.d) * T::ES;
+  const unsigned char* vp = (const unsigned char*)p.v + (n * p.vbs + (int64_t)kvh * p.d) * T::ES;
+  const unsigned char* mkey = MASK == MASK_KEYS ? p.mask + n * p.mbs : nullptr;
+  const int lk = (int)p.lk, ntile = (lk + KT - 1) / KT;
+
+  // chunks of 32 rows: part `part` of nblk equal parts, wave after wave
+  const int chunks = (int)((p.rows + 31) / 32), each = (int)((chunks + p.nblk - 1) / p.nblk);
+  const int c1 = min((part + 1) * each, chunks);
+  int ch = part * each + wave;
+  auto at = [&](int c) __attribute__((always_inline)) {  // rows past the end repeat the last one
+    const int64_t r = (int64_t)c * 32 + col;
+    return xa_row(p, kvh, r < p.rows ? r : p.rows - 1);
+  };
+  u32x4 qn[T::QN];
+  if (ch < c1) xa_load_q<DT, D>(p, n, at(ch), hl, qn);
+  constexpr int MT = xr_tiles(D, T::BYTES);
+  uint64_t kept[MT];  // the keys of each tile that count
   {
-    const unsigned char* qp = (const unsigned char*)p.q + (n * p.qbs + qi * p.ldq + (int64_t)head * p.d) * ES;
-    constexpr int E = 16 / ES;
+    int byte[MT];
 #pragma unroll
-    for (int s = 0; s < QN; ++s) {
-      const int at = (2 * s + hl) * E;
-      qf[s] = at < p.d ? *reinterpret_cast<const u32x4*>(qp + at * ES) : u32x4{0, 0, 0, 0};
+    for (int t = 0; t < MT; ++t) byte[t] = t < ntile ? xa_key_byte<KT, MASK>(mkey, (int64_t)t * KT, lk, lane) : 0;
+    const XaCopy<DT, D, W> copy(p, wave, lane);
+#pragma unroll
+    for (int t = 0; t < MT; ++t) {
+      kept[t] = __ballot(byte[t]);
+      if (kept[t])
+        copy(p, kp + (int64_t)t * KT * p.ldk * T::ES, vp + (int64_t)t * KT * p.ldv * T::ES, tiles + t * 2 * T::BYTES, kept[t]);
     }
   }
+  __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0): this wave's copies have landed
+  barrier_keep_vm();
+#pragma unroll 1
+  for (; ch < c1; ch += W) {
+    u32x4 qf[T::QN];
+#pragma unroll
+    for (int i = 0; i < T::QN; ++i) qf[i] = qn[i];
+    const XaRow r = at(ch);
+    if (ch + W < c1) xa_load_q<DT, D>(p, n, at(ch + W), hl, qn);
+    const unsigned char* mrow = MASK == MASK_PAIRS ? p.mask + n * p.mbs + r.qi * p.mqs : nullptr;
+    f32x16 o[D / 32];
+#pragma unroll
+    for (int b = 0; b < D / 32; ++b)
+#pragma unroll
+      for (int j = 0; j < 16; ++j) o[b][j] = 0.f;
+    float m = XA_FLOOR, l = 0.f;
+    // 32 keys at a time (a row of 32 keys starts where the swizzles do), half of a tile in bf16
+#pragma unroll 1
+    for (int h = 0; h < lk; h += 32) {
+      const unsigned char* ks = tiles + h / KT * 2 * T::BYTES + h % KT * T::ROWB;
+      uint32_t bits = 0;
+#pragma unroll
+      for (int t = 0; t < MT; ++t)
+        if (h / KT == t) bits = (unsigned)(kept[t] >> (h % KT));
+      unsigned pair[1][4];
+      if constexpr (MASK == MASK_PAIRS) {
+        xa_load_pairs<1>(mrow, h, lk, hl, pair);
+        if (!__any(pair[0][0] | pair[0][1] | pair[0][2] | pair[0][3])) bits = 0;
+      }
+      if (bits) xa_tile<DT, D, MASK, 1, true>(ks, ks + T::BYTES, qf, o, m, l, p.c, bits, bits == 0xffffffffu, pair);
+    }
+    l = sum32(l);
+    xa_store<D>(p, n, r, o, l, ch * 32ll + col < p.rows);
+  }
+}
 
+// ---------------------------------------------------------------- keys streamed through LDS
+template <int DT, int D, int MASK>
+__global__ void __launch_bounds__(XA_T, D <= 64 ? (MASK == MASK_PAIRS ? 3 : 4) : 2) xa_kernel(const CrossP p) {
+  using T = XaTile<DT, D>;
+  constexpr int KT = T::KT, KB = KT / 32, DB = D / 32;
+  __shared__ __align__(16) unsigned char tiles[2][2 * T::BYTES];
+
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int col = lane & 31, hl = lane >> 5;
+  // row blocks of one (image, kv head) run on one XCD, whose L2 then holds that head's K and V
+  const unsigned total = (unsigned)(p.nblk * p.nk * p.splits), span = (total + 7) >> 3;
+  const unsigned id = (blockIdx.x & 7) * span + (blockIdx.x >> 3);
+  if ((blockIdx.x >> 3) >= span || id >= total) return;
+  const unsigned hs = id / (unsigned)p.nblk, rb = id - hs * (unsigned)p.nblk;
+  const int nk = (int)(hs / (unsigned)p.splits), split = (int)(hs - nk * (unsigned)p.splits);
+  const int n = nk / p.kv_heads, kvh = nk - n * p.kv_heads;
+
+  const int64_t wrow = (int64_t)rb * XA_ROWS + wave * 32;  // the wave's first row
+  const bool busy = wrow < p.rows;
+  const int64_t row = wrow + col < p.rows ? wrow + col : p.rows - 1;  // rows past the end repeat the last one
+  const XaRow r = xa_row(p, kvh, row);
+
+  const unsigned char* kp = (const unsigned char*)p.k + (n * p.kbs + (int64_t)kvh * p.d) * T::ES;
+  const unsigned char* vp = (const unsigned char*)p.v + (n * p.vbs + (int64_t)kvh * p.d) * T::ES;
+  const unsigned char* mrow = MASK == MASK_PAIRS ? p.mask + n * p.mbs + r.qi * p.mqs : nullptr;
+  const unsigned char* mkey = MASK == MASK_KEYS ? p.mask + n * p.mbs : nullptr;
+
+  const int64_t k0 = (int64_t)split * p.split_len, k1 = k0 + p.split_len < p.lk ? k0 + p.split_len : p.lk;
+  const int ntile = (int)((k1 - k0 + KT - 1) / KT);
+
+  const XaCopy<DT, D, XA_T / 64> copy(p, wave, lane);
+  // the kept keys of a tile, one bit each. MASK_KEYS: the byte is loaded a tile ahead of its use
+  auto key_byte = [&](int t) __attribute__((always_inline)) {
+    return xa_key_byte<KT, MASK>(mkey, k0 + (int64_t)t * KT, k1, lane);
+  };
+  auto fill = [&](int t, uint64_t bits) __attribute__((always_inline)) {
+    const int64_t base = k0 + (int64_t)t * KT;
+    copy(p, kp + base * p.ldk * T::ES, vp + base * p.ldv * T::ES, tiles[t & 1], bits);
+  };
+
+  u32x4 qf[T::QN];
+  xa_load_q<DT, D>(p, n, r, hl, qf);
   f32x16 o[DB];
 #pragma unroll
   for (int b = 0; b < DB; ++b)
@@ -186,212 +473,149 @@ __global__ void __launch_bounds__(XA_T, D <= 64 ? 4 : 2) xa_kernel(const CrossP 
 
   uint64_t bits = 0;
   int byte = 0;
+  unsigned pair[KB][4], next[KB][4];
   if (ntile > 0) {
     bits = __ballot(key_byte(0));
     if (ntile > 1) byte = key_byte(1);
-    if (bits) copy(0, bits);
+    if (bits) fill(0, bits);
+    if constexpr (MASK == MASK_PAIRS) xa_load_pairs<KB>(mrow, k0, k1, hl, next);
   }
   for (int t = 0; t < ntile; ++t) {
     const uint64_t now = bits;
     __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0): this wave's copies of tile t have landed
     barrier_keep_vm();                   // everybody's have, and tile t - 1 has been read
+    if constexpr (MASK == MASK_PAIRS) {
+#pragma unroll
+      for (int b = 0; b < KB; ++b)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) pair[b][j] = next[b][j];
+    }
     if (t + 1 < ntile) {
       bits = __ballot(byte);
       if (t + 2 < ntile) byte = key_byte(t + 2);
-      if (bits) copy(t + 1, bits);
+      if (bits) fill(t + 1, bits);
+      if constexpr (MASK == MASK_PAIRS) xa_load_pairs<KB>(mrow, k0 + (int64_t)(t + 1) * KT, k1, hl, next);
     }
     if (!busy || !now) continue;
-    const unsigned char* ks = tiles[t & 1];
-    const unsigned char* vs = tiles[t & 1] + T::BYTES;
-    unsigned pair[KB][4];
     if constexpr (MASK == MASK_PAIRS) {
-      const int64_t base = k0 + (int64_t)t * KT;
       unsigned any = 0;
 #pragma unroll
-      for (int b = 0; b < KB; ++b)
-#pragma unroll
-        for (int j4 = 0; j4 < 4; ++j4) {
-          const int64_t key = base + 32 * b + 8 * j4 + 4 * hl;
-          unsigned w = 0;
-          if (now == ALL) {
-            __builtin_memcpy(&w, mrow + key, 4);
-          } else {
-#pragma unroll
-            for (int j = 0; j < 4; ++j) w |= (key + j < k1 ? (unsigned)mrow[key + j] : 0u) << (8 * j);
-          }
-          pair[b][j4] = w;
-          any |= w;
-        }
+      for (int b = 0; b < KB; ++b) any |= pair[b][0] | pair[b][1] | pair[b][2] | pair[b][3];
       if (!__any(any)) continue;
     }
-    f32x16 s[KB];
-#pragma unroll
-    for (int b = 0; b < KB; ++b) {
-#pragma unroll
-      for (int j = 0; j < 16; ++j) s[b][j] = 0.f;
-#pragma unroll
-      for (int i = 0; i < QN; ++i) {
-        const u32x4 a = *reinterpret_cast<const u32x4*>(ks + T::at_k(32 * b + col, 2 * i + hl));
-        if constexpr (DT == DT_BF16) {
-          s[b] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, qf[i]), s[b], 0, 0, 0);
-        } else {
-#pragma unroll
-          for (int e = 0; e < 4; ++e)
-            s[b] = __builtin_amdgcn_mfma_f32_32x32x2f32(__uint_as_float(a[e]), __uint_as_float(qf[i][e]), s[b], 0, 0, 0);
-        }
-      }
-    }
-    // masked and padding keys weigh nothing, whatever their scores
-    if constexpr (MASK == MASK_PAIRS) {
-#pragma unroll
-      for (int b = 0; b < KB; ++b)
-#pragma unroll
-        for (int j = 0; j < 16; ++j) s[b][j] = keep_bit(s[b][j], pair[b][j >> 2], 8 * (j & 3));
-    } else if (now != ALL) {
-#pragma unroll
-      for (int b = 0; b < KB; ++b) {
-        const unsigned w = (unsigned)(now >> (32 * b)) >> (4 * hl);
-#pragma unroll
-        for (int j = 0; j < 16; ++j) s[b][j] = keep_bit(s[b][j], w, 8 * (j >> 2) + (j & 3));
-      }
-    }
-    // the running maximum moves only when a score passes it by XA_SLACK (weights then stay below 2^XA_SLACK,
-    // and fp32 sums keep their digits): the accumulators are rescaled in few tiles instead of all
-    float mx = -INFINITY;
-#pragma unroll
-    for (int b = 0; b < KB; ++b)
-#pragma unroll
-      for (int j = 0; j < 16; ++j) mx = fmaxf(mx, s[b][j]);
-    if (__any(mx * p.c > m + XA_SLACK)) {
-      mx = fmaxf(mx, xor32(mx));
-      const float mn = fmaxf(m, mx * p.c);
-      const float alpha = __builtin_amdgcn_exp2f(m - mn);
-      m = mn;
-      l *= alpha;
-#pragma unroll
-      for (int b = 0; b < DB; ++b)
-#pragma unroll
-        for (int j = 0; j < 16; ++j) o[b][j] *= alpha;
-    }
-#pragma unroll
-    for (int b = 0; b < KB; ++b)
-#pragma unroll
-      for (int j = 0; j < 16; ++j) {
-        s[b][j] = __builtin_amdgcn_exp2f(fmaf(s[b][j], p.c, -m));
-        l += s[b][j];
-      }
-    if constexpr (DT == DT_BF16) {
-      const int i = lane & 15;
-      const int vr = 4 * hl + (i >> 2), vc = 2 * ((lane >> 4) & 1) + ((i & 3) >> 1);
-#pragma unroll
-      for (int ks2 = 0; ks2 < KT / 16; ++ks2) {
-        f32x8 pv;
-#pragma unroll
-        for (int e = 0; e < 8; ++e) pv.v[e] = s[ks2 >> 1][8 * (ks2 & 1) + e];
-        const bf16x8 pb = pack_bf16(pv);
-#pragma unroll
-        for (int b = 0; b < DB; ++b) {
-          typedef __attribute__((ext_vector_type(8))) short s16x8;
-          const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-              (__attribute__((address_space(3))) s16x4*)(vs + T::at_v(16 * ks2 + vr, 4 * b + vc) + (i & 1) * 8));
-          const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-              (__attribute__((address_space(3))) s16x4*)(vs + T::at_v(16 * ks2 + vr + 8, 4 * b + vc) + (i & 1) * 8));
-          const s16x8 a = __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
-          o[b] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), pb, o[b], 0, 0, 0);
-        }
-      }
-    } else {
-#pragma unroll
-      for (int b = 0; b < DB; ++b)
-#pragma unroll
-        for (int kb = 0; kb < KB; ++kb)
-#pragma unroll
-          for (int j = 0; j < 16; ++j) {
-            const int r = 32 * kb + 8 * (j >> 2) + 4 * hl + (j & 3);
-            const float a = *reinterpret_cast<const float*>(vs + T::at_v(r, 8 * b + (col >> 2)) + (col & 3) * 4);
-            o[b] = __builtin_amdgcn_mfma_f32_32x32x2f32(a, s[kb][j], o[b], 0, 0, 0);
-          }
-    }
+    xa_tile<DT, D, MASK, KB, false>(tiles[t & 1], tiles[t & 1] + T::BYTES, qf, o, m, l, p.c, now, now == T::ALL, pair);
   }
-  if (!busy || wrow + col >= p.rows) return;
-  l += xor32(l);
-  if (p.splits > 1) {
-    const int64_t at = ((int64_t)split * p.nk + nk) * p.rows + row, all = (int64_t)p.splits * p.nk * p.rows;
-    float* po = p.part + at * D;
-#pragma unroll
-    for (int b = 0; b < DB; ++b)
-#pragma unroll
-      for (int j4 = 0; j4 < 4; ++j4)
-        *reinterpret_cast<f32x4*>(po + 32 * b + 8 * j4 + 4 * hl) = f32x4{o[b][4 * j4], o[b][4 * j4 + 1], o[b][4 * j4 + 2], o[b][4 * j4 + 3]};
-    if (hl == 0) {
-      p.part[all * D + at] = m;
-      p.part[all * (D + 1) + at] = l;
-    }
+  if (!busy) return;
+  l = sum32(l);
+  if (p.splits == 1) {
+    xa_store<D>(p, n, r, o, l, wrow + col < p.rows);
     return;
   }
-  const float inv = l == 0.f ? 0.f : 1.f / l;
-  const int64_t at = ((n * p.lq + qi) * (int64_t)(p.kv_heads * p.rep) + head) * p.d;
+  if (wrow + col >= p.rows) return;
+  const int64_t at = ((int64_t)split * p.nk + nk) * p.rows + row, all = (int64_t)p.splits * p.nk * p.rows;
+  float* po = p.part + at * D;
 #pragma unroll
   for (int b = 0; b < DB; ++b)
 #pragma unroll
-    for (int j4 = 0; j4 < 4; ++j4) {
-      const int dd = 32 * b + 8 * j4 + 4 * hl;
-      if (dd >= p.d) continue;
-      const f32x4 y = f32x4{o[b][4 * j4] * inv, o[b][4 * j4 + 1] * inv, o[b][4 * j4 + 2] * inv, o[b][4 * j4 + 3] * inv};
-      if (p.o_dt == DT_BF16)
-        *reinterpret_cast<u32x2*>((unsigned short*)p.out + at + dd) = u32x2{pack2_bf16(y[0], y[1]), pack2_bf16(y[2], y[3])};
-      else
-        *reinterpret_cast<f32x4*>((float*)p.out + at + dd) = y;
-    }
+    for (int j4 = 0; j4 < 4; ++j4)
+      *reinterpret_cast<f32x4*>(po + 32 * b + 8 * j4 + 4 * hl) = f32x4{o[b][4 * j4], o[b][4 * j4 + 1], o[b][4 * j4 + 2], o[b][4 * j4 + 3]};
+  if (hl == 0) *reinterpret_cast<float2*>(p.part + all * D + 2 * at) = float2{m, l};
 }
 
-// one wave per row: the splits' (O, m, l) joined in split order
+// One wave per row: the splits' (O, m, l) joined. m and l of 64 splits are in flight at a time, then O of 8
 template <int D>
 __global__ void __launch_bounds__(64) xa_join_kernel(const CrossP p) {
+  constexpr int E = D > 64 ? 2 : 1;  // columns per lane (D = 32: half of the wave idles)
   const int64_t row = blockIdx.x, nk = blockIdx.y, all = (int64_t)p.splits * p.nk * p.rows;
   const int64_t step = p.nk * p.rows, first = nk * p.rows + row;
-  const float *pm = p.part + all * D + first, *pl = p.part + all * (D + 1) + first;
-  float m = XA_FLOOR;
-  for (int s = 0; s < p.splits; ++s) m = fmaxf(m, pm[s * step]);
-  float l = 0.f;
-  for (int s = 0; s < p.splits; ++s) l = fmaf(pl[s * step], __builtin_amdgcn_exp2f(pm[s * step] - m), l);
-  const float inv = l == 0.f ? 0.f : 1.f / l;
-  const int64_t n = nk / p.kv_heads, qi = row / p.rep;
-  const int head = (int)(nk - n * p.kv_heads) * p.rep + (int)(row - qi * p.rep);
-  const int64_t at = ((n * p.lq + qi) * (int64_t)(p.kv_heads * p.rep) + head) * p.d;
-  for (int dd = threadIdx.x; dd < p.d; dd += 64) {
-    float o = 0.f;
-    for (int s = 0; s < p.splits; ++s) o = fmaf(p.part[(first + s * step) * D + dd], __builtin_amdgcn_exp2f(pm[s * step] - m), o);
-    store1(p.out, p.o_dt, at + dd, o * inv);
+  const float2* ml = reinterpret_cast<const float2*>(p.part + all * D) + first;
+  const int lane = threadIdx.x, d0 = lane * E < D ? lane * E : 0;
+  const float* po = p.part + first * D + d0;
+  float m = XA_FLOOR, l = 0.f, o[E];
+#pragma unroll
+  for (int e = 0; e < E; ++e) o[e] = 0.f;
+  for (int s0 = 0; s0 < p.splits; s0 += 64) {
+    const int ns = p.splits - s0 < 64 ? p.splits - s0 : 64;
+    const float2 v = lane < ns ? ml[(s0 + lane) * step] : float2{XA_FLOOR, 0.f};
+    float mx = v.x;
+#pragma unroll
+    for (int i = 1; i < 64; i <<= 1) mx = fmaxf(mx, __shfl_xor(mx, i, 64));
+    const float mn = fmaxf(m, mx), alpha = __builtin_amdgcn_exp2f(m - mn), w = __builtin_amdgcn_exp2f(v.x - mn);
+    m = mn;
+    l = fmaf(l, alpha, group_sum<64>(v.y * w));
+#pragma unroll
+    for (int e = 0; e < E; ++e) o[e] *= alpha;
+    for (int s = 0; s < ns; s += 8) {
+      float x[8][E];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const int at = s + i < ns ? s + i : ns - 1;
+#pragma unroll
+        for (int e = 0; e < E; ++e) x[i][e] = po[(s0 + at) * step * D + e];
+      }
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const float wi = __shfl(w, s + i < ns ? s + i : 0, 64);
+#pragma unroll
+        for (int e = 0; e < E; ++e) o[e] = s + i < ns ? fmaf(x[i][e], wi, o[e]) : o[e];
+      }
+    }
   }
+  const float inv = l == 0.f ? 0.f : 1.f / l;
+  const int n = (int)(nk / p.kv_heads);
+  const XaRow r = xa_row(p, (int)nk - n * p.kv_heads, row);
+  const int64_t at = ((n * (int64_t)p.lq + r.qi) * (int64_t)(p.kv_heads * p.rep) + r.head) * p.d;
+#pragma unroll
+  for (int e = 0; e < E; ++e)
+    if (lane * E + e < p.d) store1(p.out, p.o_dt, at + lane * E + e, o[e] * inv);
 }
 
 int xa_pad(int64_t d) { return d <= 32 ? 32 : d <= 64 ? 64 : d <= 96 ? 96 : 128; }
 
+#ifndef XA_SLOTS
+#define XA_SLOTS 4LL
+#endif
 struct XaPlan {
-  int64_t nblk, split_len;
+  bool resident;
+  int64_t nblk, split_len;  // row blocks (resident: workgroups) of an (image, kv head); keys of a split
   int splits;
 };
 
-XaPlan xa_plan(int32_t dt, int64_t n, int64_t lq, int64_t lk, int64_t heads, int64_t kv_heads) {
-  XaPlan g;
-  const int kt = dt == DT_BF16 ? 64 : 32;
-  g.nblk = cdiv(lq * (heads / kv_heads), XA_ROWS);
-  const int64_t blocks = g.nblk * n * kv_heads;
+XaPlan xa_plan(int32_t dt, int64_t n, int64_t lq, int64_t lk, int64_t heads, int64_t kv_heads, int64_t d) {
+  XaPlan g{};
+  const int kt = dt == DT_BF16 ? 64 : 32, D = xa_pad(d);
+  const int64_t rows = lq * (heads / kv_heads), nk = n * kv_heads;
+  if (cdiv(lk, kt) <= xr_tiles(D, kt * D * (dt == DT_BF16 ? 2 : 4))) {
+    g.resident = true;
+    g.splits = 1;
+    g.split_len = lk;
+    const int64_t want = cdiv((D <= 64 ? 2LL : 1LL) * device_cus(), nk), most = cdiv(rows, 32 * (XR_T / 64));
+    g.nblk = want < most ? want : most;
+    return g;
+  }
+  g.nblk = cdiv(rows, XA_ROWS);
+  const int64_t blocks = g.nblk * nk;
   // split the keys while the row blocks leave CUs idle: two workgroups per CU, four tiles or more each
-  int64_t want = 2LL * device_cus() / blocks;
+  int64_t want = (D <= 64 ? XA_SLOTS : 2LL) * device_cus() / blocks;
   const int64_t most = cdiv(lk, 4 * kt);
   if (want > most) want = most;
   if (want < 1) want = 1;
   g.split_len = cdiv(cdiv(lk, want), kt) * kt;
-  if (g.split_len < kt) g.split_len = kt;
-  g.splits = (int)(lk > 0 ? cdiv(lk, g.split_len) : 1);
+  g.splits = (int)cdiv(lk, g.split_len);
   return g;
 }
 
 template <int DT, int D>
-void xa_launch(const CrossP& k, int mask, hipStream_t st) {
+void xa_launch(const CrossP& k, bool resident, int mask, hipStream_t st) {
   const dim3 grid((unsigned)(8 * ((k.nblk * k.nk * k.splits + 7) / 8)));
+  if (resident) {
+    using T = XaTile<DT, D>;
+    const unsigned lds = (unsigned)(cdiv(k.lk, T::KT) * 2 * T::BYTES);
+    if (mask == MASK_NONE) hipLaunchKernelGGL((xa_resident_kernel<DT, D, MASK_NONE>), grid, dim3(XR_T), lds, st, k);
+    else if (mask == MASK_KEYS) hipLaunchKernelGGL((xa_resident_kernel<DT, D, MASK_KEYS>), grid, dim3(XR_T), lds, st, k);
+    else hipLaunchKernelGGL((xa_resident_kernel<DT, D, MASK_PAIRS>), grid, dim3(XR_T), lds, st, k);
+    return;
+  }
   if (mask == MASK_NONE) hipLaunchKernelGGL((xa_kernel<DT, D, MASK_NONE>), grid, dim3(XA_T), 0, st, k);
   else if (mask == MASK_KEYS) hipLaunchKernelGGL((xa_kernel<DT, D, MASK_KEYS>), grid, dim3(XA_T), 0, st, k);
   else hipLaunchKernelGGL((xa_kernel<DT, D, MASK_PAIRS>), grid, dim3(XA_T), 0, st, k);
@@ -406,8 +630,8 @@ using namespace clarus;
 
 extern "C" size_t clarus_hip_cross_attention_workspace(int32_t dtype, int64_t n, int64_t lq, int64_t lk, int64_t heads,
                                                        int64_t kv_heads, int64_t d) {
-  if (n <= 0 || lq <= 0 || lk < 0 || kv_heads <= 0 || heads <= 0 || heads % kv_heads || d <= 0 || d > 128) return 0;
-  const XaPlan g = xa_plan(dtype, n, lq, lk, heads, kv_heads);
+  if (n <= 0 || lq <= 0 || lk <= 0 || kv_heads <= 0 || heads <= 0 || heads % kv_heads || d <= 0 || d > 128) return 0;
+  const XaPlan g = xa_plan(dtype, n, lq, lk, heads, kv_heads, d);
   return g.splits > 1 ? (size_t)g.splits * n * heads * lq * (xa_pad(d) + 2) * sizeof(float) : 0;
 }
 
@@ -434,7 +658,7 @@ extern "C" int clarus_hip_cross_attention(const ClarusCrossArgs* a, void* scratc
   CLARUS_REQUIRE(a->lq < ((int64_t)1 << 31) && a->lk < ((int64_t)1 << 31) && a->n * a->kv_heads < 65536 &&
                      a->lq * (a->heads / a->kv_heads) < ((int64_t)1 << 31),
                  "cross_attention: too large");
-  const XaPlan g = xa_plan(a->dtype, a->n, a->lq, a->lk, a->heads, a->kv_heads);
+  const XaPlan g = xa_plan(a->dtype, a->n, a->lq, a->lk, a->heads, a->kv_heads, a->d);
   CLARUS_REQUIRE(8 * ((g.nblk * a->n * a->kv_heads * g.splits + 7) / 8) < ((int64_t)1 << 31), "cross_attention: too large");
   const size_t need = clarus_hip_cross_attention_workspace(a->dtype, a->n, a->lq, a->lk, a->heads, a->kv_heads, a->d);
   CLARUS_REQUIRE(need == 0 || (scratch && aligned(scratch, 16) && scratch_bytes >= need),
@@ -450,13 +674,13 @@ extern "C" int clarus_hip_cross_attention(const ClarusCrossArgs* a, void* scratc
   k.c = a->scale * 1.4426950408889634f;
   hipStream_t st = (hipStream_t)stream;
   const int D = xa_pad(a->d);
-  note_kernel("xa_kernel d=%d splits=%d", D, g.splits);
+  note_kernel("%s d=%d splits=%d", g.resident ? "xa_resident_kernel" : "xa_kernel", D, g.splits);
 #define CLARUS_XA(DT)                                        \
   do {                                                       \
-    if (D == 32) xa_launch<DT, 32>(k, a->mask_mode, st);     \
-    else if (D == 64) xa_launch<DT, 64>(k, a->mask_mode, st); \
-    else if (D == 96) xa_launch<DT, 96>(k, a->mask_mode, st); \
-    else xa_launch<DT, 128>(k, a->mask_mode, st);            \
+    if (D == 32) xa_launch<DT, 32>(k, g.resident, a->mask_mode, st);     \
+    else if (D == 64) xa_launch<DT, 64>(k, g.resident, a->mask_mode, st); \
+    else if (D == 96) xa_launch<DT, 96>(k, g.resident, a->mask_mode, st); \
+    else xa_launch<DT, 128>(k, g.resident, a->mask_mode, st);            \
   } while (0)
   if (a->dtype == DT_BF16) CLARUS_XA(DT_BF16);
   else CLARUS_XA(DT_F32);

@@ -22,8 +22,9 @@ namespace clarus {
 namespace {
 
 constexpr int GN_T = 256;    // threads of an apply workgroup
-constexpr int GN_TS = 512;   // threads of a stats or small workgroup
-constexpr int UR = 8;        // rows in flight per thread (stats)
+constexpr int GN_TS = 512;   // threads of a small workgroup
+constexpr int GN_TT = 256;   // threads of a stats workgroup
+constexpr int UR = 8;         // rows in flight per thread (stats)
 constexpr int UA = 4;        // rows in flight per thread (apply)
 constexpr int NRMAX = 16;    // rows held per thread (small)
 constexpr int GN_JOIN = 8;   // partial statistics in flight per thread (join)
@@ -79,10 +80,10 @@ __device__ __forceinline__ void for_groups(int ng, int lpg, F&& f) {
 
 // WHOLE: cg % 8 == 0, an octet lies in one group and is one set of 8 values per row
 template <int DT, bool WHOLE>
-__global__ void __launch_bounds__(GN_TS) gn_stats_kernel(const GroupNormP p) {
+__global__ void __launch_bounds__(GN_TT) gn_stats_kernel(const GroupNormP p) {
   constexpr int NA = WHOLE ? 1 : 8;  // (mean, M2) pairs per thread
   constexpr int PER = WHOLE ? 8 : 1;
-  __shared__ float sm[GN_TS * NA], s2[GN_TS * NA];
+  __shared__ float sm[GN_TT * NA], s2[GN_TT * NA];
   const int tid = threadIdx.x;
   const int rl = tid / p.tr, oct = tid - rl * p.tr;
   const int64_t n = blockIdx.z, r0 = (int64_t)blockIdx.x * p.chunk;
@@ -161,7 +162,7 @@ __global__ void __launch_bounds__(GN_TS) gn_stats_kernel(const GroupNormP p) {
   const int sgroups = min(p.tr * 8, p.c - c0) / p.cg;  // groups of the strip
   const int full = rows / p.rpb, rem = rows - full * p.rpb;
   const float total = (float)rows * (float)p.cg;
-  for_groups<GN_TS>(sgroups, p.lpg, [&](int g, bool mine) {
+  for_groups<GN_TT>(sgroups, p.lpg, [&](int g, bool mine) {
     float ms = 0.f;
     for (int el = sub; el < p.rpb; el += p.lpg) {
       const float k = (float)(PER * (full + (el < rem)));
@@ -420,12 +421,12 @@ GnPlan gn_plan(int64_t n, int64_t p, int64_t c, int64_t groups) {
   }
   g.tr = (int)(c / 8 <= GN_T ? c / 8 : u * (GN_T / u));
   g.strips = (int)cdiv(c / 8, g.tr);
-  // statistics: one workgroup per CU; apply: four. Each at least UR (UA) rows per thread
+  // statistics: two workgroups per CU; apply: four. Each at least UR (UA) rows per thread
   auto split = [&](int64_t blocks, int64_t least) {
     const int64_t want = cdiv(blocks, n * g.strips), len = cdiv(p, want);
     return len < least ? least : len;
   };
-  g.schunk = split(device_cus(), (int64_t)UR * (GN_TS / g.tr));
+  g.schunk = split(2LL * device_cus(), (int64_t)UR * (GN_TT / g.tr));
   g.achunk = split(4LL * device_cus(), (int64_t)UA * (GN_T / g.tr));
   g.nchunk = (int)cdiv(p, g.schunk);
   return g;
@@ -440,7 +441,7 @@ using namespace clarus;
 extern "C" size_t clarus_hip_group_norm_workspace(int64_t n, int64_t p, int64_t c, int64_t groups) {
   if (n <= 0 || p <= 0 || c <= 0 || groups <= 0 || c % groups || c % 8 || gn_unit(c / groups) > GN_UNIT) return 0;
   const GnPlan g = gn_plan(n, p, c, groups);
-  return g.small ? 8 : (size_t)(n * groups * (g.nchunk + 1)) * sizeof(float2);
+  return g.small ? 0 : (size_t)(n * groups * (g.nchunk + 1)) * sizeof(float2);
 }
 
 extern "C" int clarus_hip_group_norm(const void* x, int32_t x_dtype, int64_t x_bstride, int64_t ldx, const float* w,
@@ -448,7 +449,7 @@ extern "C" int clarus_hip_group_norm(const void* x, int32_t x_dtype, int64_t x_b
                                      int64_t n, int64_t p, int64_t c, int64_t groups, float eps, int32_t act,
                                      void* scratch, size_t scratch_bytes, void* stream) {
   clear_error();
-  CLARUS_REQUIRE(x && out && scratch, "group_norm: null operand");
+  CLARUS_REQUIRE(x && out, "group_norm: null operand");
   CLARUS_REQUIRE(n > 0 && p > 0 && c > 0 && groups > 0, "group_norm: empty problem");
   CLARUS_REQUIRE((x_dtype == DT_BF16 || x_dtype == DT_F32) && (o_dtype == DT_BF16 || o_dtype == DT_F32),
                  "group_norm: bf16 or fp32");
@@ -463,7 +464,7 @@ extern "C" int clarus_hip_group_norm(const void* x, int32_t x_dtype, int64_t x_b
   // float counts and the pixel index of a chunk: 2^31 pixels, 65535 images and strips are the launch's limits
   CLARUS_REQUIRE(p < ((int64_t)1 << 31) && n < 65536 && c < ((int64_t)1 << 24), "group_norm: too large");
   const size_t need = clarus_hip_group_norm_workspace(n, p, c, groups);
-  CLARUS_REQUIRE(scratch_bytes >= need && aligned(scratch, 8), "group_norm: scratch %zu < %zu bytes", scratch_bytes, need);
+  CLARUS_REQUIRE(need == 0 || (scratch && scratch_bytes >= need && aligned(scratch, 8)), "group_norm: scratch %zu < %zu bytes", scratch_bytes, need);
   const GnPlan g = gn_plan(n, p, c, groups);
   GroupNormP k{};
   k.x = x; k.out = out; k.w = w; k.b = b;
@@ -476,8 +477,8 @@ extern "C" int clarus_hip_group_norm(const void* x, int32_t x_dtype, int64_t x_b
   hipStream_t st = (hipStream_t)stream;
   const bool whole = k.cg % 8 == 0;
   const int64_t sgroups = (c < 8 * g.tr ? c : 8 * g.tr) / k.cg;
-  k.rpb = GN_TS / g.tr;
-  k.lpg = gn_lanes(sgroups, k.rpb, GN_TS);
+  k.rpb = (g.small ? GN_TS : GN_TT) / g.tr;
+  k.lpg = gn_lanes(sgroups, k.rpb, g.small ? GN_TS : GN_TT);
   if (g.small) {
     const int nr = (int)cdiv(p, k.rpb);
     const dim3 grid(1, (unsigned)g.strips, (unsigned)n);
@@ -507,11 +508,11 @@ extern "C" int clarus_hip_group_norm(const void* x, int32_t x_dtype, int64_t x_b
   const dim3 sgrid((unsigned)g.nchunk, (unsigned)g.strips, (unsigned)n);
   note_kernel("gn_stats_kernel + gn_apply_kernel nchunk=%d strips=%d", g.nchunk, g.strips);
   if (x_dtype == DT_BF16) {
-    if (whole) hipLaunchKernelGGL((gn_stats_kernel<DT_BF16, true>), sgrid, dim3(GN_TS), 0, st, k);
-    else hipLaunchKernelGGL((gn_stats_kernel<DT_BF16, false>), sgrid, dim3(GN_TS), 0, st, k);
+    if (whole) hipLaunchKernelGGL((gn_stats_kernel<DT_BF16, true>), sgrid, dim3(GN_TT), 0, st, k);
+    else hipLaunchKernelGGL((gn_stats_kernel<DT_BF16, false>), sgrid, dim3(GN_TT), 0, st, k);
   } else {
-    if (whole) hipLaunchKernelGGL((gn_stats_kernel<DT_F32, true>), sgrid, dim3(GN_TS), 0, st, k);
-    else hipLaunchKernelGGL((gn_stats_kernel<DT_F32, false>), sgrid, dim3(GN_TS), 0, st, k);
+    if (whole) hipLaunchKernelGGL((gn_stats_kernel<DT_F32, true>), sgrid, dim3(GN_TT), 0, st, k);
+    else hipLaunchKernelGGL((gn_stats_kernel<DT_F32, false>), sgrid, dim3(GN_TT), 0, st, k);
   }
   hipLaunchKernelGGL(gn_join_kernel, dim3((unsigned)groups, (unsigned)n), dim3(64), 0, st, k);
   k.chunk = g.achunk;

@@ -20,7 +20,6 @@ pass), and no call synchronises.
 """
 from __future__ import annotations
 
-import contextlib
 import ctypes
 import math
 
@@ -62,6 +61,14 @@ def _vec16(t: torch.Tensor, *strides: int) -> bool:
     """Base pointer and the given element strides keep 16-byte alignment."""
     es = t.element_size()
     return t.data_ptr() % 16 == 0 and all((s * es) % 16 == 0 for s in strides)
+
+
+def _raw_stream(index: int) -> int:
+    return torch.cuda.current_stream(index).cuda_stream
+
+
+# the same without building a Stream object (0.1 instead of 1.8 us of a call)
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", _raw_stream)
 
 
 def _rows(t: torch.Tensor):
@@ -194,6 +201,7 @@ class HipOps(Backend):
         self.pair_launches = {"gemm_ln_gemm": 0, "gemm_ln_rows": 0}
         self.ffn_launches = 0  # linear_gate_linear calls served by clarus_hip_ffn
         self.ln_dw_launches = 0  # linear_dwconv calls served by clarus_hip_ln_gemm_dwconv
+        self._plans = {}  # _plan's entries
         self._ca_ws = {}  # (device, stream) -> zeroed channel-attention workspace (counters stay zero)
 
     # ------------------------------------------------------------------ plumbing
@@ -217,19 +225,33 @@ class HipOps(Backend):
     def _forward_only(self, what, *ts):
         """Declines what a forward-only op of this device cannot answer: operands elsewhere, and operands
         whose gradient autograd would lose."""
+        grad = torch.is_grad_enabled()
         for t in ts:
-            if t is None:
-                continue
-            if t.device != self.dev:
-                raise Unsupported(f"{what}: operands on {self.dev}, got {t.device}")
-            if t.requires_grad and torch.is_grad_enabled():
+            if t is not None and (t.device != self.dev or (grad and t.requires_grad)):
+                if t.device != self.dev:
+                    raise Unsupported(f"{what}: operands on {self.dev}, got {t.device}")
                 raise Unsupported(f"{what}: forward only, an operand requires its gradient")
 
-    def _current(self):
-        """Launches go to this backend's device whatever device is current."""
+    def _plan(self, key, make):
+        """What a call's sizes, strides and types alone decide (acceptance, strides, workspace size), worked out
+        once per such key; make() raises Unsupported for what the kernels decline."""
+        plan = self._plans.get(key)
+        if plan is None:
+            if len(self._plans) >= 4096:
+                self._plans.clear()
+            plan = self._plans[key] = make()
+        return plan
+
+    def _call(self, what, fn, *args):
+        """fn(*args, current stream of this backend's device), with that device current (the library
+        launches on the current one)."""
         if torch.cuda.current_device() == self.dev.index:
-            return contextlib.nullcontext()
-        return torch.cuda.device(self.dev)
+            rc = fn(*args, _raw_stream(self.dev.index))
+        else:
+            with torch.cuda.device(self.dev):
+                rc = fn(*args, _raw_stream(self.dev.index))
+        if rc:
+            _lib.check(rc, what)
 
     def _bias(self, b):
         """fp32 contiguous copy of a (weight-like) vector, once per tensor."""
@@ -813,40 +835,52 @@ class HipOps(Backend):
         C / groups channels the mean and biased variance over all pixels of the group's channels, in
         fp32, rounded once. weight, bias: [C], or [N, C] for a scale and shift of each image's own. act
         None, "silu" or "gelu". x may be a channel slice (one pixel stride); the result is contiguous."""
+        key = ("group_norm", x.shape, x.stride(), x.dtype, groups, act, out_dtype,
+               None if weight is None else (weight.shape, weight.dtype), None if bias is None else (bias.shape, bias.dtype))
+        self._forward_only("group_norm", x, weight, bias)
+        odt, n, p, c, groups, xbs, ldx, wbs, bbs, acode, need = self._plan(
+            key, lambda: self._group_norm_plan(x, groups, weight, bias, act, out_dtype or self.dtype))
+        if x.data_ptr() % 16:
+            raise Unsupported("group_norm: 16-byte aligned rows")
+        out = torch.empty(x.shape, device=x.device, dtype=odt)
+        if not p:
+            return out
+        wf = weight if weight is None or weight.dtype == torch.float32 and weight.is_contiguous() else self._affine(weight)
+        bf = bias if bias is None or bias.dtype == torch.float32 and bias.is_contiguous() else self._affine(bias)
+        scratch = torch.empty(need, device=x.device, dtype=torch.uint8) if need else None
+        self._call("group_norm", self.lib.clarus_hip_group_norm, x.data_ptr(), _lib.dtype_code(x.dtype), xbs, ldx,
+                   _lib.ptr(wf), wbs, _lib.ptr(bf), bbs, out.data_ptr(), _lib.dtype_code(odt), n, p, c, groups, float(eps),
+                   acode, _lib.ptr(scratch), need)
+        return out
+
+    def _affine(self, t):
+        """fp32 contiguous copy of a weight [C], kept, or of an image's own scale or shift [N, C], which is new with
+        every call; nor is what a capturing graph's pool holds kept, which the replay alone writes."""
+        if t.dim() == 1 and not torch.cuda.is_current_stream_capturing():
+            return self._bias(t)
+        return t.float().contiguous()
+
+    def _group_norm_plan(self, x, groups, weight, bias, act, odt):
         if x.dim() < 2 or act not in (None, "silu", "gelu") or not isinstance(groups, int) or groups < 1:
             raise Unsupported(f"group_norm: x [N, ..., C], groups >= 1, act none / silu / gelu, got {groups!r} {act!r}")
         n, c = x.shape[0], x.shape[-1]
-        odt = out_dtype or self.dtype
-        self._forward_only("group_norm", x, weight, bias)
         if not (_kdt(x) and odt in _KDT and c % 8 == 0 and c % groups == 0 and c > 0
-                and (c // groups) * 8 // math.gcd(8, c // groups) <= 2048):
+                and math.lcm(8, c // groups) <= 2048):
             raise Unsupported("group_norm: bf16 / fp32, channels a multiple of 8 and of the groups, "
                               "lcm(8, channels per group) at most 2048")
         if any(t is not None and (tuple(t.shape) not in ((c,), (n, c)) or not t.is_floating_point()) for t in (weight, bias)):
             raise Unsupported("group_norm: weight and bias [C] or [N, C]")
-        out = torch.empty(x.shape, device=x.device, dtype=odt)
-        if out.numel() == 0:
-            return out
-        at = _rows(x)
-        if at is None or at[1] < c or not _vec16(x, at[1], at[2]):
+        acode = {None: _lib.ACT_NONE, "silu": _lib.ACT_SILU, "gelu": _lib.ACT_GELU}[act]
+        wbs, bbs = (c if t is not None and t.dim() == 2 else 0 for t in (weight, bias))
+        if x.numel() == 0:
+            return odt, n, 0, c, groups, 0, c, wbs, bbs, acode, 0
+        at, es = _rows(x), x.element_size()
+        if at is None or at[1] < c or at[1] * es % 16 or at[2] * es % 16:
             raise Unsupported("group_norm: unit channel stride, one pixel stride, 16-byte aligned rows")
         p, ldx, xbs = at
         if p >= 1 << 31 or n >= 65536:
             raise Unsupported("group_norm: fewer than 2^31 pixels of an image and 65536 images")
-        with self._current():
-            # an image's own scale and shift are new with every call: converted, not kept; nor is what a graph's
-            # pool holds, which is written by the replay only
-            keep = not torch.cuda.is_current_stream_capturing()
-            wf, bf = (t if t is None else self._bias(t) if t.dim() == 1 and keep else t.float().contiguous()
-                      for t in (weight, bias))
-            need = self.lib.clarus_hip_group_norm_workspace(n, p, c, groups)
-            scratch = torch.empty(need, device=x.device, dtype=torch.uint8)
-            _lib.check(self.lib.clarus_hip_group_norm(
-                x.data_ptr(), _lib.dtype_code(x.dtype), xbs, ldx, _lib.ptr(wf), c if wf is not None and wf.dim() == 2 else 0,
-                _lib.ptr(bf), c if bf is not None and bf.dim() == 2 else 0, out.data_ptr(), _lib.dtype_code(odt), n, p, c,
-                groups, float(eps), {None: _lib.ACT_NONE, "silu": _lib.ACT_SILU, "gelu": _lib.ACT_GELU}[act],
-                scratch.data_ptr(), need, self._stream(x)), "group_norm")
-        return out
+        return odt, n, p, c, groups, xbs, ldx, wbs, bbs, acode, self.lib.clarus_hip_group_norm_workspace(n, p, c, groups)
 
     # ------------------------------------------------------------------ attention
     def cross_attention(self, q, k, v, heads, kv_heads=None, mask=None, scale=None, out_dtype=None):
@@ -857,20 +891,36 @@ class HipOps(Backend):
         keeps none, or without keys. mask: bool [N, Lk] (a masked key counts for nothing whatever k and v hold)
         or [N, Lq, Lk] (v has to be finite: a masked pair weighs 0). fp32 scores, softmax and sums; bf16 weights
         enter the product with v rounded to bf16. Returns a contiguous tensor of q's shape."""
+        kv_heads = heads if kv_heads is None else kv_heads
+        key = ("cross_attention", q.shape, q.stride(), k.shape, k.stride(), v.shape, v.stride(), q.dtype, k.dtype, v.dtype,
+               heads, kv_heads, scale, out_dtype, None if mask is None else (mask.shape, mask.stride(), mask.dtype))
+        self._forward_only("cross_attention", q, k, v, mask)
+        odt, args, need = self._plan(key, lambda: self._cross_plan(q, k, v, heads, kv_heads, mask, scale, out_dtype or self.dtype))
+        out = torch.empty(q.shape, device=q.device, dtype=odt)
+        if args is None:  # nothing asked, or nothing to attend
+            return out.zero_()
+        qp, kp, vp = q.data_ptr(), k.data_ptr(), v.data_ptr()
+        if (qp | kp | vp) % 16:
+            raise Unsupported("cross_attention: 16-byte aligned rows")
+        args = _lib.CrossArgs.from_buffer_copy(args)
+        args.q, args.k, args.v, args.out, args.mask = qp, kp, vp, out.data_ptr(), _lib.ptr(mask)
+        scratch = torch.empty(need, device=q.device, dtype=torch.uint8) if need else None
+        self._call("cross_attention", self.lib.clarus_hip_cross_attention, ctypes.byref(args), _lib.ptr(scratch), need)
+        return out
+
+    def _cross_plan(self, q, k, v, heads, kv_heads, mask, scale, odt):
         if q.dim() < 2 or k.dim() < 2 or v.dim() < 2:
             raise Unsupported("cross_attention: q, k, v [N, ..., C]")
-        kv_heads = heads if kv_heads is None else kv_heads
         n, c, ck = q.shape[0], q.shape[-1], k.shape[-1]
         if not (isinstance(heads, int) and isinstance(kv_heads, int) and heads > 0 and kv_heads > 0
-                and heads % kv_heads == 0 and c % heads == 0 and tuple(k.shape) == tuple(v.shape) and k.shape[0] == n
+                and heads % kv_heads == 0 and c % heads == 0 and k.shape == v.shape and k.shape[0] == n
                 and ck * heads == c * kv_heads):
             raise Unsupported("cross_attention: q [N, ..., heads d], k and v [N, ..., kv_heads d] of one shape, "
                               "heads a multiple of kv_heads")
         d = c // heads
-        odt = out_dtype or self.dtype
         lq, lk = math.prod(q.shape[1:-1]), math.prod(k.shape[1:-1])
-        scale = d ** -0.5 if scale is None and d else scale
-        self._forward_only("cross_attention", q, k, v, mask)
+        if scale is None and d:
+            scale = d ** -0.5
         if not (_kdt(q) and q.dtype == k.dtype == v.dtype and odt in _KDT and 8 <= d <= 128 and d % 8 == 0
                 and 0.0 < scale < math.inf):
             raise Unsupported("cross_attention: bf16 / fp32 q, k, v of one type, head width a multiple of 8 up to 128, "
@@ -879,32 +929,23 @@ class HipOps(Backend):
         if mask is not None:
             if mask.dtype != torch.bool or tuple(mask.shape) not in ((n, lk), (n, lq, lk)):
                 raise Unsupported("cross_attention: mask bool [N, Lk] or [N, Lq, Lk]")
-            if mask.stride(-1) != 1 and lk > 1 or any(s < 0 for s in mask.stride()):
+            if mask.stride(-1) != 1 and lk > 1:
                 raise Unsupported("cross_attention: mask with unit key stride")
-            # [N, Lk] where Lq is absent: a 2-D mask never stands for [Lq, Lk]
             mode = _lib.MASK_KEYS if mask.dim() == 2 else _lib.MASK_PAIRS
             mbs, mqs = mask.stride(0), mask.stride(1) if mask.dim() == 3 else 0
-        out = torch.empty(q.shape, device=q.device, dtype=odt)
-        if out.numel() == 0:
-            return out
-        if lk == 0:
-            return out.zero_()
+        if q.numel() == 0 or lk == 0:
+            return odt, None, 0
         qa, ka, va = _rows(q), _rows(k), _rows(v)
-        if None in (qa, ka, va) or not (_vec16(q, *qa[1:]) and _vec16(k, *ka[1:]) and _vec16(v, *va[1:])):
-            raise Unsupported("cross_attention: unit channel stride, one row stride, 16-byte aligned rows")
+        es = q.element_size()
+        if None in (qa, ka, va) or any(s * es % 16 for t in (qa, ka, va) for s in t[1:]) or max(ka[1], va[1]) >= 1 << 24:
+            raise Unsupported("cross_attention: unit channel stride, one row stride (k and v: below 2^24), 16-byte aligned rows")
         if max(lk, lq * (heads // kv_heads)) >= 1 << 31 or n * kv_heads >= 65536:
             raise Unsupported("cross_attention: fewer than 2^31 keys and rows, fewer than 65536 (image, kv head) pairs")
         args = _lib.CrossArgs(
-            q=q.data_ptr(), k=k.data_ptr(), v=v.data_ptr(), out=out.data_ptr(), mask=_lib.ptr(mask), n=n, lq=lq, lk=lk,
-            heads=heads, kv_heads=kv_heads, d=d, q_bstride=qa[2], ldq=qa[1], k_bstride=ka[2], ldk=ka[1], v_bstride=va[2],
-            ldv=va[1], mask_bstride=mbs, mask_qstride=mqs, dtype=_lib.dtype_code(q.dtype), o_dtype=_lib.dtype_code(odt),
-            mask_mode=mode, scale=scale)
-        with self._current():
-            need = self.lib.clarus_hip_cross_attention_workspace(args.dtype, n, lq, lk, heads, kv_heads, d)
-            scratch = torch.empty(need, device=q.device, dtype=torch.uint8) if need else None
-            _lib.check(self.lib.clarus_hip_cross_attention(ctypes.byref(args), _lib.ptr(scratch), need, self._stream(q)),
-                       "cross_attention")
-        return out
+            n=n, lq=lq, lk=lk, heads=heads, kv_heads=kv_heads, d=d, q_bstride=qa[2], ldq=qa[1], k_bstride=ka[2], ldk=ka[1],
+            v_bstride=va[2], ldv=va[1], mask_bstride=mbs, mask_qstride=mqs, dtype=_lib.dtype_code(q.dtype),
+            o_dtype=_lib.dtype_code(odt), mask_mode=mode, scale=scale)
+        return odt, args, self.lib.clarus_hip_cross_attention_workspace(args.dtype, n, lq, lk, heads, kv_heads, d)
 
     def channel_attention(self, qkv, heads, temperature):
         if not qkv.is_contiguous():

@@ -86,7 +86,7 @@ def make_mask(kind, n, lq, lk, dev, seed=0):
 def cpu_hip(dtype=torch.float32):
     from clarus_amd.hip_ops import HipOps
     h = HipOps.__new__(HipOps)
-    h.dtype, h.device, h.dev, h._cache = dtype, torch.device("cpu"), torch.device("cpu"), {}
+    h.dtype, h.device, h.dev, h._cache, h._plans = dtype, torch.device("cpu"), torch.device("cpu"), {}, {}
     return h
 
 

@@ -62,7 +62,7 @@ def cpu_hip(dtype=torch.float32):
     """HipOps' argument checks without a device: what passes them fails before anything is launched."""
     from clarus_amd.hip_ops import HipOps
     h = HipOps.__new__(HipOps)
-    h.dtype, h.device, h.dev, h._cache = dtype, torch.device("cpu"), torch.device("cpu"), {}
+    h.dtype, h.device, h.dev, h._cache, h._plans = dtype, torch.device("cpu"), torch.device("cpu"), {}, {}
     return h
 
 
@@ -101,13 +101,13 @@ def test_c_entry_refuses_before_launch():
 
     def call(x=1 << 20, xdt=0, xbs=0, ldx=64, wbs=0, out=1 << 24, odt=0, n=1, p=100, c=64, g=8, act=0, scratch=1 << 28, size=1 << 20):
         return lib.clarus_hip_group_norm(x, xdt, xbs, ldx, None, wbs, None, 0, out, odt, n, p, c, g, 1e-5, act, scratch, size, None)
-    for kw in (dict(x=None), dict(out=None), dict(scratch=None), dict(n=0), dict(p=0), dict(c=60, g=4), dict(g=7), dict(g=0),
+    for kw in (dict(x=None), dict(out=None), dict(p=100000, scratch=None), dict(n=0), dict(p=0), dict(c=60, g=4), dict(g=7), dict(g=0),
                dict(xdt=2), dict(odt=5), dict(act=2), dict(ldx=56), dict(ldx=66), dict(x=(1 << 20) + 4), dict(out=(1 << 24) + 8),
-               dict(wbs=8), dict(size=8), dict(n=1 << 16), dict(p=1 << 31), dict(c=4096, g=1, ldx=4096), dict(n=2, xbs=-64)):
+               dict(wbs=8), dict(p=100000, size=8), dict(n=1 << 16), dict(p=1 << 31), dict(c=4096, g=1, ldx=4096), dict(n=2, xbs=-64)):
         assert call(**kw) == _lib.EINVAL, kw
         assert b"group_norm" in lib.clarus_hip_last_error()
     assert lib.clarus_hip_group_norm_workspace(1, 100, 60, 4) == 0
-    assert lib.clarus_hip_group_norm_workspace(2, 100, 64, 8) > 0
+    assert lib.clarus_hip_group_norm_workspace(2, 100000, 64, 8) > 0
 
 
 @pytest.mark.parametrize("per_image", [False, True])
