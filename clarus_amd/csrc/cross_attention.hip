@@ -337,15 +337,15 @@ __device__ __forceinline__ int xa_key_byte(const unsigned char* mkey, int64_t ba
   return in;
 }
 
-// ---------------------------------------------------------------- keys that fit LDS
-// All keys of an (image, kv head) stay in a workgroup's LDS: copied once, one barrier, then its 8 waves take 32 rows
+// ---------------------------------------------------------------- few keys
+// Up to XR_KEYS keys (a prompt): all keys of an (image, kv head) stay in a workgroup's LDS: copied once, one barrier, then its 8 waves take 32 rows
 // each, chunk after chunk, the next chunk's queries in flight. Workgroups of the same rows and other heads run on one
 // XCD, whose L2 then reads and writes each line of q and out once.
 constexpr int XR_T = 512;
-__host__ __device__ constexpr int xr_tiles(int d, int tile_bytes) { return (d <= 64 ? 80 : 160) * 1024 / (2 * tile_bytes); }
+constexpr int XR_KEYS = 128;
 
 template <int DT, int D, int MASK>
-__global__ void __launch_bounds__(XR_T, D <= 64 ? 4 : 2) xa_resident_kernel(const CrossP p) {
+__global__ void __launch_bounds__(XR_T, (DT == DT_BF16 ? D <= 64 : D <= 32) ? 4 : 2) xa_resident_kernel(const CrossP p) {
   using T = XaTile<DT, D>;
   constexpr int KT = T::KT, W = XR_T / 64;
   extern __shared__ __attribute__((aligned(16))) unsigned char tiles[];
@@ -370,9 +370,10 @@ __global__ void __launch_bounds__(XR_T, D <= 64 ? 4 : 2) xa_resident_kernel(cons
     const int64_t r = (int64_t)c * 32 + col;
     return xa_row(p, kvh, r < p.rows ? r : p.rows - 1);
   };
+  constexpr bool AHEAD = T::QN <= 8;  // the next chunk's queries in flight (where registers allow it)
   u32x4 qn[T::QN];
-  if (ch < c1) xa_load_q<DT, D>(p, n, at(ch), hl, qn);
-  constexpr int MT = xr_tiles(D, T::BYTES);
+  if (AHEAD && ch < c1) xa_load_q<DT, D>(p, n, at(ch), hl, qn);
+  constexpr int MT = XR_KEYS / KT;
   uint64_t kept[MT];  // the keys of each tile that count
   {
     int byte[MT];
@@ -391,10 +392,14 @@ __global__ void __launch_bounds__(XR_T, D <= 64 ? 4 : 2) xa_resident_kernel(cons
 #pragma unroll 1
   for (; ch < c1; ch += W) {
     u32x4 qf[T::QN];
-#pragma unroll
-    for (int i = 0; i < T::QN; ++i) qf[i] = qn[i];
     const XaRow r = at(ch);
-    if (ch + W < c1) xa_load_q<DT, D>(p, n, at(ch + W), hl, qn);
+    if constexpr (AHEAD) {
+#pragma unroll
+      for (int i = 0; i < T::QN; ++i) qf[i] = qn[i];
+      if (ch + W < c1) xa_load_q<DT, D>(p, n, at(ch + W), hl, qn);
+    } else {
+      xa_load_q<DT, D>(p, n, r, hl, qf);
+    }
     const unsigned char* mrow = MASK == MASK_PAIRS ? p.mask + n * p.mbs + r.qi * p.mqs : nullptr;
     f32x16 o[D / 32];
 #pragma unroll
@@ -431,13 +436,24 @@ __global__ void __launch_bounds__(XA_T, D <= 64 ? (MASK == MASK_PAIRS ? 3 : 4) :
 
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int col = lane & 31, hl = lane >> 5;
-  // row blocks of one (image, kv head) run on one XCD, whose L2 then holds that head's K and V
-  const unsigned total = (unsigned)(p.nblk * p.nk * p.splits), span = (total + 7) >> 3;
-  const unsigned id = (blockIdx.x & 7) * span + (blockIdx.x >> 3);
-  if ((blockIdx.x >> 3) >= span || id >= total) return;
-  const unsigned hs = id / (unsigned)p.nblk, rb = id - hs * (unsigned)p.nblk;
-  const int nk = (int)(hs / (unsigned)p.splits), split = (int)(hs - nk * (unsigned)p.splits);
-  const int n = nk / p.kv_heads, kvh = nk - n * p.kv_heads;
+  // row blocks and splits of one (image, kv head) run on one XCD, whose L2 then holds that head's K and V: eight
+  // (image, kv head) pairs at a time, one on each XCD (padded batches stay balanced), the blocks of the last few
+  // pairs dealt out in equal parts
+  const unsigned per = (unsigned)(p.nblk * p.splits), xcd = blockIdx.x & 7, j = blockIdx.x >> 3, whole = (unsigned)(p.nk >> 3) * per;
+  unsigned nk, rest;
+  if (j < whole) {
+    nk = j / per;
+    rest = j - nk * per;
+    nk = nk * 8 + xcd;
+  } else {
+    const unsigned left = (unsigned)(p.nk & 7) * per, span = (left + 7) >> 3, i = xcd * span + (j - whole);
+    if (j - whole >= span || i >= left) return;
+    nk = i / per;
+    rest = i - nk * per;
+    nk += (unsigned)p.nk & ~7u;
+  }
+  const unsigned split = rest / (unsigned)p.nblk, rb = rest - split * (unsigned)p.nblk;
+  const int n = (int)nk / p.kv_heads, kvh = (int)nk - n * p.kv_heads;
 
   const int64_t wrow = (int64_t)rb * XA_ROWS + wave * 32;  // the wave's first row
   const bool busy = wrow < p.rows;
@@ -572,9 +588,6 @@ __global__ void __launch_bounds__(64) xa_join_kernel(const CrossP p) {
 
 int xa_pad(int64_t d) { return d <= 32 ? 32 : d <= 64 ? 64 : d <= 96 ? 96 : 128; }
 
-#ifndef XA_SLOTS
-#define XA_SLOTS 4LL
-#endif
 struct XaPlan {
   bool resident;
   int64_t nblk, split_len;  // row blocks (resident: workgroups) of an (image, kv head); keys of a split
@@ -585,7 +598,7 @@ XaPlan xa_plan(int32_t dt, int64_t n, int64_t lq, int64_t lk, int64_t heads, int
   XaPlan g{};
   const int kt = dt == DT_BF16 ? 64 : 32, D = xa_pad(d);
   const int64_t rows = lq * (heads / kv_heads), nk = n * kv_heads;
-  if (cdiv(lk, kt) <= xr_tiles(D, kt * D * (dt == DT_BF16 ? 2 : 4))) {
+  if (lk <= XR_KEYS) {
     g.resident = true;
     g.splits = 1;
     g.split_len = lk;
@@ -596,7 +609,7 @@ XaPlan xa_plan(int32_t dt, int64_t n, int64_t lq, int64_t lk, int64_t heads, int
   g.nblk = cdiv(rows, XA_ROWS);
   const int64_t blocks = g.nblk * nk;
   // split the keys while the row blocks leave CUs idle: two workgroups per CU, four tiles or more each
-  int64_t want = (D <= 64 ? XA_SLOTS : 2LL) * device_cus() / blocks;
+  int64_t want = 2LL * device_cus() / blocks;
   const int64_t most = cdiv(lk, 4 * kt);
   if (want > most) want = most;
   if (want < 1) want = 1;
