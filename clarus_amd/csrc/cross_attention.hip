@@ -125,23 +125,39 @@ __device__ __forceinline__ void xa_load_q(const CrossP& p, int64_t n, const XaRo
   }
 }
 
-// the mask bytes of a lane's keys of a tile that starts at key `base` and ends at k1
+// The mask bytes of a lane's row and keys (8 j + 4 hl .. + 3, j = 0 .. 3, of each 32) of a tile that starts at key `base`
+// and ends at k1: 16 bytes of each 32 as they lie in memory, exchanged with lane ^ 32 by xa_pairs once they are used
 template <int KB>
-__device__ __forceinline__ void xa_load_pairs(const unsigned char* mrow, int64_t base, int64_t k1, int hl, unsigned (&w)[KB][4]) {
-  const bool whole = k1 - base >= 32 * KB;
+__device__ __forceinline__ void xa_load_pairs(const unsigned char* mrow, int64_t base, int64_t k1, int hl, u32x4 (&w)[KB]) {
+  struct __attribute__((packed, aligned(1))) Bytes { u32x4 v; };
 #pragma unroll
-  for (int b = 0; b < KB; ++b)
+  for (int b = 0; b < KB; ++b) {
+    const int64_t key = base + 32 * b + 16 * hl;
+    if (base + 32 * (b + 1) <= k1) {
+      w[b] = reinterpret_cast<const Bytes*>(mrow + key)->v;
+    } else {
 #pragma unroll
-    for (int j4 = 0; j4 < 4; ++j4) {
-      const int64_t key = base + 32 * b + 8 * j4 + 4 * hl;
-      if (whole) {
-        __builtin_memcpy(&w[b][j4], mrow + key, 4);
-      } else {
-        w[b][j4] = 0;
+      for (int j = 0; j < 4; ++j) {
+        w[b][j] = 0;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) w[b][j4] |= (key + j < k1 ? (unsigned)mrow[key + j] : 0u) << (8 * j);
+        for (int i = 0; i < 4; ++i) w[b][j] |= (key + 4 * j + i < k1 ? (unsigned)mrow[key + 4 * j + i] : 0u) << (8 * i);
       }
     }
+  }
+}
+
+template <int KB>
+__device__ __forceinline__ void xa_pairs(const u32x4 (&w)[KB], unsigned (&pair)[KB][4]) {
+#pragma unroll
+  for (int b = 0; b < KB; ++b) {
+    unsigned w0 = w[b][0], w1 = w[b][1], w2 = w[b][2], w3 = w[b][3];
+    swap32(w0, w1);
+    swap32(w2, w3);
+    pair[b][0] = w0;
+    pair[b][1] = w2;
+    pair[b][2] = w1;
+    pair[b][3] = w3;
+  }
 }
 
 // One tile of NB x 32 keys for a wave's 32 rows: S^T = K Q^T, the softmax's step, O^T += V^T P^T. bits: the keys that
@@ -417,7 +433,9 @@ __global__ void __launch_bounds__(XR_T, (DT == DT_BF16 ? D <= 64 : D <= 32) ? 4 
         if (h / KT == t) bits = (unsigned)(kept[t] >> (h % KT));
       unsigned pair[1][4];
       if constexpr (MASK == MASK_PAIRS) {
-        xa_load_pairs<1>(mrow, h, lk, hl, pair);
+        u32x4 w[1];
+        xa_load_pairs<1>(mrow, h, lk, hl, w);
+        xa_pairs<1>(w, pair);
         if (!__any(pair[0][0] | pair[0][1] | pair[0][2] | pair[0][3])) bits = 0;
       }
       if (bits) xa_tile<DT, D, MASK, 1, true>(ks, ks + T::BYTES, qf, o, m, l, p.c, bits, bits == 0xffffffffu, pair);
@@ -489,28 +507,31 @@ __global__ void __launch_bounds__(XA_T, D <= 64 ? (MASK == MASK_PAIRS ? 3 : 4) :
 
   uint64_t bits = 0;
   int byte = 0;
-  unsigned pair[KB][4], next[KB][4];
+  unsigned pair[KB][4];
+  u32x4 next[KB], after[KB];  // MASK_PAIRS: the mask of the next two tiles
   if (ntile > 0) {
     bits = __ballot(key_byte(0));
     if (ntile > 1) byte = key_byte(1);
     if (bits) fill(0, bits);
-    if constexpr (MASK == MASK_PAIRS) xa_load_pairs<KB>(mrow, k0, k1, hl, next);
+    if constexpr (MASK == MASK_PAIRS) {
+      xa_load_pairs<KB>(mrow, k0, k1, hl, next);
+      xa_load_pairs<KB>(mrow, k0 + KT, k1, hl, after);
+    }
   }
   for (int t = 0; t < ntile; ++t) {
     const uint64_t now = bits;
     __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0): this wave's copies of tile t have landed
     barrier_keep_vm();                   // everybody's have, and tile t - 1 has been read
     if constexpr (MASK == MASK_PAIRS) {
+      xa_pairs<KB>(next, pair);
 #pragma unroll
-      for (int b = 0; b < KB; ++b)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) pair[b][j] = next[b][j];
+      for (int b = 0; b < KB; ++b) next[b] = after[b];
     }
     if (t + 1 < ntile) {
       bits = __ballot(byte);
       if (t + 2 < ntile) byte = key_byte(t + 2);
       if (bits) fill(t + 1, bits);
-      if constexpr (MASK == MASK_PAIRS) xa_load_pairs<KB>(mrow, k0 + (int64_t)(t + 1) * KT, k1, hl, next);
+      if constexpr (MASK == MASK_PAIRS) xa_load_pairs<KB>(mrow, k0 + (int64_t)(t + 2) * KT, k1, hl, after);
     }
     if (!busy || !now) continue;
     if constexpr (MASK == MASK_PAIRS) {
@@ -538,52 +559,71 @@ __global__ void __launch_bounds__(XA_T, D <= 64 ? (MASK == MASK_PAIRS ? 3 : 4) :
   if (hl == 0) *reinterpret_cast<float2*>(p.part + all * D + 2 * at) = float2{m, l};
 }
 
-// One wave per row: the splits' (O, m, l) joined. m and l of 64 splits are in flight at a time, then O of 8
+// The splits' (O, m, l) joined. TPR threads hold a row's columns (4 each), gs groups of them its splits: group i takes
+// splits i, i + gs, .., XJ_BATCH of them in flight, and the groups are joined through LDS, in a fixed order
+constexpr int XJ_BATCH = 8;
+
 template <int D>
-__global__ void __launch_bounds__(64) xa_join_kernel(const CrossP p) {
-  constexpr int E = D > 64 ? 2 : 1;  // columns per lane (D = 32: half of the wave idles)
-  const int64_t row = blockIdx.x, nk = blockIdx.y, all = (int64_t)p.splits * p.nk * p.rows;
-  const int64_t step = p.nk * p.rows, first = nk * p.rows + row;
-  const float2* ml = reinterpret_cast<const float2*>(p.part + all * D) + first;
-  const int lane = threadIdx.x, d0 = lane * E < D ? lane * E : 0;
-  const float* po = p.part + first * D + d0;
-  float m = XA_FLOOR, l = 0.f, o[E];
+__global__ void __launch_bounds__(XA_T) xa_join_kernel(const CrossP p, int gs) {
+  constexpr int TPR = D <= 32 ? 8 : D <= 64 ? 16 : 32;
+  __shared__ f32x4 so[XA_T];
+  __shared__ float2 sml[XA_T];
+  const int tid = threadIdx.x, col = (tid % TPR) * 4, part = tid / TPR % gs, rpb = XA_T / (TPR * gs);
+  const int64_t total = p.nk * p.rows, at_row = (int64_t)blockIdx.x * rpb + tid / (TPR * gs);
+  const int64_t first = at_row < total ? at_row : total - 1;  // (image, kv head) x rows + row; past the end: the last one
+  const float2* ml = reinterpret_cast<const float2*>(p.part + (int64_t)p.splits * total * D) + first;
+  const float* po = p.part + first * D + (col < D ? col : 0);
+  float m = XA_FLOOR, l = 0.f;
+  f32x4 o = {0.f, 0.f, 0.f, 0.f};
+  for (int s0 = part; s0 < p.splits; s0 += XJ_BATCH * gs) {
+    float2 t[XJ_BATCH];
+    f32x4 x[XJ_BATCH];
 #pragma unroll
-  for (int e = 0; e < E; ++e) o[e] = 0.f;
-  for (int s0 = 0; s0 < p.splits; s0 += 64) {
-    const int ns = p.splits - s0 < 64 ? p.splits - s0 : 64;
-    const float2 v = lane < ns ? ml[(s0 + lane) * step] : float2{XA_FLOOR, 0.f};
-    float mx = v.x;
+    for (int i = 0; i < XJ_BATCH; ++i) {
+      const int64_t at = (int64_t)(s0 + i * gs < p.splits ? s0 + i * gs : s0) * total;
+      t[i] = ml[at];
+      x[i] = *reinterpret_cast<const f32x4*>(po + at * D);
+    }
+    float mn = m;
 #pragma unroll
-    for (int i = 1; i < 64; i <<= 1) mx = fmaxf(mx, __shfl_xor(mx, i, 64));
-    const float mn = fmaxf(m, mx), alpha = __builtin_amdgcn_exp2f(m - mn), w = __builtin_amdgcn_exp2f(v.x - mn);
+    for (int i = 0; i < XJ_BATCH; ++i) mn = fmaxf(mn, t[i].x);
+    const float alpha = __builtin_amdgcn_exp2f(m - mn);
     m = mn;
-    l = fmaf(l, alpha, group_sum<64>(v.y * w));
+    l *= alpha;
+    o *= alpha;
 #pragma unroll
-    for (int e = 0; e < E; ++e) o[e] *= alpha;
-    for (int s = 0; s < ns; s += 8) {
-      float x[8][E];
+    for (int i = 0; i < XJ_BATCH; ++i) {
+      if (s0 + i * gs >= p.splits) break;
+      const float w = __builtin_amdgcn_exp2f(t[i].x - m);
+      l = fmaf(t[i].y, w, l);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const int at = s + i < ns ? s + i : ns - 1;
-#pragma unroll
-        for (int e = 0; e < E; ++e) x[i][e] = po[(s0 + at) * step * D + e];
-      }
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const float wi = __shfl(w, s + i < ns ? s + i : 0, 64);
-#pragma unroll
-        for (int e = 0; e < E; ++e) o[e] = s + i < ns ? fmaf(x[i][e], wi, o[e]) : o[e];
-      }
+      for (int e = 0; e < 4; ++e) o[e] = fmaf(x[i][e], w, o[e]);
     }
   }
-  const float inv = l == 0.f ? 0.f : 1.f / l;
-  const int n = (int)(nk / p.kv_heads);
-  const XaRow r = xa_row(p, (int)nk - n * p.kv_heads, row);
-  const int64_t at = ((n * (int64_t)p.lq + r.qi) * (int64_t)(p.kv_heads * p.rep) + r.head) * p.d;
+  if (gs > 1) {
+    so[tid] = o;
+    sml[tid] = float2{m, l};
+    __syncthreads();
+    if (part) return;
+    for (int i = 1; i < gs; ++i) {
+      const float2 t = sml[tid + i * TPR];
+      const f32x4 x = so[tid + i * TPR];
+      const float mn = fmaxf(m, t.x), alpha = __builtin_amdgcn_exp2f(m - mn), w = __builtin_amdgcn_exp2f(t.x - mn);
+      m = mn;
+      l = fmaf(t.y, w, l * alpha);
 #pragma unroll
-  for (int e = 0; e < E; ++e)
-    if (lane * E + e < p.d) store1(p.out, p.o_dt, at + lane * E + e, o[e] * inv);
+      for (int e = 0; e < 4; ++e) o[e] = fmaf(x[e], w, o[e] * alpha);
+    }
+  }
+  if (at_row >= total || col >= p.d) return;
+  const float inv = l == 0.f ? 0.f : 1.f / l;
+  const int64_t nk = first / p.rows, n = nk / p.kv_heads;
+  const XaRow r = xa_row(p, (int)(nk - n * p.kv_heads), first - nk * p.rows);
+  const int64_t at = ((n * p.lq + r.qi) * (int64_t)(p.kv_heads * p.rep) + r.head) * p.d + col;
+  if (p.o_dt == DT_BF16)
+    *reinterpret_cast<u32x2*>((unsigned short*)p.out + at) = u32x2{pack2_bf16(o[0] * inv, o[1] * inv), pack2_bf16(o[2] * inv, o[3] * inv)};
+  else
+    *reinterpret_cast<f32x4*>((float*)p.out + at) = f32x4{o[0] * inv, o[1] * inv, o[2] * inv, o[3] * inv};
 }
 
 int xa_pad(int64_t d) { return d <= 32 ? 32 : d <= 64 ? 64 : d <= 96 ? 96 : 128; }
@@ -632,7 +672,12 @@ void xa_launch(const CrossP& k, bool resident, int mask, hipStream_t st) {
   if (mask == MASK_NONE) hipLaunchKernelGGL((xa_kernel<DT, D, MASK_NONE>), grid, dim3(XA_T), 0, st, k);
   else if (mask == MASK_KEYS) hipLaunchKernelGGL((xa_kernel<DT, D, MASK_KEYS>), grid, dim3(XA_T), 0, st, k);
   else hipLaunchKernelGGL((xa_kernel<DT, D, MASK_PAIRS>), grid, dim3(XA_T), 0, st, k);
-  if (k.splits > 1) hipLaunchKernelGGL((xa_join_kernel<D>), dim3((unsigned)k.rows, (unsigned)k.nk), dim3(64), 0, st, k);
+  if (k.splits > 1) {
+    constexpr int TPR = D <= 32 ? 8 : D <= 64 ? 16 : 32;
+    int gs = 1;
+    while (gs * TPR < XA_T && gs * XJ_BATCH < k.splits) gs *= 2;
+    hipLaunchKernelGGL((xa_join_kernel<D>), dim3((unsigned)cdiv(k.rows * k.nk, XA_T / (TPR * gs))), dim3(XA_T), 0, st, k, gs);
+  }
 }
 
 }  // namespace
