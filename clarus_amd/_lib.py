@@ -106,7 +106,7 @@ SIGNATURES = {
     "clarus_hip_group_norm_workspace": (ctypes.c_size_t, [_i64, _i64, _i64, _i64]),
     "clarus_hip_group_norm": (_i32, [_vp, _i32, _i64, _i64, _vp, _i64, _vp, _i64, _vp, _i32, _i64, _i64, _i64, _i64,
                                      _f32, _i32, _vp, ctypes.c_size_t, _vp]),
-    "clarus_hip_cross_attention_workspace": (ctypes.c_size_t, [_i32, _i64, _i64, _i64, _i64, _i64, _i64]),
+    "clarus_hip_cross_attention_workspace": (ctypes.c_size_t, [_i32, _i64, _i64, _i64, _i64, _i64, _i64, _i32]),
     "clarus_hip_cross_attention": (_i32, [ctypes.POINTER(CrossArgs), _vp, ctypes.c_size_t, _vp]),
     "clarus_hip_abi_version": (_i32, []),
     "clarus_hip_sizeof_gemm_args": (ctypes.c_size_t, []),

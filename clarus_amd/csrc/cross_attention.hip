@@ -38,6 +38,8 @@ struct CrossP {
   const void *q, *k, *v;
   void* out;
   const unsigned char* mask;
+  const uint64_t* bits;      // MASK_PAIRS: [n][lq][nw] words of 64 keys, image stride bbs (words)
+  int64_t nw, bbs;
   float* part;               // [split][nk][rows][D] O, then [split][nk][rows] (m, l)
   int64_t qbs, ldq, kbs, ldk, vbs, ldv, mbs, mqs;
   int64_t rows;              // lq * rep
@@ -125,47 +127,28 @@ __device__ __forceinline__ void xa_load_q(const CrossP& p, int64_t n, const XaRo
   }
 }
 
-// The mask bytes of a lane's row and keys (8 j + 4 hl .. + 3, j = 0 .. 3, of each 32) of a tile that starts at key `base`
-// and ends at k1: 16 bytes of each 32 as they lie in memory, exchanged with lane ^ 32 by xa_pairs once they are used
-template <int KB>
-__device__ __forceinline__ void xa_load_pairs(const unsigned char* mrow, int64_t base, int64_t k1, int hl, u32x4 (&w)[KB]) {
+// 16 mask bytes (0 / 1) at p, the first `left` of them there, as 16 bits
+__device__ __forceinline__ unsigned xa_bits16(const unsigned char* p, int64_t left) {
   struct __attribute__((packed, aligned(1))) Bytes { u32x4 v; };
+  u32x4 w = {0, 0, 0, 0};
+  if (left >= 16) {
+    w = reinterpret_cast<const Bytes*>(p)->v;
+  } else {
 #pragma unroll
-  for (int b = 0; b < KB; ++b) {
-    const int64_t key = base + 32 * b + 16 * hl;
-    if (base + 32 * (b + 1) <= k1) {
-      w[b] = reinterpret_cast<const Bytes*>(mrow + key)->v;
-    } else {
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        w[b][j] = 0;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) w[b][j] |= (key + 4 * j + i < k1 ? (unsigned)mrow[key + 4 * j + i] : 0u) << (8 * i);
-      }
-    }
+    for (int i = 0; i < 16; ++i)
+      if (i < left) w[i >> 2] |= (unsigned)p[i] << (8 * (i & 3));
   }
-}
-
-template <int KB>
-__device__ __forceinline__ void xa_pairs(const u32x4 (&w)[KB], unsigned (&pair)[KB][4]) {
+  unsigned r = 0;
 #pragma unroll
-  for (int b = 0; b < KB; ++b) {
-    unsigned w0 = w[b][0], w1 = w[b][1], w2 = w[b][2], w3 = w[b][3];
-    swap32(w0, w1);
-    swap32(w2, w3);
-    pair[b][0] = w0;
-    pair[b][1] = w2;
-    pair[b][2] = w1;
-    pair[b][3] = w3;
-  }
+  for (int i = 0; i < 4; ++i) r |= ((w[i] & 0x01010101u) * 0x10204080u >> 28) << (4 * i);  // bytes 0 .. 3 -> bits 28 .. 31
+  return r;
 }
 
 // One tile of NB x 32 keys for a wave's 32 rows: S^T = K Q^T, the softmax's step, O^T += V^T P^T. bits: the keys that
-// count (MASK_PAIRS: pair instead).
+// count, of a lane's row under MASK_PAIRS.
 template <int DT, int D, int MASK, int NB, bool ANEW>
 __device__ __forceinline__ void xa_tile(const unsigned char* ks, const unsigned char* vs, const u32x4 (&qf)[XaTile<DT, D>::QN],
-                                        f32x16 (&o)[D / 32], float& m, float& l, float c, uint64_t bits, bool whole,
-                                        const unsigned (*pair)[4]) {
+                                        f32x16 (&o)[D / 32], float& m, float& l, float c, uint64_t bits, bool whole) {
   using T = XaTile<DT, D>;
   constexpr int DB = D / 32, QN = T::QN;
   // ANEW: the lane's LDS offsets are worked out for each tile instead of kept over the loop, where they spill
@@ -190,12 +173,7 @@ __device__ __forceinline__ void xa_tile(const unsigned char* ks, const unsigned 
     }
   }
   // masked and padding keys weigh nothing, whatever their scores
-  if constexpr (MASK == MASK_PAIRS) {
-#pragma unroll
-    for (int b = 0; b < NB; ++b)
-#pragma unroll
-      for (int j = 0; j < 16; ++j) s[b][j] = keep_bit(s[b][j], pair[b][j >> 2], 8 * (j & 3));
-  } else if (!whole) {
+  if (MASK == MASK_PAIRS || !whole) {
 #pragma unroll
     for (int b = 0; b < NB; ++b) {
       const unsigned w = (unsigned)(bits >> (32 * b)) >> (4 * hl);
@@ -353,6 +331,17 @@ __device__ __forceinline__ int xa_key_byte(const unsigned char* mkey, int64_t ba
   return in;
 }
 
+// any of the KT mask bytes at p (past `left` of them unknown: counted, and sorted out where they are used)
+template <int KT>
+__device__ __forceinline__ bool xa_any(const unsigned char* p, int64_t left) {
+  struct __attribute__((packed, aligned(1))) Bytes { u32x4 v; };
+  u32x4 any = {0, 0, 0, 0};
+#pragma unroll
+  for (int i = 0; i < KT; i += 16)
+    if (i + 16 <= left) any |= reinterpret_cast<const Bytes*>(p + i)->v;
+  return left < KT || (any[0] | any[1] | any[2] | any[3]);
+}
+
 // ---------------------------------------------------------------- few keys
 // Up to XR_KEYS keys (a prompt): all keys of an (image, kv head) stay in a workgroup's LDS: copied once, one barrier, then its 8 waves take 32 rows
 // each, chunk after chunk, the next chunk's queries in flight. Workgroups of the same rows and other heads run on one
@@ -431,14 +420,15 @@ __global__ void __launch_bounds__(XR_T, (DT == DT_BF16 ? D <= 64 : D <= 32) ? 4 
 #pragma unroll
       for (int t = 0; t < MT; ++t)
         if (h / KT == t) bits = (unsigned)(kept[t] >> (h % KT));
-      unsigned pair[1][4];
-      if constexpr (MASK == MASK_PAIRS) {
-        u32x4 w[1];
-        xa_load_pairs<1>(mrow, h, lk, hl, w);
-        xa_pairs<1>(w, pair);
-        if (!__any(pair[0][0] | pair[0][1] | pair[0][2] | pair[0][3])) bits = 0;
+      if constexpr (MASK == MASK_PAIRS) {  // a row's 32 bytes by its two lanes
+        unsigned lo = xa_bits16(mrow + h + 16 * hl, lk - h - 16 * hl) << (16 * hl), hi = lo;
+        swap32(lo, hi);
+        bits = lo | hi;
+        if (!__any(bits)) continue;
+      } else if (!bits) {
+        continue;
       }
-      if (bits) xa_tile<DT, D, MASK, 1, true>(ks, ks + T::BYTES, qf, o, m, l, p.c, bits, bits == 0xffffffffu, pair);
+      xa_tile<DT, D, MASK, 1, true>(ks, ks + T::BYTES, qf, o, m, l, p.c, bits, bits == 0xffffffffu);
     }
     l = sum32(l);
     xa_store<D>(p, n, r, o, l, ch * 32ll + col < p.rows);
@@ -451,6 +441,7 @@ __global__ void __launch_bounds__(XA_T, D <= 64 ? (MASK == MASK_PAIRS ? 3 : 4) :
   using T = XaTile<DT, D>;
   constexpr int KT = T::KT, KB = KT / 32, DB = D / 32;
   __shared__ __align__(16) unsigned char tiles[2][2 * T::BYTES];
+  __shared__ uint64_t wants[MASK == MASK_PAIRS ? XA_T / 64 : 1];
 
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int col = lane & 31, hl = lane >> 5;
@@ -480,20 +471,21 @@ __global__ void __launch_bounds__(XA_T, D <= 64 ? (MASK == MASK_PAIRS ? 3 : 4) :
 
   const unsigned char* kp = (const unsigned char*)p.k + (n * p.kbs + (int64_t)kvh * p.d) * T::ES;
   const unsigned char* vp = (const unsigned char*)p.v + (n * p.vbs + (int64_t)kvh * p.d) * T::ES;
-  const unsigned char* mrow = MASK == MASK_PAIRS ? p.mask + n * p.mbs + r.qi * p.mqs : nullptr;
+  // MASK_PAIRS: a row's mask as bits, a word per tile
+  using Word = std::conditional_t<KT == 64, uint64_t, uint32_t>;
+  const Word* words = MASK == MASK_PAIRS ? (const Word*)(p.bits + n * p.bbs + r.qi * p.nw) + (int64_t)split * (p.split_len / KT) : nullptr;
   const unsigned char* mkey = MASK == MASK_KEYS ? p.mask + n * p.mbs : nullptr;
 
   const int64_t k0 = (int64_t)split * p.split_len, k1 = k0 + p.split_len < p.lk ? k0 + p.split_len : p.lk;
   const int ntile = (int)((k1 - k0 + KT - 1) / KT);
 
   const XaCopy<DT, D, XA_T / 64> copy(p, wave, lane);
-  // the kept keys of a tile, one bit each. MASK_KEYS: the byte is loaded a tile ahead of its use
-  auto key_byte = [&](int t) __attribute__((always_inline)) {
-    return xa_key_byte<KT, MASK>(mkey, k0 + (int64_t)t * KT, k1, lane);
+  auto key_byte = [&](int t) __attribute__((always_inline)) {  // 0 for t < 0
+    return t < 0 ? 0 : xa_key_byte<KT, MASK>(mkey, k0 + (int64_t)t * KT, k1, lane);
   };
-  auto fill = [&](int t, uint64_t bits) __attribute__((always_inline)) {
+  auto fill = [&](int t, uint64_t bits, int buf) __attribute__((always_inline)) {
     const int64_t base = k0 + (int64_t)t * KT;
-    copy(p, kp + base * p.ldk * T::ES, vp + base * p.ldv * T::ES, tiles[t & 1], bits);
+    copy(p, kp + base * p.ldk * T::ES, vp + base * p.ldv * T::ES, tiles[buf], bits);
   };
 
   u32x4 qf[T::QN];
@@ -505,42 +497,65 @@ __global__ void __launch_bounds__(XA_T, D <= 64 ? (MASK == MASK_PAIRS ? 3 : 4) :
     for (int j = 0; j < 16; ++j) o[b][j] = 0.f;
   float m = XA_FLOOR, l = 0.f;
 
-  uint64_t bits = 0;
-  int byte = 0;
-  unsigned pair[KB][4];
-  u32x4 next[KB], after[KB];  // MASK_PAIRS: the mask of the next two tiles
-  if (ntile > 0) {
-    bits = __ballot(key_byte(0));
-    if (ntile > 1) byte = key_byte(1);
-    if (bits) fill(0, bits);
-    if constexpr (MASK == MASK_PAIRS) {
-      xa_load_pairs<KB>(mrow, k0, k1, hl, next);
-      xa_load_pairs<KB>(mrow, k0 + KT, k1, hl, after);
-    }
-  }
-  for (int t = 0; t < ntile; ++t) {
-    const uint64_t now = bits;
-    __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0): this wave's copies of tile t have landed
-    barrier_keep_vm();                   // everybody's have, and tile t - 1 has been read
-    if constexpr (MASK == MASK_PAIRS) {
-      xa_pairs<KB>(next, pair);
+  // 64 tiles at a time: the tiles of which the workgroup (want) and the wave (mine) keep a key, one bit each; the others
+  // are neither copied nor waited for
+#pragma unroll 1
+  for (int c0 = 0; c0 < ntile; c0 += 64) {
+    const int cn = ntile - c0 < 64 ? ntile - c0 : 64;
+    uint64_t want = ~0ull >> (64 - cn), mine = want;
+    if constexpr (MASK == MASK_KEYS) {
+      want = __ballot(lane < cn && xa_any<KT>(mkey + k0 + (int64_t)(c0 + lane) * KT, k1 - k0 - (int64_t)(c0 + lane) * KT));
+    } else if constexpr (MASK == MASK_PAIRS) {
+      // lane (row, hl): 32 tiles' words of its row
+      mine = 0;
+#pragma unroll 8
+      for (int t = 0; t < 32; ++t) {
+        const int tile = 32 * hl + t;
+        const uint64_t any = __ballot(tile < cn && words[c0 + (tile < cn ? tile : 0)] != 0);
+        mine |= (uint64_t)((unsigned)any != 0) << t | (uint64_t)((any >> 32) != 0) << (32 + t);
+      }
+      if (!busy) mine = 0;
+      __syncthreads();  // the words of the 64 tiles before have been read
+      if (lane == 0) wants[wave] = mine;
+      __syncthreads();
+      want = 0;
 #pragma unroll
-      for (int b = 0; b < KB; ++b) next[b] = after[b];
+      for (int w = 0; w < XA_T / 64; ++w) want |= wants[w];
+      want = (uint64_t)(unsigned)__builtin_amdgcn_readfirstlane((unsigned)(want >> 32)) << 32 |
+             (unsigned)__builtin_amdgcn_readfirstlane((unsigned)want);
     }
-    if (t + 1 < ntile) {
-      bits = __ballot(byte);
-      if (t + 2 < ntile) byte = key_byte(t + 2);
-      if (bits) fill(t + 1, bits);
-      if constexpr (MASK == MASK_PAIRS) xa_load_pairs<KB>(mrow, k0 + (int64_t)(t + 2) * KT, k1, hl, after);
+    auto pop = [&]() __attribute__((always_inline)) {  // the next wanted tile, -1 past the last
+      if (!want) return -1;
+      const int t = __builtin_ctzll(want);
+      want &= want - 1;
+      return c0 + t;
+    };
+    int t = pop(), t1 = pop();
+    if (t < 0) continue;
+    if (c0) barrier_keep_vm();  // the last tile of the 64 before has been read
+    // the kept keys of a tile, one bit each; the bytes of the tile after the next are on their way
+    uint64_t bits = __ballot(key_byte(t));
+    int byte = key_byte(t1), buf = 0;
+    fill(t, bits, 0);
+    Word next = MASK == MASK_PAIRS ? words[t] : 0;
+#pragma unroll 1
+    while (t >= 0) {
+      __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0): this wave's copies of tile t have landed
+      barrier_keep_vm();                   // everybody's have, and the tile before has been read
+      const uint64_t now = MASK == MASK_PAIRS ? (uint64_t)next : bits;
+      const int t2 = pop();
+      if (t1 >= 0) {
+        bits = __ballot(byte);
+        byte = key_byte(t2);
+        fill(t1, bits, buf ^ 1);
+        if constexpr (MASK == MASK_PAIRS) next = words[t1];
+      }
+      if (busy && (MASK != MASK_PAIRS || (mine >> (t - c0) & 1)))
+        xa_tile<DT, D, MASK, KB, false>(tiles[buf], tiles[buf] + T::BYTES, qf, o, m, l, p.c, now, now == T::ALL);
+      t = t1;
+      t1 = t2;
+      buf ^= 1;
     }
-    if (!busy || !now) continue;
-    if constexpr (MASK == MASK_PAIRS) {
-      unsigned any = 0;
-#pragma unroll
-      for (int b = 0; b < KB; ++b) any |= pair[b][0] | pair[b][1] | pair[b][2] | pair[b][3];
-      if (!__any(any)) continue;
-    }
-    xa_tile<DT, D, MASK, KB, false>(tiles[t & 1], tiles[t & 1] + T::BYTES, qf, o, m, l, p.c, now, now == T::ALL, pair);
   }
   if (!busy) return;
   l = sum32(l);
@@ -557,6 +572,16 @@ __global__ void __launch_bounds__(XA_T, D <= 64 ? (MASK == MASK_PAIRS ? 3 : 4) :
     for (int j4 = 0; j4 < 4; ++j4)
       *reinterpret_cast<f32x4*>(po + 32 * b + 8 * j4 + 4 * hl) = f32x4{o[b][4 * j4], o[b][4 * j4 + 1], o[b][4 * j4 + 2], o[b][4 * j4 + 3]};
   if (hl == 0) *reinterpret_cast<float2*>(p.part + all * D + 2 * at) = float2{m, l};
+}
+
+// MASK_PAIRS: the mask's bytes as bits, 64 keys a word, zeros behind the last key: read once for all heads, and an eighth
+// of the bytes for the kernels' gathers. A thread makes 16 bits
+__global__ void __launch_bounds__(XA_T) xa_bits_kernel(const unsigned char* mask, int64_t mbs, int64_t mqs, int64_t lq, int64_t lk,
+                                                       int64_t nw, int64_t total, unsigned short* out) {
+  const int64_t i = (int64_t)blockIdx.x * XA_T + threadIdx.x;
+  if (i >= total) return;
+  const int64_t row = i / (4 * nw), w = i - row * 4 * nw, n = row / lq, key = 16 * w;
+  out[i] = key < lk ? (unsigned short)xa_bits16(mask + n * mbs + (row - n * lq) * mqs + key, lk - key) : 0;
 }
 
 // The splits' (O, m, l) joined. TPR threads hold a row's columns (4 each), gs groups of them its splits: group i takes
@@ -628,13 +653,16 @@ __global__ void __launch_bounds__(XA_T) xa_join_kernel(const CrossP p, int gs) {
 
 int xa_pad(int64_t d) { return d <= 32 ? 32 : d <= 64 ? 64 : d <= 96 ? 96 : 128; }
 
+constexpr int XA_LEAST = 4;
+
 struct XaPlan {
   bool resident;
   int64_t nblk, split_len;  // row blocks (resident: workgroups) of an (image, kv head); keys of a split
   int splits;
+  size_t bits, part;        // workspace bytes: the mask's words, the splits' parts
 };
 
-XaPlan xa_plan(int32_t dt, int64_t n, int64_t lq, int64_t lk, int64_t heads, int64_t kv_heads, int64_t d) {
+XaPlan xa_plan(int32_t dt, int64_t n, int64_t lq, int64_t lk, int64_t heads, int64_t kv_heads, int64_t d, int mask) {
   XaPlan g{};
   const int kt = dt == DT_BF16 ? 64 : 32, D = xa_pad(d);
   const int64_t rows = lq * (heads / kv_heads), nk = n * kv_heads;
@@ -648,13 +676,18 @@ XaPlan xa_plan(int32_t dt, int64_t n, int64_t lq, int64_t lk, int64_t heads, int
   }
   g.nblk = cdiv(rows, XA_ROWS);
   const int64_t blocks = g.nblk * nk;
-  // split the keys while the row blocks leave CUs idle: two workgroups per CU, four tiles or more each
-  int64_t want = 2LL * device_cus() / blocks;
-  const int64_t most = cdiv(lk, 4 * kt);
+  // Split the keys where the row blocks leave a quarter of the CUs or more idle: two workgroups per CU, XA_LEAST tiles
+  // or more each. Writing and joining the parts costs about 10 us at thousands of rows (2 x 3600 queries, 1000 keys, 4
+  // heads of 64, 232 blocks: 18.7 us whole, 28.0 in two parts; 1 x 3600 x 3600, 116 blocks: 35 in two, 32.8 in four; one
+  // query of 8 images x 30001 keys, 32 blocks: 119 in eight, 94 in sixteen, 107 in twenty-four)
+  int64_t want = 4 * blocks < 3LL * device_cus() ? 2LL * device_cus() / blocks : 1;
+  const int64_t most = cdiv(lk, XA_LEAST * kt);
   if (want > most) want = most;
   if (want < 1) want = 1;
   g.split_len = cdiv(cdiv(lk, want), kt) * kt;
   g.splits = (int)cdiv(lk, g.split_len);
+  if (mask == MASK_PAIRS) g.bits = (size_t)(n * lq * cdiv(lk, 64) + 1) / 2 * 16;
+  if (g.splits > 1) g.part = (size_t)g.splits * nk * rows * (D + 2) * sizeof(float);
   return g;
 }
 
@@ -687,10 +720,10 @@ void xa_launch(const CrossP& k, bool resident, int mask, hipStream_t st) {
 using namespace clarus;
 
 extern "C" size_t clarus_hip_cross_attention_workspace(int32_t dtype, int64_t n, int64_t lq, int64_t lk, int64_t heads,
-                                                       int64_t kv_heads, int64_t d) {
+                                                       int64_t kv_heads, int64_t d, int32_t mask_mode) {
   if (n <= 0 || lq <= 0 || lk <= 0 || kv_heads <= 0 || heads <= 0 || heads % kv_heads || d <= 0 || d > 128) return 0;
-  const XaPlan g = xa_plan(dtype, n, lq, lk, heads, kv_heads, d);
-  return g.splits > 1 ? (size_t)g.splits * n * heads * lq * (xa_pad(d) + 2) * sizeof(float) : 0;
+  const XaPlan g = xa_plan(dtype, n, lq, lk, heads, kv_heads, d, mask_mode);
+  return g.bits + g.part;
 }
 
 extern "C" int clarus_hip_cross_attention(const ClarusCrossArgs* a, void* scratch, size_t scratch_bytes, void* stream) {
@@ -714,15 +747,16 @@ extern "C" int clarus_hip_cross_attention(const ClarusCrossArgs* a, void* scratc
   CLARUS_REQUIRE(a->mask_mode >= MASK_NONE && a->mask_mode <= MASK_PAIRS && (a->mask_mode == MASK_NONE || a->mask),
                  "cross_attention: mask");
   CLARUS_REQUIRE(a->lq < ((int64_t)1 << 31) && a->lk < ((int64_t)1 << 31) && a->n * a->kv_heads < 65536 &&
-                     a->lq * (a->heads / a->kv_heads) < ((int64_t)1 << 31),
+                     a->lq * (a->heads / a->kv_heads) < ((int64_t)1 << 31) &&
+                     (a->mask_mode != MASK_PAIRS || a->n * a->lq < ((int64_t)1 << 38) / a->lk),
                  "cross_attention: too large");
-  const XaPlan g = xa_plan(a->dtype, a->n, a->lq, a->lk, a->heads, a->kv_heads, a->d);
+  const XaPlan g = xa_plan(a->dtype, a->n, a->lq, a->lk, a->heads, a->kv_heads, a->d, a->mask_mode);
   CLARUS_REQUIRE(8 * ((g.nblk * a->n * a->kv_heads * g.splits + 7) / 8) < ((int64_t)1 << 31), "cross_attention: too large");
-  const size_t need = clarus_hip_cross_attention_workspace(a->dtype, a->n, a->lq, a->lk, a->heads, a->kv_heads, a->d);
+  const size_t need = g.bits + g.part;
   CLARUS_REQUIRE(need == 0 || (scratch && aligned(scratch, 16) && scratch_bytes >= need),
                  "cross_attention: scratch %zu < %zu bytes", scratch_bytes, need);
   CrossP k{};
-  k.q = a->q; k.k = a->k; k.v = a->v; k.out = a->out; k.mask = (const unsigned char*)a->mask; k.part = (float*)scratch;
+  k.q = a->q; k.k = a->k; k.v = a->v; k.out = a->out; k.mask = (const unsigned char*)a->mask; k.part = (float*)((char*)scratch + g.bits);
   k.qbs = a->q_bstride; k.ldq = a->ldq; k.kbs = a->k_bstride; k.ldk = a->ldk; k.vbs = a->v_bstride; k.ldv = a->ldv;
   k.mbs = a->mask_bstride; k.mqs = a->mask_qstride;
   k.rep = (int)(a->heads / a->kv_heads); k.kv_heads = (int)a->kv_heads; k.d = (int)a->d; k.lq = (int)a->lq;
@@ -731,6 +765,15 @@ extern "C" int clarus_hip_cross_attention(const ClarusCrossArgs* a, void* scratc
   k.o_dt = a->o_dtype;
   k.c = a->scale * 1.4426950408889634f;
   hipStream_t st = (hipStream_t)stream;
+  if (g.bits) {
+    // images or queries that share one mask row (stride 0) share its words
+    const int64_t nw = cdiv(a->lk, 64), lq = a->mask_qstride ? a->lq : 1, total = (a->mask_bstride ? a->n : 1) * lq * 4 * nw;
+    k.bits = (const uint64_t*)scratch;
+    k.nw = a->mask_qstride ? nw : 0;
+    k.bbs = a->mask_bstride ? lq * nw : 0;
+    hipLaunchKernelGGL(xa_bits_kernel, dim3((unsigned)cdiv(total, XA_T)), dim3(XA_T), 0, st, k.mask, a->mask_bstride,
+                       a->mask_qstride, lq, a->lk, nw, total, (unsigned short*)scratch);
+  }
   const int D = xa_pad(a->d);
   note_kernel("%s d=%d splits=%d", g.resident ? "xa_resident_kernel" : "xa_kernel", D, g.splits);
 #define CLARUS_XA(DT)                                        \

@@ -945,7 +945,7 @@ class HipOps(Backend):
             n=n, lq=lq, lk=lk, heads=heads, kv_heads=kv_heads, d=d, q_bstride=qa[2], ldq=qa[1], k_bstride=ka[2], ldk=ka[1],
             v_bstride=va[2], ldv=va[1], mask_bstride=mbs, mask_qstride=mqs, dtype=_lib.dtype_code(q.dtype),
             o_dtype=_lib.dtype_code(odt), mask_mode=mode, scale=scale)
-        return odt, args, self.lib.clarus_hip_cross_attention_workspace(args.dtype, n, lq, lk, heads, kv_heads, d)
+        return odt, args, self.lib.clarus_hip_cross_attention_workspace(args.dtype, n, lq, lk, heads, kv_heads, d, mode)
 
     def channel_attention(self, qkv, heads, temperature):
         if not qkv.is_contiguous():

@@ -496,7 +496,8 @@ int clarus_hip_group_norm(const void* x, int32_t x_dtype, int64_t x_bstride, int
  * so v has to be finite. dtype bf16 or fp32 (of q, k and v), o_dtype either; d a multiple of 8, at most
  * 128; scale > 0. Scores, softmax and output are accumulated in fp32; with bf16 the weights p are rounded
  * once to bf16 for the product with v. scratch holds clarus_hip_cross_attention_workspace(...) bytes
- * (partial results where few rows ask many keys; may be 0), 16-byte aligned. Deterministic.
+ * (partial results where few rows ask many keys, a
+ * mask of pairs as bits; may be 0), 16-byte aligned. Deterministic.
  * No counterpart in the reference (its attention is over channels: clarus_hip_channel_attention).
  */
 typedef struct ClarusCrossArgs {
@@ -513,7 +514,7 @@ typedef struct ClarusCrossArgs {
 } ClarusCrossArgs;
 
 size_t clarus_hip_cross_attention_workspace(int32_t dtype, int64_t n, int64_t lq, int64_t lk, int64_t heads,
-                                            int64_t kv_heads, int64_t d);
+                                            int64_t kv_heads, int64_t d, int32_t mask_mode);
 int clarus_hip_cross_attention(const ClarusCrossArgs* args, void* scratch, size_t scratch_bytes, void* stream);
 
 /* ABI version (CLARUS_HIP_ABI_VERSION) and struct sizes, for binding checks. */

@@ -87,6 +87,7 @@ def cpu_hip(dtype=torch.float32):
     from clarus_amd.hip_ops import HipOps
     h = HipOps.__new__(HipOps)
     h.dtype, h.device, h.dev, h._cache, h._plans = dtype, torch.device("cpu"), torch.device("cpu"), {}, {}
+    h.lib = _lib.load()
     return h
 
 
@@ -140,8 +141,8 @@ def test_c_entry_refuses_before_launch():
                dict(n=1 << 15), dict(lq=1, lk=100000, size=16), dict(lq=1, lk=100000, scratch=None)):
         assert call(**kw) == _lib.EINVAL, kw
         assert b"cross_attention" in lib.clarus_hip_last_error()
-    assert lib.clarus_hip_cross_attention_workspace(0, 1, 1, 100000, 4, 2, 32) > 0
-    assert lib.clarus_hip_cross_attention_workspace(0, 1, 1, 100000, 4, 3, 32) == 0
+    assert lib.clarus_hip_cross_attention_workspace(0, 1, 1, 100000, 4, 2, 32, 0) > 0
+    assert lib.clarus_hip_cross_attention_workspace(0, 1, 1, 100000, 4, 3, 32, 0) == 0
 
 
 @pytest.mark.parametrize("kind", ["none", "keys", "pairs"])

@@ -63,6 +63,7 @@ def cpu_hip(dtype=torch.float32):
     from clarus_amd.hip_ops import HipOps
     h = HipOps.__new__(HipOps)
     h.dtype, h.device, h.dev, h._cache, h._plans = dtype, torch.device("cpu"), torch.device("cpu"), {}, {}
+    h.lib = _lib.load()
     return h
 
 
