@@ -184,8 +184,20 @@ __global__ void __launch_bounds__(GN_TT) gn_stats_kernel(const GroupNormP p) {
   });
 }
 
+// GELU for an output rounded to bf16: x / (1 + e^-xP(x^2)), P an own least-squares minimax fit of ln(Phi(x) / Phi(-x)) / x
+// on |x| < 6 (the leading coefficient positive, so that it goes on to 0 and x). Off by at most 1.7e-5, and by 1.2e-4 of
+// the value from -2.4 up: a seventeenth of a bf16 half step. 12 VALU slots against the 23 of the erf form, which make
+// the apply pass wait for its arithmetic: 720 x 1280 x 64 bf16 72.4 us with it, 62.6 with this
+__device__ __forceinline__ float gelu_logistic(float x) {
+  const float y = x * x;
+  // coefficients times -log2(e)
+  const float p = fmaf(fmaf(fmaf(fmaf(-2.05391e-06f, y, 5.84004e-05f), y, 5.98691e-04f), y, -1.05898520e-01f), y, -2.30154548f);
+  return x * __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(x * p));
+}
+
+template <int ODT>
 __device__ __forceinline__ float gn_act(float y, int act) {
-  if (act == ACT_GELU) return gelu_erf(y);
+  if (act == ACT_GELU) return ODT == DT_BF16 ? gelu_logistic(y) : gelu_erf(y);
   if (act == GN_SILU) return y * __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(y * -1.4426950408889634f));
   return y;
 }
@@ -310,7 +322,7 @@ __global__ void __launch_bounds__(GN_T) gn_apply_kernel(const GroupNormP p) {
       const f32x8 x = gn_widen<DT>(u[k]);
       f32x8 y;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) y.v[i] = gn_act(fmaf(x.v[i] - mean[i], a[i], b[i]), ACT);
+      for (int i = 0; i < 8; ++i) y.v[i] = gn_act<ODT>(fmaf(x.v[i] - mean[i], a[i], b[i]), ACT);
       gn_store<ODT>(p.out, ob + (int64_t)(r + k * p.rpb) * p.c, y);
     }
   }
@@ -386,7 +398,7 @@ __global__ void __launch_bounds__(GN_TS) gn_small_kernel(const GroupNormP p) {
     if (rl + k * p.rpb >= P) continue;
     f32x8 y;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) y.v[i] = gn_act(fmaf(v[k].v[i] - mean[i / PER], a[i], b[i]), p.act);
+    for (int i = 0; i < 8; ++i) y.v[i] = gn_act<ODT>(fmaf(v[k].v[i] - mean[i / PER], a[i], b[i]), p.act);
     gn_store<ODT>(p.out, ob + (int64_t)(rl + k * p.rpb) * p.c, y);
   }
 }
