@@ -22,11 +22,11 @@ namespace clarus {
 namespace {
 
 constexpr int GN_T = 256;    // threads of an apply workgroup
-constexpr int GN_TS = 512;   // threads of a small workgroup
+constexpr int GN_TS = 256;   // threads of a small workgroup
 constexpr int GN_TT = 256;   // threads of a stats workgroup
 constexpr int UR = 8;         // rows in flight per thread (stats)
 constexpr int UA = 4;        // rows in flight per thread (apply)
-constexpr int NRMAX = 16;    // rows held per thread (small)
+constexpr int NRMAX = 8;     // rows held per thread (small), at most
 constexpr int GN_JOIN = 8;   // partial statistics in flight per thread (join)
 constexpr int GN_UNIT = 2048;  // channels that a workgroup has to hold together, at most
 constexpr int GN_SILU = CLARUS_ACT_SILU;
@@ -423,7 +423,9 @@ struct GnPlan {
 GnPlan gn_plan(int64_t n, int64_t p, int64_t c, int64_t groups) {
   GnPlan g{};
   const int64_t u = gn_unit(c / groups) / 8;  // octets a workgroup has to hold together
-  // One launch where a unit's pixels fit the registers of one workgroup
+  // One launch where a unit's pixels are at most NRMAX rows per thread of one workgroup: past that few workgroups with
+  // long chains of loads lose to the three launches over the whole chip (us, one / three launches: 16 x 24 x 512 at 3
+  // rows 5.6 / 9; 32 x 48 x 512 at 12 rows 10.8 / 9.5; 64 x 64 x 128 at 16 rows 16.5 / 10.7)
   g.small = p * u <= (int64_t)(GN_TS / u) * u * NRMAX && p <= (int64_t)(GN_TS / u) * NRMAX;
   if (g.small) {
     g.tr = (int)u;
