@@ -184,14 +184,20 @@ __global__ void __launch_bounds__(GN_TT) gn_stats_kernel(const GroupNormP p) {
   });
 }
 
-// GELU for an output rounded to bf16: x / (1 + e^-xP(x^2)), P an own least-squares minimax fit of ln(Phi(x) / Phi(-x)) / x
-// on |x| < 6 (the leading coefficient positive, so that it goes on to 0 and x). Off by at most 1.7e-5, and by 1.2e-4 of
-// the value from -2.4 up: a seventeenth of a bf16 half step. 12 VALU slots against the 23 of the erf form, which make
-// the apply pass wait for its arithmetic: 720 x 1280 x 64 bf16 72.4 us with it, 62.6 with this
+// GELU for an output rounded to bf16: x / (1 + e^-xP(x^2)), P an own minimax fit of ln(Phi(x) / Phi(-x)) / x on |x| < 5.5
+// (its leading coefficient positive, so that it goes on to 0 and x). Off by at most 6.6e-6 and, down to -5.5, by 5.6e-4
+// of the value, a seventh of a bf16 half step; further down the values are below 2e-7. 14 VALU slots against the 23 of
+// the erf form, which make the apply pass wait for its arithmetic: 720 x 1280 x 64 bf16 72.4 us with it, 63.8
+// with this
 __device__ __forceinline__ float gelu_logistic(float x) {
   const float y = x * x;
   // coefficients times -log2(e)
-  const float p = fmaf(fmaf(fmaf(fmaf(-2.05391e-06f, y, 5.84004e-05f), y, 5.98691e-04f), y, -1.05898520e-01f), y, -2.30154548f);
+  float p = fmaf(-1.38621534e-09f, y, 1.46396019e-07f);
+  p = fmaf(p, y, -5.90224226e-06f);
+  p = fmaf(p, y, 1.00142061e-04f);
+  p = fmaf(p, y, 3.82605504e-04f);
+  p = fmaf(p, y, -1.05382465e-01f);
+  p = fmaf(p, y, -2.30192351f);
   return x * __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(x * p));
 }
 
@@ -426,7 +432,7 @@ GnPlan gn_plan(int64_t n, int64_t p, int64_t c, int64_t groups) {
   // One launch where a unit's pixels are at most NRMAX rows per thread of one workgroup: past that few workgroups with
   // long chains of loads lose to the three launches over the whole chip (us, one / three launches: 16 x 24 x 512 at 3
   // rows 5.6 / 9; 32 x 48 x 512 at 12 rows 10.8 / 9.5; 64 x 64 x 128 at 16 rows 16.5 / 10.7)
-  g.small = p * u <= (int64_t)(GN_TS / u) * u * NRMAX && p <= (int64_t)(GN_TS / u) * NRMAX;
+  g.small = p <= (int64_t)(GN_TS / u) * NRMAX;
   if (g.small) {
     g.tr = (int)u;
     g.strips = (int)(c / 8 / u);
@@ -475,8 +481,9 @@ extern "C" int clarus_hip_group_norm(const void* x, int32_t x_dtype, int64_t x_b
   CLARUS_REQUIRE(aligned(x, 16) && aligned(out, 16) && ldx * es % 16 == 0 && x_bstride * es % 16 == 0,
                  "group_norm: x and out 16-byte aligned rows");
   CLARUS_REQUIRE((w_bstride == 0 || w_bstride >= c) && (b_bstride == 0 || b_bstride >= c), "group_norm: affine strides");
-  // float counts and the pixel index of a chunk: 2^31 pixels, 65535 images and strips are the launch's limits
-  CLARUS_REQUIRE(p < ((int64_t)1 << 31) && n < 65536 && c < ((int64_t)1 << 24), "group_norm: too large");
+  CLARUS_REQUIRE(eps >= 0.f && eps < INFINITY, "group_norm: eps finite and not negative");
+  // the pixel index of a chunk is 32 bits; a launch has at most 65535 images and strips (of 8 channels or more)
+  CLARUS_REQUIRE(p < ((int64_t)1 << 31) && n < 65536 && c < ((int64_t)1 << 19), "group_norm: too large");
   const size_t need = clarus_hip_group_norm_workspace(n, p, c, groups);
   CLARUS_REQUIRE(need == 0 || (scratch && scratch_bytes >= need && aligned(scratch, 8)), "group_norm: scratch %zu < %zu bytes", scratch_bytes, need);
   const GnPlan g = gn_plan(n, p, c, groups);

@@ -97,6 +97,20 @@ def test_refused_layouts_and_gradients():
         h.group_norm(torch.zeros(2, 4, 4, 16), 4, weight=torch.ones(16, requires_grad=True))
 
 
+def test_refused_values():
+    h = cpu_hip()
+    for eps in (-1e-5, float("nan"), float("inf")):
+        with pytest.raises(Unsupported):
+            h.group_norm(torch.zeros(2, 4, 4, 16), 4, eps=eps)
+    with pytest.raises(Unsupported):
+        h.group_norm(torch.zeros(1, 1, 1 << 19), 1 << 16)
+    lib = _lib.load()
+    for kw in (dict(eps=-1.0), dict(eps=float("nan")), dict(c=1 << 19, ldx=1 << 19)):
+        kw = {**dict(eps=1e-5, c=64, ldx=64), **kw}
+        assert lib.clarus_hip_group_norm(1 << 20, 0, 0, kw["ldx"], None, 0, None, 0, 1 << 24, 0, 1, 4, kw["c"], kw["c"] // 8,
+                                         kw["eps"], 0, None, 0, None) == _lib.EINVAL, kw
+
+
 def test_c_entry_refuses_before_launch():
     lib = _lib.load()
 
@@ -189,6 +203,43 @@ def test_hard_values(hips, gpu_device):
         got = hip.group_norm(y, 8, w, b)
         assert torch.equal(got[0], base[0]) and not torch.isfinite(got[1, ..., 16:24]).any()
         assert torch.equal(got[1, ..., :16], base[1, ..., :16]) and torch.equal(got[1, ..., 24:], base[1, ..., 24:])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("act", ["silu", "gelu"])
+@pytest.mark.parametrize("shape", [(1, 20, 30, 64), (1, 120, 130, 64)])
+def test_activations_over_their_range(shape, act, dt, hips, gpu_device):
+    """Values from -60 to 60: the tails go to 0 and x. In bf16, beside the general check, the values of the tail
+    themselves, down to -5.4 (below, they are under 2^-21): 2^-8 of the value for the rounding and as much for the
+    formula, and what y may be off by times the activation's slope there (its curvature times the square is nothing)."""
+    x, _, _ = inputs(shape, torch.float32, gpu_device)
+    for w, b in ((1.0, 0.0), (1.0, -3.0), (0.5, -5.0), (12.0, 5.0), (0.25, 50.0), (0.25, -50.0)):
+        wt, bt = (torch.full((shape[-1],), t, device=gpu_device) for t in (w, b))
+        got = hips[dt].group_norm(x, 8, wt, bt, act=act, out_dtype=dt)
+        check(got, x, 8, wt, bt, act=act, what=f"{act} {w} {b}")
+        if dt == torch.bfloat16:
+            y, slack = plain64(x, 8, wt, bt)
+            y.requires_grad_()
+            ref = F.silu(y) if act == "silu" else F.gelu(y)
+            slope, = torch.autograd.grad(ref.sum(), y)
+            tol = 2 * 2.0 ** -8 * ref.abs() + STAT * slack * slope.abs()
+            off = torch.where(y > -5.4, (got.double() - ref).abs() - tol, torch.zeros_like(ref))
+            assert off.max() <= 0, (w, b, off.max().item())
+
+
+@pytest.mark.gpu
+def test_a_weight_is_read_with_every_call(hips, gpu_device):
+    """A weight of another type that changes outside autograd's sight, and one used on another stream."""
+    x, w, b = inputs((1, 9, 7, 64), torch.float32, gpu_device)
+    hip = hips[torch.float32]
+    wb = w.bfloat16()
+    for i in range(3):
+        wb.data.copy_((w * (i + 1)).bfloat16())
+        check(hip.group_norm(x, 8, wb, b), x, 8, wb, b, what=str(i))
+    with torch.inference_mode():
+        wi = w.bfloat16()
+        check(hip.group_norm(x, 8, wi, b), x, 8, wi, b, what="inference")
 
 
 @pytest.mark.gpu
