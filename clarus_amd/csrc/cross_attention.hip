@@ -2,20 +2,34 @@
 // another length, on gfx950:
 //   o[q] = sum_j p_j v_j,  p = softmax_j(scale q . k_j)  over the keys the mask keeps; 0 where it keeps none.
 //
-// One pass over the keys with the running maximum m and sum l of the softmax: a workgroup holds 128
-// rows (4 waves x 32), takes K and V a tile at a time through LDS (double buffered, the next tile's
-// loads in flight during the current one's products) and never writes a score to memory. A row is a
-// query and one of the heads that share a kv head, so shared heads fill the tile of a single query.
-//   S^T = K Q^T       a lane of a 32 x 32 MFMA holds one row's scores of 16 keys: maxima and sums
-//                     need one exchange, with lane ^ 32
+// One pass over the keys with the running maximum m and sum l of the softmax; no score is written to
+// memory. A row is a query and one of the heads that share a kv head, so shared heads fill the tile of
+// a single query. A wave holds 32 rows:
+//   S^T = K Q^T       a lane of a 32 x 32 MFMA holds one row's scores of 16 keys: sums stay in the lane to
+//                     the end, a maximum needs one exchange, with lane ^ 32
 //   O^T = V^T P^T     P^T is the B operand as it is: lane l holds keys 8 (i / 4) + 4 (l / 32) + i % 4
 //                     of each 16, and V^T is read in that order (bf16: transposing LDS reads; fp32: one
 //                     float per lane), so P moves through no LDS
+// K and V go from memory straight to LDS, 16 bytes a lane, without passing through registers.
+//   xa_resident_kernel  up to XR_KEYS keys: all of them stay in LDS, rows stream by
+//   xa_kernel           any number of keys: 128 rows (4 waves) per workgroup, tiles of 64 (fp32: 32) keys, the
+//                       next one on its way during the current one's products
+//   xa_join_kernel      joins the (O, m, l) of keys split over workgroups, where rows are few
+//   xa_bits_kernel      a mask of pairs as bits
 // m, l and O are fp32. bf16: products of bf16 q, k, v are exact in fp32; P is rounded once to bf16 for
-// the product with V (half a step, 2^-9 relative per weight, of independent signs: the result's own
-// rounding to bf16 is as large). fp32: every product runs on fp32 MFMAs.
-// A masked or padding key's score is taken as -inf whatever its K holds, and its V row as 0.
-// Few rows: the keys are split over workgroups, whose (O, m, l) xa_join_kernel joins.
+// the product with V (at most half a step, 2^-8, of each weight, of independent signs: below the
+// result's own rounding to bf16). fp32: every product runs on fp32 MFMAs.
+// A masked or padding key's score is taken as -inf whatever its K holds; where no query keeps it (a mask of
+// keys, the end of the keys) its V row is taken as 0.
+//
+// What bounds it (bf16, the GPU's time alone, without the call's).
+//   Many rows and keys: the matrix cores and the softmax's arithmetic, which take turns: at 57600 queries x 3600
+//   keys, 4 heads of 128, MFMAs are busy 414k and the VALU 412k of 825k cycles, at a clock that the load lowers to
+//   1.7 GHz: 477 us, 890 TFLOP/s (a large library product reaches 1190). 14400 x 3600, 8 heads of 64, twice the
+//   arithmetic per product: 145 us, 731 TFLOP/s.
+//   A prompt (57600 x 77, 4 heads of 64): 12 us of reading q and writing o at the rate of a large copy; 21 us, a wave
+//   loading, multiplying and weighing its few keys in turn.
+//   One query of 8 images x 30001 keys: reading K and V, 492 MB in 95 us, 5.2 TB/s (a large copy: 4.8 TB/s).
 #include "capi.hpp"
 #include "common.hpp"
 
@@ -29,8 +43,7 @@ typedef __attribute__((ext_vector_type(4))) short s16x4;
 constexpr int XA_T = 256;    // threads
 constexpr int XA_ROWS = 128; // rows of a workgroup
 constexpr float XA_FLOOR = -3e38f;  // running maximum before any key: exp2(-inf - XA_FLOOR) = 0, no inf - inf
-
-constexpr float XA_SLACK = 8.f;
+constexpr float XA_SLACK = 8.f;     // a running maximum may lag the scores' by this (log2)
 
 enum : int { MASK_NONE = 0, MASK_KEYS = 1, MASK_PAIRS = 2 };
 
@@ -101,7 +114,7 @@ __device__ __forceinline__ float keep_bit(float v, unsigned w, int bit) {
   return __uint_as_float((__float_as_uint(v) & k) | (0xff800000u & ~k));
 }
 
-// one row of a wave: its query, head and mask row
+// one row of a wave: its query and head
 struct XaRow {
   int64_t qi;
   int head;
@@ -127,7 +140,7 @@ __device__ __forceinline__ void xa_load_q(const CrossP& p, int64_t n, const XaRo
   }
 }
 
-// 16 mask bytes (0 / 1) at p, the first `left` of them there, as 16 bits
+// 16 mask bytes (0 masked, any other value kept) at p, the first `left` of them there, as 16 bits
 __device__ __forceinline__ unsigned xa_bits16(const unsigned char* p, int64_t left) {
   struct __attribute__((packed, aligned(1))) Bytes { u32x4 v; };
   u32x4 w = {0, 0, 0, 0};
@@ -140,7 +153,10 @@ __device__ __forceinline__ unsigned xa_bits16(const unsigned char* p, int64_t le
   }
   unsigned r = 0;
 #pragma unroll
-  for (int i = 0; i < 4; ++i) r |= ((w[i] & 0x01010101u) * 0x10204080u >> 28) << (4 * i);  // bytes 0 .. 3 -> bits 28 .. 31
+  for (int i = 0; i < 4; ++i) {
+    const unsigned any = (((w[i] & 0x7f7f7f7fu) + 0x7f7f7f7fu) | w[i]) >> 7 & 0x01010101u;  // byte != 0
+    r |= (any * 0x10204080u >> 28) << (4 * i);                                             // bytes 0 .. 3 -> bits 28 .. 31
+  }
   return r;
 }
 
@@ -343,9 +359,9 @@ __device__ __forceinline__ bool xa_any(const unsigned char* p, int64_t left) {
 }
 
 // ---------------------------------------------------------------- few keys
-// Up to XR_KEYS keys (a prompt): all keys of an (image, kv head) stay in a workgroup's LDS: copied once, one barrier, then its 8 waves take 32 rows
-// each, chunk after chunk, the next chunk's queries in flight. Workgroups of the same rows and other heads run on one
-// XCD, whose L2 then reads and writes each line of q and out once.
+// Up to XR_KEYS keys (a prompt): all keys of an (image, kv head) stay in a workgroup's LDS: copied once, one barrier,
+// then its 8 waves take 32 rows each, chunk after chunk, the next chunk's queries in flight. Workgroups of the same rows
+// and other heads run on one XCD, whose L2 then reads and writes each line of q and out once.
 constexpr int XR_T = 512;
 constexpr int XR_KEYS = 128;
 
@@ -735,7 +751,7 @@ extern "C" int clarus_hip_cross_attention(const ClarusCrossArgs* a, void* scratc
   CLARUS_REQUIRE(a->d >= 8 && a->d <= 128 && a->d % 8 == 0, "cross_attention: head width a multiple of 8, at most 128");
   CLARUS_REQUIRE((a->dtype == DT_BF16 || a->dtype == DT_F32) && (a->o_dtype == DT_BF16 || a->o_dtype == DT_F32),
                  "cross_attention: bf16 or fp32");
-  CLARUS_REQUIRE(a->scale > 0.f && a->scale < INFINITY, "cross_attention: scale positive and finite");
+  CLARUS_REQUIRE(a->scale > 0.f && a->scale < 2e38f, "cross_attention: scale positive and below 2e38");
   const int64_t es = a->dtype == DT_BF16 ? 2 : 4;
   CLARUS_REQUIRE(aligned(a->q, 16) && aligned(a->k, 16) && aligned(a->v, 16) && aligned(a->out, 16) && a->ldq * es % 16 == 0 &&
                      a->ldk * es % 16 == 0 && a->ldv * es % 16 == 0 && a->q_bstride * es % 16 == 0 &&
@@ -744,7 +760,8 @@ extern "C" int clarus_hip_cross_attention(const ClarusCrossArgs* a, void* scratc
   CLARUS_REQUIRE(a->ldk < (1 << 24) && a->ldv < (1 << 24), "cross_attention: rows of k and v less than 2^24 elements apart");
   CLARUS_REQUIRE(a->ldq >= 0 && a->ldk >= 0 && a->ldv >= 0 && a->q_bstride >= 0 && a->k_bstride >= 0 && a->v_bstride >= 0,
                  "cross_attention: strides");
-  CLARUS_REQUIRE(a->mask_mode >= MASK_NONE && a->mask_mode <= MASK_PAIRS && (a->mask_mode == MASK_NONE || a->mask),
+  CLARUS_REQUIRE(a->mask_mode >= MASK_NONE && a->mask_mode <= MASK_PAIRS && (a->mask_mode == MASK_NONE || a->mask) &&
+                     a->mask_bstride >= 0 && a->mask_qstride >= 0,
                  "cross_attention: mask");
   CLARUS_REQUIRE(a->lq < ((int64_t)1 << 31) && a->lk < ((int64_t)1 << 31) && a->n * a->kv_heads < 65536 &&
                      a->lq * (a->heads / a->kv_heads) < ((int64_t)1 << 31) &&

@@ -842,23 +842,18 @@ class HipOps(Backend):
             key, lambda: self._group_norm_plan(x, groups, weight, bias, act, out_dtype or self.dtype))
         if x.data_ptr() % 16:
             raise Unsupported("group_norm: 16-byte aligned rows")
+        if not 0.0 <= eps < math.inf:
+            raise Unsupported("group_norm: eps finite and not negative")
         out = torch.empty(x.shape, device=x.device, dtype=odt)
         if not p:
             return out
-        wf = weight if weight is None or weight.dtype == torch.float32 and weight.is_contiguous() else self._affine(weight)
-        bf = bias if bias is None or bias.dtype == torch.float32 and bias.is_contiguous() else self._affine(bias)
+        wf = weight if weight is None else weight.float().contiguous()
+        bf = bias if bias is None else bias.float().contiguous()
         scratch = torch.empty(need, device=x.device, dtype=torch.uint8) if need else None
         self._call("group_norm", self.lib.clarus_hip_group_norm, x.data_ptr(), _lib.dtype_code(x.dtype), xbs, ldx,
                    _lib.ptr(wf), wbs, _lib.ptr(bf), bbs, out.data_ptr(), _lib.dtype_code(odt), n, p, c, groups, float(eps),
                    acode, _lib.ptr(scratch), need)
         return out
-
-    def _affine(self, t):
-        """fp32 contiguous copy of a weight [C], kept, or of an image's own scale or shift [N, C], which is new with
-        every call; nor is what a capturing graph's pool holds kept, which the replay alone writes."""
-        if t.dim() == 1 and not torch.cuda.is_current_stream_capturing():
-            return self._bias(t)
-        return t.float().contiguous()
 
     def _group_norm_plan(self, x, groups, weight, bias, act, odt):
         if x.dim() < 2 or act not in (None, "silu", "gelu") or not isinstance(groups, int) or groups < 1:
@@ -878,8 +873,8 @@ class HipOps(Backend):
         if at is None or at[1] < c or at[1] * es % 16 or at[2] * es % 16:
             raise Unsupported("group_norm: unit channel stride, one pixel stride, 16-byte aligned rows")
         p, ldx, xbs = at
-        if p >= 1 << 31 or n >= 65536:
-            raise Unsupported("group_norm: fewer than 2^31 pixels of an image and 65536 images")
+        if p >= 1 << 31 or n >= 65536 or c >= 1 << 19:
+            raise Unsupported("group_norm: fewer than 2^31 pixels of an image, 65536 images and 2^19 channels")
         return odt, n, p, c, groups, xbs, ldx, wbs, bbs, acode, self.lib.clarus_hip_group_norm_workspace(n, p, c, groups)
 
     # ------------------------------------------------------------------ attention
@@ -892,6 +887,7 @@ class HipOps(Backend):
         or [N, Lq, Lk] (v has to be finite: a masked pair weighs 0). fp32 scores, softmax and sums; bf16 weights
         enter the product with v rounded to bf16. Returns a contiguous tensor of q's shape."""
         kv_heads = heads if kv_heads is None else kv_heads
+        scale = None if scale is None else float(scale)
         key = ("cross_attention", q.shape, q.stride(), k.shape, k.stride(), v.shape, v.stride(), q.dtype, k.dtype, v.dtype,
                heads, kv_heads, scale, out_dtype, None if mask is None else (mask.shape, mask.stride(), mask.dtype))
         self._forward_only("cross_attention", q, k, v, mask)
@@ -922,9 +918,9 @@ class HipOps(Backend):
         if scale is None and d:
             scale = d ** -0.5
         if not (_kdt(q) and q.dtype == k.dtype == v.dtype and odt in _KDT and 8 <= d <= 128 and d % 8 == 0
-                and 0.0 < scale < math.inf):
+                and 0.0 < scale < 2e38):
             raise Unsupported("cross_attention: bf16 / fp32 q, k, v of one type, head width a multiple of 8 up to 128, "
-                              "scale positive and finite")
+                              "scale positive and below 2e38")
         mode, mbs, mqs = _lib.MASK_NONE, 0, 0
         if mask is not None:
             if mask.dtype != torch.bool or tuple(mask.shape) not in ((n, lk), (n, lq, lk)):
@@ -939,8 +935,10 @@ class HipOps(Backend):
         es = q.element_size()
         if None in (qa, ka, va) or any(s * es % 16 for t in (qa, ka, va) for s in t[1:]) or max(ka[1], va[1]) >= 1 << 24:
             raise Unsupported("cross_attention: unit channel stride, one row stride (k and v: below 2^24), 16-byte aligned rows")
-        if max(lk, lq * (heads // kv_heads)) >= 1 << 31 or n * kv_heads >= 65536:
-            raise Unsupported("cross_attention: fewer than 2^31 keys and rows, fewer than 65536 (image, kv head) pairs")
+        if (max(lk, lq * (heads // kv_heads)) >= 1 << 31 or n * kv_heads >= 65536
+                or (mode == _lib.MASK_PAIRS and n * lq >= (1 << 38) // lk)):
+            raise Unsupported("cross_attention: fewer than 2^31 keys and rows, fewer than 65536 (image, kv head) pairs, "
+                              "a [N, Lq, Lk] mask of fewer than 2^38 pairs")
         args = _lib.CrossArgs(
             n=n, lq=lq, lk=lk, heads=heads, kv_heads=kv_heads, d=d, q_bstride=qa[2], ldq=qa[1], k_bstride=ka[2], ldk=ka[1],
             v_bstride=va[2], ldv=va[1], mask_bstride=mbs, mask_qstride=mqs, dtype=_lib.dtype_code(q.dtype),

@@ -475,7 +475,7 @@ int clarus_hip_selective_scan(const void* u, int32_t u_dtype, const float* dbl, 
  * unless it is x itself, contiguous and of one dtype. act: CLARUS_ACT_NONE, CLARUS_ACT_GELU or
  * CLARUS_ACT_SILU. c a multiple of 8 and of groups, lcm(8, c / groups) at most 2048. Statistics and the
  * affine in fp32, rounded once. scratch holds clarus_hip_group_norm_workspace(...) bytes (the partial
- * statistics; may be 0), 8-byte aligned. Deterministic.
+ * statistics; may be 0), 8-byte aligned. Deterministic. p < 2^31, n < 2^16, c < 2^19, eps >= 0.
  * No counterpart in the reference (its norms are the LayerNorm / RMS prologues of linear).
  */
 size_t clarus_hip_group_norm_workspace(int64_t n, int64_t p, int64_t c, int64_t groups);
@@ -489,15 +489,15 @@ int clarus_hip_group_norm(const void* x, int32_t x_dtype, int64_t x_bstride, int
  *   out[n, i, h] = sum_j p_j v[n, j, g],  p = softmax_j(scale q[n, i, h] . k[n, j, g]),  g = h / (heads / kv_heads)
  * over the keys j that the mask keeps; 0 where it keeps none. q rows at q + n * q_bstride + i * ldq, head h
  * at column h * d; k, v likewise with head g (strides in elements, multiples of 16 bytes, ldk and
- * ldv below 2^24; slices of wider rows, shared rows with stride 0). out [n, lq, heads * d] contiguous, overlapping no input.
- * mask (bytes, 1 kept, 0 masked): mask_mode 1: key j of image n kept where mask[n * mask_bstride + j]; such a
+ * ldv below 2^24; slices of wider rows, shared rows with stride 0). out [n, lq, heads * d] contiguous,
+ * overlapping no input.
+ * mask (bytes, 0 masked, any other value kept): mask_mode 1: key j of image n kept where mask[n * mask_bstride + j]; such a
  * masked key counts for nothing, whatever k and v hold. mask_mode 2: kept for query i where
  * mask[n * mask_bstride + i * mask_qstride + j]; k and v of the masked pairs enter no score and weigh 0,
  * so v has to be finite. dtype bf16 or fp32 (of q, k and v), o_dtype either; d a multiple of 8, at most
- * 128; scale > 0. Scores, softmax and output are accumulated in fp32; with bf16 the weights p are rounded
+ * 128; 0 < scale < 2e38. Scores, softmax and output are accumulated in fp32; with bf16 the weights p are rounded
  * once to bf16 for the product with v. scratch holds clarus_hip_cross_attention_workspace(...) bytes
- * (partial results where few rows ask many keys, a
- * mask of pairs as bits; may be 0), 16-byte aligned. Deterministic.
+ * (partial results where few rows ask many keys, a mask of pairs as bits; may be 0), 16-byte aligned. Deterministic.
  * No counterpart in the reference (its attention is over channels: clarus_hip_channel_attention).
  */
 typedef struct ClarusCrossArgs {

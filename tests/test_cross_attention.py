@@ -119,6 +119,17 @@ def test_refusals():
             pytest.fail(f"case {i} was accepted")
 
 
+def test_refused_sizes():
+    h = cpu_hip()
+    q, k = torch.zeros(1, 1, 64).expand(1, 1 << 20, 64), torch.zeros(1, 1, 64).expand(1, 1 << 18, 64)
+    cases = [((q, k, k, 2), {"mask": torch.ones(1, 1, 1, dtype=torch.bool).expand(1, 1 << 20, 1 << 18)}),
+             ((q[:, :4], k[:, :4], k[:, :4], 2), {"scale": 2.1e38}),
+             ((torch.zeros(1, 1, 64).expand(1 << 16, 1, 64), *[torch.zeros(1, 1, 64).expand(1 << 16, 1, 64)] * 2, 1), {})]
+    for args, kw in cases:
+        with pytest.raises(Unsupported):
+            h.cross_attention(*args, **kw)
+
+
 def test_nothing_to_attend_or_to_ask_cpu():
     h = cpu_hip()
     assert h.cross_attention(torch.zeros(2, 0, 64), torch.zeros(2, 3, 64), torch.zeros(2, 3, 64), 4).shape == (2, 0, 64)
@@ -303,6 +314,139 @@ def test_repeatable_streams_and_graph(lq, lk, hips, gpu_device):
         eager = hip.cross_attention(*b, 4, 2, mask)
         torch.cuda.synchronize()
         assert torch.equal(y, ref[(i // 2) % 2]) and torch.equal(eager, ref[1]), i
+
+
+# whole keys of an image in LDS at its limit, the widest heads
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("n,lq,lk,heads,kv_heads,d", [(1, 40, 128, 2, 2, 128), (2, 300, 127, 2, 1, 128), (1, 700, 100, 1, 1, 96),
+                                                      (1, 5000, 128, 3, 3, 64), (3, 1, 128, 16, 2, 120)])
+def test_keys_that_fit(n, lq, lk, heads, kv_heads, d, dt, hips, gpu_device):
+    q, k, v = inputs(n, lq, lk, heads, kv_heads, d, dt, gpu_device, seed=lk)
+    for kind in ("none", "keys", "pairs"):
+        mask = make_mask(kind, n, lq, lk, gpu_device)
+        print(f"[xa] {n} {lq} {lk} {heads} {kv_heads} {d} {kind} {dt}", flush=True)
+        check(hips[dt].cross_attention(q, k, v, heads, kv_heads, mask), q, k, v, heads, kv_heads, mask, what=kind)
+
+
+def stretches(what, lq, lk, dev):
+    """Masks over thousands of keys in one pass: stretches of whole tiles that nothing keeps."""
+    key, row = torch.arange(lk, device=dev), torch.arange(lq, device=dev)[:, None]
+    if what == "none":
+        return None
+    if what == "last keys":
+        return (key >= lk - 150)[None]
+    if what == "both ends":
+        return ((key < 70) | (key >= lk - 37))[None]
+    if what == "one key":
+        return (key == lk - 1)[None]
+    if what == "no key":
+        return (key < 0)[None]
+    if what == "bands":  # each row its own 90 keys, every seventh none
+        return ((key - row * (lk - 90) // lq).clamp(-1, 90).remainder(90) > 0)[None] & (row % 7 != 3)[None]
+    if what == "late rows":  # only the last rows keep anything, and only the last keys
+        return ((row >= lq - 50) & (key >= lk - 200))[None]
+    return ((key < 40) | (key >= lk - 33) | (key // 500 == row // 400))[None]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("what", ["none", "last keys", "both ends", "one key", "no key", "bands", "late rows", "regions"])
+def test_long_passes(what, dt, hips, gpu_device):
+    """Enough rows that no split happens, more keys than 64 tiles (4096 in bf16, 2048 in fp32)."""
+    lq, lk, heads, d = 3105, 4501, 8, 32
+    q, k, v = inputs(1, lq, lk, heads, heads, d, dt, gpu_device, seed=11)
+    mask = stretches(what, lq, lk, gpu_device)
+    print(f"[xa] {what} {dt}", flush=True)
+    got = hips[dt].cross_attention(q, k, v, heads, mask=mask)
+    assert "xa_kernel" in _lib.last_kernel() and "splits=1" in _lib.last_kernel()
+    check(got, q, k, v, heads, mask=mask, what=what)
+    if mask is not None:
+        assert not got[:, ~mask.expand(1, lq, lk)[0].any(-1) if mask.dim() == 3 else slice(0, 0 if mask.any() else lq)].any()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("lq", [54, 26000])
+def test_layouts_of_long_keys(lq, dt, hips, gpu_device):
+    """Masks and keys with strides where the keys stream by, split (54 queries) and whole."""
+    g = torch.Generator().manual_seed(4)
+    hip, heads, d, lk = hips[dt], 2, 32, 9 * 37
+    c = heads * d
+    q = torch.randn(2, lq // 2, 2, 3 * c, generator=g).to(dt).to(gpu_device)[..., c:2 * c]
+    kv = torch.randn(2, 9, 37, 2 * c + 8, generator=g).to(dt).to(gpu_device)
+    k, v = kv[..., :c], kv[..., c:2 * c]
+    ctx = torch.randn(1, lk, 2 * c, generator=g).to(dt).to(gpu_device).expand(2, lk, 2 * c)
+    few = torch.rand(4, 7, 380, generator=g).to(gpu_device) < 0.6
+    big = torch.rand(3, lq + 3, 341, generator=g).to(gpu_device) < 0.4
+    for what, args, mask in (
+            ("keys", (q, k, v), None),
+            ("unaligned keys", (q, k, v), few[::2, 0, 5:5 + lk]),
+            ("one row for both images", (q, ctx[..., :c], ctx[..., c:]), few[:1, 3, 7:7 + lk].expand(2, lk)),
+            ("pair slice", (q, k, v), big[1:, 3:, 3:3 + lk]),
+            ("pairs of both images", (q, k, v), big[:1, 1:lq + 1, 8:8 + lk].expand(2, lq, lk)),
+            ("pairs of all queries", (q, k, v), few[2:, 6:, 1:1 + lk].expand(2, lq, lk)),
+            ("pairs of everything", (q, k, v), few[:1, :1, 47:47 + lk].expand(2, lq, lk))):
+        print(f"[xa] {what} {lq} {dt}", flush=True)
+        got = hip.cross_attention(*args, heads, mask=mask)
+        assert ("splits=1" in _lib.last_kernel()) == (lq > 54)
+        check(got, *args, heads, mask=mask, what=what)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("lk", [50, 130, 2000])
+def test_any_byte_but_zero_keeps(lk, hips, gpu_device):
+    q, k, v = inputs(2, 20, lk, 2, 2, 32, torch.bfloat16, gpu_device)
+    byte = torch.randint(0, 256, (2, 20, lk), generator=torch.Generator().manual_seed(6), dtype=torch.uint8).to(gpu_device)
+    byte[..., ::3] = 0
+    for b in (byte, byte[:, 0].contiguous()):
+        got = hips[torch.bfloat16].cross_attention(q, k, v, 2, mask=b.view(torch.bool))
+        assert torch.equal(got, hips[torch.bfloat16].cross_attention(q, k, v, 2, mask=b != 0))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("lq,lk", [(150, 900), (40, 60)])
+def test_pair_masks_on_streams_and_in_graphs(lq, lk, hips, gpu_device):
+    """Each call's bits of its mask are its own: two streams at once, two graphs in turn, eager calls between."""
+    hip = hips[torch.bfloat16]
+    q, k, v = inputs(2, lq, lk, 4, 2, 64, torch.bfloat16, gpu_device)
+    masks = [make_mask("pairs", 2, lq, lk, gpu_device, seed=s) for s in (1, 2)]
+    ref = [hip.cross_attention(q, k, v, 4, 2, m) for m in masks]
+    assert not torch.equal(*ref)
+    torch.cuda.synchronize()
+    s = torch.cuda.Stream(), torch.cuda.Stream()
+    outs = []
+    for _ in range(4):
+        for i in range(2):
+            with torch.cuda.stream(s[i]):
+                outs.append(hip.cross_attention(q, k, v, 4, 2, masks[i]))
+    torch.cuda.synchronize()
+    assert all(torch.equal(o, ref[i % 2]) for i, o in enumerate(outs))
+    made = []
+    for m in masks:
+        st = m.clone()
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            y = hip.cross_attention(q, k, v, 4, 2, st)
+        made.append((graph, st, y))
+    for i in range(6):
+        graph, st, y = made[i % 2]
+        st.copy_(masks[(i // 2) % 2])
+        graph.replay()
+        eager = hip.cross_attention(q, k, v, 4, 2, masks[1])
+        torch.cuda.synchronize()
+        assert torch.equal(y, ref[(i // 2) % 2]) and torch.equal(eager, ref[1]), i
+
+
+@pytest.mark.gpu
+def test_a_scale_is_read_with_every_call(hips, gpu_device):
+    q, k, v = inputs(1, 30, 40, 2, 2, 32, torch.float32, gpu_device)
+    scale = torch.tensor(0.25)
+    for value in (0.25, 0.5):
+        scale.fill_(value)
+        got = hips[torch.float32].cross_attention(q, k, v, 2, scale=scale)
+        check(got, q, k, v, 2, scale=value)
 
 
 @pytest.mark.gpu
