@@ -44,6 +44,7 @@ struct GroupNormP {
   int64_t schunk;    // pixels per statistics chunk
   int64_t wbs, bbs;
   int c, groups, cg, nchunk;
+  int n, strips;     // images, strips of channels (small)
   int tr, rpb;       // threads per row (octets of a strip), rows per pass of a workgroup
   int lpg;           // lanes that join a group: a power of two <= 64
   int act;
@@ -342,8 +343,13 @@ __global__ void __launch_bounds__(GN_TS) gn_small_kernel(const GroupNormP p) {
   __shared__ float stat[2][GN_UNIT];
   const int tid = threadIdx.x, sub = tid & (p.lpg - 1);
   const int rl = tid / p.tr, oct = tid - rl * p.tr;
-  const int64_t n = blockIdx.z;
-  const int s0 = blockIdx.y * p.tr * 8, c0 = s0 + oct * 8, P = (int)p.p;
+  // neighbouring strips share the lines of a row: they run on one XCD, one after the other, whose L2 joins them (64
+  // images of 2048 pixels, 512 channels, 64 groups, bf16: 71 us; dealt out over the XCDs 256)
+  const unsigned strips = (unsigned)p.strips, total_wg = strips * (unsigned)p.n, span = (total_wg + 7) >> 3;
+  const unsigned id = (blockIdx.x & 7) * span + (blockIdx.x >> 3);
+  if ((blockIdx.x >> 3) >= span || id >= total_wg) return;
+  const int64_t n = id / strips;
+  const int s0 = (int)(id - (unsigned)n * strips) * p.tr * 8, c0 = s0 + oct * 8, P = (int)p.p;
   const bool act = rl < p.rpb && c0 < p.c;
   const int sgroups = min(p.tr * 8, p.c - s0) / p.cg;
   const int units = p.cg / PER;
@@ -430,8 +436,9 @@ GnPlan gn_plan(int64_t n, int64_t p, int64_t c, int64_t groups) {
   GnPlan g{};
   const int64_t u = gn_unit(c / groups) / 8;  // octets a workgroup has to hold together
   // One launch where a unit's pixels are at most NRMAX rows per thread of one workgroup: past that few workgroups with
-  // long chains of loads lose to the three launches over the whole chip (us, one / three launches: 16 x 24 x 512 at 3
-  // rows 5.6 / 9; 32 x 48 x 512 at 12 rows 10.8 / 9.5; 64 x 64 x 128 at 16 rows 16.5 / 10.7)
+  // long chains of loads lose to the three launches over the whole chip (us, one / three launches, bf16, 32 groups: 500
+  // pixels of 512 channels at 4 rows 6.0 / 9.5, 1024 at 8 rows 7.8 / 9.4, 1536 at 12 rows 10.4 / 9.4, 2048 at 16 rows
+  // 11.9 / 9.4; 64 images of the first 18.6 / 24.6, of the second 30.3 / 37.4, of the last 63.5 / 67.3)
   g.small = p <= (int64_t)(GN_TS / u) * NRMAX;
   if (g.small) {
     g.tr = (int)u;
@@ -502,7 +509,8 @@ extern "C" int clarus_hip_group_norm(const void* x, int32_t x_dtype, int64_t x_b
   k.lpg = gn_lanes(sgroups, k.rpb, g.small ? GN_TS : GN_TT);
   if (g.small) {
     const int nr = (int)cdiv(p, k.rpb);
-    const dim3 grid(1, (unsigned)g.strips, (unsigned)n);
+    k.n = (int)n; k.strips = g.strips;
+    const dim3 grid((unsigned)(8 * cdiv(g.strips * n, 8)));
     note_kernel("gn_small_kernel strips=%d rows=%d", g.strips, nr);
 #define CLARUS_GN_S(DT, ODT, W)                                                                                  \
   do {                                                                                                           \
