@@ -45,6 +45,7 @@ struct GroupNormP {
   int64_t wbs, bbs;
   int c, groups, cg, nchunk;
   int n, strips;     // images, strips of channels (small)
+  int chunks;        // chunks of this launch
   int tr, rpb;       // threads per row (octets of a strip), rows per pass of a workgroup
   int lpg;           // lanes that join a group: a power of two <= 64
   int act;
@@ -72,6 +73,13 @@ __device__ __forceinline__ float lanes_sum(float v, int lpg) {
   return v;
 }
 
+// The chunk of pixels of this workgroup, -1 past the last: the chunks in equal parts over the XCDs, in order. The apply
+// pass then finds in its L2 what the statistics pass of the same part has read
+__device__ __forceinline__ int gn_chunk(int chunks) {
+  const int span = (chunks + 7) >> 3, i = blockIdx.x >> 3, c = (blockIdx.x & 7) * span + i;
+  return i < span && c < chunks ? c : -1;
+}
+
 // f(group) on the lpg consecutive threads of each of ng groups at a time, every lane of a wave in step
 template <int T, class F>
 __device__ __forceinline__ void for_groups(int ng, int lpg, F&& f) {
@@ -87,7 +95,9 @@ __global__ void __launch_bounds__(GN_TT) gn_stats_kernel(const GroupNormP p) {
   __shared__ float sm[GN_TT * NA], s2[GN_TT * NA];
   const int tid = threadIdx.x;
   const int rl = tid / p.tr, oct = tid - rl * p.tr;
-  const int64_t n = blockIdx.z, r0 = (int64_t)blockIdx.x * p.chunk;
+  const int at_chunk = gn_chunk(p.chunks);
+  if (at_chunk < 0) return;
+  const int64_t n = blockIdx.z, r0 = (int64_t)at_chunk * p.chunk;
   const int rows = (int)((r0 + p.chunk < p.p ? r0 + p.chunk : p.p) - r0);
   const int c0 = blockIdx.y * p.tr * 8;  // first channel of the strip
   const bool act = rl < p.rpb && c0 + oct * 8 < p.c;
@@ -181,7 +191,7 @@ __global__ void __launch_bounds__(GN_TT) gn_stats_kernel(const GroupNormP p) {
       }
     }
     q = lanes_sum(q, p.lpg);
-    if (mine && sub == 0) p.part[(n * p.groups + c0 / p.cg + g) * p.nchunk + blockIdx.x] = float2{mu, q};
+    if (mine && sub == 0) p.part[(n * p.groups + c0 / p.cg + g) * p.nchunk + at_chunk] = float2{mu, q};
   });
 }
 
@@ -289,7 +299,9 @@ __global__ void __launch_bounds__(GN_T) gn_apply_kernel(const GroupNormP p) {
   const int64_t n = blockIdx.z;
   const int rl = tid / p.tr, oct = tid - rl * p.tr, c0 = (blockIdx.y * p.tr + oct) * 8;
   const bool act = rl < p.rpb && c0 < p.c;
-  const int64_t r0 = (int64_t)blockIdx.x * p.chunk;
+  const int at_chunk = gn_chunk(p.chunks);
+  if (at_chunk < 0) return;
+  const int64_t r0 = (int64_t)at_chunk * p.chunk;
   const int rows = (int)((r0 + p.chunk < p.p ? r0 + p.chunk : p.p) - r0);
   const int64_t xb = n * p.xbs + r0 * p.ldx + c0, ob = (n * p.p + r0) * p.c + c0;
   // the first rows are on their way before the statistics and the affine are asked for
@@ -534,7 +546,8 @@ extern "C" int clarus_hip_group_norm(const void* x, int32_t x_dtype, int64_t x_b
     return check_launch("group_norm");
   }
   k.chunk = g.schunk;
-  const dim3 sgrid((unsigned)g.nchunk, (unsigned)g.strips, (unsigned)n);
+  k.chunks = g.nchunk;
+  const dim3 sgrid((unsigned)(8 * cdiv(g.nchunk, 8)), (unsigned)g.strips, (unsigned)n);
   note_kernel("gn_stats_kernel + gn_apply_kernel nchunk=%d strips=%d", g.nchunk, g.strips);
   if (x_dtype == DT_BF16) {
     if (whole) hipLaunchKernelGGL((gn_stats_kernel<DT_BF16, true>), sgrid, dim3(GN_TT), 0, st, k);
@@ -545,8 +558,9 @@ extern "C" int clarus_hip_group_norm(const void* x, int32_t x_dtype, int64_t x_b
   }
   hipLaunchKernelGGL(gn_join_kernel, dim3((unsigned)groups, (unsigned)n), dim3(64), 0, st, k);
   k.chunk = g.achunk;
+  k.chunks = (int)cdiv(p, g.achunk);
   k.rpb = GN_T / g.tr;
-  const dim3 grid((unsigned)cdiv(p, g.achunk), (unsigned)g.strips, (unsigned)n);
+  const dim3 grid((unsigned)(8 * cdiv(k.chunks, 8)), (unsigned)g.strips, (unsigned)n);
 #define CLARUS_GN_A(DT, ODT, ACT)                                                                      \
   do {                                                                                                 \
     if (whole) hipLaunchKernelGGL((gn_apply_kernel<DT, ODT, ACT, true>), grid, dim3(GN_T), 0, st, k);  \
