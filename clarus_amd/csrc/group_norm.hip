@@ -73,10 +73,12 @@ __device__ __forceinline__ float lanes_sum(float v, int lpg) {
   return v;
 }
 
-// The chunk of pixels of this workgroup, -1 past the last: the chunks in equal parts over the XCDs, in order. The apply
-// pass then finds in its L2 what the statistics pass of the same part has read
+// The chunk of pixels of this workgroup, -1 past the last: the chunks in equal parts over the XCDs, in order, BACK: the
+// last first. The apply pass goes back over the part that the statistics pass of its XCD has read, whose end is still in
+// that L2 (90 x 160 x 512 bf16 15.6 us dealt out, 14.2 in parts; 2 x 173 x 251 x 128 fp32 29.1, 28.1 in parts, 26.7 back)
+template <bool BACK>
 __device__ __forceinline__ int gn_chunk(int chunks) {
-  const int span = (chunks + 7) >> 3, i = blockIdx.x >> 3, c = (blockIdx.x & 7) * span + i;
+  const int span = (chunks + 7) >> 3, i = blockIdx.x >> 3, c = (blockIdx.x & 7) * span + (BACK ? span - 1 - i : i);
   return i < span && c < chunks ? c : -1;
 }
 
@@ -95,7 +97,7 @@ __global__ void __launch_bounds__(GN_TT) gn_stats_kernel(const GroupNormP p) {
   __shared__ float sm[GN_TT * NA], s2[GN_TT * NA];
   const int tid = threadIdx.x;
   const int rl = tid / p.tr, oct = tid - rl * p.tr;
-  const int at_chunk = gn_chunk(p.chunks);
+  const int at_chunk = gn_chunk<false>(p.chunks);
   if (at_chunk < 0) return;
   const int64_t n = blockIdx.z, r0 = (int64_t)at_chunk * p.chunk;
   const int rows = (int)((r0 + p.chunk < p.p ? r0 + p.chunk : p.p) - r0);
@@ -296,10 +298,10 @@ __device__ __forceinline__ void gn_affine(const GroupNormP& p, int64_t n, int c,
 template <int DT, int ODT, int ACT, bool WHOLE>
 __global__ void __launch_bounds__(GN_T) gn_apply_kernel(const GroupNormP p) {
   const int tid = threadIdx.x;
-  const int64_t n = blockIdx.z;
+  const int64_t n = gridDim.z - 1 - blockIdx.z;
   const int rl = tid / p.tr, oct = tid - rl * p.tr, c0 = (blockIdx.y * p.tr + oct) * 8;
   const bool act = rl < p.rpb && c0 < p.c;
-  const int at_chunk = gn_chunk(p.chunks);
+  const int at_chunk = gn_chunk<true>(p.chunks);
   if (at_chunk < 0) return;
   const int64_t r0 = (int64_t)at_chunk * p.chunk;
   const int rows = (int)((r0 + p.chunk < p.p ? r0 + p.chunk : p.p) - r0);
