@@ -27,7 +27,7 @@
 //   keys, 4 heads of 128, MFMAs are busy 414k and the VALU 412k of 825k cycles, at a clock that the load lowers to
 //   1.7 GHz: 477 us, 890 TFLOP/s (a large library product reaches 1190). 14400 x 3600, 8 heads of 64, twice the
 //   arithmetic per product: 145 us, 731 TFLOP/s.
-//   A prompt (57600 x 77, 4 heads of 64): 12 us of reading q and writing o at the rate of a large copy; 21 us, a wave
+//   A prompt (57600 x 77, 4 heads of 64): 12 us of reading q and writing o at the rate of a large copy; 19 us, a wave
 //   loading, multiplying and weighing its few keys in turn.
 //   One query of 8 images x 30001 keys: reading K and V, 492 MB in 95 us, 5.2 TB/s (a large copy: 4.8 TB/s).
 #include "capi.hpp"
@@ -136,7 +136,11 @@ __device__ __forceinline__ void xa_load_q(const CrossP& p, int64_t n, const XaRo
   for (int s = 0; s < T::QN; ++s) {
     const int at = (2 * s + hl) * E;
     qf[s] = *reinterpret_cast<const u32x4*>(qp + (at < p.d ? at : 0) * T::ES);
-    if (at >= p.d) qf[s] = u32x4{0, 0, 0, 0};
+  }
+  if (p.d < D) {
+#pragma unroll
+    for (int s = 0; s < T::QN; ++s)
+      if ((2 * s + hl) * E >= p.d) qf[s] = u32x4{0, 0, 0, 0};
   }
 }
 
@@ -161,10 +165,10 @@ __device__ __forceinline__ unsigned xa_bits16(const unsigned char* p, int64_t le
 }
 
 // One tile of NB x 32 keys for a wave's 32 rows: S^T = K Q^T, the softmax's step, O^T += V^T P^T. bits: the keys that
-// count, of a lane's row under MASK_PAIRS.
+// count, of a lane's row under MASK_PAIRS; fresh: o is still 0
 template <int DT, int D, int MASK, int NB, bool ANEW>
 __device__ __forceinline__ void xa_tile(const unsigned char* ks, const unsigned char* vs, const u32x4 (&qf)[XaTile<DT, D>::QN],
-                                        f32x16 (&o)[D / 32], float& m, float& l, float c, uint64_t bits, bool whole) {
+                                        f32x16 (&o)[D / 32], float& m, float& l, float c, uint64_t bits, bool whole, bool fresh) {
   using T = XaTile<DT, D>;
   constexpr int DB = D / 32, QN = T::QN;
   // ANEW: the lane's LDS offsets are worked out for each tile instead of kept over the loop, where they spill
@@ -210,10 +214,12 @@ __device__ __forceinline__ void xa_tile(const unsigned char* ks, const unsigned 
     const float alpha = __builtin_amdgcn_exp2f(m - mn);
     m = mn;
     l *= alpha;
+    if (!fresh) {
 #pragma unroll
-    for (int b = 0; b < DB; ++b)
+      for (int b = 0; b < DB; ++b)
 #pragma unroll
-      for (int j = 0; j < 16; ++j) o[b][j] *= alpha;
+        for (int j = 0; j < 16; ++j) o[b][j] *= alpha;
+    }
   }
 #pragma unroll
   for (int b = 0; b < NB; ++b)
@@ -260,7 +266,7 @@ __device__ __forceinline__ void xa_tile(const unsigned char* ks, const unsigned 
 template <int D>
 __device__ __forceinline__ void xa_store(const CrossP& p, int64_t n, const XaRow& r, const f32x16 (&o)[D / 32], float l, bool live) {
   const int hl = (threadIdx.x >> 5) & 1;
-  const float inv = l == 0.f ? 0.f : 1.f / l;
+  const float inv = l == 0.f ? 0.f : __builtin_amdgcn_rcpf(l);
   const int64_t at = ((n * p.lq + r.qi) * (int64_t)(p.kv_heads * p.rep) + r.head) * p.d;
 #pragma unroll
   for (int b = 0; b < D / 32; ++b)
@@ -428,6 +434,7 @@ __global__ void __launch_bounds__(XR_T, (DT == DT_BF16 ? D <= 64 : D <= 32) ? 4 
 #pragma unroll
       for (int j = 0; j < 16; ++j) o[b][j] = 0.f;
     float m = XA_FLOOR, l = 0.f;
+    bool fresh = true;  // o is 0
     // 32 keys at a time (a row of 32 keys starts where the swizzles do), half of a tile in bf16
 #pragma unroll 1
     for (int h = 0; h < lk; h += 32) {
@@ -444,7 +451,8 @@ __global__ void __launch_bounds__(XR_T, (DT == DT_BF16 ? D <= 64 : D <= 32) ? 4 
       } else if (!bits) {
         continue;
       }
-      xa_tile<DT, D, MASK, 1, true>(ks, ks + T::BYTES, qf, o, m, l, p.c, bits, bits == 0xffffffffu);
+      xa_tile<DT, D, MASK, 1, true>(ks, ks + T::BYTES, qf, o, m, l, p.c, bits, bits == 0xffffffffu, fresh);
+      fresh = false;
     }
     l = sum32(l);
     xa_store<D>(p, n, r, o, l, ch * 32ll + col < p.rows);
@@ -567,7 +575,7 @@ __global__ void __launch_bounds__(XA_T, D <= 64 ? (MASK == MASK_PAIRS ? 3 : 4) :
         if constexpr (MASK == MASK_PAIRS) next = words[t1];
       }
       if (busy && (MASK != MASK_PAIRS || (mine >> (t - c0) & 1)))
-        xa_tile<DT, D, MASK, KB, false>(tiles[buf], tiles[buf] + T::BYTES, qf, o, m, l, p.c, now, now == T::ALL);
+        xa_tile<DT, D, MASK, KB, false>(tiles[buf], tiles[buf] + T::BYTES, qf, o, m, l, p.c, now, now == T::ALL, false);
       t = t1;
       t1 = t2;
       buf ^= 1;
