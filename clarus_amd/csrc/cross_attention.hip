@@ -30,6 +30,8 @@
 //   A prompt (57600 x 77, 4 heads of 64): 12 us of reading q and writing o at the rate of a large copy; 19 us, a wave
 //   loading, multiplying and weighing its few keys in turn.
 //   One query of 8 images x 30001 keys: reading K and V, 492 MB in 95 us, 5.2 TB/s (a large copy: 4.8 TB/s).
+#include <algorithm>
+
 #include "capi.hpp"
 #include "common.hpp"
 
@@ -683,7 +685,26 @@ __global__ void __launch_bounds__(XA_T) xa_join_kernel(const CrossP p, int gs) {
 
 int xa_pad(int64_t d) { return d <= 32 ? 32 : d <= 64 ? 64 : d <= 96 ? 96 : 128; }
 
-constexpr int XA_LEAST = 4;
+// Into how many parts the keys are split: as many as make the time of a part's tiles in a row and, with more than one
+// part, of writing and joining the parts least; at most two workgroups per CU. The constants are measured (us): a tile
+// 0.73 / 0.96 / 1.4 with heads of 32 / 64 / 128, fp32 1.2 / 2.25 / 4.3; a second workgroup on a CU adds a quarter of
+// that, in fp32, where the matrix core is the bound, 0.8; parts 2.8 and, a MB of one part, 0.56 + 0.3 for each. What it
+// decides, in one / the chosen / more parts (us, bf16): one query, 8 heads of 64, 400 keys 9.6 / 7.6 (7); 8 x 256 queries,
+// 8 heads of 40, 400 keys 11.2 / - / 15.8 (2), 1600 keys 30.7 / 21.8 (4); 900 queries, 8 heads of 64, 800 keys 16.3 / 14.7
+// (4); 2 x 3600 queries, 4 heads of 64, 1000 keys 18.7 / - / 28.0 (2). One query of 8 images, 16 heads on 4 of 128, 30001
+// keys: 119 in 8 parts, 94 in 16 (two workgroups per CU), 107 in 24
+int64_t xa_splits(int32_t dt, int64_t blocks, int64_t rows, int64_t tiles, int D) {
+  const int64_t cus = device_cus(), most = std::min(tiles, std::max<int64_t>(2 * cus / blocks, 1));
+  const double tile = dt == DT_BF16 ? 0.5 + 0.0072 * D : 0.2 + 0.032 * D, share = dt == DT_BF16 ? 0.25 : 0.8;
+  const double mb = 1e-6 * (double)rows * (D + 2) * sizeof(float);
+  int64_t best = 1;
+  double least = 1e30;
+  for (int64_t s = 1; s <= most; ++s) {
+    const double t = cdiv(tiles, s) * tile * (1 + share * (cdiv(blocks * s, cus) - 1)) + (s > 1 ? 2.8 + mb * (0.56 + 0.3 * s) : 0.0);
+    if (t < least) least = t, best = s;
+  }
+  return best;
+}
 
 struct XaPlan {
   bool resident;
@@ -706,15 +727,7 @@ XaPlan xa_plan(int32_t dt, int64_t n, int64_t lq, int64_t lk, int64_t heads, int
   }
   g.nblk = cdiv(rows, XA_ROWS);
   const int64_t blocks = g.nblk * nk;
-  // Split the keys where the row blocks leave a quarter of the CUs or more idle: two workgroups per CU, XA_LEAST tiles
-  // or more each. Writing and joining the parts costs about 10 us at thousands of rows (2 x 3600 queries, 1000 keys, 4
-  // heads of 64, 232 blocks: 18.7 us whole, 28.0 in two parts; 1 x 3600 x 3600, 116 blocks: 35 in two, 32.8 in four; one
-  // query of 8 images x 30001 keys, 32 blocks: 119 in eight, 94 in sixteen, 107 in twenty-four)
-  int64_t want = 4 * blocks < 3LL * device_cus() ? 2LL * device_cus() / blocks : 1;
-  const int64_t most = cdiv(lk, XA_LEAST * kt);
-  if (want > most) want = most;
-  if (want < 1) want = 1;
-  g.split_len = cdiv(cdiv(lk, want), kt) * kt;
+  g.split_len = cdiv(cdiv(lk, xa_splits(dt, blocks, nk * rows, cdiv(lk, kt), D)), kt) * kt;
   g.splits = (int)cdiv(lk, g.split_len);
   if (mask == MASK_PAIRS) g.bits = (size_t)(n * lq * cdiv(lk, 64) + 1) / 2 * 16;
   if (g.splits > 1) g.part = (size_t)g.splits * nk * rows * (D + 2) * sizeof(float);

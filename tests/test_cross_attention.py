@@ -354,12 +354,12 @@ def stretches(what, lq, lk, dev):
 @pytest.mark.parametrize("what", ["none", "last keys", "both ends", "one key", "no key", "bands", "late rows", "regions"])
 def test_long_passes(what, dt, hips, gpu_device):
     """Enough rows that no split happens, more keys than 64 tiles (4096 in bf16, 2048 in fp32)."""
-    lq, lk, heads, d = 3105, 4501, 8, 32
+    lq, lk, heads, d = 4205, 4501, 8, 32
     q, k, v = inputs(1, lq, lk, heads, heads, d, dt, gpu_device, seed=11)
     mask = stretches(what, lq, lk, gpu_device)
     print(f"[xa] {what} {dt}", flush=True)
     got = hips[dt].cross_attention(q, k, v, heads, mask=mask)
-    assert "xa_kernel" in _lib.last_kernel() and "splits=1" in _lib.last_kernel()
+    assert "xa_kernel" in _lib.last_kernel() and _lib.last_kernel().endswith("splits=1")
     check(got, q, k, v, heads, mask=mask, what=what)
     if mask is not None:
         assert not got[:, ~mask.expand(1, lq, lk)[0].any(-1) if mask.dim() == 3 else slice(0, 0 if mask.any() else lq)].any()
@@ -389,7 +389,7 @@ def test_layouts_of_long_keys(lq, dt, hips, gpu_device):
             ("pairs of everything", (q, k, v), few[:1, :1, 47:47 + lk].expand(2, lq, lk))):
         print(f"[xa] {what} {lq} {dt}", flush=True)
         got = hip.cross_attention(*args, heads, mask=mask)
-        assert ("splits=1" in _lib.last_kernel()) == (lq > 54)
+        assert _lib.last_kernel().endswith("splits=1") == (lq > 54)
         check(got, *args, heads, mask=mask, what=what)
 
 
