@@ -12,8 +12,8 @@
 //                     float per lane), so P moves through no LDS
 // K and V go from memory straight to LDS, 16 bytes a lane, without passing through registers.
 //   xa_resident_kernel  up to XR_KEYS keys: all of them stay in LDS, rows stream by
-//   xa_kernel           any number of keys: 128 rows (4 waves) per workgroup, tiles of 64 (fp32: 32) keys, the
-//                       next one on its way during the current one's products
+//   xa_kernel           any number of keys: 128 or 256 rows (4 or 8 waves) per workgroup, tiles of 64 (fp32: 32)
+//                       keys, the next one on its way during the current one's products
 //   xa_join_kernel      joins the (O, m, l) of keys split over workgroups, where rows are few
 //   xa_bits_kernel      a mask of pairs as bits
 // m, l and O are fp32. bf16: products of bf16 q, k, v are exact in fp32; P is rounded once to bf16 for
@@ -23,13 +23,13 @@
 // keys, the end of the keys) its V row is taken as 0.
 //
 // What bounds it (bf16, the GPU's time alone, without the call's).
-//   Many rows and keys: the matrix cores and the softmax's arithmetic, which take turns: at 57600 queries x 3600
-//   keys, 4 heads of 128, MFMAs are busy 414k and the VALU 412k of 825k cycles, at a clock that the load lowers to
-//   1.7 GHz: 477 us, 890 TFLOP/s (a large library product reaches 1190). 14400 x 3600, 8 heads of 64, twice the
-//   arithmetic per product: 145 us, 731 TFLOP/s.
+//   Many rows and keys: the softmax's arithmetic and the matrix cores, which overlap in part. 14400 queries x 3600 keys, 8
+//   heads of 64: 126 us, 838 TFLOP/s (a large library product reaches 1190); 57600 x 3600, 4 heads of 128: 466 us, 910.
+//   With four waves per workgroup the first took 141 us at 1.86 GHz, the VALU busy for 64% of the cycles (an exponential
+//   counts twice), the matrix cores for 40%; the second has them at 44% and 47%.
 //   A prompt (57600 x 77, 4 heads of 64): 12 us of reading q and writing o at the rate of a large copy; 19 us, a wave
-//   loading, multiplying and weighing its few keys in turn.
-//   One query of 8 images x 30001 keys: reading K and V, 492 MB in 95 us, 5.2 TB/s (a large copy: 4.8 TB/s).
+//   loading, multiplying and weighing its few keys in turn: the VALU is busy for 62% of the cycles.
+//   One query of 8 images x 30001 keys: reading K and V, 492 MB in 94 us, 5.2 TB/s (a large copy: 4.8 TB/s).
 #include <algorithm>
 
 #include "capi.hpp"
@@ -42,8 +42,7 @@ namespace {
 typedef __attribute__((ext_vector_type(16))) float f32x16;
 typedef __attribute__((ext_vector_type(4))) short s16x4;
 
-constexpr int XA_T = 256;    // threads
-constexpr int XA_ROWS = 128; // rows of a workgroup
+constexpr int XA_T = 256;    // threads of a join or bits workgroup
 constexpr float XA_FLOOR = -3e38f;  // running maximum before any key: exp2(-inf - XA_FLOOR) = 0, no inf - inf
 constexpr float XA_SLACK = 8.f;     // a running maximum may lag the scores' by this (log2)
 
@@ -468,12 +467,13 @@ __global__ void __launch_bounds__(XR_T, (DT == DT_BF16 ? D <= 64 : D <= 32) ? 4 
 }
 
 // ---------------------------------------------------------------- keys streamed through LDS
-template <int DT, int D, int MASK>
-__global__ void __launch_bounds__(XA_T, D <= 64 ? (MASK == MASK_PAIRS ? 3 : 4) : 2) xa_kernel(const CrossP p) {
+// W waves of 32 rows. (MASK_PAIRS at 3 waves per SIMD: it spills at 4.)
+template <int DT, int D, int MASK, int W>
+__global__ void __launch_bounds__(64 * W, D <= 64 ? (MASK == MASK_PAIRS ? 3 : 4) : 2) xa_kernel(const CrossP p) {
   using T = XaTile<DT, D>;
   constexpr int KT = T::KT, KB = KT / 32, DB = D / 32;
   __shared__ __align__(16) unsigned char tiles[2][2 * T::BYTES];
-  __shared__ uint64_t wants[MASK == MASK_PAIRS ? XA_T / 64 : 1];
+  __shared__ uint64_t wants[MASK == MASK_PAIRS ? W : 1];
 
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int col = lane & 31, hl = lane >> 5;
@@ -496,7 +496,7 @@ __global__ void __launch_bounds__(XA_T, D <= 64 ? (MASK == MASK_PAIRS ? 3 : 4) :
   const unsigned split = rest / (unsigned)p.nblk, rb = rest - split * (unsigned)p.nblk;
   const int n = (int)nk / p.kv_heads, kvh = (int)nk - n * p.kv_heads;
 
-  const int64_t wrow = (int64_t)rb * XA_ROWS + wave * 32;  // the wave's first row
+  const int64_t wrow = (int64_t)rb * (32 * W) + wave * 32;  // the wave's first row
   const bool busy = wrow < p.rows;
   const int64_t row = wrow + col < p.rows ? wrow + col : p.rows - 1;  // rows past the end repeat the last one
   const XaRow r = xa_row(p, kvh, row);
@@ -511,7 +511,7 @@ __global__ void __launch_bounds__(XA_T, D <= 64 ? (MASK == MASK_PAIRS ? 3 : 4) :
   const int64_t k0 = (int64_t)split * p.split_len, k1 = k0 + p.split_len < p.lk ? k0 + p.split_len : p.lk;
   const int ntile = (int)((k1 - k0 + KT - 1) / KT);
 
-  const XaCopy<DT, D, XA_T / 64> copy(p, wave, lane);
+  const XaCopy<DT, D, W> copy(p, wave, lane);
   auto key_byte = [&](int t) __attribute__((always_inline)) {  // 0 for t < 0
     return t < 0 ? 0 : xa_key_byte<KT, MASK>(mkey, k0 + (int64_t)t * KT, k1, lane);
   };
@@ -552,7 +552,7 @@ __global__ void __launch_bounds__(XA_T, D <= 64 ? (MASK == MASK_PAIRS ? 3 : 4) :
       __syncthreads();
       want = 0;
 #pragma unroll
-      for (int w = 0; w < XA_T / 64; ++w) want |= wants[w];
+      for (int w = 0; w < W; ++w) want |= wants[w];
       want = (uint64_t)(unsigned)__builtin_amdgcn_readfirstlane((unsigned)(want >> 32)) << 32 |
              (unsigned)__builtin_amdgcn_readfirstlane((unsigned)want);
     }
@@ -706,10 +706,21 @@ int64_t xa_splits(int32_t dt, int64_t blocks, int64_t rows, int64_t tiles, int D
   return best;
 }
 
+// Waves of a workgroup: eight (bf16, heads up to 64, no mask of pairs) fill half the tiles for the same rows, 0.9 of the
+// time per row, where there are more of them than CUs; but rows are dealt out in twos as large, so the fuller CU counts
+// (us in four / eight: 14400 x 3600, 8 heads of 64 142 / 126; 57600 x 1000, 4 heads of 64 82 / 76; 10000 x 2000, 8 heads of
+// 64, 632 / 320 workgroups, 59 / 62; 5000 x 2000, 8 heads of 64, 320 / 160 workgroups, 40 / 44; fp32 and wider heads within
+// 2% or slower in eight; masks of pairs from 0.85 to 1.06 of the time)
+int xa_waves(int32_t dt, int64_t rows, int64_t nk, int D, int mask) {
+  if (dt != DT_BF16 || D > 64 || mask == MASK_PAIRS) return 4;
+  const int64_t cus = device_cus(), four = cdiv(rows, 128) * nk, eight = cdiv(rows, 256) * nk;
+  return eight > cus && 9 * 2 * cdiv(eight, cus) < 10 * cdiv(four, cus) ? 8 : 4;
+}
+
 struct XaPlan {
   bool resident;
   int64_t nblk, split_len;  // row blocks (resident: workgroups) of an (image, kv head); keys of a split
-  int splits;
+  int splits, waves;        // waves of a workgroup of xa_kernel
   size_t bits, part;        // workspace bytes: the mask's words, the splits' parts
 };
 
@@ -725,7 +736,8 @@ XaPlan xa_plan(int32_t dt, int64_t n, int64_t lq, int64_t lk, int64_t heads, int
     g.nblk = want < most ? want : most;
     return g;
   }
-  g.nblk = cdiv(rows, XA_ROWS);
+  g.waves = xa_waves(dt, rows, nk, D, mask);
+  g.nblk = cdiv(rows, 32 * g.waves);
   const int64_t blocks = g.nblk * nk;
   g.split_len = cdiv(cdiv(lk, xa_splits(dt, blocks, nk * rows, cdiv(lk, kt), D)), kt) * kt;
   g.splits = (int)cdiv(lk, g.split_len);
@@ -735,7 +747,7 @@ XaPlan xa_plan(int32_t dt, int64_t n, int64_t lq, int64_t lk, int64_t heads, int
 }
 
 template <int DT, int D>
-void xa_launch(const CrossP& k, bool resident, int mask, hipStream_t st) {
+void xa_launch(const CrossP& k, bool resident, int waves, int mask, hipStream_t st) {
   const dim3 grid((unsigned)(8 * ((k.nblk * k.nk * k.splits + 7) / 8)));
   if (resident) {
     using T = XaTile<DT, D>;
@@ -745,9 +757,16 @@ void xa_launch(const CrossP& k, bool resident, int mask, hipStream_t st) {
     else hipLaunchKernelGGL((xa_resident_kernel<DT, D, MASK_PAIRS>), grid, dim3(XR_T), lds, st, k);
     return;
   }
-  if (mask == MASK_NONE) hipLaunchKernelGGL((xa_kernel<DT, D, MASK_NONE>), grid, dim3(XA_T), 0, st, k);
-  else if (mask == MASK_KEYS) hipLaunchKernelGGL((xa_kernel<DT, D, MASK_KEYS>), grid, dim3(XA_T), 0, st, k);
-  else hipLaunchKernelGGL((xa_kernel<DT, D, MASK_PAIRS>), grid, dim3(XA_T), 0, st, k);
+  if constexpr (DT == DT_BF16 && D <= 64) {
+    if (waves == 8) {
+      if (mask == MASK_NONE) hipLaunchKernelGGL((xa_kernel<DT, D, MASK_NONE, 8>), grid, dim3(512), 0, st, k);
+      else hipLaunchKernelGGL((xa_kernel<DT, D, MASK_KEYS, 8>), grid, dim3(512), 0, st, k);
+      return;  // not split
+    }
+  }
+  if (mask == MASK_NONE) hipLaunchKernelGGL((xa_kernel<DT, D, MASK_NONE, 4>), grid, dim3(256), 0, st, k);
+  else if (mask == MASK_KEYS) hipLaunchKernelGGL((xa_kernel<DT, D, MASK_KEYS, 4>), grid, dim3(256), 0, st, k);
+  else hipLaunchKernelGGL((xa_kernel<DT, D, MASK_PAIRS, 4>), grid, dim3(256), 0, st, k);
   if (k.splits > 1) {
     constexpr int TPR = D <= 32 ? 8 : D <= 64 ? 16 : 32;
     int gs = 1;
@@ -819,13 +838,13 @@ extern "C" int clarus_hip_cross_attention(const ClarusCrossArgs* a, void* scratc
                        a->mask_qstride, lq, a->lk, nw, total, (unsigned short*)scratch);
   }
   const int D = xa_pad(a->d);
-  note_kernel("%s d=%d splits=%d", g.resident ? "xa_resident_kernel" : "xa_kernel", D, g.splits);
+  note_kernel("%s d=%d waves=%d splits=%d", g.resident ? "xa_resident_kernel" : "xa_kernel", D, g.resident ? XR_T / 64 : g.waves, g.splits);
 #define CLARUS_XA(DT)                                        \
   do {                                                       \
-    if (D == 32) xa_launch<DT, 32>(k, g.resident, a->mask_mode, st);     \
-    else if (D == 64) xa_launch<DT, 64>(k, g.resident, a->mask_mode, st); \
-    else if (D == 96) xa_launch<DT, 96>(k, g.resident, a->mask_mode, st); \
-    else xa_launch<DT, 128>(k, g.resident, a->mask_mode, st);            \
+    if (D == 32) xa_launch<DT, 32>(k, g.resident, g.waves, a->mask_mode, st);     \
+    else if (D == 64) xa_launch<DT, 64>(k, g.resident, g.waves, a->mask_mode, st); \
+    else if (D == 96) xa_launch<DT, 96>(k, g.resident, g.waves, a->mask_mode, st); \
+    else xa_launch<DT, 128>(k, g.resident, g.waves, a->mask_mode, st);            \
   } while (0)
   if (a->dtype == DT_BF16) CLARUS_XA(DT_BF16);
   else CLARUS_XA(DT_F32);

@@ -366,6 +366,20 @@ def test_long_passes(what, dt, hips, gpu_device):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("what", ["none", "last keys", "both ends", "one key", "no key"])
+def test_long_passes_of_many_rows(what, hips, gpu_device):
+    """Enough rows for workgroups of eight waves, the last of them without rows, more keys than 64 tiles."""
+    lq, lk, heads, kv_heads, d = 6200, 4501, 16, 4, 40
+    q, k, v = inputs(1, lq, lk, heads, kv_heads, d, torch.bfloat16, gpu_device, seed=12)
+    mask = stretches(what, lq, lk, gpu_device)
+    print(f"[xa] {what}", flush=True)
+    got = hips[torch.bfloat16].cross_attention(q, k, v, heads, kv_heads, mask=mask)
+    assert "waves=8" in _lib.last_kernel()
+    check(got, q, k, v, heads, kv_heads, mask=mask, what=what)
+    assert mask is None or mask.any() or not got.any()
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("dt", [torch.bfloat16, torch.float32])
 @pytest.mark.parametrize("lq", [54, 26000])
 def test_layouts_of_long_keys(lq, dt, hips, gpu_device):
