@@ -166,7 +166,7 @@ __device__ __forceinline__ unsigned xa_bits16(const unsigned char* p, int64_t le
 }
 
 // One tile of NB x 32 keys for a wave's 32 rows: S^T = K Q^T, the softmax's step, O^T += V^T P^T. bits: the keys that
-// count, of a lane's row under MASK_PAIRS; fresh: o is still 0
+// count, of a lane's row under MASK_PAIRS; whole: all of them; fresh: o is still 0
 template <int DT, int D, int MASK, int NB, bool ANEW>
 __device__ __forceinline__ void xa_tile(const unsigned char* ks, const unsigned char* vs, const u32x4 (&qf)[XaTile<DT, D>::QN],
                                         f32x16 (&o)[D / 32], float& m, float& l, float c, uint64_t bits, bool whole, bool fresh) {
@@ -199,7 +199,7 @@ __device__ __forceinline__ void xa_tile(const unsigned char* ks, const unsigned 
   }
   __builtin_amdgcn_s_setprio(1);
   // masked and padding keys weigh nothing, whatever their scores
-  if (MASK == MASK_PAIRS || !whole) {
+  if (!(MASK == MASK_PAIRS ? __all(whole) : whole)) {
 #pragma unroll
     for (int b = 0; b < NB; ++b) {
       const unsigned w = (unsigned)(bits >> (32 * b)) >> (4 * hl);
@@ -538,13 +538,21 @@ __global__ void __launch_bounds__(64 * W, D <= 64 ? (MASK == MASK_PAIRS ? 3 : 4)
     if constexpr (MASK == MASK_KEYS) {
       want = __ballot(lane < cn && xa_any<KT>(mkey + k0 + (int64_t)(c0 + lane) * KT, k1 - k0 - (int64_t)(c0 + lane) * KT));
     } else if constexpr (MASK == MASK_PAIRS) {
-      // lane (row, hl): 32 tiles' words of its row
+      // lane (row, hl): 32 tiles' words of its row, 16 in flight
       mine = 0;
-#pragma unroll 8
-      for (int t = 0; t < 32; ++t) {
-        const int tile = 32 * hl + t;
-        const uint64_t any = __ballot(tile < cn && words[c0 + (tile < cn ? tile : 0)] != 0);
-        mine |= (uint64_t)((unsigned)any != 0) << t | (uint64_t)((any >> 32) != 0) << (32 + t);
+#pragma unroll 1
+      for (int t0 = 0; t0 < 32 && t0 < cn; t0 += 16) {
+        Word w[16];
+#pragma unroll
+        for (int t = 0; t < 16; ++t) {
+          const int tile = 32 * hl + t0 + t;
+          w[t] = words[c0 + (tile < cn ? tile : 0)];
+        }
+#pragma unroll
+        for (int t = 0; t < 16; ++t) {
+          const uint64_t any = __ballot(32 * hl + t0 + t < cn && w[t] != 0);
+          mine |= (uint64_t)((unsigned)any != 0) << (t0 + t) | (uint64_t)((any >> 32) != 0) << (32 + t0 + t);
+        }
       }
       if (!busy) mine = 0;
       __syncthreads();  // the words of the 64 tiles before have been read
