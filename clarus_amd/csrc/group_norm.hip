@@ -14,6 +14,8 @@
 //   gn_apply_kernel  y: one read of x, one write
 //   gn_small_kernel  all in one launch, x held in registers between them, where the pixels of a few
 //                    whole groups fit one workgroup
+#include <algorithm>
+
 #include "capi.hpp"
 #include "common.hpp"
 
@@ -29,6 +31,7 @@ constexpr int UA = 4;        // rows in flight per thread (apply)
 constexpr int NRMAX = 8;     // rows held per thread (small), at most
 constexpr int GN_JOIN = 8;   // partial statistics in flight per thread (join)
 constexpr int GN_UNIT = 2048;  // channels that a workgroup has to hold together, at most
+constexpr int64_t GN_GRID = 1 << 23;  // workgroups of a launch, at most
 constexpr int GN_SILU = CLARUS_ACT_SILU;
 
 struct GroupNormP {
@@ -44,8 +47,7 @@ struct GroupNormP {
   int64_t schunk;    // pixels per statistics chunk
   int64_t wbs, bbs;
   int c, groups, cg, nchunk;
-  int n, strips;     // images, strips of channels (small)
-  int chunks;        // chunks of this launch
+  int n, strips, chunks;  // images, strips of channels, chunks of this launch
   int tr, rpb;       // threads per row (octets of a strip), rows per pass of a workgroup
   int lpg;           // lanes that join a group: a power of two <= 64
   int act;
@@ -73,13 +75,35 @@ __device__ __forceinline__ float lanes_sum(float v, int lpg) {
   return v;
 }
 
-// The chunk of pixels of this workgroup, -1 past the last: the chunks in equal parts over the XCDs, in order, BACK: the
-// last first. The apply pass goes back over the part that the statistics pass of its XCD has read, whose end is still in
-// that L2 (90 x 160 x 512 bf16 15.6 us dealt out, 14.2 in parts; 2 x 173 x 251 x 128 fp32 29.1, 28.1 in parts, 26.7 back)
-template <bool BACK>
-__device__ __forceinline__ int gn_chunk(int chunks) {
-  const int span = (chunks + 7) >> 3, i = blockIdx.x >> 3, c = (blockIdx.x & 7) * span + (BACK ? span - 1 - i : i);
-  return i < span && c < chunks ? c : -1;
+enum : int { GN_FRONT, GN_BACK, GN_PARTS };
+
+// What a workgroup of a one-dimensional grid works on: (image, strip of channels, chunk of pixels). False past the last.
+//   GN_FRONT, GN_BACK  one image after another (GN_BACK: the last first), its strips and chunks in equal parts over the
+//                      XCDs where there are eight of them or more. The apply pass goes back over what the statistics pass
+//                      has read, whose end is still in the last-level cache and, of its own part, in the XCD's L2 (90 x
+//                      160 x 512 bf16 15.6 us dealt out one by one, 14.2 in parts; 2 x 173 x 251 x 128 fp32 29.1, 28.1 in
+//                      parts, 26.7 back; images in parts over the XCDs: 64 x 4096 x 512 fp32 251 us, 301)
+//   GN_PARTS           the whole in equal parts over the XCDs: neighbouring strips share the lines of a row, which an L2
+//                      joins (64 images of 2048 pixels, 512 channels, 64 groups, bf16: 256 us dealt out, 71 in parts)
+template <int ORDER>
+__device__ __forceinline__ bool gn_at(const GroupNormP& p, int64_t& n, int& strip, int& chunk) {
+  const unsigned per = (unsigned)p.strips * (unsigned)p.chunks, total = (unsigned)p.n * per, xcd = blockIdx.x & 7;
+  unsigned i = blockIdx.x >> 3, rest;
+  if (ORDER != GN_PARTS && per >= 8) {
+    const unsigned m = (per + 7) >> 3;
+    if (ORDER == GN_BACK) i = (unsigned)p.n * m - 1 - i;
+    n = i / m;
+    rest = xcd * m + i % m;
+    if (rest >= per) return false;
+  } else {
+    const unsigned span = (total + 7) >> 3, id = ORDER == GN_PARTS ? xcd * span + i : ORDER == GN_BACK ? total - 1 - blockIdx.x : blockIdx.x;
+    if (i >= span || id >= total) return false;
+    n = id / per;
+    rest = id % per;
+  }
+  strip = (int)(rest / (unsigned)p.chunks);
+  chunk = (int)(rest - (unsigned)strip * (unsigned)p.chunks);
+  return true;
 }
 
 // f(group) on the lpg consecutive threads of each of ng groups at a time, every lane of a wave in step
@@ -97,11 +121,12 @@ __global__ void __launch_bounds__(GN_TT) gn_stats_kernel(const GroupNormP p) {
   __shared__ float sm[GN_TT * NA], s2[GN_TT * NA];
   const int tid = threadIdx.x;
   const int rl = tid / p.tr, oct = tid - rl * p.tr;
-  const int at_chunk = gn_chunk<false>(p.chunks);
-  if (at_chunk < 0) return;
-  const int64_t n = blockIdx.z, r0 = (int64_t)at_chunk * p.chunk;
+  int64_t n;
+  int strip, at_chunk;
+  if (!gn_at<GN_FRONT>(p, n, strip, at_chunk)) return;
+  const int64_t r0 = (int64_t)at_chunk * p.chunk;
   const int rows = (int)((r0 + p.chunk < p.p ? r0 + p.chunk : p.p) - r0);
-  const int c0 = blockIdx.y * p.tr * 8;  // first channel of the strip
+  const int c0 = strip * p.tr * 8;  // first channel of the strip
   const bool act = rl < p.rpb && c0 + oct * 8 < p.c;
   float mean[NA], m2[NA];
 #pragma unroll
@@ -298,11 +323,11 @@ __device__ __forceinline__ void gn_affine(const GroupNormP& p, int64_t n, int c,
 template <int DT, int ODT, int ACT, bool WHOLE>
 __global__ void __launch_bounds__(GN_T) gn_apply_kernel(const GroupNormP p) {
   const int tid = threadIdx.x;
-  const int64_t n = gridDim.z - 1 - blockIdx.z;
-  const int rl = tid / p.tr, oct = tid - rl * p.tr, c0 = (blockIdx.y * p.tr + oct) * 8;
+  int64_t n;
+  int strip, at_chunk;
+  if (!gn_at<GN_BACK>(p, n, strip, at_chunk)) return;
+  const int rl = tid / p.tr, oct = tid - rl * p.tr, c0 = (strip * p.tr + oct) * 8;
   const bool act = rl < p.rpb && c0 < p.c;
-  const int at_chunk = gn_chunk<true>(p.chunks);
-  if (at_chunk < 0) return;
   const int64_t r0 = (int64_t)at_chunk * p.chunk;
   const int rows = (int)((r0 + p.chunk < p.p ? r0 + p.chunk : p.p) - r0);
   const int64_t xb = n * p.xbs + r0 * p.ldx + c0, ob = (n * p.p + r0) * p.c + c0;
@@ -357,13 +382,10 @@ __global__ void __launch_bounds__(GN_TS) gn_small_kernel(const GroupNormP p) {
   __shared__ float stat[2][GN_UNIT];
   const int tid = threadIdx.x, sub = tid & (p.lpg - 1);
   const int rl = tid / p.tr, oct = tid - rl * p.tr;
-  // neighbouring strips share the lines of a row: they run on one XCD, one after the other, whose L2 joins them (64
-  // images of 2048 pixels, 512 channels, 64 groups, bf16: 71 us; dealt out over the XCDs 256)
-  const unsigned strips = (unsigned)p.strips, total_wg = strips * (unsigned)p.n, span = (total_wg + 7) >> 3;
-  const unsigned id = (blockIdx.x & 7) * span + (blockIdx.x >> 3);
-  if ((blockIdx.x >> 3) >= span || id >= total_wg) return;
-  const int64_t n = id / strips;
-  const int s0 = (int)(id - (unsigned)n * strips) * p.tr * 8, c0 = s0 + oct * 8, P = (int)p.p;
+  int64_t n;
+  int strip, at_chunk;
+  if (!gn_at<GN_PARTS>(p, n, strip, at_chunk)) return;
+  const int s0 = strip * p.tr * 8, c0 = s0 + oct * 8, P = (int)p.p;
   const bool act = rl < p.rpb && c0 < p.c;
   const int sgroups = min(p.tr * 8, p.c - s0) / p.cg;
   const int units = p.cg / PER;
@@ -429,6 +451,9 @@ __global__ void __launch_bounds__(GN_TS) gn_small_kernel(const GroupNormP p) {
   }
 }
 
+// workgroups of a launch over per (strip, chunk) pairs of each of n images, as gn_at has them
+unsigned gn_grid(int64_t n, int64_t per, bool parts) { return (unsigned)(parts || per < 8 ? 8 * cdiv(n * per, 8) : n * 8 * cdiv(per, 8)); }
+
 // least common multiple of 8 and cg
 int64_t gn_unit(int64_t cg) { return cg % 8 == 0 ? cg : cg % 4 == 0 ? 2 * cg : cg % 2 == 0 ? 4 * cg : 8 * cg; }
 
@@ -453,7 +478,7 @@ GnPlan gn_plan(int64_t n, int64_t p, int64_t c, int64_t groups) {
   // long chains of loads lose to the three launches over the whole chip (us, one / three launches, bf16, 32 groups: 500
   // pixels of 512 channels at 4 rows 6.0 / 9.5, 1024 at 8 rows 7.8 / 9.4, 1536 at 12 rows 10.4 / 9.4, 2048 at 16 rows
   // 11.9 / 9.4; 64 images of the first 18.6 / 24.6, of the second 30.3 / 37.4, of the last 63.5 / 67.3)
-  g.small = p <= (int64_t)(GN_TS / u) * NRMAX;
+  g.small = p <= (int64_t)(GN_TS / u) * NRMAX && n * (c / 8 / u) < GN_GRID;
   if (g.small) {
     g.tr = (int)u;
     g.strips = (int)(c / 8 / u);
@@ -503,11 +528,13 @@ extern "C" int clarus_hip_group_norm(const void* x, int32_t x_dtype, int64_t x_b
                  "group_norm: x and out 16-byte aligned rows");
   CLARUS_REQUIRE((w_bstride == 0 || w_bstride >= c) && (b_bstride == 0 || b_bstride >= c), "group_norm: affine strides");
   CLARUS_REQUIRE(eps >= 0.f && eps < INFINITY, "group_norm: eps finite and not negative");
-  // the pixel index of a chunk is 32 bits; a launch has at most 65535 images and strips (of 8 channels or more)
+  // 32 bits: the pixels of an image, the workgroups of a launch; the join's grid has at most 65535 images
   CLARUS_REQUIRE(p < ((int64_t)1 << 31) && n < 65536 && c < ((int64_t)1 << 19), "group_norm: too large");
   const size_t need = clarus_hip_group_norm_workspace(n, p, c, groups);
   CLARUS_REQUIRE(need == 0 || (scratch && scratch_bytes >= need && aligned(scratch, 8)), "group_norm: scratch %zu < %zu bytes", scratch_bytes, need);
   const GnPlan g = gn_plan(n, p, c, groups);
+  const int64_t achunks = g.small ? 1 : cdiv(p, g.achunk);
+  CLARUS_REQUIRE(n * g.strips * std::max<int64_t>(g.nchunk, achunks) < GN_GRID, "group_norm: too large");
   GroupNormP k{};
   k.x = x; k.out = out; k.w = w; k.b = b;
   k.stat = (float2*)scratch;
@@ -515,7 +542,7 @@ extern "C" int clarus_hip_group_norm(const void* x, int32_t x_dtype, int64_t x_b
   k.xbs = x_bstride; k.ldx = ldx; k.p = p; k.schunk = g.schunk;
   k.wbs = w_bstride; k.bbs = b_bstride;
   k.c = (int)c; k.groups = (int)groups; k.cg = (int)(c / groups); k.nchunk = g.nchunk;
-  k.tr = g.tr; k.eps = eps; k.act = act;
+  k.n = (int)n; k.strips = g.strips; k.chunks = 1; k.tr = g.tr; k.eps = eps; k.act = act;
   hipStream_t st = (hipStream_t)stream;
   const bool whole = k.cg % 8 == 0;
   const int64_t sgroups = (c < 8 * g.tr ? c : 8 * g.tr) / k.cg;
@@ -523,8 +550,7 @@ extern "C" int clarus_hip_group_norm(const void* x, int32_t x_dtype, int64_t x_b
   k.lpg = gn_lanes(sgroups, k.rpb, g.small ? GN_TS : GN_TT);
   if (g.small) {
     const int nr = (int)cdiv(p, k.rpb);
-    k.n = (int)n; k.strips = g.strips;
-    const dim3 grid((unsigned)(8 * cdiv(g.strips * n, 8)));
+    const dim3 grid(gn_grid(n, g.strips, true));
     note_kernel("gn_small_kernel strips=%d rows=%d", g.strips, nr);
 #define CLARUS_GN_S(DT, ODT, W)                                                                                  \
   do {                                                                                                           \
@@ -549,7 +575,7 @@ extern "C" int clarus_hip_group_norm(const void* x, int32_t x_dtype, int64_t x_b
   }
   k.chunk = g.schunk;
   k.chunks = g.nchunk;
-  const dim3 sgrid((unsigned)(8 * cdiv(g.nchunk, 8)), (unsigned)g.strips, (unsigned)n);
+  const dim3 sgrid(gn_grid(n, (int64_t)g.strips * g.nchunk, false));
   note_kernel("gn_stats_kernel + gn_apply_kernel nchunk=%d strips=%d", g.nchunk, g.strips);
   if (x_dtype == DT_BF16) {
     if (whole) hipLaunchKernelGGL((gn_stats_kernel<DT_BF16, true>), sgrid, dim3(GN_TT), 0, st, k);
@@ -560,9 +586,9 @@ extern "C" int clarus_hip_group_norm(const void* x, int32_t x_dtype, int64_t x_b
   }
   hipLaunchKernelGGL(gn_join_kernel, dim3((unsigned)groups, (unsigned)n), dim3(64), 0, st, k);
   k.chunk = g.achunk;
-  k.chunks = (int)cdiv(p, g.achunk);
+  k.chunks = (int)achunks;
   k.rpb = GN_T / g.tr;
-  const dim3 grid((unsigned)(8 * cdiv(k.chunks, 8)), (unsigned)g.strips, (unsigned)n);
+  const dim3 grid(gn_grid(n, g.strips * achunks, false));
 #define CLARUS_GN_A(DT, ODT, ACT)                                                                      \
   do {                                                                                                 \
     if (whole) hipLaunchKernelGGL((gn_apply_kernel<DT, ODT, ACT, true>), grid, dim3(GN_T), 0, st, k);  \

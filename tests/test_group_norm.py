@@ -161,6 +161,19 @@ def test_shapes(shape, groups, dt, hips, gpu_device):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dt", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("shape,groups", [((130, 42, 50, 64), 8), ((700, 41, 51, 32), 8), ((37, 30, 40, 264), 33), ((3, 70, 60, 2400), 12),
+                                          ((200, 3, 5, 512), 64)])
+def test_many_images_and_strips(shape, groups, dt, hips, gpu_device):
+    """Fewer chunks of an image than XCDs, several strips of channels."""
+    x, w, b = inputs(shape, dt, gpu_device, per_image=True)
+    print(f"[gn] {shape} {groups} {dt}", flush=True)
+    got = hips[dt].group_norm(x, groups, w, b, eps=EPS, act="silu")
+    print(f"[gn] {_lib.last_kernel()}", flush=True)
+    check(got, x, groups, w, b, act="silu", what=str(shape))
+
+
+@pytest.mark.gpu
 def test_types_of_operands(hips, gpu_device):
     x, w, b = inputs((2, 12, 17, 64), torch.float32, gpu_device)
     for xdt in (torch.bfloat16, torch.float32):
