@@ -454,6 +454,45 @@ def test_pair_masks_on_streams_and_in_graphs(lq, lk, hips, gpu_device):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dt", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("lq,lk", [(9, 20), (9, 2500), (40000, 150)])
+def test_output_types_and_flat_queries(lq, lk, dt, hips, gpu_device):
+    """Either output type from each form (keys in LDS, split, whole passes), and one query per image as [N, C]."""
+    q, k, v = inputs(2, lq, lk, 4, 2, 40, dt, gpu_device)
+    for odt in (torch.bfloat16, torch.float32):
+        got = hips[dt].cross_attention(q, k, v, 4, 2, out_dtype=odt)
+        assert got.dtype == odt
+        check(got, q, k, v, 4, 2, what=str(odt))
+    one = hips[dt].cross_attention(q[:, 3], k, v, 4, 2, make_mask("pairs", 2, 1, lk, gpu_device, seed=4))
+    assert one.shape == (2, 160)
+    check(one, q[:, 3], k, v, 4, 2, make_mask("pairs", 2, 1, lk, gpu_device, seed=4))
+
+
+@pytest.mark.gpu
+def test_threads(hips, gpu_device):
+    """Calls from several host threads, each on a stream of its own, sizes that share and do not share plans."""
+    import threading
+    hip = hips[torch.bfloat16]
+    cases = [inputs(1, 70 + 30 * (i % 2), 400, 4, 4, 32, torch.bfloat16, gpu_device, seed=i) for i in range(4)]
+    refs = [hip.cross_attention(*c, 4) for c in cases]
+    torch.cuda.synchronize()
+    bad, done = [], []
+
+    def work(i):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            outs = [hip.cross_attention(*cases[i], 4) for _ in range(20)]
+            torch.cuda.current_stream().synchronize()
+            bad.extend(i for o in outs if not torch.equal(o, refs[i]))
+        done.append(i)
+    ts = [threading.Thread(target=work, args=(i,)) for i in range(4)]
+    for t in ts:
+        t.start()
+    for t in ts:
+        t.join()
+    assert sorted(done) == [0, 1, 2, 3] and not bad
+
+
+@pytest.mark.gpu
 def test_a_scale_is_read_with_every_call(hips, gpu_device):
     q, k, v = inputs(1, 30, 40, 2, 2, 32, torch.float32, gpu_device)
     scale = torch.tensor(0.25)

@@ -301,6 +301,34 @@ def test_empty_repeatable_streams_and_graph(hips, gpu_device):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("shape,groups", [((2, 12, 17, 64), 16), ((2, 60, 70, 64), 16), ((1, 50, 60, 96), 12)])
+def test_output_types_and_graphs_of_each_form(shape, groups, hips, gpu_device):
+    hip = hips[torch.bfloat16]
+    x, w, b = inputs(shape, torch.float32, gpu_device)
+    for xdt in (torch.bfloat16, torch.float32):
+        for odt in (torch.bfloat16, torch.float32):
+            got = hip.group_norm(x.to(xdt), groups, w, b, act="gelu", out_dtype=odt)
+            check(got, x.to(xdt), groups, w, b, act="gelu", what=f"{xdt} -> {odt}")
+    a = [x.bfloat16(), x.flip(0, 1).mul(2).bfloat16()]
+    want = [hip.group_norm(t, groups, w, b, act="silu") for t in a]
+    made = []
+    for t in a:
+        st = t.clone()
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            y = hip.group_norm(st, groups, w, b, act="silu")
+        made.append((graph, st, y))
+    for i in range(6):
+        graph, st, y = made[i % 2]
+        st.copy_(a[(i // 2) % 2])
+        graph.replay()
+        eager = hip.group_norm(a[1], groups, w, b, act="silu")
+        torch.cuda.synchronize()
+        assert torch.equal(y, want[(i // 2) % 2]) and torch.equal(eager, want[1]), i
+
+
+@pytest.mark.gpu
 def test_chain_serves_gradients_on_torch(gpu_device):
     """An input that needs its gradient goes to the torch form of the chain, which has it."""
     from clarus_amd import spatial_torch  # noqa: F401
