@@ -844,7 +844,7 @@ class HipOps(Backend):
             raise Unsupported("group_norm: 16-byte aligned rows")
         if not 0.0 <= eps < math.inf:
             raise Unsupported("group_norm: eps finite and not negative")
-        out = torch.empty(x.shape, device=x.device, dtype=odt)
+        out = torch.empty_like(x, dtype=odt, memory_format=torch.contiguous_format)
         if not p:
             return out
         wf = weight if weight is None else weight.float().contiguous()
@@ -892,7 +892,7 @@ class HipOps(Backend):
                heads, kv_heads, scale, out_dtype, None if mask is None else (mask.shape, mask.stride(), mask.dtype))
         self._forward_only("cross_attention", q, k, v, mask)
         odt, args, need = self._plan(key, lambda: self._cross_plan(q, k, v, heads, kv_heads, mask, scale, out_dtype or self.dtype))
-        out = torch.empty(q.shape, device=q.device, dtype=odt)
+        out = torch.empty_like(q, dtype=odt, memory_format=torch.contiguous_format)
         if args is None:  # nothing asked, or nothing to attend
             return out.zero_()
         qp, kp, vp = q.data_ptr(), k.data_ptr(), v.data_ptr()
