@@ -90,7 +90,6 @@ struct XaTile {
   static constexpr int ROWB = D * ES;                 // bytes of a row in LDS
   static constexpr int CPR = ROWB / 16;               // 16-byte chunks per row
   static constexpr int BYTES = KT * ROWB;
-  static constexpr int QN = DT == DT_BF16 ? D / 16 : D / 8;  // 16-byte chunks of a row of Q per lane
   static constexpr uint64_t ALL = KT == 64 ? ~0ull : 0xffffffffull;
   // chunk c of row r sits at position c ^ swz(r). K: 16 lanes read one chunk of 16 consecutive rows; V: bf16
   // 8 rows x 4 chunks (transposing), fp32 two rows 4 apart x 8 chunks: each over all banks (fp32 V of 32 and
@@ -105,6 +104,9 @@ struct XaTile {
   static __device__ __forceinline__ int at_k(int r, int c) { return r * ROWB + (c ^ swz_k(r)) * 16; }
   static __device__ __forceinline__ int at_v(int r, int c) { return r * ROWB + (c ^ swz_v(r)) * 16; }
 };
+
+// 16-byte chunks of a row of Q per lane. C: the head's columns in sixteens, what a score sums over
+template <int DT, int C> constexpr int xa_qn = DT == DT_BF16 ? C / 16 : C / 8;
 
 // what a masked, padding or absent piece of K or V is copied from
 __device__ const u32x4 xa_zeros[1] = {u32x4{0, 0, 0, 0}};
@@ -128,19 +130,18 @@ __device__ __forceinline__ XaRow xa_row(const CrossP& p, int kvh, int64_t row) {
 }
 
 // Q^T fragments of a row
-template <int DT, int D>
-__device__ __forceinline__ void xa_load_q(const CrossP& p, int64_t n, const XaRow& r, int hl, u32x4 (&qf)[XaTile<DT, D>::QN]) {
-  using T = XaTile<DT, D>;
-  constexpr int E = 16 / T::ES;
-  const unsigned char* qp = (const unsigned char*)p.q + (n * p.qbs + r.qi * p.ldq + (int64_t)r.head * p.d) * T::ES;
+template <int DT, int C>
+__device__ __forceinline__ void xa_load_q(const CrossP& p, int64_t n, const XaRow& r, int hl, u32x4 (&qf)[xa_qn<DT, C>]) {
+  constexpr int ES = DT == DT_BF16 ? 2 : 4, E = 16 / ES, QN = xa_qn<DT, C>;
+  const unsigned char* qp = (const unsigned char*)p.q + (n * p.qbs + r.qi * p.ldq + (int64_t)r.head * p.d) * ES;
 #pragma unroll
-  for (int s = 0; s < T::QN; ++s) {
+  for (int s = 0; s < QN; ++s) {
     const int at = (2 * s + hl) * E;
-    qf[s] = *reinterpret_cast<const u32x4*>(qp + (at < p.d ? at : 0) * T::ES);
+    qf[s] = *reinterpret_cast<const u32x4*>(qp + (at < p.d ? at : 0) * ES);
   }
-  if (p.d < D) {
+  if (p.d < C) {
 #pragma unroll
-    for (int s = 0; s < T::QN; ++s)
+    for (int s = 0; s < QN; ++s)
       if ((2 * s + hl) * E >= p.d) qf[s] = u32x4{0, 0, 0, 0};
   }
 }
@@ -167,11 +168,11 @@ __device__ __forceinline__ unsigned xa_bits16(const unsigned char* p, int64_t le
 
 // One tile of NB x 32 keys for a wave's 32 rows: S^T = K Q^T, the softmax's step, O^T += V^T P^T. bits: the keys that
 // count, of a lane's row under MASK_PAIRS; whole: all of them; fresh: o is still 0
-template <int DT, int D, int MASK, int NB, bool ANEW>
-__device__ __forceinline__ void xa_tile(const unsigned char* ks, const unsigned char* vs, const u32x4 (&qf)[XaTile<DT, D>::QN],
+template <int DT, int D, int C, int MASK, int NB, bool ANEW>
+__device__ __forceinline__ void xa_tile(const unsigned char* ks, const unsigned char* vs, const u32x4 (&qf)[xa_qn<DT, C>],
                                         f32x16 (&o)[D / 32], float& m, float& l, float c, uint64_t bits, bool whole, bool fresh) {
   using T = XaTile<DT, D>;
-  constexpr int DB = D / 32, QN = T::QN;
+  constexpr int DB = D / 32, QN = xa_qn<DT, C>;
   // ANEW: the lane's LDS offsets are worked out for each tile instead of kept over the loop, where they spill
   int lane = threadIdx.x & 63;
   if constexpr (ANEW) asm volatile("" : "+v"(lane));
@@ -378,10 +379,10 @@ __device__ __forceinline__ bool xa_any(const unsigned char* p, int64_t left) {
 constexpr int XR_T = 512;
 constexpr int XR_KEYS = 128;
 
-template <int DT, int D, int MASK>
+template <int DT, int D, int C, int MASK>
 __global__ void __launch_bounds__(XR_T, (DT == DT_BF16 ? D <= 64 : D <= 32) ? 4 : 2) xa_resident_kernel(const CrossP p) {
   using T = XaTile<DT, D>;
-  constexpr int KT = T::KT, W = XR_T / 64;
+  constexpr int KT = T::KT, W = XR_T / 64, QN = xa_qn<DT, C>;
   extern __shared__ __attribute__((aligned(16))) unsigned char tiles[];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int col = lane & 31, hl = lane >> 5;
@@ -404,9 +405,9 @@ __global__ void __launch_bounds__(XR_T, (DT == DT_BF16 ? D <= 64 : D <= 32) ? 4 
     const int64_t r = (int64_t)c * 32 + col;
     return xa_row(p, kvh, r < p.rows ? r : p.rows - 1);
   };
-  constexpr bool AHEAD = T::QN <= 8;  // the next chunk's queries in flight (where registers allow it)
-  u32x4 qn[T::QN];
-  if (AHEAD && ch < c1) xa_load_q<DT, D>(p, n, at(ch), hl, qn);
+  constexpr bool AHEAD = QN <= 8;  // the next chunk's queries in flight (where registers allow it)
+  u32x4 qn[QN];
+  if (AHEAD && ch < c1) xa_load_q<DT, C>(p, n, at(ch), hl, qn);
   constexpr int MT = XR_KEYS / KT;
   uint64_t kept[MT];  // the keys of each tile that count
   {
@@ -425,14 +426,14 @@ __global__ void __launch_bounds__(XR_T, (DT == DT_BF16 ? D <= 64 : D <= 32) ? 4 
   barrier_keep_vm();
 #pragma unroll 1
   for (; ch < c1; ch += W) {
-    u32x4 qf[T::QN];
+    u32x4 qf[QN];
     const XaRow r = at(ch);
     if constexpr (AHEAD) {
 #pragma unroll
-      for (int i = 0; i < T::QN; ++i) qf[i] = qn[i];
-      if (ch + W < c1) xa_load_q<DT, D>(p, n, at(ch + W), hl, qn);
+      for (int i = 0; i < QN; ++i) qf[i] = qn[i];
+      if (ch + W < c1) xa_load_q<DT, C>(p, n, at(ch + W), hl, qn);
     } else {
-      xa_load_q<DT, D>(p, n, r, hl, qf);
+      xa_load_q<DT, C>(p, n, r, hl, qf);
     }
     const unsigned char* mrow = MASK == MASK_PAIRS ? p.mask + n * p.mbs + r.qi * p.mqs : nullptr;
     f32x16 o[D / 32];
@@ -458,7 +459,7 @@ __global__ void __launch_bounds__(XR_T, (DT == DT_BF16 ? D <= 64 : D <= 32) ? 4 
       } else if (!bits) {
         continue;
       }
-      xa_tile<DT, D, MASK, 1, true>(ks, ks + T::BYTES, qf, o, m, l, p.c, bits, bits == 0xffffffffu, fresh);
+      xa_tile<DT, D, C, MASK, 1, true>(ks, ks + T::BYTES, qf, o, m, l, p.c, bits, bits == 0xffffffffu, fresh);
       fresh = false;
     }
     l = sum32(l);
@@ -468,7 +469,7 @@ __global__ void __launch_bounds__(XR_T, (DT == DT_BF16 ? D <= 64 : D <= 32) ? 4 
 
 // ---------------------------------------------------------------- keys streamed through LDS
 // W waves of 32 rows. (MASK_PAIRS at 3 waves per SIMD: it spills at 4.)
-template <int DT, int D, int MASK, int W>
+template <int DT, int D, int C, int MASK, int W>
 __global__ void __launch_bounds__(64 * W, D <= 64 ? (MASK == MASK_PAIRS ? 3 : 4) : 2) xa_kernel(const CrossP p) {
   using T = XaTile<DT, D>;
   constexpr int KT = T::KT, KB = KT / 32, DB = D / 32;
@@ -520,8 +521,8 @@ __global__ void __launch_bounds__(64 * W, D <= 64 ? (MASK == MASK_PAIRS ? 3 : 4)
     copy(p, kp + base * p.ldk * T::ES, vp + base * p.ldv * T::ES, tiles[buf], bits);
   };
 
-  u32x4 qf[T::QN];
-  xa_load_q<DT, D>(p, n, r, hl, qf);
+  u32x4 qf[xa_qn<DT, C>];
+  xa_load_q<DT, C>(p, n, r, hl, qf);
   f32x16 o[DB];
 #pragma unroll
   for (int b = 0; b < DB; ++b)
@@ -591,7 +592,7 @@ __global__ void __launch_bounds__(64 * W, D <= 64 ? (MASK == MASK_PAIRS ? 3 : 4)
         if constexpr (MASK == MASK_PAIRS) next = words[t1];
       }
       if (busy && (MASK != MASK_PAIRS || (mine >> (t - c0) & 1)))
-        xa_tile<DT, D, MASK, KB, false>(tiles[buf], tiles[buf] + T::BYTES, qf, o, m, l, p.c, now, now == T::ALL, false);
+        xa_tile<DT, D, C, MASK, KB, false>(tiles[buf], tiles[buf] + T::BYTES, qf, o, m, l, p.c, now, now == T::ALL, false);
       t = t1;
       t1 = t2;
       buf ^= 1;
@@ -754,27 +755,27 @@ XaPlan xa_plan(int32_t dt, int64_t n, int64_t lq, int64_t lk, int64_t heads, int
   return g;
 }
 
-template <int DT, int D>
+template <int DT, int D, int C>
 void xa_launch(const CrossP& k, bool resident, int waves, int mask, hipStream_t st) {
   const dim3 grid((unsigned)(8 * ((k.nblk * k.nk * k.splits + 7) / 8)));
   if (resident) {
     using T = XaTile<DT, D>;
     const unsigned lds = (unsigned)(cdiv(k.lk, T::KT) * 2 * T::BYTES);
-    if (mask == MASK_NONE) hipLaunchKernelGGL((xa_resident_kernel<DT, D, MASK_NONE>), grid, dim3(XR_T), lds, st, k);
-    else if (mask == MASK_KEYS) hipLaunchKernelGGL((xa_resident_kernel<DT, D, MASK_KEYS>), grid, dim3(XR_T), lds, st, k);
-    else hipLaunchKernelGGL((xa_resident_kernel<DT, D, MASK_PAIRS>), grid, dim3(XR_T), lds, st, k);
+    if (mask == MASK_NONE) hipLaunchKernelGGL((xa_resident_kernel<DT, D, C, MASK_NONE>), grid, dim3(XR_T), lds, st, k);
+    else if (mask == MASK_KEYS) hipLaunchKernelGGL((xa_resident_kernel<DT, D, C, MASK_KEYS>), grid, dim3(XR_T), lds, st, k);
+    else hipLaunchKernelGGL((xa_resident_kernel<DT, D, C, MASK_PAIRS>), grid, dim3(XR_T), lds, st, k);
     return;
   }
   if constexpr (DT == DT_BF16 && D <= 64) {
     if (waves == 8) {
-      if (mask == MASK_NONE) hipLaunchKernelGGL((xa_kernel<DT, D, MASK_NONE, 8>), grid, dim3(512), 0, st, k);
-      else hipLaunchKernelGGL((xa_kernel<DT, D, MASK_KEYS, 8>), grid, dim3(512), 0, st, k);
+      if (mask == MASK_NONE) hipLaunchKernelGGL((xa_kernel<DT, D, C, MASK_NONE, 8>), grid, dim3(512), 0, st, k);
+      else hipLaunchKernelGGL((xa_kernel<DT, D, C, MASK_KEYS, 8>), grid, dim3(512), 0, st, k);
       return;  // not split
     }
   }
-  if (mask == MASK_NONE) hipLaunchKernelGGL((xa_kernel<DT, D, MASK_NONE, 4>), grid, dim3(256), 0, st, k);
-  else if (mask == MASK_KEYS) hipLaunchKernelGGL((xa_kernel<DT, D, MASK_KEYS, 4>), grid, dim3(256), 0, st, k);
-  else hipLaunchKernelGGL((xa_kernel<DT, D, MASK_PAIRS, 4>), grid, dim3(256), 0, st, k);
+  if (mask == MASK_NONE) hipLaunchKernelGGL((xa_kernel<DT, D, C, MASK_NONE, 4>), grid, dim3(256), 0, st, k);
+  else if (mask == MASK_KEYS) hipLaunchKernelGGL((xa_kernel<DT, D, C, MASK_KEYS, 4>), grid, dim3(256), 0, st, k);
+  else hipLaunchKernelGGL((xa_kernel<DT, D, C, MASK_PAIRS, 4>), grid, dim3(256), 0, st, k);
   if (k.splits > 1) {
     constexpr int TPR = D <= 32 ? 8 : D <= 64 ? 16 : 32;
     int gs = 1;
@@ -847,12 +848,17 @@ extern "C" int clarus_hip_cross_attention(const ClarusCrossArgs* a, void* scratc
   }
   const int D = xa_pad(a->d);
   note_kernel("%s d=%d waves=%d splits=%d", g.resident ? "xa_resident_kernel" : "xa_kernel", D, g.resident ? XR_T / 64 : g.waves, g.splits);
+  // V's columns come in blocks of 32, the columns that a score sums over in sixteens (14400 x 3600, 8 heads of 40: 113 us over
+  // 48 columns, 121 over 64, fp32 807 and 894; 14400 x 2000, 4 heads of 80 54 / 57, of 104 67 / 69, fp32 347 / 377, 459 / 493)
 #define CLARUS_XA(DT)                                        \
   do {                                                       \
-    if (D == 32) xa_launch<DT, 32>(k, g.resident, g.waves, a->mask_mode, st);     \
-    else if (D == 64) xa_launch<DT, 64>(k, g.resident, g.waves, a->mask_mode, st); \
-    else if (D == 96) xa_launch<DT, 96>(k, g.resident, g.waves, a->mask_mode, st); \
-    else xa_launch<DT, 128>(k, g.resident, g.waves, a->mask_mode, st);            \
+    if (D == 32) xa_launch<DT, 32, 32>(k, g.resident, g.waves, a->mask_mode, st);           \
+    else if (a->d <= 48) xa_launch<DT, 64, 48>(k, g.resident, g.waves, a->mask_mode, st);   \
+    else if (D == 64) xa_launch<DT, 64, 64>(k, g.resident, g.waves, a->mask_mode, st);      \
+    else if (a->d <= 80) xa_launch<DT, 96, 80>(k, g.resident, g.waves, a->mask_mode, st);   \
+    else if (D == 96) xa_launch<DT, 96, 96>(k, g.resident, g.waves, a->mask_mode, st);      \
+    else if (a->d <= 112) xa_launch<DT, 128, 112>(k, g.resident, g.waves, a->mask_mode, st); \
+    else xa_launch<DT, 128, 128>(k, g.resident, g.waves, a->mask_mode, st);                 \
   } while (0)
   if (a->dtype == DT_BF16) CLARUS_XA(DT_BF16);
   else CLARUS_XA(DT_F32);
