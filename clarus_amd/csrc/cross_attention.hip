@@ -17,14 +17,14 @@
 //   xa_join_kernel      joins the (O, m, l) of keys split over workgroups, where rows are few
 //   xa_bits_kernel      a mask of pairs as bits
 // m, l and O are fp32. bf16: products of bf16 q, k, v are exact in fp32; P is rounded once to bf16 for
-// the product with V (at most half a step, 2^-8, of each weight, of independent signs: below the
-// result's own rounding to bf16). fp32: every product runs on fp32 MFMAs.
+// the product with V (at most half a step, 2^-8, of each weight, of independent signs: together about
+// as much as the result's own rounding to bf16). fp32: every product runs on fp32 MFMAs.
 // A masked or padding key's score is taken as -inf whatever its K holds; where no query keeps it (a mask of
 // keys, the end of the keys) its V row is taken as 0.
 //
 // What bounds it (bf16, the GPU's time alone, without the call's).
 //   Many rows and keys: the softmax's arithmetic and the matrix cores, which overlap in part. 14400 queries x 3600 keys, 8
-//   heads of 64: 126 us, 838 TFLOP/s (a large library product reaches 1190); 57600 x 3600, 4 heads of 128: 466 us, 910.
+//   heads of 64: 122 us, 868 TFLOP/s (a large library product reaches 1190); 57600 x 3600, 4 heads of 128: 450 us, 943.
 //   In the first the VALU is busy for 72% of the cycles (an exponential counts twice), the matrix cores for 45%, in the
 //   second for 44% and 47%, at clocks that the load lowers to 1.8 and 1.9 GHz.
 //   A prompt (57600 x 77, 4 heads of 64): 12 us of reading q and writing o at the rate of a large copy; 19 us, a wave
