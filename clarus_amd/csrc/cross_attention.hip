@@ -27,7 +27,7 @@
 //   heads of 64: 122 us, 868 TFLOP/s (a large library product reaches 1190); 57600 x 3600, 4 heads of 128: 450 us, 943.
 //   In the first the VALU is busy for 72% of the cycles (an exponential counts twice), the matrix cores for 45%, in the
 //   second for 44% and 47%, at clocks that the load lowers to 1.8 and 1.9 GHz.
-//   A prompt (57600 x 77, 4 heads of 64): 12 us of reading q and writing o at the rate of a large copy; 19 us, a wave
+//   A prompt (57600 x 77, 4 heads of 64): 12 us of reading q and writing o at the rate of a large copy; 18.5 us, a wave
 //   loading, multiplying and weighing its few keys in turn: the VALU is busy for 62% of the cycles.
 //   One query of 8 images x 30001 keys: reading K and V, 492 MB in 94 us, 5.2 TB/s (a large copy: 4.8 TB/s).
 #include <algorithm>
@@ -405,6 +405,7 @@ __global__ void __launch_bounds__(XR_T, (DT == DT_BF16 ? D <= 64 : D <= 32) ? 4 
     const int64_t r = (int64_t)c * 32 + col;
     return xa_row(p, kvh, r < p.rows ? r : p.rows - 1);
   };
+  constexpr bool ANEW = DT == DT_BF16 && MASK == MASK_PAIRS && C == 64;  // (57600 x 77, 4 heads of 64: 24.6 us, 25.2 kept)
   constexpr bool AHEAD = QN <= 8;  // the next chunk's queries in flight (where registers allow it)
   u32x4 qn[QN];
   if (AHEAD && ch < c1) xa_load_q<DT, C>(p, n, at(ch), hl, qn);
@@ -459,7 +460,7 @@ __global__ void __launch_bounds__(XR_T, (DT == DT_BF16 ? D <= 64 : D <= 32) ? 4 
       } else if (!bits) {
         continue;
       }
-      xa_tile<DT, D, C, MASK, 1, true>(ks, ks + T::BYTES, qf, o, m, l, p.c, bits, bits == 0xffffffffu, fresh);
+      xa_tile<DT, D, C, MASK, 1, ANEW>(ks, ks + T::BYTES, qf, o, m, l, p.c, bits, bits == 0xffffffffu, fresh);
       fresh = false;
     }
     l = sum32(l);
