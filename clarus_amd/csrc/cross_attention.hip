@@ -11,7 +11,7 @@
 //                     of each 16, and V^T is read in that order (bf16: transposing LDS reads; fp32: one
 //                     float per lane), so P moves through no LDS
 // K and V go from memory straight to LDS, 16 bytes a lane, without passing through registers.
-//   xa_resident_kernel  up to XR_KEYS keys: all of them stay in LDS, rows stream by
+//   xa_resident_kernel  up to XR_KEYS keys: all of them stay in LDS, rows stream by (few rows of wide fp32 heads: below)
 //   xa_kernel           any number of keys: 128 or 256 rows (4 or 8 waves) per workgroup, tiles of 64 (fp32: 32)
 //                       keys, the next one on its way during the current one's products
 //   xa_join_kernel      joins the (O, m, l) of keys split over workgroups, where rows are few
@@ -696,22 +696,24 @@ __global__ void __launch_bounds__(XA_T) xa_join_kernel(const CrossP p, int gs) {
 int xa_pad(int64_t d) { return d <= 32 ? 32 : d <= 64 ? 64 : d <= 96 ? 96 : 128; }
 
 // Into how many parts the keys are split: as many as make the time of a part's tiles in a row and, with more than one
-// part, of writing and joining the parts least; at most two workgroups per CU. The constants are measured (us): a tile
-// 0.73 / 0.96 / 1.4 with heads of 32 / 64 / 128, fp32 1.2 / 2.25 / 4.3; a second workgroup on a CU adds a quarter of
-// that, in fp32, where the matrix core is the bound, 0.8; parts 2.8 and, a MB of one part, 0.56 + 0.3 for each. What it
+// part, of writing and joining the parts least, and less than most_of the time in one; at most two workgroups per CU. The
+// constants are measured (us): a tile 0.73 / 0.96 / 1.4 with heads of 32 / 64 / 128, fp32 1.2 / 2.25 / 4.3; a second
+// workgroup on a CU adds a quarter of that, in fp32, where the matrix core is the bound, 0.8; parts 2.8 and, a MB of one
+// part, 0.56 + 0.3 for each. What it
 // decides, in one / the chosen / more parts (us, bf16): one query, 8 heads of 64, 400 keys 9.6 / 7.6 (7); 8 x 256 queries,
 // 8 heads of 40, 400 keys 11.2 / - / 15.8 (2), 1600 keys 30.7 / 21.8 (4); 900 queries, 8 heads of 64, 800 keys 16.3 / 14.7
 // (4); 2 x 3600 queries, 4 heads of 64, 1000 keys 18.7 / - / 28.0 (2). One query of 8 images, 16 heads on 4 of 128, 30001
 // keys: 119 in 8 parts, 94 in 16 (two workgroups per CU), 107 in 24
-int64_t xa_splits(int32_t dt, int64_t blocks, int64_t rows, int64_t tiles, int D) {
+int64_t xa_splits(int32_t dt, int64_t blocks, int64_t rows, int64_t tiles, int D, double most_of) {
   const int64_t cus = device_cus(), most = std::min(tiles, std::max<int64_t>(2 * cus / blocks, 1));
   const double tile = dt == DT_BF16 ? 0.5 + 0.0072 * D : 0.2 + 0.032 * D, share = dt == DT_BF16 ? 0.25 : 0.8;
   const double mb = 1e-6 * (double)rows * (D + 2) * sizeof(float);
   int64_t best = 1;
-  double least = 1e30;
+  double least = 1e30, whole = 0.0;
   for (int64_t s = 1; s <= most; ++s) {
     const double t = cdiv(tiles, s) * tile * (1 + share * (cdiv(blocks * s, cus) - 1)) + (s > 1 ? 2.8 + mb * (0.56 + 0.3 * s) : 0.0);
-    if (t < least) least = t, best = s;
+    if (s == 1) whole = t;
+    if (t < least && (s == 1 || t < most_of * whole)) least = t, best = s;
   }
   return best;
 }
@@ -738,18 +740,23 @@ XaPlan xa_plan(int32_t dt, int64_t n, int64_t lq, int64_t lk, int64_t heads, int
   XaPlan g{};
   const int kt = dt == DT_BF16 ? 64 : 32, D = xa_pad(d);
   const int64_t rows = lq * (heads / kv_heads), nk = n * kv_heads;
-  if (lk <= XR_KEYS) {
+  // keys that fit LDS are split only where it takes a third off the modelled time, which knows no masks: few rows of wide fp32
+  // heads (4 x 1 queries, 8 heads on 2 of 128, 128 keys 19.8 us / 10.9 split; 71 queries 16.0 / 13.4; 225 queries, 16 heads of
+  // 80, not split, 12.4 / 13.7)
+  if (lk <= XR_KEYS && xa_splits(dt, cdiv(rows, 128) * nk, nk * rows, cdiv(lk, kt), D, 0.7) == 1) {
     g.resident = true;
     g.splits = 1;
     g.split_len = lk;
     const int64_t want = cdiv((D <= 64 ? 2LL : 1LL) * device_cus(), nk), most = cdiv(rows, 32 * (XR_T / 64));
-    g.nblk = want < most ? want : most;
+    // few rows: one chunk of 32 per workgroup while there are CUs, so that no two waves share a SIMD (900 queries, 8 heads of
+    // 64: 4.8 us, 6.0 with eight chunks per workgroup, fp32 10.0 and 17.4)
+    g.nblk = std::max(std::min(want, most), std::min(cdiv(rows, 32), device_cus() / nk));
     return g;
   }
   g.waves = xa_waves(dt, rows, nk, D, mask);
   g.nblk = cdiv(rows, 32 * g.waves);
   const int64_t blocks = g.nblk * nk;
-  g.split_len = cdiv(cdiv(lk, xa_splits(dt, blocks, nk * rows, cdiv(lk, kt), D)), kt) * kt;
+  g.split_len = cdiv(cdiv(lk, xa_splits(dt, blocks, nk * rows, cdiv(lk, kt), D, 1.0)), kt) * kt;
   g.splits = (int)cdiv(lk, g.split_len);
   if (mask == MASK_PAIRS) g.bits = (size_t)(n * lq * cdiv(lk, 64) + 1) / 2 * 16;
   if (g.splits > 1) g.part = (size_t)g.splits * nk * rows * (D + 2) * sizeof(float);
