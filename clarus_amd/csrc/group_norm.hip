@@ -4,12 +4,14 @@
 //   mean, var = biased;  y = act((x - mean) * rsqrt(var + eps) * weight[c] + bias[c])
 //
 // Statistics without cancellation: a thread takes UR rows of its channel octet into registers, has
-// their mean and squared distances exactly (two passes over registers), and joins them to its
-// running (mean, M2); threads, channels of a group and chunks of pixels are then joined by
-//   mean = sum(cnt mean) / sum(cnt),  M2 = sum(M2 + cnt (mean_i - mean)^2)
-// in a fixed order, all in fp32: no sum of squares of uncentred values occurs, so a mean far from
-// zero or a single large value costs no digits, and the result is deterministic.
-//   gn_stats_kernel  per (image, chunk of pixels) the groups' mean and M2: one read of x
+// their mean and variance in two passes over registers, and joins them to its running (mean, var);
+// threads, channels of a group and chunks of pixels are then joined by
+//   mean = sum(w mean),  var = sum(w (var_i + (mean_i - mean)^2)),  w = cnt / sum(cnt)
+// in a fixed order, all in fp32: no square of an uncentred value occurs, so a mean far from zero or
+// a single large value costs no digits, and the result is deterministic. A variance is carried and no sum
+// of squares, and nothing is joined to an empty part: whatever the count, values only have to lie within 2^60
+// of their group's mean, whose size may be more than a square holds.
+//   gn_stats_kernel  per (image, chunk of pixels) the groups' mean and variance: one read of x
 //   gn_join_kernel   per (image, group) the chunks joined: mean, rstd
 //   gn_apply_kernel  y: one read of x, one write
 //   gn_small_kernel  all in one launch, x held in registers between them, where the pixels of a few
@@ -42,7 +44,7 @@ struct GroupNormP {
   void* out;
   const float* w;    // [C] or [N][C] (wbs = C), or null
   const float* b;
-  float2* part;      // [n][G][chunk] mean, M2
+  float2* part;      // [n][G][chunk] mean, variance
   float2* stat;      // [n][G] mean, rstd
   int64_t xbs, ldx;  // image and pixel stride of x (elements)
   int64_t p;         // pixels
@@ -119,9 +121,9 @@ __device__ __forceinline__ void for_groups(int ng, int lpg, F&& f) {
 // WHOLE: cg % 8 == 0, an octet lies in one group and is one set of 8 values per row
 template <int DT, bool WHOLE>
 __global__ void __launch_bounds__(GN_TT) gn_stats_kernel(const GroupNormP p) {
-  constexpr int NA = WHOLE ? 1 : 8;  // (mean, M2) pairs per thread
+  constexpr int NA = WHOLE ? 1 : 8;  // (mean, var) pairs per thread
   constexpr int PER = WHOLE ? 8 : 1;
-  __shared__ float sm[GN_TT * NA], s2[GN_TT * NA];
+  __shared__ float sm[GN_TT * NA], sv[GN_TT * NA];
   const int tid = threadIdx.x;
   const int rl = tid / p.tr, oct = tid - rl * p.tr;
   int64_t n;
@@ -131,10 +133,16 @@ __global__ void __launch_bounds__(GN_TT) gn_stats_kernel(const GroupNormP p) {
   const int rows = (int)((r0 + p.chunk < p.p ? r0 + p.chunk : p.p) - r0);
   const int c0 = strip * p.tr * 8;  // first channel of the strip
   const bool act = rl < p.rpb && c0 + oct * 8 < p.c;
-  float mean[NA], m2[NA];
+  float mean[NA], var[NA];
 #pragma unroll
-  for (int i = 0; i < NA; ++i) mean[i] = m2[i] = 0.f;
+  for (int i = 0; i < NA; ++i) mean[i] = var[i] = 0.f;
   int cnt = 0;  // rows so far
+  // (m, v) of `part` of the rows with them joined to the rows so far (part 1: there are none)
+  auto join = [&](int a, float m, float v, float part) __attribute__((always_inline)) {
+    const float d = m - mean[a];
+    mean[a] = fmaf(d, part, mean[a]);
+    var[a] = fmaf(part, fmaf((1.f - part) * d, d, v - var[a]), var[a]);
+  };
   if (act) {
     const int64_t base = n * p.xbs + r0 * p.ldx + c0 + oct * 8;
     int r = rl;
@@ -149,7 +157,7 @@ __global__ void __launch_bounds__(GN_TT) gn_stats_kernel(const GroupNormP p) {
 #pragma unroll
       for (int k = 0; k < UR; ++k) v[k] = gn_widen<DT>(w[k]);
       if (r + (2 * UR - 1) * p.rpb < rows) fetch(r + UR * p.rpb);
-      const float part = (float)UR * __builtin_amdgcn_rcpf((float)(cnt + UR)), join = (float)cnt * part * PER;
+      const float part = cnt ? (float)UR * __builtin_amdgcn_rcpf((float)(cnt + UR)) : 1.f;
 #pragma unroll
       for (int a = 0; a < NA; ++a) {
         float s = 0.f, q = 0.f;
@@ -165,15 +173,13 @@ __global__ void __launch_bounds__(GN_TT) gn_stats_kernel(const GroupNormP p) {
             const float d = v[k].v[a * PER + i] - m;
             q = fmaf(d, d, q);
           }
-        const float d = m - mean[a];
-        mean[a] = fmaf(d, part, mean[a]);
-        m2[a] += fmaf(d * d, join, q);
+        join(a, m, q * (1.f / (UR * PER)), part);
       }
       cnt += UR;
     }
     for (; r < rows; r += p.rpb) {
       const f32x8 v = gn_load<DT>(p.x, base + (int64_t)r * p.ldx);
-      const float part = __builtin_amdgcn_rcpf((float)(cnt + 1)), join = (float)cnt * part * PER;
+      const float part = cnt ? __builtin_amdgcn_rcpf((float)(cnt + 1)) : 1.f;
 #pragma unroll
       for (int a = 0; a < NA; ++a) {
         float s = 0.f, q = 0.f;
@@ -185,9 +191,7 @@ __global__ void __launch_bounds__(GN_TT) gn_stats_kernel(const GroupNormP p) {
           const float d = v.v[a * PER + i] - m;
           q = fmaf(d, d, q);
         }
-        const float d = m - mean[a];
-        mean[a] = fmaf(d, part, mean[a]);
-        m2[a] += fmaf(d * d, join, q);
+        join(a, m, q * (1.f / PER), part);
       }
       ++cnt;
     }
@@ -195,29 +199,31 @@ __global__ void __launch_bounds__(GN_TT) gn_stats_kernel(const GroupNormP p) {
 #pragma unroll
   for (int a = 0; a < NA; ++a) {
     sm[tid * NA + a] = mean[a];
-    s2[tid * NA + a] = m2[a];
+    sv[tid * NA + a] = var[a];
   }
   __syncthreads();
   // entries of a group: row lanes (over the group's lanes) x its octets or channels of a row
   const int units = p.cg / PER, sub = tid & (p.lpg - 1);
   const int sgroups = min(p.tr * 8, p.c - c0) / p.cg;  // groups of the strip
   const int full = rows / p.rpb, rem = rows - full * p.rpb;
-  const float total = (float)rows * (float)p.cg;
+  // the part of the group's values that an entry with full rows, or one more, stands for
+  const float w0 = (float)full / ((float)rows * (float)units), w1 = (float)(full + 1) / ((float)rows * (float)units);
   for_groups<GN_TT>(sgroups, p.lpg, [&](int g, bool mine) {
+    const float base = sm[g * units];  // differences from one of the means: equal means come out as they are
     float ms = 0.f;
     for (int el = sub; el < p.rpb; el += p.lpg) {
-      const float k = (float)(PER * (full + (el < rem)));
-      for (int u = 0; u < units; ++u) ms = fmaf(k, sm[el * p.tr * NA + g * units + u], ms);
+      const float w = el < rem ? w1 : w0;
+      for (int u = 0; u < units; ++u) ms = fmaf(w, sm[el * p.tr * NA + g * units + u] - base, ms);
     }
-    const float mu = lanes_sum(ms, p.lpg) / total;  // divided: the mean of equal values is that value
+    const float mu = base + lanes_sum(ms, p.lpg);
     float q = 0.f;
     for (int el = sub; el < p.rpb; el += p.lpg) {
-      const float k = (float)(PER * (full + (el < rem)));
-      if (k == 0.f) continue;
+      const float w = el < rem ? w1 : w0;
+      if (w == 0.f) continue;
       for (int u = 0; u < units; ++u) {
         const int at = el * p.tr * NA + g * units + u;
         const float d = sm[at] - mu;
-        q += fmaf(d * d, k, s2[at]);
+        q = fmaf(w, fmaf(d, d, sv[at]), q);
       }
     }
     q = lanes_sum(q, p.lpg);
@@ -267,9 +273,10 @@ __global__ void __launch_bounds__(64) gn_join_kernel(const GroupNormP p) {
   const float2* part = p.part + (n * p.groups + blockIdx.x) * p.nchunk;
   float cnt = 0.f, mu = 0.f, q = 0.f;
   auto join = [&](float k, const float2& v) __attribute__((always_inline)) {
-    const float d = v.x - mu, f = k * __builtin_amdgcn_rcpf(fmaxf(cnt + k, 1.f));
+    if (k == 0.f) return;  // nothing there (its squared distance may be infinite, and 0 of it NaN)
+    const float d = v.x - mu, f = cnt == 0.f ? 1.f : k * __builtin_amdgcn_rcpf(cnt + k);
     mu = fmaf(d, f, mu);
-    q += fmaf(d * d, cnt * f, v.y);
+    q = fmaf(f, fmaf((1.f - f) * d, d, v.y - q), q);
     cnt += k;
   };
   for (int e0 = threadIdx.x; e0 < p.nchunk; e0 += 64 * GN_JOIN) {
@@ -284,12 +291,12 @@ __global__ void __launch_bounds__(64) gn_join_kernel(const GroupNormP p) {
       ks += k;
       ms = fmaf(k, t[j].x, ms);
     }
-    const float m = ms / ks;
+    const float m = ms / ks, per = 1.f / ks;
 #pragma unroll
     for (int j = 0; j < GN_JOIN; ++j) {
       const int e = e0 + j * 64;
       const float k = e < p.nchunk - 1 ? full : e == p.nchunk - 1 ? last : 0.f, d = t[j].x - m;
-      if (e < p.nchunk) qs += fmaf(d * d, k, t[j].y);
+      if (e < p.nchunk) qs = fmaf(k * per, fmaf(d, d, t[j].y), qs);
     }
     join(ks, float2{m, qs});
   }
@@ -299,7 +306,7 @@ __global__ void __launch_bounds__(64) gn_join_kernel(const GroupNormP p) {
     const float2 v = float2{__shfl_xor(mu, o, 64), __shfl_xor(q, o, 64)};
     join(k, v);
   }
-  if (threadIdx.x == 0) p.stat[n * p.groups + blockIdx.x] = float2{mu, rsqrtf(q / ((float)p.p * (float)p.cg) + p.eps)};
+  if (threadIdx.x == 0) p.stat[n * p.groups + blockIdx.x] = float2{mu, rsqrtf(q + p.eps)};
 }
 
 // the affine of 8 channels, all loads in flight together (4-byte aligned: a slice of a vector qualifies)
@@ -392,7 +399,7 @@ __global__ void __launch_bounds__(GN_TS) gn_small_kernel(const GroupNormP p) {
   const bool act = rl < p.rpb && c0 < p.c;
   const int sgroups = min(p.tr * 8, p.c - s0) / p.cg;
   const int units = p.cg / PER;
-  const float total = (float)P * (float)p.cg;
+  const float total = (float)P * (float)p.cg, per = 1.f / total;
   const int64_t xb = n * p.xbs + (act ? c0 : s0);
   f32x8 v[NR];
 #pragma unroll
@@ -420,15 +427,15 @@ __global__ void __launch_bounds__(GN_TS) gn_small_kernel(const GroupNormP p) {
         }
         if (act && rl + k * p.rpb < P) s += t;
       }
-      sm[tid * NA + a] = s;
+      sm[tid * NA + a] = pass ? s * per : s;
     }
     __syncthreads();
     for_groups<GN_TS>(sgroups, p.lpg, [&](int g, bool mine) {
       float s = 0.f;
       for (int el = sub; el < p.rpb; el += p.lpg)
         for (int u = 0; u < units; ++u) s += sm[el * p.tr * NA + g * units + u];
-      s = lanes_sum(s, p.lpg) / total;
-      if (mine && sub == 0) stat[pass][g] = pass ? rsqrtf(s + p.eps) : s;
+      s = lanes_sum(s, p.lpg);
+      if (mine && sub == 0) stat[pass][g] = pass ? rsqrtf(s + p.eps) : s / total;
     });
     __syncthreads();
     int g = oct * 8 / p.cg, gc = oct * 8 - g * p.cg;

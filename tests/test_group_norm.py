@@ -218,6 +218,22 @@ def test_hard_values(hips, gpu_device):
         assert torch.equal(got[1, ..., :16], base[1, ..., :16]) and torch.equal(got[1, ..., 24:], base[1, ..., 24:])
 
 
+# one launch and three, an octet in one group and in several, several strips of channels
+FORMS = [((2, 20, 30, 64), 8), ((2, 9, 11, 96), 32), ((1, 120, 130, 64), 8), ((2, 70, 90, 96), 32), ((3, 40, 50, 2400), 12)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("shape,groups", FORMS)
+def test_values_whose_square_overflows(shape, groups, dt, hips, gpu_device):
+    """Values around 1e20, whose squares fp32 does not hold, with a variance that it does."""
+    noise = torch.randn(*shape, generator=torch.Generator().manual_seed(8))
+    _, w, b = inputs(shape, dt, gpu_device)
+    for size in (1e20, -1e20):
+        x = (size * (1 + 1e-3 * noise)).to(dt).to(gpu_device)
+        check(hips[dt].group_norm(x, groups, w, b), x, groups, w, b, what=f"{size}")
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize("dt", [torch.bfloat16, torch.float32])
 @pytest.mark.parametrize("act", ["silu", "gelu"])
