@@ -10,7 +10,9 @@
 // in a fixed order, all in fp32: no square of an uncentred value occurs, so a mean far from zero or
 // a single large value costs no digits, and the result is deterministic. A variance is carried and no sum
 // of squares, and nothing is joined to an empty part: whatever the count, values only have to lie within 2^60
-// of their group's mean, whose size may be more than a square holds.
+// of their group's mean, whose size may be more than a square holds (up to 2^124, as eight of them are added).
+// The mean of equal values is that value, and their variance 0: eight values are added in pairs, which is exact for
+// equal ones, and means are joined by their differences from one of them.
 //   gn_stats_kernel  per (image, chunk of pixels) the groups' mean and variance: one read of x
 //   gn_join_kernel   per (image, group) the chunks joined: mean, rstd
 //   gn_apply_kernel  y: one read of x, one write
@@ -31,7 +33,7 @@ namespace {
 constexpr int GN_T = 256;    // threads of an apply workgroup
 constexpr int GN_TS = 256;   // threads of a small workgroup
 constexpr int GN_TT = 256;   // threads of a stats workgroup
-constexpr int UR = 8;         // rows in flight per thread (stats)
+constexpr int UR = 8;        // rows in flight per thread (stats; mean8's count)
 constexpr int UA = 4;        // rows in flight per thread (apply)
 constexpr int NRMAX = 8;     // rows held per thread (small), at most
 constexpr int GN_JOIN = 8;   // partial statistics in flight per thread (join)
@@ -73,6 +75,12 @@ __device__ __forceinline__ typename GnRaw<DT>::T gn_raw(const void* x, int64_t i
 }
 template <int DT>
 __device__ __forceinline__ f32x8 gn_widen(const typename GnRaw<DT>::T& v) { return load8<DT>(&v); }
+
+// mean of 8 values, added in pairs
+__device__ __forceinline__ float mean8(float a, float b, float c, float d, float e, float f, float g, float h) {
+  return (((a + b) + (c + d)) + ((e + f) + (g + h))) * 0.125f;
+}
+__device__ __forceinline__ float mean8(const f32x8& x) { return mean8(x.v[0], x.v[1], x.v[2], x.v[3], x.v[4], x.v[5], x.v[6], x.v[7]); }
 
 // sum over the lpg consecutive lanes of a group (lpg a power of two <= 64)
 __device__ __forceinline__ float lanes_sum(float v, int lpg) {
@@ -160,12 +168,10 @@ __global__ void __launch_bounds__(GN_TT) gn_stats_kernel(const GroupNormP p) {
       const float part = cnt ? (float)UR * __builtin_amdgcn_rcpf((float)(cnt + UR)) : 1.f;
 #pragma unroll
       for (int a = 0; a < NA; ++a) {
-        float s = 0.f, q = 0.f;
+        float t[UR], q = 0.f;
 #pragma unroll
-        for (int k = 0; k < UR; ++k)
-#pragma unroll
-          for (int i = 0; i < PER; ++i) s += v[k].v[a * PER + i];
-        const float m = s * (1.f / (UR * PER));
+        for (int k = 0; k < UR; ++k) t[k] = WHOLE ? mean8(v[k]) : v[k].v[a];
+        const float m = mean8(t[0], t[1], t[2], t[3], t[4], t[5], t[6], t[7]);
 #pragma unroll
         for (int k = 0; k < UR; ++k)
 #pragma unroll
@@ -182,10 +188,8 @@ __global__ void __launch_bounds__(GN_TT) gn_stats_kernel(const GroupNormP p) {
       const float part = cnt ? __builtin_amdgcn_rcpf((float)(cnt + 1)) : 1.f;
 #pragma unroll
       for (int a = 0; a < NA; ++a) {
-        float s = 0.f, q = 0.f;
-#pragma unroll
-        for (int i = 0; i < PER; ++i) s += v.v[a * PER + i];
-        const float m = s * (1.f / PER);
+        float q = 0.f;
+        const float m = WHOLE ? mean8(v) : v.v[a];
 #pragma unroll
         for (int i = 0; i < PER; ++i) {
           const float d = v.v[a * PER + i] - m;
@@ -289,9 +293,9 @@ __global__ void __launch_bounds__(64) gn_join_kernel(const GroupNormP p) {
       const int e = e0 + j * 64;
       const float k = e < p.nchunk - 1 ? full : e == p.nchunk - 1 ? last : 0.f;
       ks += k;
-      ms = fmaf(k, t[j].x, ms);
+      if (e < p.nchunk) ms = fmaf(k, t[j].x - t[0].x, ms);
     }
-    const float m = ms / ks, per = 1.f / ks;
+    const float per = 1.f / ks, m = fmaf(ms, per, t[0].x);
 #pragma unroll
     for (int j = 0; j < GN_JOIN; ++j) {
       const int e = e0 + j * 64;
@@ -399,7 +403,7 @@ __global__ void __launch_bounds__(GN_TS) gn_small_kernel(const GroupNormP p) {
   const bool act = rl < p.rpb && c0 < p.c;
   const int sgroups = min(p.tr * 8, p.c - s0) / p.cg;
   const int units = p.cg / PER;
-  const float total = (float)P * (float)p.cg, per = 1.f / total;
+  const float per = 1.f / ((float)P * (float)p.cg);
   const int64_t xb = n * p.xbs + (act ? c0 : s0);
   f32x8 v[NR];
 #pragma unroll
@@ -409,33 +413,43 @@ __global__ void __launch_bounds__(GN_TS) gn_small_kernel(const GroupNormP p) {
   }
   float a[8], b[8];
   gn_affine(p, n, act ? c0 : 0, a, b);
+  const int full = P / p.rpb, rem = P - full * p.rpb, mine_rows = full + (rl < rem);
+  // the part of the group's values that an entry with full rows, or one more, stands for
+  const float w0 = (float)full / ((float)P * (float)units), w1 = (float)(full + 1) / ((float)P * (float)units);
   float mean[NA], rstd[NA];
-#pragma unroll
-  for (int i = 0; i < NA; ++i) mean[i] = 0.f;
 #pragma unroll
   for (int pass = 0; pass < 2; ++pass) {
 #pragma unroll
     for (int a = 0; a < NA; ++a) {
-      float s = 0.f;
+      float s = 0.f, first = 0.f;
 #pragma unroll
       for (int k = 0; k < NR; ++k) {
         float t = 0.f;
+        if (pass) {
 #pragma unroll
-        for (int i = 0; i < PER; ++i) {
-          const float d = v[k].v[a * PER + i] - mean[a];
-          t = pass ? fmaf(d, d, t) : t + d;
+          for (int i = 0; i < PER; ++i) {
+            const float d = v[k].v[a * PER + i] - mean[a];
+            t = fmaf(d, d, t);
+          }
+        } else {
+          t = WHOLE ? mean8(v[k]) : v[k].v[a];
+          if (k == 0) first = t;
+          t -= first;
         }
-        if (act && rl + k * p.rpb < P) s += t;
+        if (act && k < mine_rows) s += t;
       }
-      sm[tid * NA + a] = pass ? s * per : s;
+      sm[tid * NA + a] = pass ? s * per : fmaf(s, 1.f / (float)max(mine_rows, 1), first);
     }
     __syncthreads();
     for_groups<GN_TS>(sgroups, p.lpg, [&](int g, bool mine) {
+      const float base = pass ? 0.f : sm[g * units];
       float s = 0.f;
-      for (int el = sub; el < p.rpb; el += p.lpg)
-        for (int u = 0; u < units; ++u) s += sm[el * p.tr * NA + g * units + u];
+      for (int el = sub; el < p.rpb; el += p.lpg) {
+        const float w = pass ? 1.f : el < rem ? w1 : w0;
+        for (int u = 0; u < units; ++u) s = fmaf(w, sm[el * p.tr * NA + g * units + u] - base, s);
+      }
       s = lanes_sum(s, p.lpg);
-      if (mine && sub == 0) stat[pass][g] = pass ? rsqrtf(s + p.eps) : s / total;
+      if (mine && sub == 0) stat[pass][g] = pass ? rsqrtf(s + p.eps) : base + s;
     });
     __syncthreads();
     int g = oct * 8 / p.cg, gc = oct * 8 - g * p.cg;

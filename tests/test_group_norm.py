@@ -236,6 +236,17 @@ def test_values_whose_square_overflows(shape, groups, dt, hips, gpu_device):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("dt", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("shape,groups", FORMS)
+def test_equal_values(shape, groups, dt, hips, gpu_device):
+    """A group of one value, its mantissa full, has that mean and no variance: the bias comes out."""
+    _, w, b = inputs(shape, dt, gpu_device)
+    for value in (1000.1, 0.1, -100.3, 1e-30, 3e36):
+        x = torch.full(shape, value, dtype=dt, device=gpu_device)
+        assert torch.equal(hips[dt].group_norm(x, groups, w, b), b.to(dt).expand(shape)), value
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt", [torch.bfloat16, torch.float32])
 @pytest.mark.parametrize("act", ["silu", "gelu"])
 @pytest.mark.parametrize("shape", [(1, 20, 30, 64), (1, 120, 130, 64)])
 def test_activations_over_their_range(shape, act, dt, hips, gpu_device):
