@@ -45,6 +45,7 @@ typedef __attribute__((ext_vector_type(4))) short s16x4;
 constexpr int XA_T = 256;    // threads of a join or bits workgroup
 constexpr float XA_FLOOR = -3e38f;  // running maximum before any key: exp2(-inf - XA_FLOOR) = 0, no inf - inf
 constexpr float XA_SLACK = 8.f;     // a running maximum may lag the scores' by this (log2)
+constexpr float XA_FAR = 8388608.f;  // 2^23: up to this size a running maximum is within a quarter of the product it rounds
 
 enum : int { MASK_NONE = 0, MASK_KEYS = 1, MASK_PAIRS = 2 };
 
@@ -167,10 +168,11 @@ __device__ __forceinline__ unsigned xa_bits16(const unsigned char* p, int64_t le
 }
 
 // One tile of NB x 32 keys for a wave's 32 rows: S^T = K Q^T, the softmax's step, O^T += V^T P^T. bits: the keys that
-// count, of a lane's row under MASK_PAIRS; whole: all of them; fresh: o is still 0
+// count, of a lane's row under MASK_PAIRS; whole: all of them; fresh: o is still 0; far: the maximum of
+// a row of the wave has been past XA_FAR
 template <int DT, int D, int C, int MASK, int NB, bool ANEW>
 __device__ __forceinline__ void xa_tile(const unsigned char* ks, const unsigned char* vs, const u32x4 (&qf)[xa_qn<DT, C>],
-                                        f32x16 (&o)[D / 32], float& m, float& l, float c, uint64_t bits, bool whole, bool fresh) {
+                                        f32x16 (&o)[D / 32], float& m, float& l, bool& far, float c, uint64_t bits, bool whole, bool fresh) {
   using T = XaTile<DT, D>;
   constexpr int DB = D / 32, QN = xa_qn<DT, C>;
   // ANEW: the lane's LDS offsets are worked out for each tile instead of kept over the loop, where they spill
@@ -221,12 +223,23 @@ __device__ __forceinline__ void xa_tile(const unsigned char* ks, const unsigned 
     const float alpha = __builtin_amdgcn_exp2f(m - mn);
     m = mn;
     l *= alpha;
+    far |= __any(fabsf(m) > XA_FAR && fabsf(m) < -XA_FLOOR) != 0;
     if (!fresh) {
 #pragma unroll
       for (int b = 0; b < DB; ++b)
 #pragma unroll
         for (int j = 0; j < 16; ++j) o[b][j] *= alpha;
     }
+  }
+  // The product in fmaf(s, c, -m) is exact and m is rounded: past XA_FAR half a step of m would, as an exponent, overflow or
+  // leave nothing of the weights, so there the products are rounded as m was. One bit of the wave, which moves with m alone:
+  // times within 1% (heads of 40 and 80 3%) of those without
+  if (far) {
+#pragma unroll
+    for (int b = 0; b < NB; ++b)
+#pragma unroll
+      for (int j = 0; j < 16; ++j) s[b][j] *= c;
+    c = 1.f;
   }
 #pragma unroll
   for (int b = 0; b < NB; ++b)
@@ -443,7 +456,7 @@ __global__ void __launch_bounds__(XR_T, (DT == DT_BF16 ? D <= 64 : D <= 32) ? 4 
 #pragma unroll
       for (int j = 0; j < 16; ++j) o[b][j] = 0.f;
     float m = XA_FLOOR, l = 0.f;
-    bool fresh = true;  // o is 0
+    bool far = false, fresh = true;  // fresh: o is 0
     // 32 keys at a time (a row of 32 keys starts where the swizzles do), half of a tile in bf16
 #pragma unroll 1
     for (int h = 0; h < lk; h += 32) {
@@ -460,7 +473,7 @@ __global__ void __launch_bounds__(XR_T, (DT == DT_BF16 ? D <= 64 : D <= 32) ? 4 
       } else if (!bits) {
         continue;
       }
-      xa_tile<DT, D, C, MASK, 1, ANEW>(ks, ks + T::BYTES, qf, o, m, l, p.c, bits, bits == 0xffffffffu, fresh);
+      xa_tile<DT, D, C, MASK, 1, ANEW>(ks, ks + T::BYTES, qf, o, m, l, far, p.c, bits, bits == 0xffffffffu, fresh);
       fresh = false;
     }
     l = sum32(l);
@@ -530,6 +543,7 @@ __global__ void __launch_bounds__(64 * W, D <= 64 ? (MASK == MASK_PAIRS ? 3 : 4)
 #pragma unroll
     for (int j = 0; j < 16; ++j) o[b][j] = 0.f;
   float m = XA_FLOOR, l = 0.f;
+  bool far = false;
 
   // 64 tiles at a time: the tiles of which the workgroup (want) and the wave (mine) keep a key, one bit each; the others
   // are neither copied nor waited for
@@ -593,7 +607,7 @@ __global__ void __launch_bounds__(64 * W, D <= 64 ? (MASK == MASK_PAIRS ? 3 : 4)
         if constexpr (MASK == MASK_PAIRS) next = words[t1];
       }
       if (busy && (MASK != MASK_PAIRS || (mine >> (t - c0) & 1)))
-        xa_tile<DT, D, C, MASK, KB, false>(tiles[buf], tiles[buf] + T::BYTES, qf, o, m, l, p.c, now, now == T::ALL, false);
+        xa_tile<DT, D, C, MASK, KB, false>(tiles[buf], tiles[buf] + T::BYTES, qf, o, m, l, far, p.c, now, now == T::ALL, false);
       t = t1;
       t1 = t2;
       buf ^= 1;

@@ -265,6 +265,35 @@ def test_extreme_scores(dt, hips, gpu_device):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dt", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("lq,lk", [(70, 100), (3, 3001), (6200, 700)])
+def test_scores_of_any_size(lq, lk, dt, hips, gpu_device):
+    """Scores up to 2^60 (exact products, equal ones among them, everything else far below): the largest alone count, in
+    equal parts. Their weights are 1 and their sum exact up to the mean's rounding: 2^-8 of the largest value in bf16; in
+    fp32 sums of up to 31 values and two roundings, under 64 * 2^-24 of it. Rows of ordinary scores among them too."""
+    heads, d = 8, 32
+    q0, _, v = inputs(1, lq, lk, heads, heads, d, dt, gpu_device)
+    for size in (2.0 ** 14, 2.0 ** 17, 2.0 ** 30):
+        for sign in (1, -1):
+            q = torch.zeros(1, lq, heads, d, device=gpu_device)
+            q[..., 3] = sign * size * (1 + torch.arange(lq, device=gpu_device) % 7 / 8.)[None, :, None]
+            k = torch.zeros(1, lk, heads, d, device=gpu_device)
+            level = 1 + (torch.arange(lk, device=gpu_device) * 37 % 100) / 128.
+            k[..., 3] = size * level[None, :, None]
+            best = level == (level.max() if sign > 0 else level.min())
+            want = v[:, best].double().mean(1, keepdim=True)
+            q, k = q.flatten(2).to(dt), k.flatten(2).to(dt)
+            tol = (2.0 ** -8 if dt == torch.bfloat16 else 64 * U) * v.double().abs().max()
+            for mask in (None, torch.ones(1, lk, dtype=torch.bool, device=gpu_device), best[None, None].expand(1, lq, lk)):
+                got = hips[dt].cross_attention(q, k, v, heads, mask=mask)
+                assert (got.double() - want).abs().max() <= tol, (size, sign, mask is None or mask.dim())
+            # the other rows of a wave keep their accuracy
+            qm = torch.where((torch.arange(lq, device=gpu_device) % 3 == 0)[None, :, None], q, q0 / size)
+            got = hips[dt].cross_attention(qm, k, v, heads)[:, 1::3].contiguous()
+            check(got, qm[:, 1::3], k, v, heads, what="beside far rows")
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("lq", [1, 300])
 def test_offsets_past_32_bits(lq, hips, gpu_device):
     """Keys and values in rows 2^19 elements apart: the last ones lie past 2^31 elements."""
