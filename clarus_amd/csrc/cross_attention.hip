@@ -43,6 +43,7 @@ typedef __attribute__((ext_vector_type(16))) float f32x16;
 typedef __attribute__((ext_vector_type(4))) short s16x4;
 
 constexpr int XA_T = 256;    // threads of a join or bits workgroup
+constexpr int64_t XA_BITS_GRID = 1 << 20;  // bits workgroups, at most
 constexpr float XA_FLOOR = -3e38f;  // running maximum before any key: exp2(-inf - XA_FLOOR) = 0, no inf - inf
 constexpr float XA_SLACK = 8.f;     // a running maximum may lag the scores' by this (log2)
 constexpr float XA_FAR = 8388608.f;  // 2^23: up to this size a running maximum is within a quarter of the product it rounds
@@ -631,13 +632,13 @@ __global__ void __launch_bounds__(64 * W, D <= 64 ? (MASK == MASK_PAIRS ? 3 : 4)
 }
 
 // MASK_PAIRS: the mask's bytes as bits, 64 keys a word, zeros behind the last key: read once for all heads, and an eighth
-// of the bytes for the kernels' gathers. A thread makes 16 bits
+// of the bytes for the kernels' gathers. A thread makes 16 bits at a time
 __global__ void __launch_bounds__(XA_T) xa_bits_kernel(const unsigned char* mask, int64_t mbs, int64_t mqs, int64_t lq, int64_t lk,
                                                        int64_t nw, int64_t total, unsigned short* out) {
-  const int64_t i = (int64_t)blockIdx.x * XA_T + threadIdx.x;
-  if (i >= total) return;
-  const int64_t row = i / (4 * nw), w = i - row * 4 * nw, n = row / lq, key = 16 * w;
-  out[i] = key < lk ? (unsigned short)xa_bits16(mask + n * mbs + (row - n * lq) * mqs + key, lk - key) : 0;
+  for (int64_t i = (int64_t)blockIdx.x * XA_T + threadIdx.x; i < total; i += (int64_t)gridDim.x * XA_T) {
+    const int64_t row = i / (4 * nw), w = i - row * 4 * nw, n = row / lq, key = 16 * w;
+    out[i] = key < lk ? (unsigned short)xa_bits16(mask + n * mbs + (row - n * lq) * mqs + key, lk - key) : 0;
+  }
 }
 
 // The splits' (O, m, l) joined. TPR threads hold a row's columns (4 each), gs groups of them its splits: group i takes
@@ -845,7 +846,10 @@ extern "C" int clarus_hip_cross_attention(const ClarusCrossArgs* a, void* scratc
                      (a->mask_mode != MASK_PAIRS || a->n * a->lq < ((int64_t)1 << 38) / a->lk),
                  "cross_attention: too large");
   const XaPlan g = xa_plan(a->dtype, a->n, a->lq, a->lk, a->heads, a->kv_heads, a->d, a->mask_mode);
-  CLARUS_REQUIRE(8 * ((g.nblk * a->n * a->kv_heads * g.splits + 7) / 8) < ((int64_t)1 << 31), "cross_attention: too large");
+  // a launch has fewer than 2^32 threads: two for each row here, of n * heads * lq < 2^31 rows (so heads fit an int too)
+  CLARUS_REQUIRE(8 * ((g.nblk * a->n * a->kv_heads * g.splits + 7) / 8) < ((int64_t)1 << 32) / (g.resident ? XR_T : 64 * g.waves) &&
+                     a->n * a->kv_heads * (a->lq * (a->heads / a->kv_heads)) < ((int64_t)1 << 31),
+                 "cross_attention: too large");
   const size_t need = g.bits + g.part;
   CLARUS_REQUIRE(need == 0 || (scratch && aligned(scratch, 16) && scratch_bytes >= need),
                  "cross_attention: scratch %zu < %zu bytes", scratch_bytes, need);
@@ -865,8 +869,9 @@ extern "C" int clarus_hip_cross_attention(const ClarusCrossArgs* a, void* scratc
     k.bits = (const uint64_t*)scratch;
     k.nw = a->mask_qstride ? nw : 0;
     k.bbs = a->mask_bstride ? lq * nw : 0;
-    hipLaunchKernelGGL(xa_bits_kernel, dim3((unsigned)cdiv(total, XA_T)), dim3(XA_T), 0, st, k.mask, a->mask_bstride,
-                       a->mask_qstride, lq, a->lk, nw, total, (unsigned short*)scratch);
+    hipLaunchKernelGGL(xa_bits_kernel, dim3((unsigned)std::min(cdiv(total, XA_T), XA_BITS_GRID)), dim3(XA_T), 0, st, k.mask,
+                       a->mask_bstride, a->mask_qstride, lq, a->lk, nw, total, (unsigned short*)scratch);
+    if (const int rc = check_launch("cross_attention")) return rc;
   }
   const int D = xa_pad(a->d);
   note_kernel("%s d=%d waves=%d splits=%d", g.resident ? "xa_resident_kernel" : "xa_kernel", D, g.resident ? XR_T / 64 : g.waves, g.splits);

@@ -873,8 +873,11 @@ class HipOps(Backend):
         if at is None or at[1] < c or at[1] * es % 16 or at[2] * es % 16:
             raise Unsupported("group_norm: unit channel stride, one pixel stride, 16-byte aligned rows")
         p, ldx, xbs = at
-        if p >= 1 << 31 or n >= 65536 or c >= 1 << 19:
-            raise Unsupported("group_norm: fewer than 2^31 pixels of an image, 65536 images and 2^19 channels")
+        unit = math.lcm(8, c // groups)
+        strips = 1 if c <= 2048 else -(-c // (2048 // unit * unit))  # of channels that a workgroup takes
+        if p >= 1 << 31 or n >= 65536 or c >= 1 << 19 or n * strips >= (1 << 23) - 4096:
+            raise Unsupported("group_norm: fewer than 2^31 pixels of an image, 65536 images, 2^19 channels and 2^23 - 4096 "
+                              "strips of up to 2048 channels in all images")
         return odt, n, p, c, groups, xbs, ldx, wbs, bbs, acode, self.lib.clarus_hip_group_norm_workspace(n, p, c, groups)
 
     # ------------------------------------------------------------------ attention
@@ -935,10 +938,12 @@ class HipOps(Backend):
         es = q.element_size()
         if None in (qa, ka, va) or any(s * es % 16 for t in (qa, ka, va) for s in t[1:]) or max(ka[1], va[1]) >= 1 << 24:
             raise Unsupported("cross_attention: unit channel stride, one row stride (k and v: below 2^24), 16-byte aligned rows")
-        if (max(lk, lq * (heads // kv_heads)) >= 1 << 31 or n * kv_heads >= 65536
+        rows = -(-lq * (heads // kv_heads) // 256) * 256  # of an (image, kv head) pair, in whole workgroups
+        if (lk >= 1 << 31 or n * kv_heads * rows >= (1 << 31) - 4096 or n * kv_heads >= 65536
                 or (mode == _lib.MASK_PAIRS and n * lq >= (1 << 38) // lk)):
-            raise Unsupported("cross_attention: fewer than 2^31 keys and rows, fewer than 65536 (image, kv head) pairs, "
-                              "a [N, Lq, Lk] mask of fewer than 2^38 pairs")
+            raise Unsupported("cross_attention: fewer than 2^31 keys, fewer than 2^31 - 4096 rows (n * heads * lq, those of an "
+                              "(image, kv head) pair rounded up to 256), fewer than 65536 such pairs, a [N, Lq, Lk] mask of "
+                              "fewer than 2^38 pairs")
         args = _lib.CrossArgs(
             n=n, lq=lq, lk=lk, heads=heads, kv_heads=kv_heads, d=d, q_bstride=qa[2], ldq=qa[1], k_bstride=ka[2], ldk=ka[1],
             v_bstride=va[2], ldv=va[1], mask_bstride=mbs, mask_qstride=mqs, dtype=_lib.dtype_code(q.dtype),

@@ -475,7 +475,8 @@ int clarus_hip_selective_scan(const void* u, int32_t u_dtype, const float* dbl, 
  * unless it is x itself, contiguous and of one dtype. act: CLARUS_ACT_NONE, CLARUS_ACT_GELU or
  * CLARUS_ACT_SILU. c a multiple of 8 and of groups, lcm(8, c / groups) at most 2048. Statistics and the
  * affine in fp32, rounded once. scratch holds clarus_hip_group_norm_workspace(...) bytes (the partial
- * statistics; may be 0), 8-byte aligned. Deterministic. p < 2^31, n < 2^16, c < 2^19, eps >= 0.
+ * statistics; may be 0), 8-byte aligned. Deterministic. p < 2^31, n < 2^16, c < 2^19,
+ * fewer than 2^23 - 4096 strips (the most whole lcm(8, c / groups) up to 2048 channels) in all images, eps >= 0.
  * No counterpart in the reference (its norms are the LayerNorm / RMS prologues of linear).
  */
 size_t clarus_hip_group_norm_workspace(int64_t n, int64_t p, int64_t c, int64_t groups);
@@ -495,8 +496,9 @@ int clarus_hip_group_norm(const void* x, int32_t x_dtype, int64_t x_bstride, int
  * masked key counts for nothing, whatever k and v hold. mask_mode 2: kept for query i where
  * mask[n * mask_bstride + i * mask_qstride + j]; k and v of the masked pairs enter no score and weigh 0,
  * so v has to be finite. dtype bf16 or fp32 (of q, k and v), o_dtype either; d a multiple of 8, at most
- * 128; 0 < scale < 2e38. Scores, softmax and output are accumulated in fp32; with bf16 the weights p are rounded
- * once to bf16 for the product with v. scratch holds clarus_hip_cross_attention_workspace(...) bytes
+ * 128; 0 < scale < 2e38; lk < 2^31, n * kv_heads < 2^16, n * heads * lq < 2^31 - 4096 with each (image, kv head)'s
+ * rows rounded up to 256, n * lq * lk < 2^38 with mask_mode 2. Scores, softmax and output are accumulated in fp32; with
+ * bf16 the weights p are rounded once to bf16 for the product with v. scratch holds clarus_hip_cross_attention_workspace(...) bytes
  * (partial results where few rows ask many keys, a mask of pairs as bits; may be 0), 16-byte aligned. Deterministic.
  * No counterpart in the reference (its attention is over channels: clarus_hip_channel_attention).
  */

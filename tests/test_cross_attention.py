@@ -130,6 +130,25 @@ def test_refused_sizes():
             h.cross_attention(*args, **kw)
 
 
+def test_refused_launches():
+    """A launch of 2^32 threads (two for a row) is declined, just below it is not."""
+    import ctypes
+    h, z = cpu_hip(torch.bfloat16), torch.zeros(1, 1, 8, dtype=torch.bfloat16)
+    for heads, lq in ((16, 1 << 27), (1, (1 << 31) - 4097), (2, 1 << 30), (128, (1 << 24) - 40)):
+        with pytest.raises(Unsupported):
+            h.cross_attention(z.expand(1, 1, 8).repeat(1, 1, heads).expand(1, lq, 8 * heads), *[z.repeat(1, 1, heads)] * 2, heads)
+    for heads, lq in ((16, (1 << 27) - 512), (1, (1 << 31) - 4352), (2, (1 << 30) - 2304)):
+        q, kv = torch.zeros(1, 1, 8 * heads, dtype=torch.bfloat16).expand(1, lq, 8 * heads), torch.zeros(1, 1, 8 * heads, dtype=torch.bfloat16)
+        h._cross_plan(q, kv, kv, heads, heads, None, None, torch.bfloat16)
+    lib = _lib.load()
+    for kw in (dict(lq=1 << 28, heads=16, kv_heads=16), dict(lq=1 << 23, n=256, heads=8, kv_heads=1), dict(lq=1, heads=1 << 31, kv_heads=2)):
+        base = dict(q=1 << 20, k=1 << 21, v=1 << 22, out=1 << 23, n=1, lk=200, d=8, ldq=128, ldk=128, ldv=128, dtype=1, o_dtype=1,
+                    mask_mode=0, scale=0.2)
+        args = _lib.CrossArgs(**{**base, **kw})
+        assert lib.clarus_hip_cross_attention(ctypes.byref(args), 1 << 30, 1 << 40, None) == _lib.EINVAL, kw
+        assert b"too large" in lib.clarus_hip_last_error()
+
+
 def test_nothing_to_attend_or_to_ask_cpu():
     h = cpu_hip()
     assert h.cross_attention(torch.zeros(2, 0, 64), torch.zeros(2, 3, 64), torch.zeros(2, 3, 64), 4).shape == (2, 0, 64)
@@ -304,6 +323,19 @@ def test_offsets_past_32_bits(lq, hips, gpu_device):
     got = hips[torch.bfloat16].cross_attention(q, buf[..., :64], buf[..., 128:192], heads)
     assert torch.equal(got, hips[torch.bfloat16].cross_attention(q, k, v, heads))
     check(got, q, k, v, heads)
+
+
+@pytest.mark.gpu
+def test_a_mask_of_billions_of_pairs(hips, gpu_device):
+    """4.4e9 bytes of mask: more words than one pass of the bits kernel's grid makes."""
+    lq, lk, d = (1 << 20) + 1000, 4200, 8
+    q, k, v = inputs(1, 1000, lk, 1, 1, d, torch.bfloat16, gpu_device)
+    row, key = torch.arange(1024, device=gpu_device)[:, None], torch.arange(lk, device=gpu_device)
+    at = torch.arange(lq, device=gpu_device)
+    mask = ((row * 7 + key) % 1024 < 40)[at % 1024][None]
+    got = hips[torch.bfloat16].cross_attention(q[:, at % 1000], k, v, 1, mask=mask)
+    for at in (0, lq // 2 // 1000 * 1000, lq // 1000 * 1000 - 1000):
+        check(got[:, at:at + 1000].contiguous(), q, k, v, 1, mask=mask[:, at:at + 1000], what=str(at))
 
 
 @pytest.mark.gpu

@@ -111,6 +111,13 @@ def test_refused_values():
                                          kw["eps"], 0, None, 0, None) == _lib.EINVAL, kw
 
 
+def test_refused_launches():
+    """As many strips of channels as a launch has no workgroups for."""
+    with pytest.raises(Unsupported):
+        cpu_hip().group_norm(torch.zeros(1, 1, 1 << 18).expand(65535, 1, 1 << 18), 1 << 8)
+    cpu_hip()._group_norm_plan(torch.zeros(1, 1, 1 << 18).expand(65000, 1, 1 << 18), 1 << 8, None, None, None, torch.float32)
+
+
 def test_c_entry_refuses_before_launch():
     lib = _lib.load()
 
