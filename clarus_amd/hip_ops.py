@@ -835,6 +835,8 @@ class HipOps(Backend):
         C / groups channels the mean and biased variance over all pixels of the group's channels, in
         fp32, rounded once. weight, bias: [C], or [N, C] for a scale and shift of each image's own. act
         None, "silu" or "gelu". x may be a channel slice (one pixel stride); the result is contiguous."""
+        if not isinstance(groups, int):  # before the plans, whose keys 4.0 and 4 share
+            raise Unsupported(f"group_norm: groups an integer, got {groups!r}")
         key = ("group_norm", x.shape, x.stride(), x.dtype, groups, act, out_dtype,
                None if weight is None else (weight.shape, weight.dtype), None if bias is None else (bias.shape, bias.dtype))
         self._forward_only("group_norm", x, weight, bias)
@@ -856,7 +858,7 @@ class HipOps(Backend):
         return out
 
     def _group_norm_plan(self, x, groups, weight, bias, act, odt):
-        if x.dim() < 2 or act not in (None, "silu", "gelu") or not isinstance(groups, int) or groups < 1:
+        if x.dim() < 2 or act not in (None, "silu", "gelu") or groups < 1:
             raise Unsupported(f"group_norm: x [N, ..., C], groups >= 1, act none / silu / gelu, got {groups!r} {act!r}")
         n, c = x.shape[0], x.shape[-1]
         if not (_kdt(x) and odt in _KDT and c % 8 == 0 and c % groups == 0 and c > 0
@@ -890,6 +892,8 @@ class HipOps(Backend):
         or [N, Lq, Lk] (v has to be finite: a masked pair weighs 0). fp32 scores, softmax and sums; bf16 weights
         enter the product with v rounded to bf16. Returns a contiguous tensor of q's shape."""
         kv_heads = heads if kv_heads is None else kv_heads
+        if not (isinstance(heads, int) and isinstance(kv_heads, int)):  # before the plans, whose keys 4.0 and 4 share
+            raise Unsupported(f"cross_attention: heads and kv_heads integers, got {heads!r} {kv_heads!r}")
         scale = None if scale is None else float(scale)
         key = ("cross_attention", q.shape, q.stride(), k.shape, k.stride(), v.shape, v.stride(), q.dtype, k.dtype, v.dtype,
                heads, kv_heads, scale, out_dtype, None if mask is None else (mask.shape, mask.stride(), mask.dtype))
@@ -911,8 +915,7 @@ class HipOps(Backend):
         if q.dim() < 2 or k.dim() < 2 or v.dim() < 2:
             raise Unsupported("cross_attention: q, k, v [N, ..., C]")
         n, c, ck = q.shape[0], q.shape[-1], k.shape[-1]
-        if not (isinstance(heads, int) and isinstance(kv_heads, int) and heads > 0 and kv_heads > 0
-                and heads % kv_heads == 0 and c % heads == 0 and k.shape == v.shape and k.shape[0] == n
+        if not (heads > 0 and kv_heads > 0 and heads % kv_heads == 0 and c % heads == 0 and k.shape == v.shape and k.shape[0] == n
                 and ck * heads == c * kv_heads):
             raise Unsupported("cross_attention: q [N, ..., heads d], k and v [N, ..., kv_heads d] of one shape, "
                               "heads a multiple of kv_heads")

@@ -149,6 +149,16 @@ def test_refused_launches():
         assert b"too large" in lib.clarus_hip_last_error()
 
 
+def test_a_refusal_does_not_depend_on_earlier_calls():
+    h = cpu_hip()
+    q, k = torch.zeros(2, 5, 64), torch.zeros(2, 0, 64)
+    for ok, bad in (((4,), (4.0,)), ((4, 2), (4, 2.0)), ((4, 2), (4.0, 2))):
+        kv = k[..., :32] if len(ok) == 2 else k
+        assert h.cross_attention(q, kv, kv, *ok).shape == q.shape
+        with pytest.raises(Unsupported):
+            h.cross_attention(q, kv, kv, *bad)
+
+
 def test_nothing_to_attend_or_to_ask_cpu():
     h = cpu_hip()
     assert h.cross_attention(torch.zeros(2, 0, 64), torch.zeros(2, 3, 64), torch.zeros(2, 3, 64), 4).shape == (2, 0, 64)

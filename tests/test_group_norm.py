@@ -111,6 +111,13 @@ def test_refused_values():
                                          kw["eps"], 0, None, 0, None) == _lib.EINVAL, kw
 
 
+def test_a_refusal_does_not_depend_on_earlier_calls():
+    h, x = cpu_hip(), torch.zeros(2, 0, 4, 16)
+    assert h.group_norm(x, 4).shape == x.shape
+    with pytest.raises(Unsupported):
+        h.group_norm(x, 4.0)
+
+
 def test_refused_launches():
     """As many strips of channels as a launch has no workgroups for."""
     with pytest.raises(Unsupported):
