@@ -24,6 +24,7 @@ import ctypes
 import math
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 from .dft import dft_matrices
@@ -69,6 +70,12 @@ def _raw_stream(index: int) -> int:
 
 # the same without building a Stream object (0.1 instead of 1.8 us of a call)
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", _raw_stream)
+
+
+def _dual_level() -> bool:
+    """A forward-mode level is open (asked first: unpacking an operand costs a microsecond); where torch does not
+    say, one may be."""
+    return getattr(forward_ad, "_current_level", 0) >= 0
 
 
 def _rows(t: torch.Tensor):
@@ -224,8 +231,12 @@ class HipOps(Backend):
 
     def _forward_only(self, what, *ts):
         """Declines what a forward-only op of this device cannot answer: operands elsewhere, and operands
-        whose gradient autograd would lose."""
+        whose gradient or forward-mode tangent autograd would lose."""
         grad = torch.is_grad_enabled()
+        if _dual_level():
+            for t in ts:
+                if t is not None and forward_ad.unpack_dual(t).tangent is not None:
+                    raise Unsupported(f"{what}: an operand carries a forward-mode tangent")
         for t in ts:
             if t is not None and (t.device != self.dev or (grad and t.requires_grad)):
                 if t.device != self.dev:

@@ -159,6 +159,20 @@ def test_a_refusal_does_not_depend_on_earlier_calls():
             h.cross_attention(q, kv, kv, *bad)
 
 
+def test_tangents_are_declined():
+    """A forward-mode tangent would be lost, with gradients enabled or not; outside its level there is none."""
+    from torch.autograd import forward_ad
+    h, q, k = cpu_hip(), torch.zeros(2, 5, 64), torch.zeros(2, 0, 64)
+    with forward_ad.dual_level(), torch.no_grad():
+        dual = forward_ad.make_dual(q, torch.ones_like(q))
+        with pytest.raises(Unsupported, match="tangent"):
+            h.cross_attention(dual, k, k, 4)
+        with pytest.raises(Unsupported, match="tangent"):
+            h.cross_attention(q, k, forward_ad.make_dual(k, k + 1), 4)
+        assert h.cross_attention(q, k, k, 4).shape == q.shape
+    assert h.cross_attention(dual, k, k, 4).shape == q.shape
+
+
 def test_nothing_to_attend_or_to_ask_cpu():
     h = cpu_hip()
     assert h.cross_attention(torch.zeros(2, 0, 64), torch.zeros(2, 3, 64), torch.zeros(2, 3, 64), 4).shape == (2, 0, 64)

@@ -118,6 +118,18 @@ def test_a_refusal_does_not_depend_on_earlier_calls():
         h.group_norm(x, 4.0)
 
 
+def test_tangents_go_to_the_torch_form():
+    from torch.autograd import forward_ad
+    from clarus_amd.spatial_torch import TorchSpatialOps
+    h, be, x, w = cpu_hip(), TorchSpatialOps(torch.float32, "cpu"), torch.randn(2, 4, 4, 16), torch.ones(16)
+    with forward_ad.dual_level():
+        dual = forward_ad.make_dual(x, torch.ones_like(x))
+        for args in ((dual, 4, w), (x, 4, forward_ad.make_dual(w, w))):
+            with pytest.raises(Unsupported, match="tangent"):
+                h.group_norm(*args)
+            assert forward_ad.unpack_dual(be.group_norm(*args)).tangent is not None
+
+
 def test_refused_launches():
     """As many strips of channels as a launch has no workgroups for."""
     with pytest.raises(Unsupported):
