@@ -855,8 +855,8 @@ class HipOps(Backend):
             key, lambda: self._group_norm_plan(x, groups, weight, bias, act, out_dtype or self.dtype))
         if x.data_ptr() % 16:
             raise Unsupported("group_norm: 16-byte aligned rows")
-        if not 0.0 <= eps < math.inf:
-            raise Unsupported("group_norm: eps finite and not negative")
+        if not 0.0 <= eps < 3.4028235e38:
+            raise Unsupported("group_norm: eps finite (as fp32) and not negative")
         out = torch.empty_like(x, dtype=odt, memory_format=torch.contiguous_format)
         if not p:
             return out
@@ -934,10 +934,11 @@ class HipOps(Backend):
         lq, lk = math.prod(q.shape[1:-1]), math.prod(k.shape[1:-1])
         if scale is None and d:
             scale = d ** -0.5
+        held, limit = (ctypes.c_float(s or 0.0).value for s in (scale, 2e38))  # as the call passes them on
         if not (_kdt(q) and q.dtype == k.dtype == v.dtype and odt in _KDT and 8 <= d <= 128 and d % 8 == 0
-                and 0.0 < scale < 2e38):
+                and 0.0 < held < limit):
             raise Unsupported("cross_attention: bf16 / fp32 q, k, v of one type, head width a multiple of 8 up to 128, "
-                              "scale positive and below 2e38")
+                              "scale positive and below 2e38 (as fp32)")
         mode, mbs, mqs = _lib.MASK_NONE, 0, 0
         if mask is not None:
             if mask.dtype != torch.bool or tuple(mask.shape) not in ((n, lk), (n, lq, lk)):

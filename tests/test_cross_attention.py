@@ -173,6 +173,13 @@ def test_tangents_are_declined():
     assert h.cross_attention(dual, k, k, 4).shape == q.shape
 
 
+def test_scales_that_fp32_does_not_hold_are_declined():
+    h, q, k = cpu_hip(), torch.zeros(1, 5, 64), torch.zeros(1, 7, 64)
+    for scale in (1e-46, 7e-46, 1e39, math.nextafter(2e38, 0.0)):  # 0, 0, inf, above 2e38 as fp32
+        with pytest.raises(Unsupported):
+            h.cross_attention(q, k, k, 4, scale=scale)
+
+
 def test_nothing_to_attend_or_to_ask_cpu():
     h = cpu_hip()
     assert h.cross_attention(torch.zeros(2, 0, 64), torch.zeros(2, 3, 64), torch.zeros(2, 3, 64), 4).shape == (2, 0, 64)

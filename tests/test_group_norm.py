@@ -130,6 +130,12 @@ def test_tangents_go_to_the_torch_form():
             assert forward_ad.unpack_dual(be.group_norm(*args)).tangent is not None
 
 
+def test_an_eps_that_fp32_does_not_hold_is_declined():
+    for eps in (1e39, 3.5e38, -1e-50):
+        with pytest.raises(Unsupported):
+            cpu_hip().group_norm(torch.zeros(2, 4, 4, 16), 4, eps=eps)
+
+
 def test_refused_launches():
     """As many strips of channels as a launch has no workgroups for."""
     with pytest.raises(Unsupported):
