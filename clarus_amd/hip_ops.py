@@ -253,6 +253,13 @@ class HipOps(Backend):
             plan = self._plans[key] = make()
         return plan
 
+    def _workspace(self, fn, *args):
+        """fn(*args) with this backend's device current: the library's plans go by its compute units."""
+        if self.dev.type != "cuda" or torch.cuda.current_device() == self.dev.index:
+            return fn(*args)
+        with torch.cuda.device(self.dev):
+            return fn(*args)
+
     def _call(self, what, fn, *args):
         """fn(*args, current stream of this backend's device), with that device current (the library
         launches on the current one)."""
@@ -891,7 +898,8 @@ class HipOps(Backend):
         if p >= 1 << 31 or n >= 65536 or c >= 1 << 19 or n * strips >= (1 << 23) - 4096:
             raise Unsupported("group_norm: fewer than 2^31 pixels of an image, 65536 images, 2^19 channels and 2^23 - 4096 "
                               "strips of up to 2048 channels in all images")
-        return odt, n, p, c, groups, xbs, ldx, wbs, bbs, acode, self.lib.clarus_hip_group_norm_workspace(n, p, c, groups)
+        need = self._workspace(self.lib.clarus_hip_group_norm_workspace, n, p, c, groups)
+        return odt, n, p, c, groups, xbs, ldx, wbs, bbs, acode, need
 
     # ------------------------------------------------------------------ attention
     def cross_attention(self, q, k, v, heads, kv_heads=None, mask=None, scale=None, out_dtype=None):
@@ -963,7 +971,8 @@ class HipOps(Backend):
             n=n, lq=lq, lk=lk, heads=heads, kv_heads=kv_heads, d=d, q_bstride=qa[2], ldq=qa[1], k_bstride=ka[2], ldk=ka[1],
             v_bstride=va[2], ldv=va[1], mask_bstride=mbs, mask_qstride=mqs, dtype=_lib.dtype_code(q.dtype),
             o_dtype=_lib.dtype_code(odt), mask_mode=mode, scale=scale)
-        return odt, args, self.lib.clarus_hip_cross_attention_workspace(args.dtype, n, lq, lk, heads, kv_heads, d, mode)
+        return odt, args, self._workspace(self.lib.clarus_hip_cross_attention_workspace, args.dtype, n, lq, lk, heads, kv_heads,
+                                          d, mode)
 
     def channel_attention(self, qkv, heads, temperature):
         if not qkv.is_contiguous():

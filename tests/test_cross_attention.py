@@ -180,6 +180,34 @@ def test_scales_that_fp32_does_not_hold_are_declined():
             h.cross_attention(q, k, k, 4, scale=scale)
 
 
+def test_workspaces_are_sized_with_the_backends_device_current(monkeypatch):
+    """The splits and chunks go by the current device's compute units: the query runs where the launch will."""
+    h, on, asked = cpu_hip(), [0], []
+    h.dev = torch.device("cuda", 1)
+
+    class Current:
+        def __init__(self, dev):
+            self.dev = dev
+
+        def __enter__(self):
+            on.append(self.dev.index)
+
+        def __exit__(self, *exc):
+            on.pop()
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: on[-1])
+    monkeypatch.setattr(torch.cuda, "device", Current)
+
+    class Lib:
+        def clarus_hip_cross_attention_workspace(self, *args):
+            asked.append(on[-1])
+            return 0
+        clarus_hip_group_norm_workspace = clarus_hip_cross_attention_workspace
+    h.lib, x = Lib(), torch.zeros(1, 5, 64)
+    h._cross_plan(x, x, x, 4, 4, None, None, torch.float32)
+    h._group_norm_plan(x, 8, None, None, None, torch.float32)
+    assert asked == [1, 1] and on == [0]
+
+
 def test_nothing_to_attend_or_to_ask_cpu():
     h = cpu_hip()
     assert h.cross_attention(torch.zeros(2, 0, 64), torch.zeros(2, 3, 64), torch.zeros(2, 3, 64), 4).shape == (2, 0, 64)
