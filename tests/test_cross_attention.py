@@ -449,6 +449,33 @@ def test_keys_that_fit(n, lq, lk, heads, kv_heads, d, dt, hips, gpu_device):
         check(hips[dt].cross_attention(q, k, v, heads, kv_heads, mask), q, k, v, heads, kv_heads, mask, what=kind)
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("n,lq,lk,heads,kv_heads,d", [(1, 6000, 128, 8, 8, 128), (1, 6000, 128, 8, 8, 96), (2, 3000, 97, 4, 4, 72),
+                                                      (2, 3000, 128, 4, 2, 80), (1, 6000, 128, 4, 4, 104), (1, 6000, 75, 4, 4, 112),
+                                                      (1, 2000, 128, 8, 8, 112), (2, 2000, 65, 8, 8, 80)])
+def test_many_rows_on_keys_that_fit(n, lq, lk, heads, kv_heads, d, dt, hips, gpu_device):
+    """Rows enough that the keys stay in LDS, up to 128 KB of them, for every width over 64 that the kernels tell apart."""
+    q, k, v = inputs(n, lq, lk, heads, kv_heads, d, dt, gpu_device, seed=lk)
+    for kind in ("none", "keys", "pairs"):
+        mask = make_mask(kind, n, lq, lk, gpu_device)
+        print(f"[xa] {n} {lq} {lk} {heads} {kv_heads} {d} {kind} {dt}", flush=True)
+        got = hips[dt].cross_attention(q, k, v, heads, kv_heads, mask)
+        assert "xa_resident_kernel" in _lib.last_kernel()
+        check(got, q, k, v, heads, kv_heads, mask, what=kind)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("n,lq,lk,heads,kv_heads,d", [(1, 40, 128, 2, 2, 128), (2, 300, 127, 2, 1, 128), (1, 700, 100, 1, 1, 96), (3, 1, 128, 16, 2, 120)])
+def test_few_rows_of_wide_fp32_heads_split_keys_that_would_fit(n, lq, lk, heads, kv_heads, d, hips, gpu_device):
+    q, k, v = inputs(n, lq, lk, heads, kv_heads, d, torch.float32, gpu_device, seed=lk)
+    for kind in ("none", "keys", "pairs"):
+        mask = make_mask(kind, n, lq, lk, gpu_device)
+        got = hips[torch.float32].cross_attention(q, k, v, heads, kv_heads, mask)
+        assert "xa_kernel" in _lib.last_kernel() and not _lib.last_kernel().endswith("splits=1")
+        check(got, q, k, v, heads, kv_heads, mask, what=kind)
+
+
 def stretches(what, lq, lk, dev):
     """Masks over thousands of keys in one pass: stretches of whole tiles that nothing keeps."""
     key, row = torch.arange(lk, device=dev), torch.arange(lq, device=dev)[:, None]
@@ -483,6 +510,25 @@ def test_long_passes(what, dt, hips, gpu_device):
     check(got, q, k, v, heads, mask=mask, what=what)
     if mask is not None:
         assert not got[:, ~mask.expand(1, lq, lk)[0].any(-1) if mask.dim() == 3 else slice(0, 0 if mask.any() else lq)].any()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("what", ["none", "last keys", "both ends", "one key", "no key", "bands", "late rows", "regions", "scattered keys",
+                                  "scattered pairs"])
+def test_long_parts(what, dt, hips, gpu_device):
+    """Keys split into parts of more than 64 tiles each: the second part's masks past its first 64 tiles."""
+    n, lq, lk, heads, d = 2, 700, 8450, 17, 32
+    q, k, v = inputs(n, lq, lk, heads, heads, d, dt, gpu_device, seed=13)
+    if what.startswith("scattered"):
+        mask = make_mask(what.split()[1], n, lq, lk, gpu_device)
+    else:
+        mask = stretches(what, lq, lk, gpu_device)
+        mask = mask if mask is None else mask.expand(n, *mask.shape[1:])
+    print(f"[xa] {what} {dt}", flush=True)
+    got = hips[dt].cross_attention(q, k, v, heads, mask=mask)
+    assert _lib.last_kernel().endswith("splits=2")
+    check(got, q, k, v, heads, mask=mask, what=what)
 
 
 @pytest.mark.gpu
