@@ -14,7 +14,7 @@ import math
 import torch
 import torch.nn.functional as F
 
-from .dispatch import Backend, _host, register_backend
+from .dispatch import Backend, Unsupported, _host, register_backend
 from .geometry import Small, box_geometry
 
 
@@ -47,7 +47,13 @@ class TorchSpatialOps(Backend):
     def group_norm(self, x, groups, weight=None, bias=None, eps=1e-5, act=None, out_dtype=None):
         """Group norm of x [N, ..., C], channels last, in fp32 (weight and bias [C] or [N, C]), then
         SiLU / GELU."""
+        if x.dim() < 2 or act not in (None, "silu", "gelu") or not isinstance(groups, int) or groups < 1 or x.shape[-1] % groups:
+            raise Unsupported(f"group_norm: x [N, ..., C], groups of C, act none / silu / gelu, got {groups!r} {act!r}")
         n, c = x.shape[0], x.shape[-1]
+        if any(t is not None and (tuple(t.shape) not in ((c,), (n, c)) or not t.is_floating_point()) for t in (weight, bias)):
+            raise Unsupported("group_norm: weight and bias [C] or [N, C]")
+        if not 0.0 <= eps < math.inf or not (out_dtype or self.dtype).is_floating_point:
+            raise Unsupported("group_norm: eps finite and not negative, a floating-point output")
         p = math.prod(x.shape[1:-1])
         y = x.float().reshape(n, p, groups, c // groups)
         var, mean = torch.var_mean(y, (1, 3), correction=0, keepdim=True)

@@ -86,6 +86,20 @@ def test_refusals(shape, groups, kw):
         cpu_hip().group_norm(torch.zeros(shape), groups, **kw)
 
 
+@pytest.mark.parametrize("kw", [{"act": "relu"}, {"act": True}, {"groups": 3}, {"groups": 0}, {"groups": 2.0}, {"weight": torch.ones(16, 2)},
+                                {"weight": torch.ones(32)}, {"bias": torch.ones(1, 1, 16)}, {"bias": torch.ones(16, dtype=torch.int64)},
+                                {"eps": -1.0}, {"eps": float("nan")}, {"out_dtype": torch.int32}])
+def test_what_no_backend_answers_is_declined_by_all(kw):
+    """The torch form of the chain declines too what is no group norm, instead of answering something else."""
+    from clarus_amd.spatial_torch import TorchSpatialOps
+    args = {"groups": 4, **kw}
+    for be in (cpu_hip(), TorchSpatialOps(torch.float32, "cpu")):
+        with pytest.raises(Unsupported):
+            be.group_norm(torch.zeros(2, 4, 4, 16), **args)
+    with pytest.raises(Unsupported):
+        TorchSpatialOps(torch.float32, "cpu").group_norm(torch.zeros(16), 4)
+
+
 def test_refused_layouts_and_gradients():
     h = cpu_hip()
     for x in (torch.zeros(2, 4, 4, 32)[..., ::2], torch.zeros(2, 16, 4, 4).permute(0, 2, 3, 1),
