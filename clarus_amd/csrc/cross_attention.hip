@@ -778,6 +778,15 @@ XaPlan xa_plan(int32_t dt, int64_t n, int64_t lq, int64_t lk, int64_t heads, int
   return g;
 }
 
+// What 32-bit counts and a launch of fewer than 2^32 threads (two for each of n * heads * lq rows) hold. Each size on its own
+// first, so that no product wraps
+bool xa_fits(int64_t n, int64_t lq, int64_t lk, int64_t heads, int64_t kv_heads, int mask) {
+  const int64_t big = (int64_t)1 << 31;
+  return n < 65536 && kv_heads < 65536 && n * kv_heads < 65536 && heads < big && lq < big && lk < big &&
+         lq * (heads / kv_heads) < big && n * kv_heads * (lq * (heads / kv_heads)) < big &&
+         (mask != MASK_PAIRS || n * lq < ((int64_t)1 << 38) / lk);
+}
+
 template <int DT, int D, int C>
 void xa_launch(const CrossP& k, bool resident, int waves, int mask, hipStream_t st) {
   const dim3 grid((unsigned)(8 * ((k.nblk * k.nk * k.splits + 7) / 8)));
@@ -815,7 +824,9 @@ using namespace clarus;
 
 extern "C" size_t clarus_hip_cross_attention_workspace(int32_t dtype, int64_t n, int64_t lq, int64_t lk, int64_t heads,
                                                        int64_t kv_heads, int64_t d, int32_t mask_mode) {
-  if (n <= 0 || lq <= 0 || lk <= 0 || kv_heads <= 0 || heads <= 0 || heads % kv_heads || d <= 0 || d > 128) return 0;
+  if (n <= 0 || lq <= 0 || lk <= 0 || kv_heads <= 0 || heads <= 0 || heads % kv_heads || d <= 0 || d > 128 ||
+      !xa_fits(n, lq, lk, heads, kv_heads, mask_mode))
+    return 0;
   const XaPlan g = xa_plan(dtype, n, lq, lk, heads, kv_heads, d, mask_mode);
   return g.bits + g.part;
 }
@@ -841,15 +852,10 @@ extern "C" int clarus_hip_cross_attention(const ClarusCrossArgs* a, void* scratc
   CLARUS_REQUIRE(a->mask_mode >= MASK_NONE && a->mask_mode <= MASK_PAIRS && (a->mask_mode == MASK_NONE || a->mask) &&
                      a->mask_bstride >= 0 && a->mask_qstride >= 0,
                  "cross_attention: mask");
-  CLARUS_REQUIRE(a->lq < ((int64_t)1 << 31) && a->lk < ((int64_t)1 << 31) && a->n * a->kv_heads < 65536 &&
-                     a->lq * (a->heads / a->kv_heads) < ((int64_t)1 << 31) &&
-                     (a->mask_mode != MASK_PAIRS || a->n * a->lq < ((int64_t)1 << 38) / a->lk),
-                 "cross_attention: too large");
+  CLARUS_REQUIRE(xa_fits(a->n, a->lq, a->lk, a->heads, a->kv_heads, a->mask_mode), "cross_attention: too large");
   const XaPlan g = xa_plan(a->dtype, a->n, a->lq, a->lk, a->heads, a->kv_heads, a->d, a->mask_mode);
-  // a launch has fewer than 2^32 threads: two for each row here, of n * heads * lq < 2^31 rows (so heads fit an int too)
-  CLARUS_REQUIRE(8 * ((g.nblk * a->n * a->kv_heads * g.splits + 7) / 8) < ((int64_t)1 << 32) / (g.resident ? XR_T : 64 * g.waves) &&
-                     a->n * a->kv_heads * (a->lq * (a->heads / a->kv_heads)) < ((int64_t)1 << 31),
-                 "cross_attention: too large");
+  CLARUS_REQUIRE(8 * ((g.nblk * a->n * a->kv_heads * g.splits + 7) / 8) < ((int64_t)1 << 32) / (g.resident ? XR_T : 64 * g.waves),
+                 "cross_attention: too large");  // rows that fill few of their workgroups
   const size_t need = g.bits + g.part;
   CLARUS_REQUIRE(need == 0 || (scratch && aligned(scratch, 16) && scratch_bytes >= need),
                  "cross_attention: scratch %zu < %zu bytes", scratch_bytes, need);

@@ -478,6 +478,9 @@ __global__ void __launch_bounds__(GN_TS) gn_small_kernel(const GroupNormP p) {
 // workgroups of a launch over per (strip, chunk) pairs of each of n images, as gn_at has them
 unsigned gn_grid(int64_t n, int64_t per, bool parts) { return (unsigned)(parts || per < 8 ? 8 * cdiv(n * per, 8) : n * 8 * cdiv(per, 8)); }
 
+// 32 bits: the pixels of an image, the workgroups of a launch; the join's grid has at most 65535 images
+bool gn_fits(int64_t n, int64_t p, int64_t c) { return p < ((int64_t)1 << 31) && n < 65536 && c < ((int64_t)1 << 19); }
+
 // least common multiple of 8 and cg
 int64_t gn_unit(int64_t cg) { return cg % 8 == 0 ? cg : cg % 4 == 0 ? 2 * cg : cg % 2 == 0 ? 4 * cg : 8 * cg; }
 
@@ -529,7 +532,7 @@ GnPlan gn_plan(int64_t n, int64_t p, int64_t c, int64_t groups) {
 using namespace clarus;
 
 extern "C" size_t clarus_hip_group_norm_workspace(int64_t n, int64_t p, int64_t c, int64_t groups) {
-  if (n <= 0 || p <= 0 || c <= 0 || groups <= 0 || c % groups || c % 8 || gn_unit(c / groups) > GN_UNIT) return 0;
+  if (n <= 0 || p <= 0 || c <= 0 || groups <= 0 || c % groups || c % 8 || !gn_fits(n, p, c) || gn_unit(c / groups) > GN_UNIT) return 0;
   const GnPlan g = gn_plan(n, p, c, groups);
   return g.small ? 0 : (size_t)(n * groups * (g.nchunk + 1)) * sizeof(float2);
 }
@@ -544,6 +547,7 @@ extern "C" int clarus_hip_group_norm(const void* x, int32_t x_dtype, int64_t x_b
   CLARUS_REQUIRE((x_dtype == DT_BF16 || x_dtype == DT_F32) && (o_dtype == DT_BF16 || o_dtype == DT_F32),
                  "group_norm: bf16 or fp32");
   CLARUS_REQUIRE(c % 8 == 0 && c % groups == 0, "group_norm: channels a multiple of 8 and of the groups");
+  CLARUS_REQUIRE(gn_fits(n, p, c), "group_norm: too large");
   CLARUS_REQUIRE(gn_unit(c / groups) <= GN_UNIT, "group_norm: lcm(8, channels per group) at most %d", GN_UNIT);
   CLARUS_REQUIRE(act == ACT_NONE || act == ACT_GELU || act == CLARUS_ACT_SILU, "group_norm: act none, GELU or SiLU");
   const int64_t es = x_dtype == DT_BF16 ? 2 : 4;
@@ -552,8 +556,6 @@ extern "C" int clarus_hip_group_norm(const void* x, int32_t x_dtype, int64_t x_b
                  "group_norm: x and out 16-byte aligned rows");
   CLARUS_REQUIRE((w_bstride == 0 || w_bstride >= c) && (b_bstride == 0 || b_bstride >= c), "group_norm: affine strides");
   CLARUS_REQUIRE(eps >= 0.f && eps < INFINITY, "group_norm: eps finite and not negative");
-  // 32 bits: the pixels of an image, the workgroups of a launch; the join's grid has at most 65535 images
-  CLARUS_REQUIRE(p < ((int64_t)1 << 31) && n < 65536 && c < ((int64_t)1 << 19), "group_norm: too large");
   const size_t need = clarus_hip_group_norm_workspace(n, p, c, groups);
   CLARUS_REQUIRE(need == 0 || (scratch && scratch_bytes >= need && aligned(scratch, 8)), "group_norm: scratch %zu < %zu bytes", scratch_bytes, need);
   const GnPlan g = gn_plan(n, p, c, groups);

@@ -208,6 +208,22 @@ def test_workspaces_are_sized_with_the_backends_device_current(monkeypatch):
     assert asked == [1, 1] and on == [0]
 
 
+def test_sizes_whose_products_overflow_are_refused():
+    """Products of the C entry's sizes that wrap around 64 bits do not pass for small ones."""
+    import ctypes
+    lib = _lib.load()
+    base = dict(q=1 << 20, k=1 << 21, v=1 << 22, out=1 << 23, n=1, lq=4, lk=64, heads=4, kv_heads=1, d=8, ldq=32, ldk=32, ldv=32,
+                dtype=1, o_dtype=1, mask_mode=0, scale=0.2)
+    for kw in (dict(heads=1 << 62), dict(n=1 << 62, kv_heads=4), dict(n=1 << 60, kv_heads=16, heads=16), dict(kv_heads=1 << 62, heads=1 << 62),
+               dict(n=1 << 61, lq=8, mask_mode=2, mask=16), dict(heads=1 << 33, kv_heads=4, lq=1 << 31)):
+        assert lib.clarus_hip_cross_attention(ctypes.byref(_lib.CrossArgs(**{**base, **kw})), 1 << 30, 1 << 40, None) == _lib.EINVAL, kw
+        assert b"too large" in lib.clarus_hip_last_error(), kw
+    assert lib.clarus_hip_cross_attention_workspace(1, 1 << 62, 1, 100000, 4, 4, 8, 0) == 0
+    assert lib.clarus_hip_cross_attention_workspace(1, 1, 4, 100000, 1 << 62, 1, 8, 0) == 0
+    assert lib.clarus_hip_group_norm_workspace(1 << 62, 100000, 64, 8) == 0
+    assert lib.clarus_hip_group_norm_workspace(1, 1 << 62, 64, 8) == 0
+
+
 def test_nothing_to_attend_or_to_ask_cpu():
     h = cpu_hip()
     assert h.cross_attention(torch.zeros(2, 0, 64), torch.zeros(2, 3, 64), torch.zeros(2, 3, 64), 4).shape == (2, 0, 64)
