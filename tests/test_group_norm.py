@@ -292,6 +292,42 @@ def test_equal_values(shape, groups, dt, hips, gpu_device):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("shape,groups", FORMS)
+def test_what_is_not_finite_stays_in_its_group(shape, groups, hips, gpu_device):
+    """First and last values of a group among them: what other values are taken relative to."""
+    hip, size = hips[torch.float32], shape[-1] // groups
+    x, w, b = inputs(shape, torch.float32, gpu_device)
+    base = hip.group_norm(x, groups, w, b)
+    g = groups // 2
+    inside = slice(g * size, (g + 1) * size)
+    for bad in (float("nan"), float("inf"), -float("inf")):
+        for at in ((0, 0, g * size), (shape[1] - 1, shape[2] - 1, (g + 1) * size - 1), (shape[1] // 2, 3, g * size + size // 2)):
+            y = x.clone()
+            y[(shape[0] - 1, *at)] = bad
+            got = hip.group_norm(y, groups, w, b)
+            assert torch.equal(got[:-1], base[:-1]) and not torch.isfinite(got[-1, ..., inside]).any(), (bad, at)
+            assert torch.equal(got[-1, ..., :g * size], base[-1, ..., :g * size]), (bad, at)
+            assert torch.equal(got[-1, ..., (g + 1) * size:], base[-1, ..., (g + 1) * size:]), (bad, at)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("shape,groups", FORMS)
+def test_c_entry_in_place(shape, groups, dt, hips, gpu_device):
+    """out may be x itself."""
+    hip = hips[dt]
+    x, w, b = inputs(shape, dt, gpu_device)
+    want = hip.group_norm(x, groups, w, b, act="silu")
+    n, p, c, code = shape[0], shape[1] * shape[2], shape[-1], _lib.dtype_code(dt)
+    need = hip.lib.clarus_hip_group_norm_workspace(n, p, c, groups)
+    scratch = torch.empty(max(need, 8), dtype=torch.uint8, device=gpu_device)
+    _lib.check(hip.lib.clarus_hip_group_norm(x.data_ptr(), code, p * c, c, w.data_ptr(), 0, b.data_ptr(), 0, x.data_ptr(), code, n, p, c,
+                                             groups, EPS, _lib.ACT_SILU, scratch.data_ptr(), need,
+                                             torch.cuda.current_stream().cuda_stream), "group_norm")
+    assert torch.equal(x, want)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("dt", [torch.bfloat16, torch.float32])
 @pytest.mark.parametrize("act", ["silu", "gelu"])
 @pytest.mark.parametrize("shape", [(1, 20, 30, 64), (1, 120, 130, 64)])
