@@ -43,7 +43,7 @@ typedef __attribute__((ext_vector_type(16))) float f32x16;
 typedef __attribute__((ext_vector_type(4))) short s16x4;
 
 constexpr int XA_T = 256;    // threads of a join or bits workgroup
-constexpr int64_t XA_BITS_GRID = 1 << 20;  // bits workgroups, at most
+constexpr int64_t XA_BITS_GRID = 1 << 20;  // workgroups of a bits launch, at most
 constexpr float XA_FLOOR = -3e38f;  // running maximum before any key: exp2(-inf - XA_FLOOR) = 0, no inf - inf
 constexpr float XA_SLACK = 8.f;     // a running maximum may lag the scores' by this (log2)
 constexpr float XA_FAR = 8388608.f;  // 2^23: up to this size a running maximum is within a quarter of the product it rounds
@@ -483,7 +483,8 @@ __global__ void __launch_bounds__(XR_T, (DT == DT_BF16 ? D <= 64 : D <= 32) ? 4 
 }
 
 // ---------------------------------------------------------------- keys streamed through LDS
-// W waves of 32 rows. (MASK_PAIRS at 3 waves per SIMD: it spills at 4.)
+// W waves of 32 rows. (MASK_PAIRS at 3 waves per SIMD: at 4 it spills. Of those at 4, two forms of masked keys in four waves keep
+// a few registers in scratch: bf16 heads of 40 and 48 three, fp32 heads of 56 and 64 four.)
 template <int DT, int D, int C, int MASK, int W>
 __global__ void __launch_bounds__(64 * W, D <= 64 ? (MASK == MASK_PAIRS ? 3 : 4) : 2) xa_kernel(const CrossP p) {
   using T = XaTile<DT, D>;
@@ -632,13 +633,13 @@ __global__ void __launch_bounds__(64 * W, D <= 64 ? (MASK == MASK_PAIRS ? 3 : 4)
 }
 
 // MASK_PAIRS: the mask's bytes as bits, 64 keys a word, zeros behind the last key: read once for all heads, and an eighth
-// of the bytes for the kernels' gathers. A thread makes 16 bits at a time
+// of the bytes for the kernels' gathers. A thread makes 16 bits. first: what the launches before have made
 __global__ void __launch_bounds__(XA_T) xa_bits_kernel(const unsigned char* mask, int64_t mbs, int64_t mqs, int64_t lq, int64_t lk,
-                                                       int64_t nw, int64_t total, unsigned short* out) {
-  for (int64_t i = (int64_t)blockIdx.x * XA_T + threadIdx.x; i < total; i += (int64_t)gridDim.x * XA_T) {
-    const int64_t row = i / (4 * nw), w = i - row * 4 * nw, n = row / lq, key = 16 * w;
-    out[i] = key < lk ? (unsigned short)xa_bits16(mask + n * mbs + (row - n * lq) * mqs + key, lk - key) : 0;
-  }
+                                                       int64_t nw, int64_t first, int64_t total, unsigned short* out) {
+  const int64_t i = first + (int64_t)blockIdx.x * XA_T + threadIdx.x;
+  if (i >= total) return;
+  const int64_t row = i / (4 * nw), w = i - row * 4 * nw, n = row / lq, key = 16 * w;
+  out[i] = key < lk ? (unsigned short)xa_bits16(mask + n * mbs + (row - n * lq) * mqs + key, lk - key) : 0;
 }
 
 // The splits' (O, m, l) joined. TPR threads hold a row's columns (4 each), gs groups of them its splits: group i takes
@@ -875,8 +876,9 @@ extern "C" int clarus_hip_cross_attention(const ClarusCrossArgs* a, void* scratc
     k.bits = (const uint64_t*)scratch;
     k.nw = a->mask_qstride ? nw : 0;
     k.bbs = a->mask_bstride ? lq * nw : 0;
-    hipLaunchKernelGGL(xa_bits_kernel, dim3((unsigned)std::min(cdiv(total, XA_T), XA_BITS_GRID)), dim3(XA_T), 0, st, k.mask,
-                       a->mask_bstride, a->mask_qstride, lq, a->lk, nw, total, (unsigned short*)scratch);
+    for (int64_t first = 0; first < total; first += XA_BITS_GRID * XA_T)
+      hipLaunchKernelGGL(xa_bits_kernel, dim3((unsigned)std::min(cdiv(total - first, XA_T), XA_BITS_GRID)), dim3(XA_T), 0, st,
+                         k.mask, a->mask_bstride, a->mask_qstride, lq, a->lk, nw, first, total, (unsigned short*)scratch);
     if (const int rc = check_launch("cross_attention")) return rc;
   }
   const int D = xa_pad(a->d);

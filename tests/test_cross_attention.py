@@ -402,7 +402,7 @@ def test_offsets_past_32_bits(lq, hips, gpu_device):
 
 @pytest.mark.gpu
 def test_a_mask_of_billions_of_pairs(hips, gpu_device):
-    """4.4e9 bytes of mask: more words than one pass of the bits kernel's grid makes."""
+    """4.4e9 bytes of mask: more words than one launch of the bits kernel makes."""
     lq, lk, d = (1 << 20) + 1000, 4200, 8
     q, k, v = inputs(1, 1000, lk, 1, 1, d, torch.bfloat16, gpu_device)
     row, key = torch.arange(1024, device=gpu_device)[:, None], torch.arange(lk, device=gpu_device)
