@@ -24,11 +24,11 @@
 //
 // What bounds it (bf16, the GPU's time alone, without the call's).
 //   Many rows and keys: the softmax's arithmetic and the matrix cores, which overlap in part. 14400 queries x 3600 keys, 8
-//   heads of 64: 122 us, 868 TFLOP/s (a large library product reaches 1190); 57600 x 3600, 4 heads of 128: 450 us, 943.
-//   In the first the VALU is busy for 72% of the cycles (an exponential counts twice), the matrix cores for 45%, in the
-//   second for 44% and 47%, at clocks that the load lowers to 1.8 and 1.9 GHz.
-//   A prompt (57600 x 77, 4 heads of 64): 12 us of reading q and writing o at the rate of a large copy; 18.5 us, a wave
-//   loading, multiplying and weighing its few keys in turn: the VALU is busy for 62% of the cycles.
+//   heads of 64: 117 to 129 us by the card, 822 to 907 TFLOP/s (a large library product reaches 1190); 57600 x 3600, 4 heads of
+//   128: 434 to 477 us, 890 to 979. In the first the VALU is busy for 70% of the cycles (an exponential counts twice), the
+//   matrix cores for 44%, in the second for 43% and 45%, at clocks that the load lowers to 1.8 and 1.9 GHz.
+//   A prompt (57600 x 77, 4 heads of 64): 12 us of reading q and writing o at the rate of a large copy; 18.3 us, a wave
+//   loading, multiplying and weighing its few keys in turn: the VALU is busy for 55% of the cycles.
 //   One query of 8 images x 30001 keys: reading K and V, 492 MB in 94 us, 5.2 TB/s (a large copy: 4.8 TB/s).
 #include <algorithm>
 

@@ -19,8 +19,8 @@
 //   gn_small_kernel  all in one launch, x held in registers between them, where the pixels of a few
 //                    whole groups fit one workgroup
 // What bounds it: memory. 720 x 1280 x 64 bf16 with GELU, 236 MB in and out: 62 us with x in the last-level cache
-// (statistics 24, join 5, apply 36 us traced, the last at 96% VALU issue), 81 us cold; 2 x 173 x 251 x 128 fp32 with SiLU,
-// 89 MB: 27 us. Small maps: the launches (90 x 160 x 512 bf16, 29 MB: 8 + 3 + 7 us).
+// (statistics 24, join 5, apply 36 us traced, the last at 97% VALU issue), 81 us cold; 2 x 173 x 251 x 128 fp32 with SiLU,
+// 89 MB: 27 us. Small maps: the launches (90 x 160 x 512 bf16, 29 MB: 8 + 3 + 8 us).
 #include <algorithm>
 
 #include "capi.hpp"

@@ -475,7 +475,8 @@ int clarus_hip_selective_scan(const void* u, int32_t u_dtype, const float* dbl, 
  * unless it is x itself, contiguous and of one dtype. act: CLARUS_ACT_NONE, CLARUS_ACT_GELU or
  * CLARUS_ACT_SILU. c a multiple of 8 and of groups, lcm(8, c / groups) at most 2048. Statistics and the
  * affine in fp32, rounded once. scratch holds clarus_hip_group_norm_workspace(...) bytes (the partial
- * statistics; may be 0), 8-byte aligned. Deterministic. p < 2^31, n < 2^16, c < 2^19,
+ * statistics; may be 0), 8-byte aligned. Deterministic. Values below 2^124 in size and within 2^60 of their group's
+ * mean (further away the statistics overflow). p < 2^31, n < 2^16, c < 2^19,
  * fewer than 2^23 - 4096 strips (the most whole lcm(8, c / groups) up to 2048 channels) in all images, eps >= 0.
  * No counterpart in the reference (its norms are the LayerNorm / RMS prologues of linear).
  */
