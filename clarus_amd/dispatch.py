@@ -1,7 +1,7 @@
 """Per-operator backend dispatch: the contract the `hip` backend plugs into.
 
 This restates clarus's dispatcher (python/clarus/ops/__init__.py:27-138) so the HIP backend
-can be registered, exercised and tested without the reference package on the GPU box.
+can be registered, exercised and tested without the reference package installed.
 
 Contract (same names, arguments and error behaviour as the reference):
   * `Unsupported` raised by a backend op hands the call to the next backend in the chain;
