@@ -1,6 +1,6 @@
 """ctypes binding of libclarus_hip.so (declarations: include/clarus_hip.h).
 
-The structures below mirror ClarusGemmArgs / ClarusConvArgs / ClarusCrossArgs field by field; `load()` checks
+The structures below mirror ClarusGemmArgs, ClarusConvArgs, ClarusCrossArgs and their like field by field; `load()` checks
 their sizes against the library's own sizeof and the ABI version before handing it out.
 torch is imported first so that the process's HIP runtime is torch's (the library links the
 same soname, libamdhip64.so.7, and binds to the already-loaded copy).
@@ -24,6 +24,8 @@ A_ROWS, A_S2D = 0, 1
 C_ROWS, C_SHUFFLE, C_NCHW = 0, 1, 2
 ACT_NONE, ACT_GELU, ACT_LRELU, ACT_SILU = 0, 1, 2, 3
 MASK_NONE, MASK_KEYS, MASK_PAIRS = 0, 1, 2  # mask_mode of clarus_hip_cross_attention
+ROTARY_AXES, ROTARY_PAIRS = 4, 128
+POS_GRID, POS_F32, POS_I32, POS_I64 = 0, 1, 2, 3  # pos_kind of clarus_hip_rotary
 CHANNEL_ATTENTION_SCRATCH_MAX = 16 << 20  # bytes of clarus_hip_channel_attention_noalloc's static scratch
 
 _vp, _i64, _i32, _f32 = ctypes.c_void_p, ctypes.c_int64, ctypes.c_int32, ctypes.c_float
@@ -69,6 +71,28 @@ class CrossArgs(ctypes.Structure):
     ]
 
 
+class RotaryArgs(ctypes.Structure):
+    _fields_ = [
+        ("x", _vp), ("out", _vp), ("positions", _vp),
+        ("n", _i64), ("l", _i64), ("heads", _i64), ("d", _i64),
+        ("x_bstride", _i64), ("ldx", _i64), ("pos_bstride", _i64), ("ldpos", _i64),
+        ("grid", _i64 * ROTARY_AXES), ("sections", _i64 * ROTARY_AXES), ("turn", ctypes.c_double * ROTARY_PAIRS),
+        ("axes", _i32), ("pairs_mode", _i32), ("pos_kind", _i32), ("dtype", _i32), ("o_dtype", _i32),
+    ]
+
+
+class AddNormArgs(ctypes.Structure):
+    _fields_ = [
+        ("x", _vp), ("y", _vp), ("sum", _vp), ("norm", _vp),
+        ("gate", _vp), ("post_w", _vp), ("post_b", _vp), ("w", _vp), ("b", _vp),
+        ("n", _i64), ("rows", _i64), ("c", _i64),
+        ("x_bstride", _i64), ("ldx", _i64), ("y_bstride", _i64), ("ldy", _i64),
+        ("gate_bstride", _i64), ("post_w_bstride", _i64), ("post_b_bstride", _i64), ("w_bstride", _i64), ("b_bstride", _i64),
+        ("x_dtype", _i32), ("y_dtype", _i32), ("sum_dtype", _i32), ("norm_dtype", _i32), ("post", _i32), ("pre", _i32),
+        ("scale", _f32), ("eps", _f32),
+    ]
+
+
 # name -> (restype, argtypes); every function declared in include/clarus_hip.h
 SIGNATURES = {
     "clarus_hip_gemm": (_i32, [ctypes.POINTER(GemmArgs), _vp]),
@@ -108,10 +132,14 @@ SIGNATURES = {
                                      _f32, _i32, _vp, ctypes.c_size_t, _vp]),
     "clarus_hip_cross_attention_workspace": (ctypes.c_size_t, [_i32, _i64, _i64, _i64, _i64, _i64, _i64, _i32]),
     "clarus_hip_cross_attention": (_i32, [ctypes.POINTER(CrossArgs), _vp, ctypes.c_size_t, _vp]),
+    "clarus_hip_rotary": (_i32, [ctypes.POINTER(RotaryArgs), _vp]),
+    "clarus_hip_add_norm": (_i32, [ctypes.POINTER(AddNormArgs), _vp]),
     "clarus_hip_abi_version": (_i32, []),
     "clarus_hip_sizeof_gemm_args": (ctypes.c_size_t, []),
     "clarus_hip_sizeof_conv_args": (ctypes.c_size_t, []),
     "clarus_hip_sizeof_cross_args": (ctypes.c_size_t, []),
+    "clarus_hip_sizeof_rotary_args": (ctypes.c_size_t, []),
+    "clarus_hip_sizeof_add_norm_args": (ctypes.c_size_t, []),
     "clarus_hip_last_error": (ctypes.c_char_p, []),
     "clarus_hip_last_kernel": (ctypes.c_char_p, []),
 }
@@ -144,6 +172,9 @@ def load(path: str = LIB_PATH):
         raise RuntimeError("ClarusConvArgs layout differs between the library and the binding")
     if lib.clarus_hip_sizeof_cross_args() != ctypes.sizeof(CrossArgs):
         raise RuntimeError("ClarusCrossArgs layout differs between the library and the binding")
+    for cls, name in ((RotaryArgs, "rotary"), (AddNormArgs, "add_norm")):
+        if getattr(lib, f"clarus_hip_sizeof_{name}_args")() != ctypes.sizeof(cls):
+            raise RuntimeError(f"{cls.__name__} layout differs between the library and the binding")
     _LIB = lib
     return lib
 

@@ -51,6 +51,10 @@ size_t clarus_hip_sizeof_conv_args(void) { return sizeof(ClarusConvArgs); }
 
 size_t clarus_hip_sizeof_cross_args(void) { return sizeof(ClarusCrossArgs); }
 
+size_t clarus_hip_sizeof_rotary_args(void) { return sizeof(ClarusRotaryArgs); }
+
+size_t clarus_hip_sizeof_add_norm_args(void) { return sizeof(ClarusAddNormArgs); }
+
 const char* clarus_hip_last_error(void) { return clarus::g_err; }
 
 const char* clarus_hip_last_kernel(void) { return clarus::g_kernel; }

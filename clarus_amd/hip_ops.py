@@ -22,6 +22,7 @@ from __future__ import annotations
 
 import ctypes
 import math
+import operator
 
 import torch
 from torch.autograd import forward_ad
@@ -900,6 +901,131 @@ class HipOps(Backend):
                               "strips of up to 2048 channels in all images")
         need = self._workspace(self.lib.clarus_hip_group_norm_workspace, n, p, c, groups)
         return odt, n, p, c, groups, xbs, ldx, wbs, bbs, acode, need
+
+    # ------------------------------------------------------------------ around a block's token mixer
+    def rotary(self, x, heads, sections, positions=None, base=10000.0, pairs="adjacent", out_dtype=None):
+        """Rotary positions with several axes on x [N, ..., heads * d] (NHWC pixels, frames of them, or tokens; a slice of
+        wider rows qualifies, so the queries and keys of a joint projection turn in one call). sections: pairs of
+        columns of each axis, in order; pair i of axis a turns by position_a * base ** (-i / sections[a]). pairs:
+        "adjacent" (columns 2 j and 2 j + 1 of a head) or "halves" (columns j and j + sum(sections)); columns behind
+        the pairs stay. positions: [L, axes] or [N, L, axes] of the L tokens of an image, int32, int64 or fp32;
+        None: x's inner dimensions are the axes and their indices the positions. Angles are worked out in 64 bits.
+        Returns a contiguous tensor of x's shape."""
+        if not isinstance(heads, int):
+            raise Unsupported(f"rotary: heads an integer, got {heads!r}")
+        try:
+            sections, base = tuple(map(operator.index, sections)), float(base)
+        except TypeError as exc:
+            raise Unsupported("rotary: sections integers, base a number") from exc
+        key = ("rotary", x.shape, x.stride(), x.dtype, heads, sections, base, pairs, out_dtype,
+               None if positions is None else (positions.shape, positions.stride(), positions.dtype))
+        self._forward_only("rotary", x, positions)
+        odt, args = self._plan(key, lambda: self._rotary_plan(x, heads, sections, positions, base, pairs, out_dtype or self.dtype))
+        out = torch.empty_like(x, dtype=odt, memory_format=torch.contiguous_format)
+        if args is None:
+            return out
+        if x.data_ptr() % 16:
+            raise Unsupported("rotary: 16-byte aligned rows")
+        args = _lib.RotaryArgs.from_buffer_copy(args)
+        args.x, args.out, args.positions = x.data_ptr(), out.data_ptr(), _lib.ptr(positions)
+        self._call("rotary", self.lib.clarus_hip_rotary, ctypes.byref(args))
+        return out
+
+    def _rotary_plan(self, x, heads, sections, positions, base, pairs, odt):
+        if x.dim() < 2 or heads < 1 or x.shape[-1] % heads or pairs not in ("adjacent", "halves"):
+            raise Unsupported(f"rotary: x [N, ..., heads d], pairs adjacent or halves, got {heads!r} {pairs!r}")
+        n, c = x.shape[0], x.shape[-1]
+        d, inner = c // heads, x.shape[1:-1]
+        l, axes = math.prod(inner), len(sections)
+        if not (_kdt(x) and odt in _KDT and d > 0 and d % 8 == 0 and d <= 2 * _lib.ROTARY_PAIRS and c < 1 << 24):
+            raise Unsupported("rotary: bf16 / fp32, head width a multiple of 8 up to 256, rows below 2^24 columns")
+        if not (1 <= axes <= _lib.ROTARY_AXES and min(sections) >= 0 and 1 <= sum(sections) <= d // 2):
+            raise Unsupported("rotary: 1 to 4 axes with 1 to d / 2 pairs in all")
+        if not 1e-30 < base < 1e30:
+            raise Unsupported("rotary: base positive and finite")
+        kind, pbs, ldp = _lib.POS_GRID, 0, 0
+        if positions is None:
+            if axes != len(inner):
+                raise Unsupported(f"rotary: {axes} sections without positions for {len(inner)} inner dimensions")
+        else:
+            kind = {torch.float32: _lib.POS_F32, torch.int32: _lib.POS_I32, torch.int64: _lib.POS_I64}.get(positions.dtype)
+            if kind is None or tuple(positions.shape) not in ((l, axes), (n, l, axes)):
+                raise Unsupported("rotary: positions [L, axes] or [N, L, axes], int32, int64 or fp32")
+            if positions.stride(-1) != 1 and axes > 1:
+                raise Unsupported("rotary: positions with unit axis stride")
+            pbs, ldp = positions.stride(0) if positions.dim() == 3 else 0, positions.stride(-2)
+        if x.numel() == 0:
+            return odt, None
+        at, es = _rows(x), x.element_size()
+        if at is None or at[1] * es % 16 or at[2] * es % 16:
+            raise Unsupported("rotary: unit channel stride, one row stride, 16-byte aligned rows")
+        if n * l >= 1 << 28:
+            raise Unsupported("rotary: fewer than 2^28 tokens")
+        turns = [base ** (-i / s) / math.tau for s in sections for i in range(s)]
+        return odt, _lib.RotaryArgs(
+            n=n, l=l, heads=heads, d=d, x_bstride=at[2], ldx=at[1], pos_bstride=pbs, ldpos=ldp,
+            grid=(ctypes.c_int64 * _lib.ROTARY_AXES)(*(inner if positions is None else ())),
+            sections=(ctypes.c_int64 * _lib.ROTARY_AXES)(*sections), turn=(ctypes.c_double * _lib.ROTARY_PAIRS)(*turns),
+            axes=axes, pairs_mode=int(pairs == "halves"), pos_kind=kind, dtype=_lib.dtype_code(x.dtype),
+            o_dtype=_lib.dtype_code(odt))
+
+    def add_norm(self, x, y=None, gate=None, scale=1.0, post=False, post_weight=None, post_bias=None, ln=True, weight=None,
+                 bias=None, eps=1e-6, out_dtype=None):
+        """A block's output y joined to the residual stream x (both [N, ..., C]), and the norm that the next block reads:
+        sum = x + scale * gate * (post(y) * post_weight + post_bias) in x's dtype, norm = ln(sum) * weight + bias in
+        out_dtype (the compute dtype). post and ln: False (the value itself; ln=False returns no norm), True
+        (LayerNorm) or "rms", over the channels with eps. gate, post_weight, post_bias, weight and bias: [C], or
+        [N, C] for each image's own (a conditioned block's gate, 1 + scale and shift). y None: the sum is x itself. The
+        norm is taken of the sum before its rounding. Returns (sum, norm); norm None with ln=False."""
+        if not all(isinstance(k, (bool, str)) for k in (post, ln)):
+            raise Unsupported(f"add_norm: post and ln False, True or 'rms', got {post!r} {ln!r}")
+        affine = (gate, post_weight, post_bias, weight, bias)
+        key = ("add_norm", x.shape, x.stride(), x.dtype, None if y is None else (y.shape, y.stride(), y.dtype), post, ln, out_dtype,
+               tuple(None if t is None else (t.shape, t.dtype) for t in affine))
+        self._forward_only("add_norm", x, y, *affine)
+        odt, args = self._plan(key, lambda: self._add_norm_plan(x, y, affine, post, ln, out_dtype or self.dtype))
+        eps, scale = (ctypes.c_float(v).value for v in (eps, scale))  # as the call passes them on
+        if not (0.0 <= eps < math.inf and math.isfinite(scale)):
+            raise Unsupported("add_norm: eps finite (as fp32) and not negative, scale finite")
+        total = x if y is None else torch.empty_like(x, memory_format=torch.contiguous_format)
+        norm = torch.empty_like(x, dtype=odt, memory_format=torch.contiguous_format) if ln else None
+        if args is None or (y is None and norm is None):
+            return total, norm
+        if x.data_ptr() % 16 or (y is not None and y.data_ptr() % 16):
+            raise Unsupported("add_norm: 16-byte aligned rows")
+        args = _lib.AddNormArgs.from_buffer_copy(args)
+        held = [t if t is None or (t.dtype == torch.float32 and t.is_contiguous() and t.data_ptr() % 16 == 0)
+                else torch.empty_like(t, dtype=torch.float32, memory_format=torch.contiguous_format).copy_(t) for t in affine]
+        args.gate, args.post_w, args.post_b, args.w, args.b = map(_lib.ptr, held)
+        args.x, args.y, args.norm, args.scale, args.eps = x.data_ptr(), _lib.ptr(y), _lib.ptr(norm), scale, eps
+        args.sum = None if y is None else total.data_ptr()
+        self._call("add_norm", self.lib.clarus_hip_add_norm, ctypes.byref(args))
+        return total, norm
+
+    def _add_norm_plan(self, x, y, affine, post, ln, odt):
+        kinds = {False: _lib.PRO_NONE, True: _lib.PRO_LN, "rms": _lib.PRO_RMS}
+        if x.dim() < 2 or post not in kinds or ln not in kinds:
+            raise Unsupported(f"add_norm: x [N, ..., C], post and ln False, True or 'rms', got {post!r} {ln!r}")
+        n, c = x.shape[0], x.shape[-1]
+        if not (_kdt(x, y) and odt in _KDT and 0 < c <= 16384 and c % 8 == 0 and (y is None or y.shape == x.shape)):
+            raise Unsupported("add_norm: bf16 / fp32, y of x's shape, channels a multiple of 8 up to 16384")
+        if any(t is not None and (tuple(t.shape) not in ((c,), (n, c)) or not t.is_floating_point()) for t in affine):
+            raise Unsupported("add_norm: gate, weights and biases [C] or [N, C]")
+        if x.numel() == 0:
+            return odt, None
+        xa, ya = _rows(x), None if y is None else _rows(y)
+        if xa is None or any(s * x.element_size() % 16 for s in xa[1:]) or (
+                y is not None and (ya is None or any(s * y.element_size() % 16 for s in ya[1:]))):
+            raise Unsupported("add_norm: unit channel stride, one row stride, 16-byte aligned rows")
+        rows = xa[0]
+        if n * rows >= 1 << 31 or n >= 1 << 23:
+            raise Unsupported("add_norm: fewer than 2^31 rows and 2^23 images")
+        strides = [c if t is not None and t.dim() == 2 else 0 for t in affine]
+        return odt, _lib.AddNormArgs(
+            n=n, rows=rows, c=c, x_bstride=xa[2], ldx=xa[1], y_bstride=ya[2] if ya else 0, ldy=ya[1] if ya else 0,
+            gate_bstride=strides[0], post_w_bstride=strides[1], post_b_bstride=strides[2], w_bstride=strides[3],
+            b_bstride=strides[4], x_dtype=_lib.dtype_code(x.dtype), y_dtype=_lib.dtype_code((x if y is None else y).dtype),
+            sum_dtype=_lib.dtype_code(x.dtype), norm_dtype=_lib.dtype_code(odt), post=kinds[post], pre=kinds[ln])
 
     # ------------------------------------------------------------------ attention
     def cross_attention(self, q, k, v, heads, kv_heads=None, mask=None, scale=None, out_dtype=None):

@@ -1,5 +1,5 @@
 """PyTorch backend for the NON-GEMM ops the NAFNet harness needs (depthwise conv, TLC local
-mean, scaled add, pixel (un)shuffle) and group norm, run on the device with torch.
+mean, scaled add, pixel (un)shuffle), group norm, rotary positions and add_norm, run on the device with torch.
 
 These ops are outside the HIP hot path; in clarus they fall through to the reference torch
 backend (python/clarus/ops/torch_ref.py:133-218), whose semantics this follows. Registered as
@@ -64,6 +64,59 @@ class TorchSpatialOps(Backend):
             y = y + bias.float().reshape(-1, 1, c)
         y = F.silu(y) if act == "silu" else F.gelu(y) if act == "gelu" else y
         return y.reshape(x.shape).to(out_dtype or self.dtype)
+
+    def rotary(self, x, heads, sections, positions=None, base=10000.0, pairs="adjacent", out_dtype=None):
+        """Rotary positions with an axis for each of `sections` on the heads of x [N, ..., heads d], angles in 64 bits
+        (positions [L, axes] or [N, L, axes]; None: x's inner dimensions)."""
+        sections = tuple(sections)
+        p, inner = sum(sections), x.shape[1:-1]
+        if (not isinstance(heads, int) or heads < 1 or x.dim() < 2 or x.shape[-1] % heads or pairs not in ("adjacent", "halves")
+                or min(sections, default=-1) < 0 or not 0 < 2 * p <= x.shape[-1] // heads or not 0.0 < base < math.inf):
+            raise Unsupported("rotary: x [N, ..., heads d], sections of up to d / 2 pairs, pairs adjacent or halves")
+        n, d, l = x.shape[0], x.shape[-1] // heads, math.prod(inner)
+        if positions is None:
+            if len(inner) != len(sections):
+                raise Unsupported("rotary: without positions a section for each inner dimension")
+            at = torch.stack(torch.meshgrid(*[torch.arange(s, device=x.device) for s in inner], indexing="ij"), -1)
+            positions = at.reshape(l, len(sections))
+        elif tuple(positions.shape) not in ((l, len(sections)), (n, l, len(sections))):
+            raise Unsupported("rotary: positions [L, axes] or [N, L, axes]")
+        t = torch.cat([positions[..., a, None].double() * base ** (-torch.arange(s, device=x.device, dtype=torch.float64) / max(s, 1))
+                       for a, s in enumerate(sections)], -1)[..., None, :]
+        cos, sin = t.cos().float(), t.sin().float()
+        y = x.float().reshape(n, l, heads, d)
+        a, b = (y[..., 0:2 * p:2], y[..., 1:2 * p:2]) if pairs == "adjacent" else (y[..., :p], y[..., p:2 * p])
+        a, b = a * cos - b * sin, a * sin + b * cos
+        z = torch.stack((a, b), -1).flatten(-2) if pairs == "adjacent" else torch.cat((a, b), -1)
+        return torch.cat((z, y[..., 2 * p:]), -1).reshape(x.shape).to(out_dtype or self.dtype)
+
+    def add_norm(self, x, y=None, gate=None, scale=1.0, post=False, post_weight=None, post_bias=None, ln=True, weight=None,
+                 bias=None, eps=1e-6, out_dtype=None):
+        """(x + scale gate (post(y) post_weight + post_bias) in x's dtype, ln(that) weight + bias), norms over the channels
+        in fp32 (False, True or "rms"), vectors [C] or [N, C]."""
+        n, c = x.shape[0], x.shape[-1]
+        affine = (gate, post_weight, post_bias, weight, bias)
+        if x.dim() < 2 or any(k not in (False, True, "rms") for k in (post, ln)) or (y is not None and y.shape != x.shape):
+            raise Unsupported(f"add_norm: x [N, ..., C], y of its shape, post and ln False, True or 'rms', got {post!r} {ln!r}")
+        if any(t is not None and (tuple(t.shape) not in ((c,), (n, c)) or not t.is_floating_point()) for t in affine):
+            raise Unsupported("add_norm: gate, weights and biases [C] or [N, C]")
+        if not 0.0 <= eps < math.inf or not math.isfinite(scale) or not (out_dtype or self.dtype).is_floating_point:
+            raise Unsupported("add_norm: eps finite and not negative, scale finite, a floating-point output")
+
+        def norm(v, kind, w, b):
+            if kind is True:
+                var, mean = torch.var_mean(v, -1, correction=0, keepdim=True)
+                v = (v - mean) * torch.rsqrt(var + eps)
+            elif kind:
+                v = v * torch.rsqrt(v.square().mean(-1, keepdim=True) + eps)
+            v = v if w is None else v * w.float().reshape(-1, 1, c)
+            return v if b is None else v + b.float().reshape(-1, 1, c)
+        r, total = x.float().reshape(n, math.prod(x.shape[1:-1]), c), x
+        if y is not None:
+            add = norm(y.float().reshape(r.shape), post, post_weight, post_bias)
+            r = r + (add if gate is None else add * gate.float().reshape(-1, 1, c)) * scale
+            total = r.reshape(x.shape).to(x.dtype)
+        return total, norm(r, ln, weight, bias).reshape(x.shape).to(out_dtype or self.dtype) if ln else None
 
     def add_scaled(self, a, b, alpha, out_dtype=None, out=None):
         """a * alpha + b (torch_ref.py:201-207)."""

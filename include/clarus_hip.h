@@ -520,11 +520,70 @@ size_t clarus_hip_cross_attention_workspace(int32_t dtype, int64_t n, int64_t lq
                                             int64_t kv_heads, int64_t d, int32_t mask_mode);
 int clarus_hip_cross_attention(const ClarusCrossArgs* args, void* scratch, size_t scratch_bytes, void* stream);
 
+/*
+ * Rotary positions with up to CLARUS_ROTARY_AXES axes (time, height, width) on the heads of token rows: pair j of
+ * every head (a, b) becomes (a cos t - b sin t, a sin t + b cos t), t = 2 pi position[token][axis of j] * turn[j];
+ * the columns behind the pairs are copied. sections[i]: pairs of axis i, in order (1 to d / 2 in all); pairs_mode 0:
+ * pair j is columns 2 j and 2 j + 1 of a head, 1: columns j and j + (all pairs). turn: turns of pair j for a step of its
+ * axis (frequency / 2 pi).
+ * x rows at x + n * x_bstride + token * ldx, heads * d columns (d a multiple of 8, at most 256; 16-byte aligned rows,
+ * slices of wider rows); out [n, l, heads * d] contiguous, not overlapping x unless it is x itself, contiguous and of
+ * one dtype. positions: pos_kind 0: none, token t stands at its place in a grid[0] x grid[1] x .. of l tokens; 1 / 2 / 3:
+ * fp32 / int32 / int64 at positions + n * pos_bstride + token * ldpos + axis (elements). Angles are reduced in 64 bits.
+ * n * l < 2^28, heads * d < 2^24. No counterpart in the reference.
+ */
+#define CLARUS_ROTARY_AXES 4
+#define CLARUS_ROTARY_PAIRS 128
+typedef struct ClarusRotaryArgs {
+  const void* x;
+  void* out;
+  const void* positions; /* NULL with pos_kind 0 */
+  int64_t n, l, heads, d;
+  int64_t x_bstride, ldx, pos_bstride, ldpos;
+  int64_t grid[CLARUS_ROTARY_AXES], sections[CLARUS_ROTARY_AXES];
+  double turn[CLARUS_ROTARY_PAIRS];
+  int32_t axes, pairs_mode, pos_kind, dtype, o_dtype;
+} ClarusRotaryArgs;
+
+int clarus_hip_rotary(const ClarusRotaryArgs* args, void* stream);
+
+/*
+ * A block's output added to the residual stream, and the norm that the next block reads, per row of c channels:
+ *   sum = x + scale * gate[ch] * (post(y) * post_w[ch] + post_b[ch]);  norm = pre(sum) * w[ch] + b[ch]
+ * post and pre: CLARUS_PRO_NONE (the value itself), CLARUS_PRO_LN ((v - mean) * rsqrt(var + eps)) or CLARUS_PRO_RMS
+ * (v * rsqrt(mean(v^2) + eps)). y NULL: no block, sum = x, which is not written (sum may be NULL). norm NULL: only the sum.
+ * pre works on the sum before its rounding. x, y rows at x + n * x_bstride + row * ldx (16-byte aligned, slices of wider
+ * rows); sum, norm [n, rows, c] contiguous (sum may be x itself where x is contiguous and of sum's type; nothing else
+ * overlaps). gate, post_w, post_b, w, b: fp32 [c] (stride 0) or one row per image (stride >= c), or NULL
+ * for 1 / 0. c a multiple of 8 up to 16384, n * rows < 2^31, statistics and affine in fp32; values within 2^60 of zero.
+ * No counterpart in the reference (whose norms are the prologues of linear).
+ */
+typedef struct ClarusAddNormArgs {
+  const void* x;
+  const void* y;
+  void* sum;
+  void* norm;
+  const float* gate;
+  const float* post_w;
+  const float* post_b;
+  const float* w;
+  const float* b;
+  int64_t n, rows, c;
+  int64_t x_bstride, ldx, y_bstride, ldy;
+  int64_t gate_bstride, post_w_bstride, post_b_bstride, w_bstride, b_bstride;
+  int32_t x_dtype, y_dtype, sum_dtype, norm_dtype, post, pre;
+  float scale, eps;
+} ClarusAddNormArgs;
+
+int clarus_hip_add_norm(const ClarusAddNormArgs* args, void* stream);
+
 /* ABI version (CLARUS_HIP_ABI_VERSION) and struct sizes, for binding checks. */
 int clarus_hip_abi_version(void);
 size_t clarus_hip_sizeof_gemm_args(void);
 size_t clarus_hip_sizeof_conv_args(void);
 size_t clarus_hip_sizeof_cross_args(void);
+size_t clarus_hip_sizeof_rotary_args(void);
+size_t clarus_hip_sizeof_add_norm_args(void);
 
 /* Text of the calling thread's last failure ("" if none). */
 const char* clarus_hip_last_error(void);

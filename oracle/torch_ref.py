@@ -174,6 +174,39 @@ class TorchRef:
         p = torch.softmax(s.masked_fill(none, 0), -1).masked_fill(none, 0)
         return (p @ vh).permute(0, 2, 1, 3).reshape(q.shape).to(self._odt(out_dtype))
 
+    def rotary(self, x, heads, sections, positions=None, base=10000.0, pairs="adjacent", out_dtype=None):
+        """No reference op: pairs of each head's columns turned by position * base^(-i / pairs of the axis)."""
+        n, d, p = x.shape[0], x.shape[-1] // heads, sum(sections)
+        y = x.float().reshape(n, -1, heads, d)
+        if positions is None:
+            positions = torch.cartesian_prod(*[torch.arange(s, device=x.device) for s in x.shape[1:-1]]).reshape(-1, x.dim() - 2)
+        t = torch.cat([positions[..., a, None].double() * base ** (-torch.arange(s, device=x.device).double() / s)
+                       for a, s in enumerate(sections)], -1).reshape(-1, y.shape[1], 1, p)
+        cos, sin = t.cos().float(), t.sin().float()
+        z = y[..., :2 * p]
+        a, b = z.unflatten(-1, (p, 2)).unbind(-1) if pairs == "adjacent" else z.chunk(2, -1)
+        a, b = a * cos - b * sin, b * cos + a * sin
+        z = torch.stack((a, b), -1).flatten(-2) if pairs == "adjacent" else torch.cat((a, b), -1)
+        return torch.cat((z, y[..., 2 * p:]), -1).reshape(x.shape).to(self._odt(out_dtype))
+
+    def add_norm(self, x, y=None, gate=None, scale=1.0, post=False, post_weight=None, post_bias=None, ln=True, weight=None,
+                 bias=None, eps=1e-6, out_dtype=None):
+        """No reference op: (x + scale gate (post(y) pw + pb), ln(that) w + b), vectors [C] or [N, C]."""
+        n, c = x.shape[0], x.shape[-1]
+
+        def norm(v, kind, w, b):
+            if kind:
+                v = v - v.mean(-1, keepdim=True) if kind != "rms" else v
+                v = v * torch.rsqrt(v.square().mean(-1, keepdim=True) + eps)
+            v = v if w is None else v * w.float().reshape(-1, 1, c)
+            return v if b is None else v + b.float().reshape(-1, 1, c)
+        r = x.float().reshape(n, -1, c)
+        if y is not None:
+            add = norm(y.float().reshape(n, -1, c), post, post_weight, post_bias) * scale
+            r = r + (add if gate is None else add * gate.float().reshape(-1, 1, c))
+        h = norm(r, ln, weight, bias).reshape(x.shape).to(self._odt(out_dtype)) if ln else None
+        return r.reshape(x.shape).to(x.dtype), h
+
     def channel_attention(self, qkv, heads, temperature):
         """torch_ref.py:220-235: softmax((q/|q|)(k/|k|)^T * t) per image and head, fp32."""
         n, h, w, c3 = qkv.shape
