@@ -93,6 +93,15 @@ class AddNormArgs(ctypes.Structure):
     ]
 
 
+class LinearArgs(ctypes.Structure):
+    _fields_ = [
+        ("q", _vp), ("k", _vp), ("v", _vp), ("out", _vp), ("log_decay", _vp), ("state_in", _vp), ("state_out", _vp),
+        ("n", _i64), ("l", _i64), ("heads", _i64), ("kv_heads", _i64), ("dk", _i64), ("dv", _i64),
+        ("q_bstride", _i64), ("ldq", _i64), ("k_bstride", _i64), ("ldk", _i64), ("v_bstride", _i64), ("ldv", _i64),
+        ("dtype", _i32), ("o_dtype", _i32), ("scale", _f32),
+    ]
+
+
 # name -> (restype, argtypes); every function declared in include/clarus_hip.h
 SIGNATURES = {
     "clarus_hip_gemm": (_i32, [ctypes.POINTER(GemmArgs), _vp]),
@@ -134,12 +143,15 @@ SIGNATURES = {
     "clarus_hip_cross_attention": (_i32, [ctypes.POINTER(CrossArgs), _vp, ctypes.c_size_t, _vp]),
     "clarus_hip_rotary": (_i32, [ctypes.POINTER(RotaryArgs), _vp]),
     "clarus_hip_add_norm": (_i32, [ctypes.POINTER(AddNormArgs), _vp]),
+    "clarus_hip_linear_attention_workspace": (ctypes.c_size_t, [_i32] + [_i64] * 6),
+    "clarus_hip_linear_attention": (_i32, [ctypes.POINTER(LinearArgs), _vp, ctypes.c_size_t, _vp]),
     "clarus_hip_abi_version": (_i32, []),
     "clarus_hip_sizeof_gemm_args": (ctypes.c_size_t, []),
     "clarus_hip_sizeof_conv_args": (ctypes.c_size_t, []),
     "clarus_hip_sizeof_cross_args": (ctypes.c_size_t, []),
     "clarus_hip_sizeof_rotary_args": (ctypes.c_size_t, []),
     "clarus_hip_sizeof_add_norm_args": (ctypes.c_size_t, []),
+    "clarus_hip_sizeof_linear_args": (ctypes.c_size_t, []),
     "clarus_hip_last_error": (ctypes.c_char_p, []),
     "clarus_hip_last_kernel": (ctypes.c_char_p, []),
 }
@@ -172,7 +184,7 @@ def load(path: str = LIB_PATH):
         raise RuntimeError("ClarusConvArgs layout differs between the library and the binding")
     if lib.clarus_hip_sizeof_cross_args() != ctypes.sizeof(CrossArgs):
         raise RuntimeError("ClarusCrossArgs layout differs between the library and the binding")
-    for cls, name in ((RotaryArgs, "rotary"), (AddNormArgs, "add_norm")):
+    for cls, name in ((RotaryArgs, "rotary"), (AddNormArgs, "add_norm"), (LinearArgs, "linear")):
         if getattr(lib, f"clarus_hip_sizeof_{name}_args")() != ctypes.sizeof(cls):
             raise RuntimeError(f"{cls.__name__} layout differs between the library and the binding")
     _LIB = lib

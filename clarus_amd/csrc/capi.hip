@@ -55,6 +55,8 @@ size_t clarus_hip_sizeof_rotary_args(void) { return sizeof(ClarusRotaryArgs); }
 
 size_t clarus_hip_sizeof_add_norm_args(void) { return sizeof(ClarusAddNormArgs); }
 
+size_t clarus_hip_sizeof_linear_args(void) { return sizeof(ClarusLinearArgs); }
+
 const char* clarus_hip_last_error(void) { return clarus::g_err; }
 
 const char* clarus_hip_last_kernel(void) { return clarus::g_kernel; }

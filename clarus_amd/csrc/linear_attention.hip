@@ -1,0 +1,612 @@
+// Causal linear attention with a decay for each head, from a state and to one, on gfx950; per image and kv head
+//   S_t = e^g S_{t-1} + k_t v_t^T,   o_t[h] = scale q_t[h]^T S_t   for the heads h that share the kv head.
+//
+//   la_step_kernel   a few tokens: the state in registers, read and written once, token after token
+//   la_chunk_kernel  longer sequences, in segments of whole chunks of 64 (fp32: 32) tokens. Within a chunk
+//                      o_i = e^{g (i + 1)} q_i^T S + sum_{j <= i} e^{g (i - j)} (q_i . k_j) v_j,
+//                      S <- e^{g c} S + sum_j e^{g (c - 1 - j)} k_j v_j^T
+//                    as matrix products; once without outputs for what a segment adds to the state, once from the
+//                    state that it starts with
+//   la_carry_kernel  the segments' start states, and the state after the last
+// A sequence that is no whole number of chunks is padded in front (k, v = 0), so that every factor is a power of e^g with
+// an exponent that is not negative. States, sums and factors are fp32 (a segment's factor is kept as two fp32 numbers from
+// 64 bits: a state held over many calls and segments does not drift by the factor's rounding).
+//
+// A wave holds 32 columns of values: S as MFMA accumulators, rows dk. As an A operand (rows = values) the accumulators
+// stand as they are for S^T, in the order of dk in which q's fragments are put by exchanging halves with lane ^ 32; P^T
+// goes from the accumulators of K Q^T into the product with V^T likewise, and V^T is both that product's operand and,
+// weighted, the state's. bf16: products of bf16 q, k, v are exact in fp32; the weighted values go in three bf16 parts
+// (2^-24 of them left out) where a segment's sum for the state is made, in two (2^-16) where only outputs follow, S in two
+// as an operand, and the weights q . k within a chunk are rounded once to bf16 (2^-8 of each, of independent
+// signs: about as much as the output's own rounding). fp32: every product on fp32 MFMAs.
+#include <algorithm>
+#include <math.h>
+
+#include "attention_tile.hpp"
+#include "capi.hpp"
+
+namespace clarus {
+
+namespace {
+
+constexpr int LA_T = 256;  // threads of a step or carry workgroup
+constexpr float LA_LEAST = -1000.f;  // log2 of a decay: 2^-1000 is 0 in fp32, and 0 times it no NaN
+
+struct LinP {
+  const void *q, *k, *v;
+  void* out;
+  const float *s_in, *decay;
+  float *s_out, *part;
+  int64_t qbs, ldq, kbs, ldk, vbs, ldv;
+  int64_t l;             // tokens
+  int64_t nk, nseg, seg; // (image, kv head) pairs, segments, tokens of one
+  int64_t pad;           // in front of the first token
+  int rep, kv_heads, dk, dv, o_dt;
+  int slices;            // of the values' columns (step)
+  float scale;
+};
+
+// log2 of a head's decay
+__device__ __forceinline__ float la_log2(const LinP& p, int h) {
+  const float g = p.decay[h] * 1.4426950408889634f;
+  return g < LA_LEAST ? LA_LEAST : g;
+}
+
+// e^{g n} as two floats
+struct Factor { float hi, lo; };
+__device__ __forceinline__ Factor la_factor(const LinP& p, int h, int64_t n) {
+  double e = (double)p.decay[h] * (double)n * 1.4426950408889634074;
+  e = n == 0 ? 0.0 : e < (double)LA_LEAST ? (double)LA_LEAST : e;
+  const double f = exp2(e);
+  Factor r;
+  r.hi = (float)f;
+  r.lo = r.hi < 3e38f ? (float)(f - (double)r.hi) : 0.f;
+  return r;
+}
+__device__ __forceinline__ float la_scaled(float s, const Factor& f, float add) { return fmaf(s, f.hi, fmaf(s, f.lo, add)); }
+
+// ---------------------------------------------------------------- a few tokens
+// A workgroup holds DVS columns of a state, a thread four of them in NP rows RG apart
+template <int DT, int DVS, int NP>
+__global__ void __launch_bounds__(LA_T) la_step_kernel(const LinP p) {
+  constexpr int TPR = DVS / 4, RG = LA_T / TPR, ES = DT == DT_BF16 ? 2 : 4;
+  __shared__ float ks[RG * NP], qs[RG * NP];
+  __shared__ f32x4 po[LA_T];
+  const int tid = threadIdx.x, rg = tid / TPR, c4 = tid - rg * TPR;
+  const int64_t nk = blockIdx.x / p.slices;
+  const int slice = (int)(blockIdx.x - nk * p.slices);
+  const int64_t n = nk / p.kv_heads;
+  const int h = (int)(nk - n * p.kv_heads), col = slice * DVS + c4 * 4;
+  const bool mine = col < p.dv;
+  const Factor f = la_factor(p, h, 1);
+  const unsigned char* kp = (const unsigned char*)p.k + (n * p.kbs + (int64_t)h * p.dk) * ES;
+  const unsigned char* vp = (const unsigned char*)p.v + (n * p.vbs + (int64_t)h * p.dv) * ES;
+  f32x4 s[NP];
+  const int64_t at = nk * p.dk * p.dv + col;
+#pragma unroll
+  for (int i = 0; i < NP; ++i) {
+    const int r = rg + RG * i;
+    s[i] = p.s_in && mine && r < p.dk ? *reinterpret_cast<const f32x4*>(p.s_in + at + (int64_t)r * p.dv) : f32x4{0.f, 0.f, 0.f, 0.f};
+  }
+  for (int64_t t = 0; t < p.l; ++t) {
+    __syncthreads();
+    for (int i = tid; i < RG * NP; i += LA_T) ks[i] = i < p.dk ? load1(kp, DT, t * p.ldk + i) : 0.f;
+    f32x4 v = {0.f, 0.f, 0.f, 0.f};
+    if (mine)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) v[e] = load1(vp, DT, t * p.ldv + col + e);
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < NP; ++i) {
+      const float k = ks[rg + RG * i];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) s[i][e] = la_scaled(s[i][e], f, k * v[e]);
+    }
+    for (int r = 0; r < p.rep; ++r) {
+      const int head = h * p.rep + r;
+      const unsigned char* qp = (const unsigned char*)p.q + (n * p.qbs + t * p.ldq + (int64_t)head * p.dk) * ES;
+      if (r) __syncthreads();
+      for (int i = tid; i < RG * NP; i += LA_T) qs[i] = i < p.dk ? load1(qp, DT, i) : 0.f;
+      __syncthreads();
+      f32x4 o = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int i = 0; i < NP; ++i) {
+        const float q = qs[rg + RG * i];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[e] = fmaf(q, s[i][e], o[e]);
+      }
+      po[tid] = o;
+      __syncthreads();
+      if (rg == 0 && mine) {
+        for (int i = 1; i < RG; ++i) o += po[tid + i * TPR];
+        const int64_t to = ((n * p.l + t) * (int64_t)(p.kv_heads * p.rep) + head) * p.dv + col;
+        if (p.o_dt == DT_BF16)
+          *reinterpret_cast<u32x2*>((unsigned short*)p.out + to) =
+              u32x2{pack2_bf16(o[0] * p.scale, o[1] * p.scale), pack2_bf16(o[2] * p.scale, o[3] * p.scale)};
+        else
+          *reinterpret_cast<f32x4*>((float*)p.out + to) = o * p.scale;
+      }
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < NP; ++i) {
+    const int r = rg + RG * i;
+    if (mine && r < p.dk) *reinterpret_cast<f32x4*>(p.s_out + at + (int64_t)r * p.dv) = s[i];
+  }
+}
+
+// ---------------------------------------------------------------- chunks
+// Tokens of a chunk: 64 in bf16, 32 in fp32 and with wide keys in bf16, whose state and queries fill the registers
+template <int DT, int DK> constexpr int la_kt = DT == DT_BF16 && DK <= 64 ? 64 : 32;
+
+// The copies of one tile (KT tokens, D columns of LDS) by W waves, 1 KiB each
+template <int DT, int D, int KT, int W>
+struct LaCopy {
+  using T = XaTile<DT, D>;
+  static constexpr int BYTES = KT * T::ROWB, NI = (BYTES / 1024 + W - 1) / W;
+  static constexpr bool EVEN = BYTES / 1024 % W == 0;
+  uint32_t off[NI];  // from the tile's first row
+
+  __device__ __forceinline__ LaCopy(int64_t ld, int wave, int lane) {
+#pragma unroll
+    for (int j = 0; j < NI; ++j) {
+      const int at = (wave + W * j) * 1024 + lane * 16, r = at / T::ROWB, c = ((at % T::ROWB) / 16) ^ T::swz_k(r);
+      off[j] = (uint32_t)(r * ld * T::ES) + c * 16;
+    }
+  }
+  // rows before `pad` and columns from d on as zeros
+  __device__ __forceinline__ void operator()(const unsigned char* src, int d, int pad, unsigned char* dst, int wave, int lane) const {
+#define LA_COPY(from)                                                                          \
+  __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(from),     \
+                                   (__attribute__((address_space(3))) void*)(dst + (wave + W * j) * 1024), 16, 0, 0)
+    if (pad == 0 && d == D) {
+#pragma unroll
+      for (int j = 0; j < NI; ++j) {
+        if (!EVEN && wave + W * j >= BYTES / 1024) break;
+        LA_COPY(src + off[j]);
+      }
+    } else {
+      const unsigned char* zero = (const unsigned char*)xa_zeros;
+#pragma unroll
+      for (int j = 0; j < NI; ++j) {
+        if (!EVEN && wave + W * j >= BYTES / 1024) break;
+        const int at = (wave + W * j) * 1024 + lane * 16, r = at / T::ROWB, c = ((at % T::ROWB) / 16) ^ T::swz_k(r);
+        LA_COPY(r >= pad && c * 16 < d * T::ES ? src + off[j] : zero);
+      }
+    }
+#undef LA_COPY
+  }
+};
+
+// 32 x 16 fragment of a tile's transpose (rows = columns 32 b .. of the tile, 16 tokens 16 ks ..), tokens in the order of
+// the accumulators
+template <int D>
+__device__ __forceinline__ bf16x8 la_turned(const unsigned char* tile, int ks, int b, int lane) {
+  using T = XaTile<DT_BF16, D>;
+  typedef __attribute__((ext_vector_type(8))) short s16x8;
+  const int i = lane & 15, vr = 16 * ks + 4 * (lane >> 5) + (i >> 2), vc = 4 * b + 2 * ((lane >> 4) & 1) + ((i & 3) >> 1);
+  const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+      (__attribute__((address_space(3))) s16x4*)(tile + T::at_k(vr, vc) + (i & 1) * 8));
+  const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+      (__attribute__((address_space(3))) s16x4*)(tile + T::at_k(vr + 8, vc) + (i & 1) * 8));
+  return __builtin_bit_cast(bf16x8, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+}
+
+__device__ __forceinline__ f32x16 la_mfma(const bf16x8& a, const bf16x8& b, const f32x16& c) {
+  return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
+}
+
+// W waves, 32 columns of values each. OUT: outputs, from the segment's start state; else what the segment adds
+template <int DT, int DK, int W, bool OUT>
+__global__ void __launch_bounds__(64 * W, 2) la_chunk_kernel(const LinP p) {
+  using TK = XaTile<DT, DK>;
+  using TV = XaTile<DT, 32 * W>;
+  constexpr int KT = la_kt<DT, DK>, QT = KT / 32, DB = DK / 32, QN = xa_qn<DT, DK>, ES = TK::ES;
+  constexpr int KBYTES = KT * TK::ROWB, VBYTES = KT * TV::ROWB;
+  __shared__ __align__(16) unsigned char tiles[2][KBYTES + VBYTES];
+  const int tid = threadIdx.x, lane0 = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int col = lane0 & 31, hl = lane0 >> 5;
+  // neighbouring heads of a segment, which share lines of rows, on one XCD
+  const unsigned total = (unsigned)(p.nk * p.nseg), span = (total + 7) >> 3, id = (blockIdx.x & 7) * span + (blockIdx.x >> 3);
+  if ((blockIdx.x >> 3) >= span || id >= total) return;
+  const unsigned rest = id / (unsigned)p.kv_heads, h = id - rest * (unsigned)p.kv_heads;
+  const unsigned n = rest / (unsigned)p.nseg, seg = rest - n * (unsigned)p.nseg;
+  const int64_t nk = (int64_t)n * p.kv_heads + h;
+  // padded places: token = place - pad
+  const int64_t t0 = seg * p.seg, t1 = t0 + p.seg < p.l + p.pad ? t0 + p.seg : p.l + p.pad;
+  const int nchunk = (int)((t1 - t0) / KT);
+
+  const float g = la_log2(p, h);
+  f32x16 s[DB];
+  float* part = p.part + ((nk * p.nseg + seg) * W + wave) * (DB * 16 * 64) + lane0;
+#pragma unroll
+  for (int b = 0; b < DB; ++b)
+#pragma unroll
+    for (int j = 0; j < 16; ++j) s[b][j] = OUT ? part[(b * 16 + j) * 64] : 0.f;
+  // e^{g (c - 1 - r)} of row r = 16 ks + 8 (i / 4) + 4 hl + i % 4 of a chunk (fp32: 16 values of i)
+  float fi[DT == DT_BF16 ? 8 : 16], fk[KT / 16];
+  constexpr int LAST = DT == DT_BF16 ? 15 : KT - 1;
+#pragma unroll
+  for (int i = 0; i < (DT == DT_BF16 ? 8 : 16); ++i) fi[i] = __builtin_amdgcn_exp2f(g * (float)(LAST - (8 * (i >> 2) + 4 * hl + (i & 3))));
+#pragma unroll
+  for (int i = 0; i < KT / 16; ++i) fk[i] = __builtin_amdgcn_exp2f(g * (float)(KT - 16 - 16 * i));
+  // e^{g (i - j)} of query i = col of a tile of 32 and key j of the same tile (0 behind the query), and of the one before
+  float same[OUT ? 16 : 1], before[OUT && QT == 2 ? 16 : 1];
+  if constexpr (OUT) {
+#pragma unroll
+    for (int j = 0; j < 16; ++j) {
+      const int gap = col - (8 * (j >> 2) + 4 * hl + (j & 3));
+      same[j] = gap >= 0 ? __builtin_amdgcn_exp2f(g * (float)gap) : 0.f;
+      if constexpr (QT == 2) before[j] = __builtin_amdgcn_exp2f(g * (float)(gap + 32));
+    }
+  }
+  const float whole = __builtin_amdgcn_exp2f(g * (float)KT);
+
+  const unsigned char* kp = (const unsigned char*)p.k + (n * p.kbs + (int64_t)h * p.dk) * ES;
+  const unsigned char* vp = (const unsigned char*)p.v + (n * p.vbs + (int64_t)h * p.dv) * ES;
+  const LaCopy<DT, DK, KT, W> copy_k(p.ldk, wave, lane0);
+  const LaCopy<DT, 32 * W, KT, W> copy_v(p.ldv, wave, lane0);
+  auto fill = [&](int c, int buf) __attribute__((always_inline)) {
+    const int64_t at = t0 + (int64_t)c * KT - p.pad;  // token of the chunk's first place, negative in the padding
+    const int pad = at < 0 ? (int)-at : 0;
+    copy_k(kp + at * p.ldk * ES, p.dk, pad, tiles[buf], wave, lane0);
+    copy_v(vp + at * p.ldv * ES, p.dv, pad, tiles[buf] + KBYTES, wave, lane0);
+  };
+  u32x4 qf[OUT ? QT : 1][QN];  // of the next chunk from where this one's outputs are done
+  auto load_q = [&](int c, int r) __attribute__((always_inline)) {
+#pragma unroll
+    for (int t = 0; t < QT; ++t) {
+      const int64_t place = t0 + (int64_t)c * KT + 32 * t + col - p.pad;
+      const unsigned char* qp = (const unsigned char*)p.q + (n * p.qbs + (place < 0 ? 0 : place) * p.ldq + (int64_t)(h * p.rep + r) * p.dk) * ES;
+#pragma unroll
+      for (int i = 0; i < QN; ++i) {
+        const int at = (2 * i + hl) * (16 / ES);
+        qf[t][i] = *reinterpret_cast<const u32x4*>(qp + (at < p.dk ? at : 0) * ES);
+        if (p.dk < DK && at >= p.dk) qf[t][i] = u32x4{0, 0, 0, 0};
+      }
+    }
+  };
+  fill(0, 0);
+  if constexpr (OUT) load_q(0, 0);
+#pragma unroll 1
+  for (int c = 0; c < nchunk; ++c) {
+    // LDS and output offsets are worked out for each chunk instead of kept over the loop, where they spill
+    int lane = lane0;
+    asm volatile("" : "+v"(lane));
+    const int col = lane & 31, hl = lane >> 5;
+    const int64_t first = t0 + (int64_t)c * KT - p.pad;
+    const int pad = first < 0 ? (int)-first : 0;
+    __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0): this wave's copies have landed
+    barrier_keep_vm();                   // everybody's have, and the chunk before has been read
+    const unsigned char *kt = tiles[c & 1], *vt = tiles[c & 1] + KBYTES;
+    if (c + 1 < nchunk) fill(c + 1, (c & 1) ^ 1);
+    bf16x8 vf[DT == DT_BF16 ? KT / 16 : 1];
+    float vx[DT == DT_BF16 ? 1 : 16];
+    if constexpr (DT == DT_BF16) {
+#pragma unroll
+      for (int ks = 0; ks < KT / 16; ++ks) vf[ks] = la_turned<32 * W>(vt, ks, wave, lane);
+    } else {
+#pragma unroll
+      for (int j = 0; j < 16; ++j)
+        vx[j] = *reinterpret_cast<const float*>(vt + TV::at_k(8 * (j >> 2) + 4 * hl + (j & 3), 8 * wave + (col >> 2)) + (col & 3) * 4);
+    }
+    if constexpr (OUT) {
+#pragma unroll 1
+      for (int r = 0; r < p.rep; ++r) {
+        if (r) load_q(c, r);
+        f32x16 o[QT];
+#pragma unroll
+        for (int t = 0; t < QT; ++t)
+#pragma unroll
+          for (int j = 0; j < 16; ++j) o[t][j] = 0.f;
+        // S^T Q^T
+        if constexpr (DT == DT_BF16) {
+#pragma unroll
+          for (int i = 0; i < QN; ++i) {
+            f32x8 x;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) x.v[e] = s[i >> 1][8 * (i & 1) + e];
+            bf16x8 hi, lo;
+            split_bf16(x, hi, lo);
+#pragma unroll
+            for (int t = 0; t < QT; ++t) {
+              unsigned x0 = qf[t][i][0], x1 = qf[t][i][1], y0 = qf[t][i][2], y1 = qf[t][i][3];
+              swap32(x0, y0);
+              swap32(x1, y1);
+              const bf16x8 q = __builtin_bit_cast(bf16x8, u32x4{x0, x1, y0, y1});
+              o[t] = la_mfma(hi, q, o[t]);
+              o[t] = la_mfma(lo, q, o[t]);
+            }
+          }
+        } else {
+#pragma unroll
+          for (int b = 0; b < DB; ++b)
+#pragma unroll
+            for (int j = 0; j < 16; ++j)
+              o[0] = __builtin_amdgcn_mfma_f32_32x32x2f32(s[b][j], __uint_as_float(qf[0][4 * b + (j >> 2)][j & 3]), o[0], 0, 0, 0);
+        }
+#pragma unroll
+        for (int t = 0; t < QT; ++t) {
+          const int since = 32 * t + col + 1 - pad;
+          const float f = __builtin_amdgcn_exp2f(g * (float)(since > 0 ? since : 0));
+#pragma unroll
+          for (int j = 0; j < 16; ++j) o[t][j] *= f;
+        }
+        __builtin_amdgcn_sched_barrier(0);
+        // P^T = (K Q^T) weighted, O^T += V^T P^T
+#pragma unroll
+        for (int t = 0; t < QT; ++t)
+#pragma unroll
+          for (int b = 0; b <= t; ++b) {
+            f32x16 w;
+#pragma unroll
+            for (int j = 0; j < 16; ++j) w[j] = 0.f;
+#pragma unroll
+            for (int i = 0; i < QN; ++i) {
+              const u32x4 a = *reinterpret_cast<const u32x4*>(kt + TK::at_k(32 * b + col, 2 * i + hl));
+              if constexpr (DT == DT_BF16) {
+                w = la_mfma(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, qf[t][i]), w);
+              } else {
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                  w = __builtin_amdgcn_mfma_f32_32x32x2f32(__uint_as_float(a[e]), __uint_as_float(qf[t][i][e]), w, 0, 0, 0);
+              }
+            }
+#pragma unroll
+            for (int j = 0; j < 16; ++j) {
+              if (b != t) w[j] *= before[QT == 2 ? j : 0];
+              else w[j] = col >= 8 * (j >> 2) + 4 * hl + (j & 3) ? w[j] * same[j] : 0.f;  // whatever a later key holds
+            }
+            __builtin_amdgcn_sched_barrier(0);
+            if constexpr (DT == DT_BF16) {
+#pragma unroll
+              for (int half = 0; half < 2; ++half) {
+                f32x8 x;
+#pragma unroll
+                for (int e = 0; e < 8; ++e) x.v[e] = w[8 * half + e];
+                o[t] = la_mfma(vf[2 * b + half], pack_bf16(x), o[t]);
+              }
+            } else {
+#pragma unroll
+              for (int j = 0; j < 16; ++j) o[t] = __builtin_amdgcn_mfma_f32_32x32x2f32(vx[j], w[j], o[t], 0, 0, 0);
+            }
+          }
+#pragma unroll
+        for (int t = 0; t < QT; ++t) {
+          const bool live = 32 * t + col >= pad;
+          const int64_t at = ((n * p.l + first + 32 * t + col) * (int64_t)(p.kv_heads * p.rep) + h * p.rep + r) * p.dv + 32 * wave;
+#pragma unroll
+          for (int j = 0; j < 16; j += 8) {
+            f32x4 y[2];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) y[i >> 2][i & 3] = o[t][j + i] * p.scale;
+            if (p.o_dt == DT_BF16) {
+              unsigned a0 = pack2_bf16(y[0][0], y[0][1]), a1 = pack2_bf16(y[0][2], y[0][3]), b0 = pack2_bf16(y[1][0], y[1][1]),
+                       b1 = pack2_bf16(y[1][2], y[1][3]);
+              swap32(a0, b0);
+              swap32(a1, b1);
+              const int c8 = 2 * j + 8 * hl;
+              if (live && 32 * wave + c8 < p.dv) *reinterpret_cast<u32x4*>((unsigned short*)p.out + at + c8) = u32x4{a0, a1, b0, b1};
+            } else {
+#pragma unroll
+              for (int i = 0; i < 2; ++i) {
+                const int c4 = 2 * j + 8 * i + 4 * hl;
+                if (live && 32 * wave + c4 < p.dv) *reinterpret_cast<f32x4*>((float*)p.out + at + c4) = y[i];
+              }
+            }
+          }
+        }
+      }
+      if (c + 1 == nchunk) break;  // no output needs the state behind the last chunk
+      load_q(c + 1, 0);
+    }
+    __builtin_amdgcn_sched_barrier(0);
+    // the state behind this chunk
+    const float keep = pad ? __builtin_amdgcn_exp2f(g * (float)(KT - pad)) : whole;
+#pragma unroll
+    for (int b = 0; b < DB; ++b)
+#pragma unroll
+      for (int j = 0; j < 16; ++j) s[b][j] *= keep;
+    if constexpr (DT == DT_BF16) {
+#pragma unroll
+      for (int ks = 0; ks < KT / 16; ++ks) {
+        f32x8 x;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) x.v[e] = (float)vf[ks][e] * (fi[e] * fk[ks]);
+        bf16x8 part3[3];
+        split_bf16(x, part3[0], part3[1]);
+        if constexpr (!OUT) {
+#pragma unroll
+          for (int e = 0; e < 8; ++e) part3[2][e] = (bf16_t)(x.v[e] - (float)part3[0][e] - (float)part3[1][e]);
+        }
+#pragma unroll
+        for (int b = 0; b < DB; ++b) {
+          const bf16x8 a = la_turned<DK>(kt, ks, b, lane);
+#pragma unroll
+          for (int i = 0; i < (OUT ? 2 : 3); ++i) s[b] = la_mfma(a, part3[i], s[b]);
+        }
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < 16; ++j) {
+        const float x = vx[j] * fi[j];
+#pragma unroll
+        for (int b = 0; b < DB; ++b) {
+          const float a = *reinterpret_cast<const float*>(kt + TK::at_k(8 * (j >> 2) + 4 * hl + (j & 3), 8 * b + (col >> 2)) + (col & 3) * 4);
+          s[b] = __builtin_amdgcn_mfma_f32_32x32x2f32(a, x, s[b], 0, 0, 0);
+        }
+      }
+    }
+  }
+  if constexpr (!OUT) {
+#pragma unroll
+    for (int b = 0; b < DB; ++b)
+#pragma unroll
+      for (int j = 0; j < 16; ++j) part[(b * 16 + j) * 64] = s[b][j];
+  }
+}
+
+// In place of what each segment adds the state that it starts with; the state behind the last. A thread per element, in the
+// accumulators' order; the next CB segments' loads in flight
+template <int CB>
+__global__ void __launch_bounds__(LA_T) la_carry_kernel(const LinP p, int waves, int db) {
+  const int per = waves * db * 16 * 64;  // elements of a state, padded
+  const int64_t i = (int64_t)blockIdx.x * LA_T + threadIdx.x;
+  if (i >= p.nk * per) return;
+  const int64_t nk = i / per;
+  const int e = (int)(i - nk * per), lane = e & 63, reg = (e >> 6) % (db * 16), wave = e / (db * 16 * 64), j = reg & 15;
+  const int r = 32 * (reg >> 4) + 8 * (j >> 2) + 4 * (lane >> 5) + (j & 3), c = 32 * wave + (lane & 31);
+  const bool in = r < p.dk && c < p.dv;
+  const int64_t at = nk * p.dk * p.dv + (int64_t)r * p.dv + c;
+  const int h = (int)(nk % p.kv_heads);
+  const Factor first = la_factor(p, h, p.seg - p.pad < p.l ? p.seg - p.pad : p.l), f = la_factor(p, h, p.seg),
+               last = la_factor(p, h, p.l + p.pad - (p.nseg - 1) * p.seg);
+  float* part = p.part + nk * p.nseg * per + e;
+  float s = p.s_in && in ? p.s_in[at] : 0.f;
+  float add[2][CB];
+  auto load = [&](int buf, int64_t s0) __attribute__((always_inline)) {
+#pragma unroll
+    for (int k = 0; k < CB; ++k) add[buf][k] = part[(s0 + k < p.nseg ? s0 + k : p.nseg - 1) * per];
+  };
+  auto run = [&](int buf, int64_t s0) __attribute__((always_inline)) {
+#pragma unroll
+    for (int k = 0; k < CB; ++k) {
+      if (s0 + k >= p.nseg) break;
+      part[(s0 + k) * per] = s;
+      const Factor& by = s0 + k == 0 ? first : s0 + k == p.nseg - 1 ? last : f;
+      s = la_scaled(s, by, add[buf][k]);
+    }
+  };
+  load(0, 0);
+  for (int64_t s0 = 0; s0 < p.nseg; s0 += 2 * CB) {
+    load(1, s0 + CB);
+    run(0, s0);
+    load(0, s0 + 2 * CB);
+    run(1, s0 + CB);
+  }
+  if (in) p.s_out[at] = s;
+}
+
+struct LaPlan {
+  bool chunks;
+  int64_t seg, nseg, pad;
+  int waves, slice;  // of values: waves of 32 columns; columns of a step workgroup
+  size_t part;
+};
+
+LaPlan la_plan(int32_t dt, int64_t n, int64_t l, int64_t kv_heads, int64_t dk, int64_t dv) {
+  LaPlan g{};
+  const int64_t nk = n * kv_heads;
+  if (l <= 16) {
+    g.slice = dv <= 32 ? 32 : dv <= 64 ? 64 : 128;
+    while (g.slice > 32 && nk * cdiv(dv, g.slice) < 2 * device_cus()) g.slice /= 2;
+    return g;
+  }
+  const int64_t kt = dt == DT_BF16 && dk <= 64 ? 64 : 32, chunks = cdiv(l, kt);
+  g.chunks = true;
+  g.waves = (int)cdiv(dv, 32);
+  g.pad = chunks * kt - l;
+  const int64_t want = cdiv(8LL * device_cus(), nk * g.waves);  // segments for two waves per SIMD
+  g.seg = cdiv(chunks, std::max<int64_t>(std::min(want, cdiv(chunks, 2)), 1)) * kt;
+  g.nseg = cdiv(chunks * kt, g.seg);
+  g.part = (size_t)(nk * g.nseg) * g.waves * cdiv(dk, 32) * 4096;
+  return g;
+}
+
+bool la_fits(int64_t n, int64_t l, int64_t heads, int64_t kv_heads) {
+  return n < (1 << 20) && kv_heads < (1 << 20) && n * kv_heads < (1 << 20) && heads < (1 << 20) && l < ((int64_t)1 << 31);
+}
+
+template <int DT, int DK, int W>
+void la_launch(const LinP& k, hipStream_t st) {
+  const dim3 grid((unsigned)(8 * cdiv(k.nk * k.nseg, 8)));
+  constexpr int DB = DK / 32;
+  hipLaunchKernelGGL((la_chunk_kernel<DT, DK, W, false>), grid, dim3(64 * W), 0, st, k);
+  hipLaunchKernelGGL((la_carry_kernel<8>), dim3((unsigned)cdiv(k.nk * W * DB * 1024, LA_T)), dim3(LA_T), 0, st, k, W, DB);
+  hipLaunchKernelGGL((la_chunk_kernel<DT, DK, W, true>), grid, dim3(64 * W), 0, st, k);
+}
+
+template <int DT, int DK>
+void la_launch_dk(const LinP& k, int waves, hipStream_t st) {
+  if (waves == 1) la_launch<DT, DK, 1>(k, st);
+  else if (waves == 2) la_launch<DT, DK, 2>(k, st);
+  else if (waves == 3) la_launch<DT, DK, 3>(k, st);
+  else la_launch<DT, DK, 4>(k, st);
+}
+
+template <int DT>
+void la_launch_dt(const LinP& k, const LaPlan& g, hipStream_t st) {
+  if (g.chunks) {
+    if (k.dk <= 32) la_launch_dk<DT, 32>(k, g.waves, st);
+    else if (k.dk <= 64) la_launch_dk<DT, 64>(k, g.waves, st);
+    else if (k.dk <= 96) la_launch_dk<DT, 96>(k, g.waves, st);
+    else la_launch_dk<DT, 128>(k, g.waves, st);
+    return;
+  }
+  const dim3 grid((unsigned)(k.nk * k.slices));
+#define CLARUS_LA(DVS)                                                                                                   \
+  do {                                                                                                                   \
+    if (k.dk <= 32) hipLaunchKernelGGL((la_step_kernel<DT, DVS, 32 * DVS / 1024>), grid, dim3(LA_T), 0, st, k);          \
+    else if (k.dk <= 64) hipLaunchKernelGGL((la_step_kernel<DT, DVS, 64 * DVS / 1024>), grid, dim3(LA_T), 0, st, k);     \
+    else hipLaunchKernelGGL((la_step_kernel<DT, DVS, 128 * DVS / 1024>), grid, dim3(LA_T), 0, st, k);                    \
+  } while (0)
+  if (g.slice == 32) CLARUS_LA(32);
+  else if (g.slice == 64) CLARUS_LA(64);
+  else CLARUS_LA(128);
+#undef CLARUS_LA
+}
+
+}  // namespace
+
+}  // namespace clarus
+
+using namespace clarus;
+
+extern "C" size_t clarus_hip_linear_attention_workspace(int32_t dtype, int64_t n, int64_t l, int64_t heads, int64_t kv_heads,
+                                                        int64_t dk, int64_t dv) {
+  if (n <= 0 || l <= 0 || heads <= 0 || kv_heads <= 0 || heads % kv_heads || dk <= 0 || dk > 128 || dv <= 0 || dv > 128 ||
+      !la_fits(n, l, heads, kv_heads))
+    return 0;
+  return la_plan(dtype, n, l, kv_heads, dk, dv).part;
+}
+
+extern "C" int clarus_hip_linear_attention(const ClarusLinearArgs* a, void* scratch, size_t scratch_bytes, void* stream) {
+  clear_error();
+  CLARUS_REQUIRE(a, "linear_attention: null arguments");
+  CLARUS_REQUIRE(a->q && a->k && a->v && a->out && a->log_decay && a->state_out, "linear_attention: null operand");
+  CLARUS_REQUIRE(a->n > 0 && a->l > 0 && a->heads > 0 && a->kv_heads > 0, "linear_attention: empty problem");
+  CLARUS_REQUIRE(a->heads % a->kv_heads == 0, "linear_attention: heads a multiple of kv_heads");
+  CLARUS_REQUIRE(a->dk >= 8 && a->dk <= 128 && a->dk % 8 == 0 && a->dv >= 8 && a->dv <= 128 && a->dv % 8 == 0,
+                 "linear_attention: head widths multiples of 8, at most 128");
+  CLARUS_REQUIRE((a->dtype == DT_BF16 || a->dtype == DT_F32) && (a->o_dtype == DT_BF16 || a->o_dtype == DT_F32),
+                 "linear_attention: bf16 or fp32");
+  CLARUS_REQUIRE(a->scale == a->scale && fabsf(a->scale) < INFINITY, "linear_attention: scale");
+  const int64_t es = a->dtype == DT_BF16 ? 2 : 4;
+  CLARUS_REQUIRE(aligned(a->q, 16) && aligned(a->k, 16) && aligned(a->v, 16) && aligned(a->out, 16) && a->ldq * es % 16 == 0 &&
+                     a->ldk * es % 16 == 0 && a->ldv * es % 16 == 0 && a->q_bstride * es % 16 == 0 &&
+                     a->k_bstride * es % 16 == 0 && a->v_bstride * es % 16 == 0,
+                 "linear_attention: 16-byte aligned rows");
+  CLARUS_REQUIRE(a->ldq >= 0 && a->ldk >= 0 && a->ldv >= 0 && a->q_bstride >= 0 && a->k_bstride >= 0 && a->v_bstride >= 0,
+                 "linear_attention: strides");
+  CLARUS_REQUIRE(a->ldk < (1 << 24) && a->ldv < (1 << 24), "linear_attention: rows of k and v less than 2^24 elements apart");
+  CLARUS_REQUIRE(aligned(a->state_in, 16) && aligned(a->state_out, 16) && aligned(a->log_decay, 4), "linear_attention: aligned states");
+  CLARUS_REQUIRE(la_fits(a->n, a->l, a->heads, a->kv_heads), "linear_attention: too large");
+  const LaPlan g = la_plan(a->dtype, a->n, a->l, a->kv_heads, a->dk, a->dv);
+  CLARUS_REQUIRE(!g.chunks || (a->n * a->kv_heads * g.nseg < (1 << 23) && a->n * a->kv_heads * g.waves * cdiv(a->dk, 32) * 4 < (1 << 23)),
+                 "linear_attention: too large");
+  CLARUS_REQUIRE(g.part == 0 || (scratch && aligned(scratch, 16) && scratch_bytes >= g.part),
+                 "linear_attention: scratch %zu < %zu bytes", scratch_bytes, g.part);
+  LinP k{};
+  k.q = a->q; k.k = a->k; k.v = a->v; k.out = a->out;
+  k.s_in = a->state_in; k.s_out = a->state_out; k.decay = a->log_decay; k.part = (float*)scratch;
+  k.qbs = a->q_bstride; k.ldq = a->ldq; k.kbs = a->k_bstride; k.ldk = a->ldk; k.vbs = a->v_bstride; k.ldv = a->ldv;
+  k.l = a->l; k.nk = a->n * a->kv_heads; k.nseg = g.nseg; k.seg = g.seg; k.pad = g.pad;
+  k.rep = (int)(a->heads / a->kv_heads); k.kv_heads = (int)a->kv_heads; k.dk = (int)a->dk; k.dv = (int)a->dv;
+  k.o_dt = a->o_dtype; k.scale = a->scale;
+  k.slices = g.chunks ? 1 : (int)cdiv(a->dv, g.slice);
+  note_kernel(g.chunks ? "la_chunk_kernel segments=%lld waves=%d" : "la_step_kernel slices=%lld of %d",
+              (long long)(g.chunks ? g.nseg : k.slices), g.chunks ? g.waves : g.slice);
+  if (a->dtype == DT_BF16) la_launch_dt<DT_BF16>(k, g, (hipStream_t)stream);
+  else la_launch_dt<DT_F32>(k, g, (hipStream_t)stream);
+  return check_launch("linear_attention");
+}

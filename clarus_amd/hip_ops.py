@@ -1100,6 +1100,76 @@ class HipOps(Backend):
         return odt, args, self._workspace(self.lib.clarus_hip_cross_attention_workspace, args.dtype, n, lq, lk, heads, kv_heads,
                                           d, mode)
 
+    def linear_attention(self, q, k, v, log_decay, heads, kv_heads=None, state=None, scale=None, state_out=None, out_dtype=None):
+        """Causal linear attention with a decay for each head over tokens in order (rasters, frames): per image and kv
+        head S_t = exp(log_decay) S_{t-1} + k_t v_t^T, out_t = scale q_t^T S_t for the heads that share it. q [N, ...,
+        heads * dk], k [N, ..., kv_heads * dk], v [N, ..., kv_heads * dv] with the same tokens (slices of wider rows qualify);
+        log_decay [kv_heads], at most 0; scale 1 / sqrt(dk) by default. state [N, kv_heads, dk, dv] fp32: S before the first
+        token (None: zeros), so that a sequence can go on where an earlier call ended, piece by piece or token by
+        token. Returns (out [N, ..., heads * dv], the state behind the last token); state_out: a tensor to write the
+        state to, which may be `state` itself. fp32 states and sums; with bf16, products q . k within 64 tokens are rounded
+        to bf16."""
+        kv_heads = heads if kv_heads is None else kv_heads
+        if not (isinstance(heads, int) and isinstance(kv_heads, int)):  # before the plans, whose keys 4.0 and 4 share
+            raise Unsupported(f"linear_attention: heads and kv_heads integers, got {heads!r} {kv_heads!r}")
+        scale = None if scale is None else float(scale)
+        key = ("linear_attention", q.shape, q.stride(), k.shape, k.stride(), v.shape, v.stride(), q.dtype, k.dtype, v.dtype, heads,
+               kv_heads, scale, out_dtype, log_decay.shape, log_decay.dtype,
+               *(None if t is None else (t.shape, t.stride(), t.dtype) for t in (state, state_out)))
+        self._forward_only("linear_attention", q, k, v, log_decay, state, state_out)
+        odt, shape, sshape, args, need = self._plan(key, lambda: self._linear_plan_state(
+            q, k, v, log_decay, heads, kv_heads, state, scale, state_out, out_dtype or self.dtype))
+        qp, kp, vp = q.data_ptr(), k.data_ptr(), v.data_ptr()
+        sp, op = _lib.ptr(state), _lib.ptr(state_out)
+        if (qp | kp | vp | (sp or 0) | (op or 0)) % 16:
+            raise Unsupported("linear_attention: 16-byte aligned rows and states")
+        out = torch.empty(shape, device=q.device, dtype=odt)
+        last = torch.empty(sshape, device=q.device, dtype=torch.float32) if state_out is None else state_out
+        if args is None:  # no token: the state stays
+            if last is not state:
+                last.zero_() if state is None else last.copy_(state)
+            return out, last
+        decay = log_decay if log_decay.dtype == torch.float32 and log_decay.is_contiguous() else log_decay.float().contiguous()
+        args = _lib.LinearArgs.from_buffer_copy(args)
+        args.q, args.k, args.v, args.out, args.log_decay = qp, kp, vp, out.data_ptr(), decay.data_ptr()
+        args.state_in, args.state_out = sp, last.data_ptr()
+        scratch = torch.empty(need, device=q.device, dtype=torch.uint8) if need else None
+        self._call("linear_attention", self.lib.clarus_hip_linear_attention, ctypes.byref(args), _lib.ptr(scratch), need)
+        return out, last
+
+    def _linear_plan_state(self, q, k, v, log_decay, heads, kv_heads, state, scale, state_out, odt):
+        if q.dim() < 2 or k.dim() < 2 or v.dim() < 2:
+            raise Unsupported("linear_attention: q, k, v [N, ..., C]")
+        n, ck, cv = q.shape[0], k.shape[-1], v.shape[-1]
+        if not (heads > 0 and kv_heads > 0 and heads % kv_heads == 0 and ck % kv_heads == 0 and cv % kv_heads == 0
+                and q.shape[-1] * kv_heads == ck * heads and q.shape[:-1] == k.shape[:-1] == v.shape[:-1]):
+            raise Unsupported("linear_attention: q [N, ..., heads dk], k [N, ..., kv_heads dk], v [N, ..., kv_heads dv] of the same "
+                              "tokens, heads a multiple of kv_heads")
+        dk, dv, l = ck // kv_heads, cv // kv_heads, math.prod(q.shape[1:-1])
+        held = ctypes.c_float(dk ** -0.5 if scale is None and dk else scale or 0.0).value  # as the call passes it on
+        if not (_kdt(q) and q.dtype == k.dtype == v.dtype and odt in _KDT and all(8 <= d <= 128 and d % 8 == 0 for d in (dk, dv))
+                and math.isfinite(held)):
+            raise Unsupported("linear_attention: bf16 / fp32 q, k, v of one type, head widths multiples of 8 up to 128, scale finite")
+        if tuple(log_decay.shape) != (kv_heads,) or not log_decay.is_floating_point():
+            raise Unsupported("linear_attention: log_decay [kv_heads]")
+        sshape = (n, kv_heads, dk, dv)
+        if any(t is not None and not (tuple(t.shape) == sshape and t.dtype == torch.float32 and t.is_contiguous())
+               for t in (state, state_out)):
+            raise Unsupported("linear_attention: states [N, kv_heads, dk, dv], fp32, contiguous")
+        shape = (*q.shape[:-1], heads * dv)
+        if n * l == 0:
+            return odt, shape, sshape, None, 0
+        at, es = [_rows(t) for t in (q, k, v)], q.element_size()
+        if None in at or any(s * es % 16 for t in at for s in t[1:]) or max(at[1][1], at[2][1]) >= 1 << 24:
+            raise Unsupported("linear_attention: unit channel stride, one row stride (k and v: below 2^24), 16-byte aligned rows")
+        if n * kv_heads >= 1 << 20 or heads >= 1 << 20 or l >= 1 << 31:
+            raise Unsupported("linear_attention: fewer than 2^20 (image, kv head) pairs and 2^31 tokens")
+        args = _lib.LinearArgs(n=n, l=l, heads=heads, kv_heads=kv_heads, dk=dk, dv=dv, q_bstride=at[0][2], ldq=at[0][1],
+                               k_bstride=at[1][2], ldk=at[1][1], v_bstride=at[2][2], ldv=at[2][1], dtype=_lib.dtype_code(q.dtype),
+                               o_dtype=_lib.dtype_code(odt), scale=held)
+        return odt, shape, sshape, args, self._workspace(self.lib.clarus_hip_linear_attention_workspace, args.dtype, n, l, heads,
+                                                         kv_heads, dk, dv)
+
     def channel_attention(self, qkv, heads, temperature):
         if not qkv.is_contiguous():
             raise Unsupported("channel_attention: contiguous qkv only")

@@ -577,6 +577,35 @@ typedef struct ClarusAddNormArgs {
 
 int clarus_hip_add_norm(const ClarusAddNormArgs* args, void* stream);
 
+/*
+ * Causal linear attention with a decay for each head, carried by a state; per image and kv head g
+ *   S_t = exp(log_decay[g]) S_{t-1} + k_t v_t^T,   out_t[h] = scale q_t[h]^T S_t   for heads h of kv head h / (heads / kv_heads).
+ * q rows at q + n * q_bstride + t * ldq, head h at column h * dk; k likewise, v and out with heads of dv (16-byte aligned
+ * rows, slices of wider rows, ldk and ldv below 2^24; dk, dv multiples of 8, at most 128); out [n, l, heads * dv] contiguous. state_in
+ * [n, kv_heads, dk, dv] fp32 or NULL for zeros; state_out the same, may be state_in itself; nothing else overlaps. log_decay
+ * fp32 [kv_heads], at most 0 (0 keeps all, -inf nothing but the token). States, sums and factors in fp32; with bf16 the
+ * products q . k of tokens up to 64 apart are rounded once to bf16. n * kv_heads < 2^20, l < 2^31. scratch holds
+ * clarus_hip_linear_attention_workspace(...) bytes (may be 0), 16-byte aligned. Deterministic. No counterpart in the reference
+ * (its recurrence is selective_scan's).
+ */
+typedef struct ClarusLinearArgs {
+  const void* q;
+  const void* k;
+  const void* v;
+  void* out;
+  const float* log_decay;
+  const float* state_in;
+  float* state_out;
+  int64_t n, l, heads, kv_heads, dk, dv;
+  int64_t q_bstride, ldq, k_bstride, ldk, v_bstride, ldv;
+  int32_t dtype, o_dtype;
+  float scale;
+} ClarusLinearArgs;
+
+size_t clarus_hip_linear_attention_workspace(int32_t dtype, int64_t n, int64_t l, int64_t heads, int64_t kv_heads, int64_t dk,
+                                             int64_t dv);
+int clarus_hip_linear_attention(const ClarusLinearArgs* args, void* scratch, size_t scratch_bytes, void* stream);
+
 /* ABI version (CLARUS_HIP_ABI_VERSION) and struct sizes, for binding checks. */
 int clarus_hip_abi_version(void);
 size_t clarus_hip_sizeof_gemm_args(void);
@@ -584,6 +613,7 @@ size_t clarus_hip_sizeof_conv_args(void);
 size_t clarus_hip_sizeof_cross_args(void);
 size_t clarus_hip_sizeof_rotary_args(void);
 size_t clarus_hip_sizeof_add_norm_args(void);
+size_t clarus_hip_sizeof_linear_args(void);
 
 /* Text of the calling thread's last failure ("" if none). */
 const char* clarus_hip_last_error(void);

@@ -207,6 +207,21 @@ class TorchRef:
         h = norm(r, ln, weight, bias).reshape(x.shape).to(self._odt(out_dtype)) if ln else None
         return r.reshape(x.shape).to(x.dtype), h
 
+    def linear_attention(self, q, k, v, log_decay, heads, kv_heads=None, state=None, scale=None, state_out=None, out_dtype=None):
+        """No reference op: S <- e^g S + k v^T, out = scale q^T S, token after token."""
+        kv_heads = kv_heads or heads
+        n, rep, dk = q.shape[0], heads // kv_heads, q.shape[-1] // heads
+        qh = q.float().reshape(n, -1, kv_heads, rep, dk) * (dk ** -0.5 if scale is None else scale)
+        kh, vh = (t.float().reshape(n, qh.shape[1], kv_heads, -1) for t in (k, v))
+        s = torch.zeros(n, kv_heads, dk, vh.shape[-1], device=q.device) if state is None else state.clone()
+        f = log_decay.float().exp()[:, None, None]
+        out = []
+        for t in range(qh.shape[1]):
+            s = s * f + kh[:, t, :, :, None] * vh[:, t, :, None]
+            out.append(qh[:, t] @ s)
+        y = torch.stack(out, 1).reshape(*q.shape[:-1], -1).to(self._odt(out_dtype))
+        return (y, s) if state_out is None else (y, state_out.copy_(s))
+
     def channel_attention(self, qkv, heads, temperature):
         """torch_ref.py:220-235: softmax((q/|q|)(k/|k|)^T * t) per image and head, fp32."""
         n, h, w, c3 = qkv.shape
