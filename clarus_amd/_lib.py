@@ -102,6 +102,16 @@ class LinearArgs(ctypes.Structure):
     ]
 
 
+class SparseArgs(ctypes.Structure):
+    _fields_ = [
+        ("q", _vp), ("k", _vp), ("v", _vp), ("out", _vp), ("mask", _vp), ("means", _vp), ("chosen", _vp),
+        ("n", _i64), ("lq", _i64), ("lk", _i64), ("heads", _i64), ("kv_heads", _i64), ("d", _i64),
+        ("top", _i64), ("block", _i64), ("group", _i64),
+        ("q_bstride", _i64), ("ldq", _i64), ("k_bstride", _i64), ("ldk", _i64), ("v_bstride", _i64), ("ldv", _i64),
+        ("mask_bstride", _i64), ("dtype", _i32), ("o_dtype", _i32), ("scale", _f32),
+    ]
+
+
 # name -> (restype, argtypes); every function declared in include/clarus_hip.h
 SIGNATURES = {
     "clarus_hip_gemm": (_i32, [ctypes.POINTER(GemmArgs), _vp]),
@@ -145,6 +155,9 @@ SIGNATURES = {
     "clarus_hip_add_norm": (_i32, [ctypes.POINTER(AddNormArgs), _vp]),
     "clarus_hip_linear_attention_workspace": (ctypes.c_size_t, [_i32] + [_i64] * 6),
     "clarus_hip_linear_attention": (_i32, [ctypes.POINTER(LinearArgs), _vp, ctypes.c_size_t, _vp]),
+    "clarus_hip_block_means": (_i32, [_vp, _i32, _i64, _i64, _vp, _i64, _vp, _i64, _i64, _i64, _i64, _vp]),
+    "clarus_hip_sparse_attention_workspace": (ctypes.c_size_t, [_i32] + [_i64] * 9 + [_i32] * 2),
+    "clarus_hip_sparse_attention": (_i32, [ctypes.POINTER(SparseArgs), _vp, ctypes.c_size_t, _vp]),
     "clarus_hip_abi_version": (_i32, []),
     "clarus_hip_sizeof_gemm_args": (ctypes.c_size_t, []),
     "clarus_hip_sizeof_conv_args": (ctypes.c_size_t, []),
@@ -152,6 +165,7 @@ SIGNATURES = {
     "clarus_hip_sizeof_rotary_args": (ctypes.c_size_t, []),
     "clarus_hip_sizeof_add_norm_args": (ctypes.c_size_t, []),
     "clarus_hip_sizeof_linear_args": (ctypes.c_size_t, []),
+    "clarus_hip_sizeof_sparse_args": (ctypes.c_size_t, []),
     "clarus_hip_last_error": (ctypes.c_char_p, []),
     "clarus_hip_last_kernel": (ctypes.c_char_p, []),
 }
@@ -184,7 +198,8 @@ def load(path: str = LIB_PATH):
         raise RuntimeError("ClarusConvArgs layout differs between the library and the binding")
     if lib.clarus_hip_sizeof_cross_args() != ctypes.sizeof(CrossArgs):
         raise RuntimeError("ClarusCrossArgs layout differs between the library and the binding")
-    for cls, name in ((RotaryArgs, "rotary"), (AddNormArgs, "add_norm"), (LinearArgs, "linear")):
+    for cls, name in ((RotaryArgs, "rotary"), (AddNormArgs, "add_norm"), (LinearArgs, "linear"),
+                      (SparseArgs, "sparse")):
         if getattr(lib, f"clarus_hip_sizeof_{name}_args")() != ctypes.sizeof(cls):
             raise RuntimeError(f"{cls.__name__} layout differs between the library and the binding")
     _LIB = lib

@@ -57,6 +57,8 @@ size_t clarus_hip_sizeof_add_norm_args(void) { return sizeof(ClarusAddNormArgs);
 
 size_t clarus_hip_sizeof_linear_args(void) { return sizeof(ClarusLinearArgs); }
 
+size_t clarus_hip_sizeof_sparse_args(void) { return sizeof(ClarusSparseArgs); }
+
 const char* clarus_hip_last_error(void) { return clarus::g_err; }
 
 const char* clarus_hip_last_kernel(void) { return clarus::g_kernel; }

@@ -1,0 +1,498 @@
+// Attention over the blocks of keys that a cheap score selects, on gfx950. Per image and head:
+//   m_b = mean of the kept keys of block b,  a_g = mean of the queries of group g  (64 bits, rounded to fp32)
+//   the `top` blocks of the largest a_g . m_b (64 bits; equal ones: the lowest index; a block without a kept key: never)
+//   o_i = softmax_j(scale q_i . k_j) v_j  over the kept keys j of the blocks chosen by i's group; 0 where there are none.
+//
+//   sp_means_kernel   the means of blocks of keys, or of groups of queries
+//   sp_score_kernel   scores of a slab of rows (image, head, group), 64 bits
+//   sp_choose_kernel  a row's choice as bits, 64 blocks a word
+//   sp_kernel         the attention: 32 rows per wave as in cross_attention.hip (a row is a query and one of the heads that
+//                     share a kv head); a workgroup takes the blocks that any of its rows has chosen, one after another
+//                     through LDS, and a wave those of its own rows, the bits of each row masking what the others chose
+//   xa_join_kernel    joins the parts of blocks split over workgroups, where rows are few
+#include <algorithm>
+
+#include "attention_tile.hpp"
+#include "capi.hpp"
+
+namespace clarus {
+
+namespace {
+
+constexpr int SP_T = 256;
+constexpr int SP_WORDS = 32;   // words of 64 blocks that a workgroup of sp_kernel lists at a time
+constexpr int SP_TILE = 64;    // rows and blocks of a score workgroup
+constexpr int64_t SP_SLAB = 128 << 20;  // bytes of scores at a time, about
+
+struct SparseP {
+  CrossP x;
+  uint64_t* chosen;       // [n][heads][groups][nw]
+  const float* means;     // [n][nb][kv_heads * d]
+  const void* asks;       // rows of queries, or of their groups' means (fp32)
+  int64_t abs, lda;
+  double* score;          // of a slab, [row][nb]
+  int64_t nw, nb, groups, first;  // first: the slab's first row (image, head, group)
+  int64_t slab;           // rows of this slab
+  int block, group, top, heads, ask_dt;
+  int tpb;                // tiles of a block
+};
+
+// ---------------------------------------------------------------- means
+// A workgroup: one block of rows (of `size`; the last may be shorter) and up to 8 x SP_T / rg columns, rg rows at a time
+template <int DT>
+__global__ void __launch_bounds__(SP_T) sp_means_kernel(const unsigned char* x, int64_t xbs, int64_t ldx, const unsigned char* mask, int64_t mbs,
+                                                        float* out, int64_t rows, int64_t c, int64_t size, unsigned nb, int rg) {
+  constexpr int ES = DT == DT_BF16 ? 2 : 4;
+  __shared__ double part[SP_T][8];
+  __shared__ int count[SP_T];
+  const int tid = threadIdx.x, per = SP_T / rg, r0 = tid / per;
+  const unsigned n = blockIdx.x / nb, b = blockIdx.x - n * nb;
+  const int64_t col = ((int64_t)blockIdx.y * per + tid - r0 * per) * 8;
+  const bool in = col < c;
+  const int64_t first = (int64_t)b * size, last = first + size < rows ? first + size : rows;
+  double s[8];
+#pragma unroll
+  for (int e = 0; e < 8; ++e) s[e] = 0.0;
+  int kept = 0;
+  const unsigned char* xp = x + (n * xbs + (in ? col : 0)) * ES;
+  for (int64_t r = first + r0; r < last; r += rg) {
+    if (mask && !mask[n * mbs + r]) continue;
+    ++kept;
+    const f32x8 v = load8<DT>(xp + r * ldx * ES);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) s[e] += (double)v.v[e];
+  }
+#pragma unroll
+  for (int e = 0; e < 8; ++e) part[tid][e] = s[e];
+  count[tid] = kept;
+  __syncthreads();
+  if (r0 || !in) return;
+  for (int i = 1; i < rg; ++i) {
+    kept += count[tid + i * per];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) s[e] += part[tid + i * per][e];
+  }
+  float* to = out + ((int64_t)n * nb + b) * c + col;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) to[e] = (float)(s[e] / (double)kept);  // 0 / 0 where nothing is kept
+}
+
+// ---------------------------------------------------------------- scores
+__global__ void __launch_bounds__(SP_T) sp_score_kernel(const SparseP p) {
+  constexpr int KC = 32;  // columns at a time
+  __shared__ float sa[SP_TILE][KC + 1], sm[SP_TILE][KC + 1];
+  const int tid = threadIdx.x, tx = tid & 15, ty = tid >> 4, d = p.x.d;
+  const int64_t row0 = (int64_t)blockIdx.x * SP_TILE, b0 = (int64_t)blockIdx.y * SP_TILE;
+  double acc[4][4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) acc[i][j] = 0.0;
+  // rows of one workgroup may be of several heads, each with means of its own: one head after another
+  const int64_t all = p.slab - row0 < SP_TILE ? p.slab - row0 : SP_TILE;
+  for (int64_t i0 = 0; i0 < all;) {
+    const int64_t nh = (p.first + row0 + i0) / p.groups, g0 = p.first + row0 + i0 - nh * p.groups;
+    const int64_t i1 = std::min(all, i0 + p.groups - g0);
+    const int64_t n = nh / p.heads, h = nh - n * p.heads;
+    const float* mp = p.means + (n * p.nb * p.x.kv_heads + h / p.x.rep) * d;
+    for (int c0 = 0; c0 < d; c0 += KC) {
+      __syncthreads();
+      for (int i = tid; i < SP_TILE * KC; i += SP_T) {
+        const int r = i / KC, c = i - r * KC;
+        const bool mine = r >= i0 && r < i1 && c0 + c < d;
+        sa[r][c] = mine ? load1(p.asks, p.ask_dt, n * p.abs + (g0 + r - i0) * p.lda + h * d + c0 + c) : 0.f;
+        sm[r][c] = b0 + r < p.nb && c0 + c < d ? mp[(b0 + r) * p.x.kv_heads * d + c0 + c] : 0.f;
+      }
+      __syncthreads();
+#pragma unroll 4
+      for (int c = 0; c < KC; ++c) {
+        double a[4], m[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) a[i] = sa[ty + 16 * i][c], m[i] = sm[tx + 16 * i][c];
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if (ty + 16 * i >= i0 && ty + 16 * i < i1)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) acc[i][j] = fma(a[i], m[j], acc[i][j]);
+      }
+    }
+    i0 = i1;
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      if (ty + 16 * i < all && b0 + tx + 16 * j < p.nb) p.score[(row0 + ty + 16 * i) * p.nb + b0 + tx + 16 * j] = acc[i][j];
+}
+
+// order of scores as whole numbers; 0: none (NaN, -inf)
+__device__ __forceinline__ uint64_t sp_key(double v) {
+  if (!(v > -INFINITY)) return 0;
+  const uint64_t u = __builtin_bit_cast(uint64_t, v + 0.0);
+  return u >> 63 ? ~u : u | 1ull << 63;
+}
+
+// a workgroup per row: the top-th largest score found byte by byte from the highest, then the bits
+__global__ void __launch_bounds__(SP_T) sp_choose_kernel(const SparseP p) {
+  __shared__ int hist[256], at[2], ties[SP_T / 64];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const double* s = p.score + (int64_t)blockIdx.x * p.nb;
+  uint64_t* to = p.chosen + (p.first + blockIdx.x) * p.nw;
+  uint64_t prefix = 0;
+  int left = p.top;  // of the top ones, those whose higher bytes are `prefix`
+  for (int shift = 56; shift >= 0; shift -= 8) {
+    __syncthreads();
+    hist[tid] = 0;
+    __syncthreads();
+    for (int64_t b = tid; b < p.nb; b += SP_T) {
+      const uint64_t k = sp_key(s[b]);
+      if (shift == 56 || k >> (shift + 8) == prefix) atomicAdd(&hist[k >> shift & 255], 1);
+    }
+    __syncthreads();
+    if (tid == 0) {
+      int i = 255, seen = 0;
+      while (i > 0 && seen + hist[i] < left) seen += hist[i--];
+      at[0] = i;
+      at[1] = left - seen;
+    }
+    __syncthreads();
+    prefix = prefix << 8 | (uint64_t)at[0];
+    left = at[1];
+  }
+  // every score above prefix, and the first `left` equal to it
+  int before = 0;
+  for (int64_t b0 = 0; b0 < p.nb; b0 += SP_T) {
+    const int64_t b = b0 + tid;
+    const uint64_t k = b < p.nb ? sp_key(s[b]) : 0;
+    const uint64_t same = __ballot(k == prefix && k != 0);
+    __syncthreads();
+    if (lane == 0) ties[wave] = __popcll(same);
+    __syncthreads();
+    int rank = before;
+    for (int w = 0; w < wave; ++w) rank += ties[w];
+    for (int w = 0; w < SP_T / 64; ++w) before += ties[w];
+    rank += __popcll(same & ((1ull << lane) - 1));
+    const uint64_t word = __ballot(k > prefix || (k == prefix && k != 0 && rank < left));
+    if (lane == 0 && b0 / 64 + wave < p.nw) to[b0 / 64 + wave] = word;
+  }
+}
+
+// ---------------------------------------------------------------- attention
+__device__ __forceinline__ uint64_t or32(uint64_t v) {  // over the 32 lanes of a half
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) v |= __shfl_xor(v, o, 64);
+  return v;
+}
+
+template <int DT, int D, int C, int MASK, int W>
+__global__ void __launch_bounds__(64 * W, D <= 64 ? 3 : 2) sp_kernel(const SparseP sp) {
+  using T = XaTile<DT, D>;
+  constexpr int KT = T::KT, KB = KT / 32, DB = D / 32;
+  const CrossP& p = sp.x;
+  __shared__ __align__(16) unsigned char tiles[2][2 * T::BYTES];
+  __shared__ uint64_t wants[W][SP_WORDS];
+  __shared__ unsigned short list[SP_WORDS * 64];  // blocks of the words at hand that a row of the workgroup has chosen
+
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int col = lane & 31, hl = lane >> 5;
+  // as xa_kernel: row blocks and splits of one (image, kv head) on one XCD
+  const unsigned per = (unsigned)(p.nblk * p.splits), xcd = blockIdx.x & 7, j = blockIdx.x >> 3, whole = (unsigned)(p.nk >> 3) * per;
+  unsigned nk, rest;
+  if (j < whole) {
+    nk = j / per;
+    rest = j - nk * per;
+    nk = nk * 8 + xcd;
+  } else {
+    const unsigned left = (unsigned)(p.nk & 7) * per, span = (left + 7) >> 3, i = xcd * span + (j - whole);
+    if (j - whole >= span || i >= left) return;
+    nk = i / per;
+    rest = i - nk * per;
+    nk += (unsigned)p.nk & ~7u;
+  }
+  const unsigned split = rest / (unsigned)p.nblk, rb = rest - split * (unsigned)p.nblk;
+  const int n = (int)nk / p.kv_heads, kvh = (int)nk - n * p.kv_heads;
+  const int64_t wrow = (int64_t)rb * (32 * W) + wave * 32;
+  const bool busy = wrow < p.rows;
+  const int64_t row = wrow + col < p.rows ? wrow + col : p.rows - 1;  // rows past the end repeat the last one
+  const XaRow r = xa_row(p, kvh, row);
+  const unsigned char* kp = (const unsigned char*)p.k + (n * p.kbs + (int64_t)kvh * p.d) * T::ES;
+  const unsigned char* vp = (const unsigned char*)p.v + (n * p.vbs + (int64_t)kvh * p.d) * T::ES;
+  const unsigned char* mkey = MASK == MASK_KEYS ? p.mask + n * p.mbs : nullptr;
+  const uint64_t* words = sp.chosen + (((int64_t)n * sp.heads + r.head) * sp.groups + (unsigned)r.qi / (unsigned)sp.group) * sp.nw;
+
+  const XaCopy<DT, D, W> copy(p, wave, lane);
+  auto fill = [&](int64_t t, uint64_t bits, int buf) __attribute__((always_inline)) {
+    const int64_t base = t * KT;
+    copy(p, kp + base * p.ldk * T::ES, vp + base * p.ldv * T::ES, tiles[buf], bits);
+  };
+  u32x4 qf[xa_qn<DT, C>];
+  xa_load_q<DT, C>(p, n, r, hl, qf);
+  f32x16 o[DB];
+#pragma unroll
+  for (int b = 0; b < DB; ++b)
+#pragma unroll
+    for (int i = 0; i < 16; ++i) o[b][i] = 0.f;
+  float m = XA_FLOOR, l = 0.f;
+  bool far = false;
+
+#pragma unroll 1
+  for (int64_t w0 = 0; w0 < sp.nw; w0 += SP_WORDS) {
+    const int wn = sp.nw - w0 < SP_WORDS ? (int)(sp.nw - w0) : SP_WORDS;
+    if (w0) __syncthreads();  // the words and the last tile before have been read
+    for (int w = 0; w < wn; ++w) {
+      const uint64_t any = or32(busy ? words[w0 + w] : 0);
+      if (lane == 0) wants[wave][w] = any;
+    }
+    __syncthreads();
+    // every wave lists the wanted blocks in order (the same list)
+    int count = 0;
+    for (int w = 0; w < wn; ++w) {
+      uint64_t want = 0;
+#pragma unroll
+      for (int i = 0; i < W; ++i) want |= wants[i][w];
+      if (wave == 0 && (want >> lane & 1)) list[count + __popcll(want & ((1ull << lane) - 1))] = (unsigned short)(w * 64 + lane);
+      count += __popcll(want);
+    }
+    count = __builtin_amdgcn_readfirstlane(count);
+    __syncthreads();
+    const int i1 = (int)((int64_t)count * (split + 1) / p.splits);
+    int at = (int)((int64_t)count * split / p.splits) - 1, blk = 0, sub = sp.tpb;
+    auto pop = [&](int& b) __attribute__((always_inline)) -> int64_t {  // the next tile and its block, -1 past the last
+      if (++sub >= sp.tpb || ((w0 * 64 + blk) * sp.tpb + sub) * KT >= p.lk) {
+        if (++at >= i1) {
+          sub = sp.tpb;
+          --at;
+          return -1;
+        }
+        blk = __builtin_amdgcn_readfirstlane((int)list[at]);
+        sub = 0;
+      }
+      b = blk;
+      return (w0 * 64 + blk) * sp.tpb + sub;
+    };
+    auto key_byte = [&](int64_t t) __attribute__((always_inline)) { return t < 0 ? 0 : xa_key_byte<KT, MASK>(mkey, t * KT, p.lk, lane); };
+    auto word_of = [&](int b) __attribute__((always_inline)) { return words[w0 + (b >> 6)] >> (b & 63); };
+    int b = 0, b1 = 0, b2 = 0;
+    int64_t t = pop(b), t1 = pop(b1);
+    if (t < 0) continue;
+    uint64_t bits = __ballot(key_byte(t));
+    int byte = key_byte(t1), buf = 0;
+    fill(t, bits, 0);
+    uint64_t next = word_of(b);
+#pragma unroll 1
+    while (t >= 0) {
+      __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0): this wave's copies of tile t have landed
+      barrier_keep_vm();                   // everybody's have, and the tile before has been read
+      const uint64_t now = next & 1 ? bits : 0;  // of this lane's row
+      const bool mine = busy && (wants[wave][b >> 6] >> (b & 63) & 1);
+      const int64_t t2 = pop(b2);
+      if (t1 >= 0) {
+        bits = __ballot(byte);
+        byte = key_byte(t2);
+        fill(t1, bits, buf ^ 1);
+        next = word_of(b1);
+      }
+      if (mine) xa_tile<DT, D, C, MASK_PAIRS, KB, false>(tiles[buf], tiles[buf] + T::BYTES, qf, o, m, l, far, p.c, now, now == T::ALL, false);
+      t = t1;
+      b = b1;
+      t1 = t2;
+      b1 = b2;
+      buf ^= 1;
+    }
+  }
+  if (!busy) return;
+  l = sum32(l);
+  if (p.splits == 1) {
+    xa_store<D>(p, n, r, o, l, wrow + col < p.rows);
+    return;
+  }
+  if (wrow + col >= p.rows) return;
+  const int64_t to = ((int64_t)split * p.nk + nk) * p.rows + row, all = (int64_t)p.splits * p.nk * p.rows;
+  float* po = p.part + to * D;
+#pragma unroll
+  for (int b = 0; b < DB; ++b)
+#pragma unroll
+    for (int j4 = 0; j4 < 4; ++j4)
+      *reinterpret_cast<f32x4*>(po + 32 * b + 8 * j4 + 4 * hl) = f32x4{o[b][4 * j4], o[b][4 * j4 + 1], o[b][4 * j4 + 2], o[b][4 * j4 + 3]};
+  if (hl == 0) *reinterpret_cast<float2*>(p.part + all * D + 2 * to) = float2{m, l};
+}
+
+int sp_pad(int64_t d) { return d <= 32 ? 32 : d <= 64 ? 64 : d <= 96 ? 96 : 128; }
+
+struct SpPlan {
+  int64_t nb, nw, groups, nblk, slab;  // slab: rows of scores at a time
+  int splits, waves;
+  size_t means, asks, chosen, score, part;  // workspace bytes, each a multiple of 16
+  size_t total() const { return means + asks + chosen + score + part; }
+};
+
+SpPlan sp_plan(int32_t dt, int64_t n, int64_t lq, int64_t lk, int64_t heads, int64_t kv_heads, int64_t d, int64_t top, int64_t block, int64_t group,
+               bool has_means, bool has_chosen) {
+  SpPlan g{};
+  g.nb = cdiv(lk, block);
+  g.nw = cdiv(g.nb, 64);
+  g.groups = cdiv(lq, group);
+  const int64_t rows = lq * (heads / kv_heads), nk = n * kv_heads, asks = n * heads * g.groups;
+  if (!has_means) g.means = (size_t)(n * g.nb * kv_heads * d) * sizeof(float);
+  if (group > 1) g.asks = (size_t)(n * g.groups * heads * d) * sizeof(float);
+  if (!has_chosen) g.chosen = (size_t)cdiv(asks * g.nw, 2) * 16;
+  g.slab = std::min(asks, std::min<int64_t>(cdiv(SP_SLAB / 8, g.nb * SP_TILE), 1 << 16) * SP_TILE);
+  g.score = (size_t)cdiv(g.slab * g.nb, 2) * 16;
+  g.waves = rows <= 32 ? 1 : 4;
+  g.nblk = cdiv(rows, 32 * g.waves);
+  const int64_t blocks = g.nblk * nk, cus = device_cus();
+  // few rows: the blocks that they can choose split until every CU has two workgroups
+  const int64_t most = std::min(g.nb, std::min<int64_t>(rows, 32 * g.waves) * std::min(top, g.nb));
+  g.splits = (int)std::max<int64_t>(1, std::min(2 * cus / blocks, most));
+  if (g.splits > 1) g.part = (size_t)cdiv((int64_t)g.splits * nk * rows * (sp_pad(d) + 2), 4) * 16;
+  return g;
+}
+
+bool sp_fits(int64_t n, int64_t lq, int64_t lk, int64_t heads, int64_t kv_heads, int64_t block, int64_t group) {
+  const int64_t big = (int64_t)1 << 31;
+  if (!(n < 65536 && kv_heads < 65536 && n * kv_heads < 65536 && heads < 65536 && lq < big && lk < big && lq * (heads / kv_heads) < big &&
+        n * heads < big && n * kv_heads * (cdiv(lq * (heads / kv_heads), 128) * 128) < big - 4096))
+    return false;
+  const int64_t nb = cdiv(lk, block), groups = cdiv(lq, group);
+  return nb < (1 << 21) && n * nb < (1 << 23) && (group == 1 || n * groups < (1 << 23)) && n * heads * groups < big;
+}
+
+template <int DT, int D, int C, int MASK>
+void sp_launch_mask(const SparseP& k, int waves, hipStream_t st) {
+  const dim3 grid((unsigned)(8 * ((k.x.nblk * k.x.nk * k.x.splits + 7) / 8)));
+  if (waves == 1) hipLaunchKernelGGL((sp_kernel<DT, D, C, MASK, 1>), grid, dim3(64), 0, st, k);
+  else hipLaunchKernelGGL((sp_kernel<DT, D, C, MASK, 4>), grid, dim3(256), 0, st, k);
+}
+
+template <int DT, int D, int C>
+void sp_launch(const SparseP& k, int waves, hipStream_t st) {
+  if (k.x.mask) sp_launch_mask<DT, D, C, MASK_KEYS>(k, waves, st);
+  else sp_launch_mask<DT, D, C, MASK_NONE>(k, waves, st);
+  if (k.x.splits > 1) {
+    constexpr int TPR = D <= 32 ? 8 : D <= 64 ? 16 : 32;
+    int gs = 1;
+    while (gs * TPR < XA_T && gs * XJ_BATCH < k.x.splits) gs *= 2;
+    hipLaunchKernelGGL((xa_join_kernel<D>), dim3((unsigned)cdiv(k.x.rows * k.x.nk, XA_T / (TPR * gs))), dim3(XA_T), 0, st, k.x, gs);
+  }
+}
+
+void sp_means(const void* x, int dt, int64_t xbs, int64_t ldx, const void* mask, int64_t mbs, float* out, int64_t n, int64_t rows, int64_t c,
+              int64_t size, hipStream_t st) {
+  const int64_t nb = cdiv(rows, size), oct = c / 8;
+  int rg = 1;
+  while (rg < 32 && rg < size && oct * rg * 2 <= SP_T) rg *= 2;
+  const dim3 grid((unsigned)(n * nb), (unsigned)cdiv(oct, SP_T / rg));
+  if (dt == DT_BF16)
+    hipLaunchKernelGGL(sp_means_kernel<DT_BF16>, grid, dim3(SP_T), 0, st, (const unsigned char*)x, xbs, ldx, (const unsigned char*)mask, mbs, out,
+                       rows, c, size, (unsigned)nb, rg);
+  else
+    hipLaunchKernelGGL(sp_means_kernel<DT_F32>, grid, dim3(SP_T), 0, st, (const unsigned char*)x, xbs, ldx, (const unsigned char*)mask, mbs, out,
+                       rows, c, size, (unsigned)nb, rg);
+}
+
+}  // namespace
+
+}  // namespace clarus
+
+using namespace clarus;
+
+extern "C" int clarus_hip_block_means(const void* k, int32_t dtype, int64_t k_bstride, int64_t ldk, const void* mask, int64_t mask_bstride,
+                                      float* means, int64_t n, int64_t lk, int64_t c, int64_t block, void* stream) {
+  clear_error();
+  CLARUS_REQUIRE(k && means, "block_means: null operand");
+  CLARUS_REQUIRE(n > 0 && lk > 0 && c > 0 && block > 0, "block_means: empty problem");
+  CLARUS_REQUIRE(dtype == DT_BF16 || dtype == DT_F32, "block_means: bf16 or fp32");
+  CLARUS_REQUIRE(c % 8 == 0 && c < (1 << 20), "block_means: columns a multiple of 8, below 2^20");
+  const int64_t es = dtype == DT_BF16 ? 2 : 4;
+  CLARUS_REQUIRE(aligned(k, 16) && aligned(means, 16) && ldk * es % 16 == 0 && k_bstride * es % 16 == 0, "block_means: 16-byte aligned rows");
+  CLARUS_REQUIRE(ldk >= 0 && k_bstride >= 0 && mask_bstride >= 0, "block_means: strides");
+  CLARUS_REQUIRE(n < (1 << 23) && lk < ((int64_t)1 << 31) && block < ((int64_t)1 << 31) && n * cdiv(lk, block) < (1 << 23), "block_means: too large");
+  note_kernel("sp_means_kernel");
+  sp_means(k, dtype, k_bstride, ldk, mask, mask_bstride, means, n, lk, c, block, (hipStream_t)stream);
+  return check_launch("block_means");
+}
+
+extern "C" size_t clarus_hip_sparse_attention_workspace(int32_t dtype, int64_t n, int64_t lq, int64_t lk, int64_t heads, int64_t kv_heads, int64_t d, int64_t top,
+                                                        int64_t block, int64_t group, int32_t has_means, int32_t has_chosen) {
+  if (n <= 0 || lq <= 0 || lk <= 0 || kv_heads <= 0 || heads <= 0 || heads % kv_heads || d <= 0 || d > 128 || top <= 0 || block < 64 ||
+      block % 64 || block >= (1 << 20) || group <= 0 || !sp_fits(n, lq, lk, heads, kv_heads, block, std::min(group, lq)))
+    return 0;
+  return sp_plan(dtype, n, lq, lk, heads, kv_heads, d, std::min(top, lk), block, std::min(group, lq), has_means != 0, has_chosen != 0).total();
+}
+
+extern "C" int clarus_hip_sparse_attention(const ClarusSparseArgs* a, void* scratch, size_t scratch_bytes, void* stream) {
+  clear_error();
+  CLARUS_REQUIRE(a, "sparse_attention: null arguments");
+  CLARUS_REQUIRE(a->q && a->k && a->v && a->out, "sparse_attention: null operand");
+  CLARUS_REQUIRE(a->n > 0 && a->lq > 0 && a->lk > 0 && a->heads > 0 && a->kv_heads > 0, "sparse_attention: empty problem");
+  CLARUS_REQUIRE(a->heads % a->kv_heads == 0, "sparse_attention: heads a multiple of kv_heads");
+  CLARUS_REQUIRE(a->d >= 8 && a->d <= 128 && a->d % 8 == 0, "sparse_attention: head width a multiple of 8, at most 128");
+  CLARUS_REQUIRE(a->top > 0 && a->group > 0 && a->block >= 64 && a->block % 64 == 0 && a->block < (1 << 20),
+                 "sparse_attention: top and group positive, block a multiple of 64 below 2^20");
+  CLARUS_REQUIRE((a->dtype == DT_BF16 || a->dtype == DT_F32) && (a->o_dtype == DT_BF16 || a->o_dtype == DT_F32),
+                 "sparse_attention: bf16 or fp32");
+  CLARUS_REQUIRE(a->scale > 0.f && a->scale < 2e38f, "sparse_attention: scale positive and below 2e38");
+  const int64_t es = a->dtype == DT_BF16 ? 2 : 4;
+  CLARUS_REQUIRE(aligned(a->q, 16) && aligned(a->k, 16) && aligned(a->v, 16) && aligned(a->out, 16) && aligned(a->means, 16) &&
+                     aligned(a->chosen, 8) && a->ldq * es % 16 == 0 && a->ldk * es % 16 == 0 && a->ldv * es % 16 == 0 &&
+                     a->q_bstride * es % 16 == 0 && a->k_bstride * es % 16 == 0 && a->v_bstride * es % 16 == 0,
+                 "sparse_attention: 16-byte aligned rows");
+  CLARUS_REQUIRE(a->ldk < (1 << 24) && a->ldv < (1 << 24), "sparse_attention: rows of k and v less than 2^24 elements apart");
+  CLARUS_REQUIRE(a->ldq >= 0 && a->ldk >= 0 && a->ldv >= 0 && a->q_bstride >= 0 && a->k_bstride >= 0 && a->v_bstride >= 0 &&
+                     a->mask_bstride >= 0,
+                 "sparse_attention: strides");
+  const int64_t group = std::min(a->group, a->lq), top = std::min(a->top, a->lk);
+  CLARUS_REQUIRE(sp_fits(a->n, a->lq, a->lk, a->heads, a->kv_heads, a->block, group), "sparse_attention: too large");
+  const SpPlan g = sp_plan(a->dtype, a->n, a->lq, a->lk, a->heads, a->kv_heads, a->d, top, a->block, group, a->means != nullptr, a->chosen != nullptr);
+  CLARUS_REQUIRE(g.total() == 0 || (scratch && aligned(scratch, 16) && scratch_bytes >= g.total()),
+                 "sparse_attention: scratch %zu < %zu bytes", scratch_bytes, g.total());
+  char* at = (char*)scratch;
+  auto take = [&](size_t bytes) { char* r = at; at += bytes; return r; };
+  SparseP k{};
+  CrossP& x = k.x;
+  x.q = a->q; x.k = a->k; x.v = a->v; x.out = a->out; x.mask = (const unsigned char*)a->mask;
+  x.qbs = a->q_bstride; x.ldq = a->ldq; x.kbs = a->k_bstride; x.ldk = a->ldk; x.vbs = a->v_bstride; x.ldv = a->ldv; x.mbs = a->mask_bstride;
+  x.rep = (int)(a->heads / a->kv_heads); x.kv_heads = (int)a->kv_heads; x.d = (int)a->d; x.lq = (int)a->lq;
+  x.rows = a->lq * x.rep; x.lk = a->lk; x.nk = a->n * a->kv_heads; x.nblk = g.nblk; x.splits = g.splits;
+  x.o_dt = a->o_dtype; x.c = a->scale * 1.4426950408889634f;
+  k.nw = g.nw; k.nb = g.nb; k.groups = g.groups; k.block = (int)a->block; k.group = (int)group; k.top = (int)top; k.heads = (int)a->heads;
+  k.tpb = (int)(a->block / (a->dtype == DT_BF16 ? 64 : 32));
+  hipStream_t st = (hipStream_t)stream;
+  const int64_t c = a->heads * a->d, ck = a->kv_heads * a->d;
+  float* means = (float*)take(g.means);
+  if (!a->means) sp_means(a->k, a->dtype, a->k_bstride, a->ldk, a->mask, a->mask_bstride, means, a->n, a->lk, ck, a->block, st);
+  k.means = a->means ? a->means : means;
+  float* asks = (float*)take(g.asks);
+  if (group > 1) {
+    sp_means(a->q, a->dtype, a->q_bstride, a->ldq, nullptr, 0, asks, a->n, a->lq, c, group, st);
+    k.asks = asks; k.abs = g.groups * c; k.lda = c; k.ask_dt = DT_F32;
+  } else {
+    k.asks = a->q; k.abs = a->q_bstride; k.lda = a->ldq; k.ask_dt = a->dtype;
+  }
+  uint64_t* chosen = (uint64_t*)take(g.chosen);
+  k.chosen = a->chosen ? a->chosen : chosen;
+  k.score = (double*)take(g.score);
+  x.part = (float*)take(g.part);
+  const int64_t rows = a->n * a->heads * g.groups;
+  for (k.first = 0; k.first < rows; k.first += g.slab) {
+    k.slab = std::min(g.slab, rows - k.first);
+    hipLaunchKernelGGL(sp_score_kernel, dim3((unsigned)cdiv(k.slab, SP_TILE), (unsigned)cdiv(g.nb, SP_TILE)), dim3(SP_T), 0, st, k);
+    hipLaunchKernelGGL(sp_choose_kernel, dim3((unsigned)k.slab), dim3(SP_T), 0, st, k);
+  }
+  if (const int rc = check_launch("sparse_attention")) return rc;
+  note_kernel("sp_kernel d=%d waves=%d splits=%d", sp_pad(a->d), g.waves, g.splits);
+#define CLARUS_SP(DT)                                          \
+  do {                                                         \
+    if (a->d <= 32) sp_launch<DT, 32, 32>(k, g.waves, st);     \
+    else if (a->d <= 48) sp_launch<DT, 64, 48>(k, g.waves, st); \
+    else if (a->d <= 64) sp_launch<DT, 64, 64>(k, g.waves, st); \
+    else if (a->d <= 80) sp_launch<DT, 96, 80>(k, g.waves, st); \
+    else if (a->d <= 96) sp_launch<DT, 96, 96>(k, g.waves, st); \
+    else if (a->d <= 112) sp_launch<DT, 128, 112>(k, g.waves, st); \
+    else sp_launch<DT, 128, 128>(k, g.waves, st);              \
+  } while (0)
+  if (a->dtype == DT_BF16) CLARUS_SP(DT_BF16);
+  else CLARUS_SP(DT_F32);
+#undef CLARUS_SP
+  return check_launch("sparse_attention");
+}

@@ -1100,6 +1100,120 @@ class HipOps(Backend):
         return odt, args, self._workspace(self.lib.clarus_hip_cross_attention_workspace, args.dtype, n, lq, lk, heads, kv_heads,
                                           d, mode)
 
+    def block_means(self, k, block=64, mask=None):
+        """Means of the blocks of `block` consecutive keys of k [N, ..., C] that sparse_attention chooses by: fp32 [N, blocks,
+        C], of the keys that mask [N, Lk] keeps, NaN for a block that keeps none. Worth keeping while the keys stay."""
+        key = ("block_means", k.shape, k.stride(), k.dtype, block, None if mask is None else (mask.shape, mask.stride(), mask.dtype))
+        self._forward_only("block_means", k, mask)
+        if not isinstance(block, int):
+            raise Unsupported(f"block_means: block an integer, got {block!r}")
+        n, lk, c, kbs, ldk, mbs = self._plan(key, lambda: self._means_plan("block_means", k, block, mask))
+        out = torch.empty((n, -(-lk // block), c), device=k.device, dtype=torch.float32)
+        if out.numel() == 0:
+            return out
+        if k.data_ptr() % 16:
+            raise Unsupported("block_means: 16-byte aligned rows")
+        self._call("block_means", self.lib.clarus_hip_block_means, k.data_ptr(), _lib.dtype_code(k.dtype), kbs, ldk, _lib.ptr(mask), mbs,
+                   out.data_ptr(), n, lk, c, block)
+        return out
+
+    def _means_plan(self, what, k, block, mask):
+        if k.dim() < 2 or not _kdt(k) or k.shape[-1] % 8 or not 0 < k.shape[-1] < 1 << 20:
+            raise Unsupported(f"{what}: bf16 / fp32 k [N, ..., C], C a multiple of 8 below 2^20")
+        if block < 64 or block % 64 or block >= 1 << 20:
+            raise Unsupported(f"{what}: block a multiple of 64 below 2^20, got {block!r}")
+        n, c, lk = k.shape[0], k.shape[-1], math.prod(k.shape[1:-1])
+        if mask is not None:
+            if mask.dtype != torch.bool or tuple(mask.shape) != (n, lk):
+                raise Unsupported(f"{what}: mask bool [N, Lk]")
+            if mask.stride(-1) != 1 and lk > 1:
+                raise Unsupported(f"{what}: mask with unit key stride")
+        at, es = _rows(k), k.element_size()
+        if k.numel() and (at is None or any(s * es % 16 for s in at[1:])):
+            raise Unsupported(f"{what}: unit channel stride, one row stride, 16-byte aligned rows")
+        if lk >= 1 << 31 or n * -(-lk // block) >= 1 << 23:
+            raise Unsupported(f"{what}: fewer than 2^31 keys, fewer than 2^23 blocks in all images")
+        return n, lk, c, at[2] if at else 0, at[1] if at else 0, 0 if mask is None else mask.stride(0)
+
+    def sparse_attention(self, q, k, v, heads, top, kv_heads=None, block=64, group=1, mask=None, means=None, scale=None, out_dtype=None,
+                         return_blocks=False):
+        """cross_attention over the blocks of keys that a cheap score selects (self-attention of a large map, or a few
+        tokens over a long context). The keys of k and v [N, ..., kv_heads * d] fall into blocks of `block` consecutive ones, the
+        queries q [N, ..., heads * d] into groups of `group`. A head's group attends the kept keys of the `top` blocks whose
+        mean key has the largest product with the group's mean query (means rounded to fp32, products in 64 bits; of equal
+        ones the lowest index). mask: bool [N, Lk], a masked key counts for nothing whatever k and v hold; a block
+        without a kept key is not chosen. means: block_means(k, block, mask), kept while the keys stay (None: made in the
+        call). 0 for a query without a block. Returns a contiguous tensor of q's shape; with return_blocks also the choice,
+        bool [N, heads, groups, blocks]."""
+        kv_heads = heads if kv_heads is None else kv_heads
+        if not all(isinstance(i, int) for i in (heads, kv_heads, top, block, group)):  # before the plans, whose keys 4.0 and 4 share
+            raise Unsupported("sparse_attention: heads, kv_heads, top, block and group integers, got "
+                              f"{heads!r} {kv_heads!r} {top!r} {block!r} {group!r}")
+        scale, return_blocks = None if scale is None else float(scale), bool(return_blocks)
+        key = ("sparse_attention", q.shape, q.stride(), k.shape, k.stride(), v.shape, v.stride(), q.dtype, k.dtype, v.dtype, heads,
+               kv_heads, top, block, group, scale, out_dtype, return_blocks,
+               *(None if t is None else (t.shape, t.stride(), t.dtype) for t in (mask, means)))
+        self._forward_only("sparse_attention", q, k, v, mask, means)
+        odt, args, need, shape = self._plan(key, lambda: self._sparse_plan(q, k, v, heads, top, kv_heads, block, group, mask, means, scale,
+                                                                           out_dtype or self.dtype, return_blocks))
+        out = torch.empty_like(q, dtype=odt, memory_format=torch.contiguous_format)
+        if args is None:  # nothing asked, or nothing to attend
+            out.zero_()
+            return (out, torch.zeros(shape, device=q.device, dtype=torch.bool)) if return_blocks else out
+        qp, kp, vp, mp = q.data_ptr(), k.data_ptr(), v.data_ptr(), _lib.ptr(means)
+        if (qp | kp | vp | (mp or 0)) % 16:
+            raise Unsupported("sparse_attention: 16-byte aligned rows")
+        words = torch.empty((*shape[:3], -(-shape[3] // 64)), device=q.device, dtype=torch.int64) if return_blocks else None
+        args = _lib.SparseArgs.from_buffer_copy(args)
+        args.q, args.k, args.v, args.out, args.mask, args.means, args.chosen = qp, kp, vp, out.data_ptr(), _lib.ptr(mask), mp, _lib.ptr(words)
+        scratch = torch.empty(need, device=q.device, dtype=torch.uint8) if need else None
+        self._call("sparse_attention", self.lib.clarus_hip_sparse_attention, ctypes.byref(args), _lib.ptr(scratch), need)
+        if not return_blocks:
+            return out
+        bits = words[..., None] >> torch.arange(64, device=q.device) & 1
+        return out, bits.flatten(-2)[..., :shape[3]].bool()
+
+    def _sparse_plan(self, q, k, v, heads, top, kv_heads, block, group, mask, means, scale, odt, return_blocks):
+        if q.dim() < 2 or k.dim() < 2 or v.dim() < 2:
+            raise Unsupported("sparse_attention: q, k, v [N, ..., C]")
+        n, c, ck = q.shape[0], q.shape[-1], k.shape[-1]
+        if not (heads > 0 and kv_heads > 0 and heads % kv_heads == 0 and c % heads == 0 and k.shape == v.shape and k.shape[0] == n
+                and ck * heads == c * kv_heads):
+            raise Unsupported("sparse_attention: q [N, ..., heads d], k and v [N, ..., kv_heads d] of one shape, "
+                              "heads a multiple of kv_heads")
+        d = c // heads
+        lq, lk = math.prod(q.shape[1:-1]), math.prod(k.shape[1:-1])
+        if scale is None and d:
+            scale = d ** -0.5
+        held, limit = (ctypes.c_float(s or 0.0).value for s in (scale, 2e38))  # as the call passes them on
+        if not (_kdt(q) and q.dtype == k.dtype == v.dtype and odt in _KDT and 8 <= d <= 128 and d % 8 == 0
+                and 0.0 < held < limit):
+            raise Unsupported("sparse_attention: bf16 / fp32 q, k, v of one type, head width a multiple of 8 up to 128, "
+                              "scale positive and below 2e38 (as fp32)")
+        if top < 1 or group < 1:
+            raise Unsupported(f"sparse_attention: top and group positive, got {top!r} {group!r}")
+        _, _, _, kbs, ldk, mbs = self._means_plan("sparse_attention", k, block, mask)
+        blocks, groups = -(-lk // block), -(-lq // min(group, max(lq, 1)))
+        if means is not None and not (tuple(means.shape) == (n, blocks, ck) and means.dtype == torch.float32 and means.is_contiguous()):
+            raise Unsupported("sparse_attention: means [N, blocks, kv_heads d], fp32, contiguous, as block_means makes them")
+        shape = (n, heads, groups, blocks)
+        if q.numel() == 0 or lk == 0:
+            return odt, None, 0, shape
+        qa, va, es = _rows(q), _rows(v), q.element_size()
+        if None in (qa, va) or any(s * es % 16 for t in (qa, va) for s in t[1:]) or max(ldk, va[1]) >= 1 << 24:
+            raise Unsupported("sparse_attention: unit channel stride, one row stride (k and v: below 2^24), 16-byte aligned rows")
+        rows = -(-lq * (heads // kv_heads) // 128) * 128  # of an (image, kv head) pair, in whole workgroups
+        if (n * kv_heads * rows >= (1 << 31) - 4096 or n * kv_heads >= 65536 or heads >= 65536 or blocks >= 1 << 21
+                or (min(group, lq) > 1 and n * groups >= 1 << 23) or n * heads * groups >= 1 << 31):
+            raise Unsupported("sparse_attention: fewer than 2^31 - 4096 rows (n * heads * lq, those of an (image, kv head) pair rounded "
+                              "up to 128), 65536 such pairs, 2^21 blocks of an image, 2^23 groups of several queries, 2^31 choices")
+        args = _lib.SparseArgs(
+            n=n, lq=lq, lk=lk, heads=heads, kv_heads=kv_heads, d=d, top=min(top, lk), block=block, group=min(group, lq), q_bstride=qa[2],
+            ldq=qa[1], k_bstride=kbs, ldk=ldk, v_bstride=va[2], ldv=va[1], mask_bstride=mbs, dtype=_lib.dtype_code(q.dtype),
+            o_dtype=_lib.dtype_code(odt), scale=scale)
+        return odt, args, self._workspace(self.lib.clarus_hip_sparse_attention_workspace, args.dtype, n, lq, lk, heads, kv_heads, d, args.top,
+                                          block, args.group, int(means is not None), int(return_blocks)), shape
+
     def linear_attention(self, q, k, v, log_decay, heads, kv_heads=None, state=None, scale=None, state_out=None, out_dtype=None):
         """Causal linear attention with a decay for each head over tokens in order (rasters, frames): per image and kv
         head S_t = exp(log_decay) S_{t-1} + k_t v_t^T, out_t = scale q_t^T S_t for the heads that share it. q [N, ...,

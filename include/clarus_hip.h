@@ -606,6 +606,48 @@ size_t clarus_hip_linear_attention_workspace(int32_t dtype, int64_t n, int64_t l
                                              int64_t dv);
 int clarus_hip_linear_attention(const ClarusLinearArgs* args, void* scratch, size_t scratch_bytes, void* stream);
 
+/*
+ * Means of blocks of `block` consecutive rows (the last one may be shorter): means [n, ceil(lk / block), c] fp32
+ * contiguous, of the rows that mask keeps (bytes at mask + n * mask_bstride + row, any value but 0; NULL: all), summed and
+ * divided in 64 bits; NaN for a block that keeps none. k rows at k + n * k_bstride + row * ldk (bf16 or fp32, 16-byte aligned);
+ * c a multiple of 8 below 2^20, n * blocks < 2^23. No counterpart in the reference.
+ */
+int clarus_hip_block_means(const void* k, int32_t dtype, int64_t k_bstride, int64_t ldk, const void* mask, int64_t mask_bstride, float* means,
+                           int64_t n, int64_t lk, int64_t c, int64_t block, void* stream);
+
+/*
+ * Attention over the blocks of keys that a score selects. The keys of an image fall into blocks of `block`, its queries into
+ * groups of `group` consecutive ones (the last of each may be shorter). For head h of group g, the `top` blocks of the
+ * largest (mean of the group's queries) . (mean of the block's kept keys) are chosen, means as clarus_hip_block_means
+ * makes them (a group of one: the query itself) and the product in 64 bits, of equal ones the lowest index; a block whose score is NaN
+ * or -inf (one that keeps no key) never is. Then
+ *   out[n, i, h] = sum_j p_j v[n, j, g'],  p = softmax_j(scale q[n, i, h] . k[n, j, g']),  g' = h / (heads / kv_heads)
+ * over the kept keys j of the blocks chosen for i's group; 0 where there are none. q, k, v, out, scale, types, sizes and
+ * arithmetic as clarus_hip_cross_attention's; mask NULL or bytes at mask + n * mask_bstride + j (0 masked: such a key
+ * counts for nothing, whatever k and v hold). means: those of k's blocks, kept by the caller while the keys stay, or NULL.
+ * chosen: NULL or [n, heads, groups, ceil(blocks / 64)] words that receive the choice, block b in bit b % 64 of word b / 64.
+ * block a multiple of 64 below 2^20, n * blocks < 2^23 and fewer than 2^21 blocks, n * groups < 2^23 where group > 1,
+ * n * heads * groups < 2^31. scratch holds clarus_hip_sparse_attention_workspace(...) bytes, 16-byte aligned.
+ * Deterministic. No counterpart in the reference.
+ */
+typedef struct ClarusSparseArgs {
+  const void* q;
+  const void* k;
+  const void* v;
+  void* out;
+  const void* mask;
+  const float* means;
+  uint64_t* chosen;
+  int64_t n, lq, lk, heads, kv_heads, d, top, block, group;
+  int64_t q_bstride, ldq, k_bstride, ldk, v_bstride, ldv, mask_bstride;
+  int32_t dtype, o_dtype;
+  float scale;
+} ClarusSparseArgs;
+
+size_t clarus_hip_sparse_attention_workspace(int32_t dtype, int64_t n, int64_t lq, int64_t lk, int64_t heads, int64_t kv_heads, int64_t d,
+                                             int64_t top, int64_t block, int64_t group, int32_t has_means, int32_t has_chosen);
+int clarus_hip_sparse_attention(const ClarusSparseArgs* args, void* scratch, size_t scratch_bytes, void* stream);
+
 /* ABI version (CLARUS_HIP_ABI_VERSION) and struct sizes, for binding checks. */
 int clarus_hip_abi_version(void);
 size_t clarus_hip_sizeof_gemm_args(void);
@@ -614,6 +656,7 @@ size_t clarus_hip_sizeof_cross_args(void);
 size_t clarus_hip_sizeof_rotary_args(void);
 size_t clarus_hip_sizeof_add_norm_args(void);
 size_t clarus_hip_sizeof_linear_args(void);
+size_t clarus_hip_sizeof_sparse_args(void);
 
 /* Text of the calling thread's last failure ("" if none). */
 const char* clarus_hip_last_error(void);

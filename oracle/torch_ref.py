@@ -207,6 +207,39 @@ class TorchRef:
         h = norm(r, ln, weight, bias).reshape(x.shape).to(self._odt(out_dtype)) if ln else None
         return r.reshape(x.shape).to(x.dtype), h
 
+    def block_means(self, k, block=64, mask=None):
+        """No reference op: means of the kept rows of each block, in 64 bits, as fp32."""
+        k = k.reshape(k.shape[0], -1, k.shape[-1]).double()
+        keep = torch.ones(k.shape[:2], dtype=torch.bool, device=k.device) if mask is None else mask
+        k = k.masked_fill(~keep[..., None], 0)
+        return torch.stack([a.sum(1) / b.sum(1, keepdim=True) for a, b in zip(k.split(block, 1), keep.split(block, 1))], 1).float()
+
+    def sparse_attention(self, q, k, v, heads, top, kv_heads=None, block=64, group=1, mask=None, means=None, scale=None, out_dtype=None,
+                         return_blocks=False):
+        """No reference op: cross_attention under a mask that keeps, for each head and group of queries, the blocks of keys
+        of the `top` largest products of means."""
+        kv_heads = kv_heads or heads
+        n, d, rep = q.shape[0], q.shape[-1] // heads, heads // kv_heads
+        q3, k3, v3 = (t.reshape(n, -1, t.shape[-1]) for t in (q, k, v))
+        lq, lk = q3.shape[1], k3.shape[1]
+        m = (self.block_means(k3, block, mask) if means is None else means).double()
+        a = torch.stack([t.double().mean(1) for t in q3.split(group, 1)], 1).float().double() if group > 1 else q3.double()
+        kept = torch.ones(n, lk, dtype=torch.bool, device=q.device) if mask is None else mask
+        out, chosen = torch.zeros(n, lq, heads * d, device=q.device), []
+        for h in range(heads):
+            sl, kv = slice(h * d, h * d + d), slice(h // rep * d, h // rep * d + d)
+            score = a[..., sl] @ m[..., kv].transpose(1, 2).contiguous()
+            score = score.nan_to_num(nan=-float("inf"), posinf=float("inf"), neginf=-float("inf"))
+            order = score.sort(dim=-1, descending=True, stable=True)[1][..., :top]
+            pick = torch.zeros_like(score, dtype=torch.bool).scatter_(-1, order, True) & (score > -float("inf"))
+            chosen.append(pick)
+            see = pick.repeat_interleave(group, 1)[:, :lq].repeat_interleave(block, 2)[..., :lk] & kept[:, None]
+            out[..., sl] = self.cross_attention(q3[..., sl], k3[..., kv].masked_fill(~kept[..., None], 0),
+                                                v3[..., kv].masked_fill(~kept[..., None], 0), 1, mask=see,
+                                                scale=d ** -0.5 if scale is None else scale, out_dtype=torch.float32)
+        out = out.reshape(q.shape).to(self._odt(out_dtype))
+        return (out, torch.stack(chosen, 1)) if return_blocks else out
+
     def linear_attention(self, q, k, v, log_decay, heads, kv_heads=None, state=None, scale=None, state_out=None, out_dtype=None):
         """No reference op: S <- e^g S + k v^T, out = scale q^T S, token after token."""
         kv_heads = kv_heads or heads
