@@ -4,8 +4,9 @@
 //   o_i = softmax_j(scale q_i . k_j) v_j  over the kept keys j of the blocks chosen by i's group; 0 where there are none.
 //
 //   sp_means_kernel   the means of blocks of keys, or of groups of queries
-//   sp_score_kernel   scores of a slab of rows (image, head, group), 64 bits
-//   sp_choose_kernel  a row's choice as bits, 64 blocks a word
+//   sp_pick_kernel    up to 1024 blocks: scores and choice, as bits, 64 blocks a word
+//   sp_score_kernel   more blocks: scores of a slab of rows (image, head, group), 64 bits
+//   sp_choose_kernel  a row's choice from them
 //   sp_kernel         the attention: 32 rows per wave as in cross_attention.hip (a row is a query and one of the heads that
 //                     share a kv head); a workgroup takes the blocks that any of its rows has chosen, one after another
 //                     through LDS, and a wave those of its own rows, the bits of each row masking what the others chose
@@ -177,6 +178,272 @@ __global__ void __launch_bounds__(SP_T) sp_choose_kernel(const SparseP p) {
   }
 }
 
+// ---------------------------------------------------------------- scores and choice in one
+// A workgroup: W waves, 32 rows (groups and the heads that share a kv head) of one (image, kv head). A wave holds the scores of
+// NT tiles of 32 blocks in registers, from fp32 MFMAs (S^T = means asks^T: a lane holds a row's scores of 16 blocks of
+// each tile, its partner in lane ^ 32 the other 16). They are off by at most e = 2 (d + 8) 2^-24 |ask| |mean| (Cauchy-Schwarz over
+// the terms). A row's threshold is searched between its least and largest score, by counts; where the least score
+// chosen and the largest left out are more than 2 e apart, 64 bits would choose the same. Where they are not, the blocks
+// within 2 e of the threshold are scored again in 64 bits by a wave, up to 64 of them; a row with more of them (equal blocks,
+// an ask of zeros), or with a norm that is not finite, is done by the whole workgroup, every block's rank counted.
+constexpr int SP_PICK = 1024;  // blocks, at most
+
+template <int D, int NT, int W>
+__global__ void __launch_bounds__(64 * W, W > 8 ? 4 : 2) sp_pick_kernel(const SparseP p, unsigned row_tiles) {
+  constexpr int QN = D / 8;
+  __shared__ float xf[3][W][32];  // exchanged by the waves: per row
+  __shared__ int xi[W][32];
+  __shared__ float wide[W];
+  __shared__ unsigned redo[2];    // rows to do again: a few blocks, all of them
+  __shared__ unsigned words[32][NT * W], cands[32][NT * W];
+  __shared__ double ask64[D];
+  __shared__ uint64_t keys[32 * NT * W];
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), col = lane & 31, hl = lane >> 5;
+  const unsigned nk = blockIdx.x / row_tiles, tile = blockIdx.x - nk * row_tiles;
+  const int64_t n = nk / p.x.kv_heads, kvh = nk - n * p.x.kv_heads, rows = p.groups * p.x.rep;
+  const int d = p.x.d;
+  const int64_t row = (int64_t)tile * 32 + col;
+  const bool there = row < rows;
+  const int64_t g = (there ? row : rows - 1) / p.x.rep, head = kvh * p.x.rep + (there ? row : rows - 1) - g * p.x.rep;
+  const int64_t ask = n * p.abs + g * p.lda + head * d, mld = (int64_t)p.x.kv_heads * d;
+  const float* mp = p.means + (n * p.nb * p.x.kv_heads + kvh) * d;
+  const int nb = (int)p.nb;
+
+  f32x4 q[QN];
+  float qq = 0.f;
+#pragma unroll
+  for (int i = 0; i < QN; ++i) {
+    const int c = 8 * i + 4 * hl;
+    q[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+    if (8 * i < d) {
+      if (p.ask_dt == DT_BF16) {
+        const u32x2 w = *reinterpret_cast<const u32x2*>((const unsigned short*)p.asks + ask + c);
+#pragma unroll
+        for (int e = 0; e < 2; ++e) q[i][2 * e] = __uint_as_float(w[e] << 16), q[i][2 * e + 1] = __uint_as_float(w[e] & 0xffff0000u);
+      } else {
+        q[i] = *reinterpret_cast<const f32x4*>((const float*)p.asks + ask + c);
+      }
+    }
+#pragma unroll
+    for (int e = 0; e < 4; ++e) qq = fmaf(q[i][e], q[i][e], qq);
+  }
+  qq = sum32(qq);
+
+  f32x16 s[NT];
+  float mm = 0.f, least = INFINITY, most = -INFINITY;
+  int valid = 0;
+#pragma unroll
+  for (int t = 0; t < NT; ++t) {
+    const int b0 = 32 * (t * W + wave), b = b0 + col;
+#pragma unroll
+    for (int j = 0; j < 16; ++j) s[t][j] = 0.f;
+    if (b0 >= nb) {
+#pragma unroll
+      for (int j = 0; j < 16; ++j) s[t][j] = -INFINITY;
+      continue;
+    }
+    const float* m = mp + (b < nb ? b : 0) * mld + 4 * hl;
+    float norm = 0.f;
+#pragma unroll
+    for (int i = 0; i < QN; ++i)
+      if (8 * i < d) {
+        const f32x4 a = *reinterpret_cast<const f32x4*>(m + 8 * i);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          norm = fmaf(a[e], a[e], norm);
+          s[t] = __builtin_amdgcn_mfma_f32_32x32x2f32(a[e], q[i][e], s[t], 0, 0, 0);
+        }
+      }
+    norm = sum32(norm);
+    const bool ok = b < nb && norm == norm;  // a mean of NaN has no score, whatever the row asks
+    if (ok) mm = fmaxf(mm, norm);
+    const unsigned keep = (unsigned)__ballot(ok) >> (4 * hl);
+#pragma unroll
+    for (int j = 0; j < 16; ++j) {
+      const int at = 8 * (j >> 2) + (j & 3);
+      s[t][j] = keep_bit(s[t][j], keep, at);
+      most = fmaxf(most, s[t][j]);
+      least = fminf(least, keep >> at & 1 ? s[t][j] : INFINITY);
+    }
+    valid += __popc((unsigned)__ballot(ok));
+  }
+  // over the row's lanes and waves
+  auto all_max = [&](float v, int slot) __attribute__((always_inline)) {
+    v = max32(v);
+    if constexpr (W > 1) {
+      if (hl == 0) xf[slot][wave][col] = v;
+      __syncthreads();
+#pragma unroll
+      for (int w = 0; w < W; ++w) v = fmaxf(v, xf[slot][w][col]);
+    }
+    return v;
+  };
+  auto all_sum = [&](int v) __attribute__((always_inline)) {  // v of this lane's half of the blocks
+    unsigned a = (unsigned)v, b = a;
+    swap32(a, b);
+    v = (int)(a + b);
+    if constexpr (W > 1) {
+      __syncthreads();  // the counts before have been read
+      if (hl == 0) xi[wave][col] = v;
+      __syncthreads();
+      v = 0;
+#pragma unroll
+      for (int w = 0; w < W; ++w) v += xi[w][col];
+    }
+    return v;
+  };
+  auto count = [&](float t) __attribute__((always_inline)) {
+    int c = 0;
+#pragma unroll
+    for (int i = 0; i < NT; ++i)
+#pragma unroll
+      for (int j = 0; j < 16; ++j) c += s[i][j] >= t;
+    return all_sum(c);
+  };
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) mm = fmaxf(mm, __shfl_xor(mm, o, 64));  // a wave's blocks lie over its lanes
+  if (W > 1 && lane == 0) wide[wave] = mm;
+  most = all_max(most, 0);
+  least = -all_max(-least, 1);
+  if constexpr (W > 1) {  // all_max's barriers lie behind
+    mm = wide[0];
+#pragma unroll
+    for (int w = 1; w < W; ++w) mm = fmaxf(mm, wide[w]);
+  }
+  valid = all_sum(hl == 0 ? valid : 0);
+  const float e = 2.f * (float)(d + 8) * 0x1p-24f * 1.01f * sqrtf(qq) * sqrtf(mm) + 1e-35f;
+  const bool wild = !(qq < INFINITY && mm < INFINITY);  // products may leave fp32
+  bool done = wild || valid <= p.top, exact = false;
+  float thr = -3.402823466e38f;  // every block with a score
+  // more than `top` scores from lo on, fewer from hi on: between them as far as the counts' logarithms say (the tail of
+  // a bell falls about so), halfway every third time
+  float lo = least, hi = most + fabsf(most) * 0x1p-20f + e, clo = (float)valid, chi = 0.5f;
+  const float want = (float)p.top;
+#pragma unroll 1
+  for (int i = 0; i < 48 && !__all(done); ++i) {
+    const float w = i % 3 == 2 ? 0.5f : __builtin_amdgcn_logf(clo / want) / __builtin_amdgcn_logf(clo / chi);
+    const float mid = lo + (hi - lo) * fminf(fmaxf(w, 0.03f), 0.97f);
+    const int c = count(mid);
+    if (!done) {
+      if (c == p.top) thr = mid, done = exact = true;
+      else if (c > p.top) lo = mid, clo = (float)c;
+      else hi = mid, chi = fmaxf((float)c, 0.5f);
+      if (!(hi - lo > e)) done = true;
+    }
+  }
+  float in = INFINITY, out = -INFINITY;
+#pragma unroll
+  for (int t = 0; t < NT; ++t)
+#pragma unroll
+    for (int j = 0; j < 16; ++j) {
+      const bool sel = s[t][j] >= thr;
+      in = fminf(in, sel ? s[t][j] : INFINITY);
+      out = fmaxf(out, sel ? -INFINITY : s[t][j]);
+    }
+  in = -all_max(-in, 2);
+  out = all_max(out, 0);
+  const bool near = there && (wild || (valid > p.top && !(exact && in - out > 2.f * e)));
+  unsigned* to = reinterpret_cast<unsigned*>(p.chosen + ((n * p.heads + head) * p.groups + g) * p.nw);
+#pragma unroll
+  for (int t = 0; t < NT; ++t) {
+    unsigned w = 0;
+#pragma unroll
+    for (int j = 0; j < 16; ++j) w |= (unsigned)(s[t][j] >= thr) << (8 * (j >> 2) + (j & 3));
+    w <<= 4 * hl;
+    unsigned other = w;
+    swap32(w, other);
+    if (hl == 0 && there && !near && t * W + wave < 2 * p.nw) to[t * W + wave] = w | other;
+  }
+  if (!__any(near)) return;  // the same in every wave
+  // the top-th largest score lies within [lo, hi]: what is more than 2 e above is chosen, what is more than 2 e below is not,
+  // and 64 bits decide between them
+  if (exact) lo = hi = in;
+  const float sure = hi + 2.f * e, maybe = lo - 2.f * e;
+#pragma unroll
+  for (int t = 0; t < NT; ++t) {
+    unsigned w = 0, c = 0;
+#pragma unroll
+    for (int j = 0; j < 16; ++j) {
+      w |= (unsigned)(s[t][j] > sure) << (8 * (j >> 2) + (j & 3));
+      c |= (unsigned)(s[t][j] >= maybe && s[t][j] <= sure) << (8 * (j >> 2) + (j & 3));
+    }
+    w <<= 4 * hl, c <<= 4 * hl;
+    unsigned w2 = w, c2 = c;
+    swap32(w, w2);
+    swap32(c, c2);
+    if (hl == 0) words[col][t * W + wave] = w | w2, cands[col][t * W + wave] = c | c2;
+  }
+  if (wave == 0) {
+    const unsigned few = (unsigned)__ballot(near && !wild), whole = (unsigned)__ballot(near && wild);
+    if (lane == 0) redo[0] = few, redo[1] = whole;
+  }
+  __syncthreads();
+  int turn = 0;
+  for (unsigned left = __builtin_amdgcn_readfirstlane(redo[0]); left; left &= left - 1) {
+    if (turn++ % W != wave) continue;
+    const int at = __builtin_ctz(left);
+    const int64_t r = (int64_t)tile * 32 + at, rg = r / p.x.rep, rh = kvh * p.x.rep + r - rg * p.x.rep;
+    const int64_t from = n * p.abs + rg * p.lda + rh * d;
+    double a[(D + 63) / 64];
+#pragma unroll
+    for (int i = 0; i < (D + 63) / 64; ++i) a[i] = lane + 64 * i < d ? load1(p.asks, p.ask_dt, from + lane + 64 * i) : 0.f;
+    int some = 0, taken = 0, mine = 0;  // candidates, chosen already, the lane's candidate
+    for (int t = 0; t < NT * W; ++t) {
+      taken += __popc(words[at][t]);
+      for (unsigned c = __builtin_amdgcn_readfirstlane(cands[at][t]); c; c &= c - 1) {
+        if (lane == some) mine = 32 * t + __builtin_ctz(c);
+        ++some;
+      }
+    }
+    if (some > 64) {
+      if (lane == 0) atomicOr(&redo[1], 1u << at);
+      continue;
+    }
+    uint64_t key = 0;
+#pragma unroll 4
+    for (int i = 0; i < some; ++i) {
+      const float* m = mp + __builtin_amdgcn_readlane(mine, i) * mld;
+      double v = 0.0;
+#pragma unroll
+      for (int k = 0; k < (D + 63) / 64; ++k)
+        if (lane + 64 * k < d) v = fma(a[k], (double)m[lane + 64 * k], v);
+#pragma unroll
+      for (int o = 32; o; o >>= 1) v += __shfl_xor(v, o, 64);
+      if (lane == i) key = sp_key(v);
+    }
+    int rank = 0;
+    for (int i = 0; i < some; ++i) {
+      const uint64_t k = (uint64_t)__builtin_amdgcn_readlane((unsigned)(key >> 32), i) << 32 | (unsigned)__builtin_amdgcn_readlane((unsigned)key, i);
+      rank += k > key || (k == key && i < lane);
+    }
+    if (key != 0 && rank < p.top - taken) atomicOr(&words[at][mine >> 5], 1u << (mine & 31));
+    __builtin_amdgcn_s_waitcnt(0xc07f);  // lgkmcnt(0): the wave's own LDS operations, in order
+    unsigned* rto = reinterpret_cast<unsigned*>(p.chosen + ((n * p.heads + rh) * p.groups + rg) * p.nw);
+    for (int t = lane; t < 2 * p.nw; t += 64) rto[t] = words[at][t];
+  }
+  __syncthreads();
+  for (unsigned left = __builtin_amdgcn_readfirstlane(redo[1]); left; left &= left - 1) {
+    const int64_t r = (int64_t)tile * 32 + __builtin_ctz(left), rg = r / p.x.rep, rh = kvh * p.x.rep + r - rg * p.x.rep;
+    for (int c = tid; c < d; c += 64 * W) ask64[c] = load1(p.asks, p.ask_dt, n * p.abs + rg * p.lda + rh * d + c);
+    __syncthreads();
+    for (int b = tid; b < nb; b += 64 * W) {
+      double v = 0.0;
+      for (int c = 0; c < d; ++c) v = fma(ask64[c], (double)mp[b * mld + c], v);
+      keys[b] = sp_key(v);
+    }
+    __syncthreads();
+    for (int b0 = 64 * wave; b0 < nb; b0 += 64 * W) {
+      const int b = b0 + lane;
+      const uint64_t k = b < nb ? keys[b] : 0;
+      int rank = 0;
+      for (int i = 0; i < nb; ++i) rank += keys[i] > k || (keys[i] == k && i < b);
+      const uint64_t word = __ballot(k != 0 && rank < p.top);
+      if (lane == 0) p.chosen[((n * p.heads + rh) * p.groups + rg) * p.nw + b0 / 64] = word;
+    }
+    __syncthreads();
+  }
+}
+
 // ---------------------------------------------------------------- attention
 __device__ __forceinline__ uint64_t or32(uint64_t v) {  // over the 32 lanes of a half
 #pragma unroll
@@ -322,6 +589,7 @@ int sp_pad(int64_t d) { return d <= 32 ? 32 : d <= 64 ? 64 : d <= 96 ? 96 : 128;
 struct SpPlan {
   int64_t nb, nw, groups, nblk, slab;  // slab: rows of scores at a time
   int splits, waves;
+  int pick_tiles, pick_waves;  // of 32 blocks per wave of sp_pick_kernel; 0: sp_score_kernel and sp_choose_kernel
   size_t means, asks, chosen, score, part;  // workspace bytes, each a multiple of 16
   size_t total() const { return means + asks + chosen + score + part; }
 };
@@ -336,8 +604,17 @@ SpPlan sp_plan(int32_t dt, int64_t n, int64_t lq, int64_t lk, int64_t heads, int
   if (!has_means) g.means = (size_t)(n * g.nb * kv_heads * d) * sizeof(float);
   if (group > 1) g.asks = (size_t)(n * g.groups * heads * d) * sizeof(float);
   if (!has_chosen) g.chosen = (size_t)cdiv(asks * g.nw, 2) * 16;
-  g.slab = std::min(asks, std::min<int64_t>(cdiv(SP_SLAB / 8, g.nb * SP_TILE), 1 << 16) * SP_TILE);
-  g.score = (size_t)cdiv(g.slab * g.nb, 2) * 16;
+  if (g.nb <= SP_PICK) {
+    // few rows: two tiles per wave and more waves
+    const int64_t tiles = 2 * g.nw, wgs = nk * cdiv(g.groups * (heads / kv_heads), 32);
+    const int most = wgs < 2 * device_cus() ? 2 : d <= 64 ? 8 : 4;
+    g.pick_tiles = tiles <= 2 ? 2 : most;
+    g.pick_waves = 1;
+    while (g.pick_tiles * g.pick_waves < tiles) g.pick_waves *= 2;
+  } else {
+    g.slab = std::min(asks, std::min<int64_t>(cdiv(SP_SLAB / 8, g.nb * SP_TILE), 1 << 16) * SP_TILE);
+    g.score = (size_t)cdiv(g.slab * g.nb, 2) * 16;
+  }
   g.waves = rows <= 32 ? 1 : 4;
   g.nblk = cdiv(rows, 32 * g.waves);
   const int64_t blocks = g.nblk * nk, cus = device_cus();
@@ -354,7 +631,31 @@ bool sp_fits(int64_t n, int64_t lq, int64_t lk, int64_t heads, int64_t kv_heads,
         n * heads < big && n * kv_heads * (cdiv(lq * (heads / kv_heads), 128) * 128) < big - 4096))
     return false;
   const int64_t nb = cdiv(lk, block), groups = cdiv(lq, group);
-  return nb < (1 << 21) && n * nb < (1 << 23) && (group == 1 || n * groups < (1 << 23)) && n * heads * groups < big;
+  return nb < (1 << 21) && n * nb < (1 << 23) && (group == 1 || n * groups < (1 << 23)) && n * heads * groups < (1 << 26);
+}
+
+template <int D>
+void sp_pick(const SparseP& k, const SpPlan& g, hipStream_t st) {
+  const unsigned tiles = (unsigned)cdiv(k.groups * k.x.rep, 32);
+  const dim3 grid((unsigned)k.x.nk * tiles), block(64 * g.pick_waves);
+#define CLARUS_PICK(NT, W) \
+  if (g.pick_tiles == NT && g.pick_waves == W) hipLaunchKernelGGL((sp_pick_kernel<D, NT, W>), grid, block, 0, st, k, tiles)
+  CLARUS_PICK(2, 1);
+  CLARUS_PICK(2, 2);
+  CLARUS_PICK(2, 4);
+  CLARUS_PICK(2, 8);
+  CLARUS_PICK(2, 16);
+  if constexpr (D <= 64) {
+    CLARUS_PICK(8, 1);
+    CLARUS_PICK(8, 2);
+    CLARUS_PICK(8, 4);
+  } else {
+    CLARUS_PICK(4, 1);
+    CLARUS_PICK(4, 2);
+    CLARUS_PICK(4, 4);
+    CLARUS_PICK(4, 8);
+  }
+#undef CLARUS_PICK
 }
 
 template <int DT, int D, int C, int MASK>
@@ -474,7 +775,11 @@ extern "C" int clarus_hip_sparse_attention(const ClarusSparseArgs* a, void* scra
   k.score = (double*)take(g.score);
   x.part = (float*)take(g.part);
   const int64_t rows = a->n * a->heads * g.groups;
-  for (k.first = 0; k.first < rows; k.first += g.slab) {
+  if (g.pick_tiles) {
+    if (a->d <= 64) sp_pick<64>(k, g, st);
+    else sp_pick<128>(k, g, st);
+  }
+  for (k.first = 0; !g.pick_tiles && k.first < rows; k.first += g.slab) {
     k.slab = std::min(g.slab, rows - k.first);
     hipLaunchKernelGGL(sp_score_kernel, dim3((unsigned)cdiv(k.slab, SP_TILE), (unsigned)cdiv(g.nb, SP_TILE)), dim3(SP_T), 0, st, k);
     hipLaunchKernelGGL(sp_choose_kernel, dim3((unsigned)k.slab), dim3(SP_T), 0, st, k);

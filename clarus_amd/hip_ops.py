@@ -1204,9 +1204,9 @@ class HipOps(Backend):
             raise Unsupported("sparse_attention: unit channel stride, one row stride (k and v: below 2^24), 16-byte aligned rows")
         rows = -(-lq * (heads // kv_heads) // 128) * 128  # of an (image, kv head) pair, in whole workgroups
         if (n * kv_heads * rows >= (1 << 31) - 4096 or n * kv_heads >= 65536 or heads >= 65536 or blocks >= 1 << 21
-                or (min(group, lq) > 1 and n * groups >= 1 << 23) or n * heads * groups >= 1 << 31):
+                or (min(group, lq) > 1 and n * groups >= 1 << 23) or n * heads * groups >= 1 << 26):
             raise Unsupported("sparse_attention: fewer than 2^31 - 4096 rows (n * heads * lq, those of an (image, kv head) pair rounded "
-                              "up to 128), 65536 such pairs, 2^21 blocks of an image, 2^23 groups of several queries, 2^31 choices")
+                              "up to 128), 65536 such pairs, 2^21 blocks of an image, 2^23 groups of several queries, 2^26 choices")
         args = _lib.SparseArgs(
             n=n, lq=lq, lk=lk, heads=heads, kv_heads=kv_heads, d=d, top=min(top, lk), block=block, group=min(group, lq), q_bstride=qa[2],
             ldq=qa[1], k_bstride=kbs, ldk=ldk, v_bstride=va[2], ldv=va[1], mask_bstride=mbs, dtype=_lib.dtype_code(q.dtype),

@@ -627,7 +627,7 @@ int clarus_hip_block_means(const void* k, int32_t dtype, int64_t k_bstride, int6
  * counts for nothing, whatever k and v hold). means: those of k's blocks, kept by the caller while the keys stay, or NULL.
  * chosen: NULL or [n, heads, groups, ceil(blocks / 64)] words that receive the choice, block b in bit b % 64 of word b / 64.
  * block a multiple of 64 below 2^20, n * blocks < 2^23 and fewer than 2^21 blocks, n * groups < 2^23 where group > 1,
- * n * heads * groups < 2^31. scratch holds clarus_hip_sparse_attention_workspace(...) bytes, 16-byte aligned.
+ * n * heads * groups < 2^26. scratch holds clarus_hip_sparse_attention_workspace(...) bytes, 16-byte aligned.
  * Deterministic. No counterpart in the reference.
  */
 typedef struct ClarusSparseArgs {
