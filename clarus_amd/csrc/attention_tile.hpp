@@ -17,7 +17,7 @@ constexpr float XA_FLOOR = -3e38f;  // running maximum before any key: exp2(-inf
 constexpr float XA_SLACK = 8.f;     // a running maximum may lag the scores' by this (log2)
 constexpr float XA_FAR = 8388608.f;  // 2^23: up to this size a running maximum is within a quarter of the product it rounds
 
-enum : int { MASK_NONE = 0, MASK_KEYS = 1, MASK_PAIRS = 2 };
+enum : int { MASK_NONE = 0, MASK_KEYS = 1, MASK_PAIRS = 2, MASK_ROWS = 3 };
 
 struct CrossP {
   const void *q, *k, *v;
@@ -139,10 +139,11 @@ __device__ __forceinline__ unsigned xa_bits16(const unsigned char* p, int64_t le
 
 // One tile of NB x 32 keys for a wave's 32 rows: S^T = K Q^T, the softmax's step, O^T += V^T P^T. bits: the keys that
 // count, of a lane's row under MASK_PAIRS; whole: all of them; fresh: o is still 0; far: the maximum of
-// a row of the wave has been past XA_FAR
+// a row of the wave has been past XA_FAR; MASK_ROWS: the rows that are not live keep nothing of the tile, the others `bits`
 template <int DT, int D, int C, int MASK, int NB, bool ANEW>
 __device__ __forceinline__ void xa_tile(const unsigned char* ks, const unsigned char* vs, const u32x4 (&qf)[xa_qn<DT, C>],
-                                        f32x16 (&o)[D / 32], float& m, float& l, bool& far, float c, uint64_t bits, bool whole, bool fresh) {
+                                        f32x16 (&o)[D / 32], float& m, float& l, bool& far, float c, uint64_t bits, bool whole, bool fresh,
+                                        bool live = true) {
   using T = XaTile<DT, D>;
   constexpr int DB = D / 32, QN = xa_qn<DT, C>;
   // ANEW: the lane's LDS offsets are worked out for each tile instead of kept over the loop, where they spill
@@ -187,6 +188,7 @@ __device__ __forceinline__ void xa_tile(const unsigned char* ks, const unsigned 
   for (int b = 0; b < NB; ++b)
 #pragma unroll
     for (int j = 0; j < 16; ++j) mx = fmaxf(mx, s[b][j]);
+  if (MASK == MASK_ROWS && !live) mx = -INFINITY;
   if (__any(mx * c > m + XA_SLACK)) {
     mx = max32(mx);
     const float mn = fmaxf(m, mx * c);
@@ -211,11 +213,12 @@ __device__ __forceinline__ void xa_tile(const unsigned char* ks, const unsigned 
       for (int j = 0; j < 16; ++j) s[b][j] *= c;
     c = 1.f;
   }
+  const float mw = MASK == MASK_ROWS && !live ? INFINITY : m;
 #pragma unroll
   for (int b = 0; b < NB; ++b)
 #pragma unroll
     for (int j = 0; j < 16; ++j) {
-      s[b][j] = __builtin_amdgcn_exp2f(fmaf(s[b][j], c, -m));
+      s[b][j] = __builtin_amdgcn_exp2f(fmaf(s[b][j], c, -mw));
       l += s[b][j];
     }
   __builtin_amdgcn_s_setprio(2);

@@ -9,7 +9,7 @@
 //   sp_choose_kernel  a row's choice from them
 //   sp_kernel         the attention: 32 rows per wave as in cross_attention.hip (a row is a query and one of the heads that
 //                     share a kv head); a workgroup takes the blocks that any of its rows has chosen, one after another
-//                     through LDS, and a wave those of its own rows, the bits of each row masking what the others chose
+//                     through LDS, and a wave those of its own rows; a row that has not chosen a block weighs it by 0
 //   xa_join_kernel    joins the parts of blocks split over workgroups, where rows are few
 #include <algorithm>
 
@@ -21,7 +21,7 @@ namespace clarus {
 namespace {
 
 constexpr int SP_T = 256;
-constexpr int SP_WORDS = 32;   // words of 64 blocks that a workgroup of sp_kernel lists at a time
+constexpr int SP_WORDS = 16;   // words of 64 blocks that a workgroup of sp_kernel lists at a time
 constexpr int SP_TILE = 64;    // rows and blocks of a score workgroup
 constexpr int64_t SP_SLAB = 128 << 20;  // bytes of scores at a time, about
 
@@ -35,7 +35,6 @@ struct SparseP {
   int64_t nw, nb, groups, first;  // first: the slab's first row (image, head, group)
   int64_t slab;           // rows of this slab
   int block, group, top, heads, ask_dt;
-  int tpb;                // tiles of a block
 };
 
 // ---------------------------------------------------------------- means
@@ -451,12 +450,69 @@ __device__ __forceinline__ uint64_t or32(uint64_t v) {  // over the 32 lanes of 
   return v;
 }
 
+// The copies of one operand of a tile to LDS by W waves, 1 KiB each: XaCopy's layout. Where the rows of a wave's
+// copies lie a multiple of 16 apart (what the swizzles repeat after), one offset serves all of them
+template <int DT, int D, int W, bool V>
+struct SpCopy {
+  using T = XaTile<DT, D>;
+  static constexpr int BYTES = T::BYTES, NI = (BYTES / 1024 + W - 1) / W;
+  static constexpr bool EVEN = BYTES / 1024 % W == 0, SAME = W * 1024 % (16 * T::ROWB) == 0;
+  uint32_t off[SAME ? 1 : NI];
+  static __device__ __forceinline__ void place(int j, int wave, int lane, int& r, int& c) {
+    const int at = (wave + W * j) * 1024 + lane * 16;
+    r = at / T::ROWB;
+    c = at % T::ROWB / 16;
+    c ^= V ? T::swz_v(r) : T::swz_k(r);
+  }
+  __device__ __forceinline__ SpCopy(int64_t ld, int wave, int lane) {
+#pragma unroll
+    for (int j = 0; j < (SAME ? 1 : NI); ++j) {
+      int r, c;
+      place(j, wave, lane, r, c);
+      off[j] = (uint32_t)(r * ld * T::ES) + c * 16;
+    }
+  }
+  // bits: the keys that count; the others, and columns from d on, are zeros
+  __device__ __forceinline__ void operator()(const unsigned char* src, int64_t ld, int d, unsigned char* tile, uint64_t bits, int wave,
+                                             int lane) const {
+    unsigned char* dst = tile + wave * 1024;
+#define SP_COPY(from)                                                                          \
+  __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void*)(from),     \
+                                   (__attribute__((address_space(3))) void*)(dst + j * W * 1024), 16, 0, 0)
+    const unsigned step = SAME ? (unsigned)(W * 1024 / T::ROWB * ld * T::ES) : 0;  // bytes between a wave's copies
+    if (bits == T::ALL && d == D) {
+#pragma unroll
+      for (int j = 0; j < NI; ++j) {
+        if (!EVEN && wave + W * j >= BYTES / 1024) break;
+        SP_COPY(src + (size_t)j * step + off[SAME ? 0 : j]);
+      }
+    } else {
+      const unsigned char* zero = (const unsigned char*)xa_zeros;
+#pragma unroll
+      for (int j = 0; j < NI; ++j) {
+        if (!EVEN && wave + W * j >= BYTES / 1024) break;
+        int r, c;
+        place(j, wave, lane, r, c);
+        SP_COPY((bits >> r & 1) && c * 16 < d * T::ES ? src + (size_t)j * step + off[SAME ? 0 : j] : zero);
+      }
+    }
+#undef SP_COPY
+  }
+};
+
+__device__ __forceinline__ const unsigned char* uniform(const unsigned char* p) {
+  const uint64_t u = (uint64_t)p;
+  return (const unsigned char*)((uint64_t)(unsigned)__builtin_amdgcn_readfirstlane((unsigned)(u >> 32)) << 32 |
+                                (unsigned)__builtin_amdgcn_readfirstlane((unsigned)u));
+}
+
 template <int DT, int D, int C, int MASK, int W>
-__global__ void __launch_bounds__(64 * W, D <= 64 ? 3 : 2) sp_kernel(const SparseP sp) {
+__global__ void __launch_bounds__(64 * W, DT == DT_BF16 && D <= 64 ? 4 : 2) sp_kernel(const SparseP sp) {
   using T = XaTile<DT, D>;
   constexpr int KT = T::KT, KB = KT / 32, DB = D / 32;
   const CrossP& p = sp.x;
-  __shared__ __align__(16) unsigned char tiles[2][2 * T::BYTES];
+  const int tpb = sp.block / KT, lk = (int)p.lk;  // tiles of a block, keys
+  __shared__ __align__(16) unsigned char tile[2 * T::BYTES];
   __shared__ uint64_t wants[W][SP_WORDS];
   __shared__ unsigned short list[SP_WORDS * 64];  // blocks of the words at hand that a row of the workgroup has chosen
 
@@ -480,20 +536,25 @@ __global__ void __launch_bounds__(64 * W, D <= 64 ? 3 : 2) sp_kernel(const Spars
   const int n = (int)nk / p.kv_heads, kvh = (int)nk - n * p.kv_heads;
   const int64_t wrow = (int64_t)rb * (32 * W) + wave * 32;
   const bool busy = wrow < p.rows;
-  const int64_t row = wrow + col < p.rows ? wrow + col : p.rows - 1;  // rows past the end repeat the last one
-  const XaRow r = xa_row(p, kvh, row);
+  // the lane's row, worked out anew where it is needed (kept over the loop it would spill); past the end the last one
+  auto place = [&]() __attribute__((always_inline)) {
+    int at = lane & 31;
+    asm volatile("" : "+v"(at));
+    return wrow + at < p.rows ? wrow + at : p.rows - 1;
+  };
   const unsigned char* kp = (const unsigned char*)p.k + (n * p.kbs + (int64_t)kvh * p.d) * T::ES;
   const unsigned char* vp = (const unsigned char*)p.v + (n * p.vbs + (int64_t)kvh * p.d) * T::ES;
   const unsigned char* mkey = MASK == MASK_KEYS ? p.mask + n * p.mbs : nullptr;
-  const uint64_t* words = sp.chosen + (((int64_t)n * sp.heads + r.head) * sp.groups + (unsigned)r.qi / (unsigned)sp.group) * sp.nw;
 
-  const XaCopy<DT, D, W> copy(p, wave, lane);
-  auto fill = [&](int64_t t, uint64_t bits, int buf) __attribute__((always_inline)) {
-    const int64_t base = t * KT;
-    copy(p, kp + base * p.ldk * T::ES, vp + base * p.ldv * T::ES, tiles[buf], bits);
+  const SpCopy<DT, D, W, false> copy_k(p.ldk, wave, lane);
+  const SpCopy<DT, D, W, true> copy_v(p.ldv, wave, lane);
+  auto fill = [&](int t, uint64_t bits) __attribute__((always_inline)) {
+    const int64_t base = (int64_t)t * KT;
+    copy_k(uniform(kp + base * p.ldk * T::ES), p.ldk, p.d, tile, bits, wave, lane);
+    copy_v(uniform(vp + base * p.ldv * T::ES), p.ldv, p.d, tile + T::BYTES, bits, wave, lane);
   };
   u32x4 qf[xa_qn<DT, C>];
-  xa_load_q<DT, C>(p, n, r, hl, qf);
+  xa_load_q<DT, C>(p, n, xa_row(p, kvh, place()), hl, qf);
   f32x16 o[DB];
 #pragma unroll
   for (int b = 0; b < DB; ++b)
@@ -506,6 +567,8 @@ __global__ void __launch_bounds__(64 * W, D <= 64 ? 3 : 2) sp_kernel(const Spars
   for (int64_t w0 = 0; w0 < sp.nw; w0 += SP_WORDS) {
     const int wn = sp.nw - w0 < SP_WORDS ? (int)(sp.nw - w0) : SP_WORDS;
     if (w0) __syncthreads();  // the words and the last tile before have been read
+    const XaRow r = xa_row(p, kvh, place());
+    const uint64_t* words = sp.chosen + (((int64_t)n * sp.heads + r.head) * sp.groups + (unsigned)r.qi / (unsigned)sp.group) * sp.nw;
     for (int w = 0; w < wn; ++w) {
       const uint64_t any = or32(busy ? words[w0 + w] : 0);
       if (lane == 0) wants[wave][w] = any;
@@ -523,57 +586,65 @@ __global__ void __launch_bounds__(64 * W, D <= 64 ? 3 : 2) sp_kernel(const Spars
     count = __builtin_amdgcn_readfirstlane(count);
     __syncthreads();
     const int i1 = (int)((int64_t)count * (split + 1) / p.splits);
-    int at = (int)((int64_t)count * split / p.splits) - 1, blk = 0, sub = sp.tpb;
-    auto pop = [&](int& b) __attribute__((always_inline)) -> int64_t {  // the next tile and its block, -1 past the last
-      if (++sub >= sp.tpb || ((w0 * 64 + blk) * sp.tpb + sub) * KT >= p.lk) {
-        if (++at >= i1) {
-          sub = sp.tpb;
-          --at;
+    // 32 listed blocks at a time: lane i holds the i-th, bit i of `keep` says whether the lane's row has chosen it, so that
+    // the steps between the products read no list
+#pragma unroll 1
+    for (int i0 = (int)((int64_t)count * split / p.splits); i0 < i1; i0 += 32) {
+      const int cn = i1 - i0 < 32 ? i1 - i0 : 32;
+      const int blk = lane < cn ? list[i0 + lane] : 0;
+      unsigned keep = 0;
+      const unsigned* row_words = reinterpret_cast<const unsigned*>(words + w0);
+      if (busy) {
+#pragma unroll 4
+        for (int i = 0; i < cn; ++i) {
+          const int b = __builtin_amdgcn_readlane(blk, i);
+          keep |= (row_words[b >> 5] >> (b & 31) & 1) << i;
+        }
+      }
+      int e = -1, sub = tpb;
+      auto pop = [&](int& i) __attribute__((always_inline)) {  // the next tile and its place in the list, -1 past the last
+        if (++sub < tpb) {
+          const int t = ((int)w0 * 64 + __builtin_amdgcn_readlane(blk, e)) * tpb + sub;
+          if (t * KT < lk) return t;
+        }
+        if (e + 1 >= cn) {
+          sub = tpb;
           return -1;
         }
-        blk = __builtin_amdgcn_readfirstlane((int)list[at]);
+        i = ++e;
         sub = 0;
-      }
-      b = blk;
-      return (w0 * 64 + blk) * sp.tpb + sub;
-    };
-    auto key_byte = [&](int64_t t) __attribute__((always_inline)) { return t < 0 ? 0 : xa_key_byte<KT, MASK>(mkey, t * KT, p.lk, lane); };
-    auto word_of = [&](int b) __attribute__((always_inline)) { return words[w0 + (b >> 6)] >> (b & 63); };
-    int b = 0, b1 = 0, b2 = 0;
-    int64_t t = pop(b), t1 = pop(b1);
-    if (t < 0) continue;
-    uint64_t bits = __ballot(key_byte(t));
-    int byte = key_byte(t1), buf = 0;
-    fill(t, bits, 0);
-    uint64_t next = word_of(b);
+        return ((int)w0 * 64 + __builtin_amdgcn_readlane(blk, e)) * tpb;
+      };
+      auto key_byte = [&](int t) __attribute__((always_inline)) {  // this lane's key of a tile counts
+        const bool in = lane < KT && lane < lk - t * KT && t >= 0;
+        if constexpr (MASK == MASK_KEYS) return in ? (int)mkey[t * KT + lane] : 0;
+        return (int)in;
+      };
+      int i = 0, t = pop(i);
+      int byte = key_byte(t);
 #pragma unroll 1
-    while (t >= 0) {
-      __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0): this wave's copies of tile t have landed
-      barrier_keep_vm();                   // everybody's have, and the tile before has been read
-      const uint64_t now = next & 1 ? bits : 0;  // of this lane's row
-      const bool mine = busy && (wants[wave][b >> 6] >> (b & 63) & 1);
-      const int64_t t2 = pop(b2);
-      if (t1 >= 0) {
-        bits = __ballot(byte);
-        byte = key_byte(t2);
-        fill(t1, bits, buf ^ 1);
-        next = word_of(b1);
+      while (t >= 0) {
+        const uint64_t bits = __ballot(byte);
+        barrier_keep_vm();  // the tile before has been read
+        fill(t, bits);
+        const bool live = keep >> i & 1;  // this lane's row has chosen it
+        t = pop(i);
+        byte = key_byte(t);
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // this wave's copies have landed
+        barrier_keep_vm();                   // everybody's have
+        if (__any(live)) xa_tile<DT, D, C, MASK_ROWS, KB, DT == DT_BF16 && C == 64>(tile, tile + T::BYTES, qf, o, m, l, far, p.c, bits, bits == T::ALL, false, live);
       }
-      if (mine) xa_tile<DT, D, C, MASK_PAIRS, KB, false>(tiles[buf], tiles[buf] + T::BYTES, qf, o, m, l, far, p.c, now, now == T::ALL, false);
-      t = t1;
-      b = b1;
-      t1 = t2;
-      b1 = b2;
-      buf ^= 1;
     }
   }
   if (!busy) return;
   l = sum32(l);
+  const int64_t row = place();
+  const bool there = wrow + col < p.rows;
   if (p.splits == 1) {
-    xa_store<D>(p, n, r, o, l, wrow + col < p.rows);
+    xa_store<D>(p, n, xa_row(p, kvh, row), o, l, there);
     return;
   }
-  if (wrow + col >= p.rows) return;
+  if (!there) return;
   const int64_t to = ((int64_t)split * p.nk + nk) * p.rows + row, all = (int64_t)p.splits * p.nk * p.rows;
   float* po = p.part + to * D;
 #pragma unroll
@@ -585,6 +656,14 @@ __global__ void __launch_bounds__(64 * W, D <= 64 ? 3 : 2) sp_kernel(const Spars
 }
 
 int sp_pad(int64_t d) { return d <= 32 ? 32 : d <= 64 ? 64 : d <= 96 ? 96 : 128; }
+
+// Waves of a workgroup, 32 rows each: they share the copies of a block, but wait for each other's blocks. Rows that choose
+// together fill four; else two (fp32, bound by the products: one). us with 1 / 2 / 4 waves, one tile in LDS: 14400 queries
+// of 8 heads of 64 each choosing 16 of 225 blocks 357 / 292 / 341; 57600, 64 choosing together, 16 of 900 354 / 242 / 298, 256
+// together 329 / 224 / 195; 28800 of 128, 256 together 381 / 197 / 183; 7200 of 4 heads of 64 in fp32, each 453 / 659 / 435, 14400,
+// 64 together 169 / 173 / 279; 14400 of 2 of 128 in fp32, 256 together 184 / 272 / 154. (A second tile in LDS, on its way
+// during the first one's products, halves the workgroups of a CU: 57600, 64 together, 555 / 336 / 335)
+int sp_waves(int32_t dt, int64_t rows, int64_t alike) { return rows <= 32 ? 1 : alike >= 128 ? 4 : dt == DT_BF16 ? 2 : 1; }
 
 struct SpPlan {
   int64_t nb, nw, groups, nblk, slab;  // slab: rows of scores at a time
@@ -615,7 +694,7 @@ SpPlan sp_plan(int32_t dt, int64_t n, int64_t lq, int64_t lk, int64_t heads, int
     g.slab = std::min(asks, std::min<int64_t>(cdiv(SP_SLAB / 8, g.nb * SP_TILE), 1 << 16) * SP_TILE);
     g.score = (size_t)cdiv(g.slab * g.nb, 2) * 16;
   }
-  g.waves = rows <= 32 ? 1 : 4;
+  g.waves = sp_waves(dt, rows, group * (heads / kv_heads));
   g.nblk = cdiv(rows, 32 * g.waves);
   const int64_t blocks = g.nblk * nk, cus = device_cus();
   // few rows: the blocks that they can choose split until every CU has two workgroups
@@ -662,7 +741,8 @@ template <int DT, int D, int C, int MASK>
 void sp_launch_mask(const SparseP& k, int waves, hipStream_t st) {
   const dim3 grid((unsigned)(8 * ((k.x.nblk * k.x.nk * k.x.splits + 7) / 8)));
   if (waves == 1) hipLaunchKernelGGL((sp_kernel<DT, D, C, MASK, 1>), grid, dim3(64), 0, st, k);
-  else hipLaunchKernelGGL((sp_kernel<DT, D, C, MASK, 4>), grid, dim3(256), 0, st, k);
+  else if (waves == 4) hipLaunchKernelGGL((sp_kernel<DT, D, C, MASK, 4>), grid, dim3(256), 0, st, k);
+  else if constexpr (DT == DT_BF16) hipLaunchKernelGGL((sp_kernel<DT, D, C, MASK, 2>), grid, dim3(128), 0, st, k);
 }
 
 template <int DT, int D, int C>
@@ -757,7 +837,6 @@ extern "C" int clarus_hip_sparse_attention(const ClarusSparseArgs* a, void* scra
   x.rows = a->lq * x.rep; x.lk = a->lk; x.nk = a->n * a->kv_heads; x.nblk = g.nblk; x.splits = g.splits;
   x.o_dt = a->o_dtype; x.c = a->scale * 1.4426950408889634f;
   k.nw = g.nw; k.nb = g.nb; k.groups = g.groups; k.block = (int)a->block; k.group = (int)group; k.top = (int)top; k.heads = (int)a->heads;
-  k.tpb = (int)(a->block / (a->dtype == DT_BF16 ? 64 : 32));
   hipStream_t st = (hipStream_t)stream;
   const int64_t c = a->heads * a->d, ck = a->kv_heads * a->d;
   float* means = (float*)take(g.means);
