@@ -37,6 +37,7 @@ struct LinP {
   void* out;
   const float *s_in, *decay;
   float *s_out, *part;
+  int* careful;          // segments with values that are not finite, for each wave's columns
   int64_t qbs, ldq, kbs, ldk, vbs, ldv;
   int64_t l;             // tokens
   int64_t nk, nseg, seg; // (image, kv head) pairs, segments, tokens of one
@@ -137,7 +138,7 @@ __global__ void __launch_bounds__(LA_T) la_step_kernel(const LinP p) {
 
 // ---------------------------------------------------------------- chunks
 // Tokens of a chunk: 64 in bf16, 32 in fp32 and with wide keys in bf16, whose state and queries fill the registers
-template <int DT, int DK> constexpr int la_kt = DT == DT_BF16 && DK <= 64 ? 64 : 32;
+template <int DT, int DK> constexpr int la_kt = DT == DT_BF16 && DK <= 32 ? 64 : 32;
 
 // The copies of one tile (KT tokens, D columns of LDS) by W waves, 1 KiB each
 template <int DT, int D, int KT, int W>
@@ -196,21 +197,26 @@ __device__ __forceinline__ f32x16 la_mfma(const bf16x8& a, const bf16x8& b, cons
   return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
 }
 
-// W waves, 32 columns of values each. OUT: outputs, from the segment's start state; else what the segment adds
+// chunks in LDS: the one at work and the next (fp32), or the next two on their way (bf16); K, V and Q of the first head
 template <int DT, int DK, int W, bool OUT>
-__global__ void __launch_bounds__(64 * W, 2) la_chunk_kernel(const LinP p) {
+struct LaChunk {
+  static constexpr int KT = la_kt<DT, DK>, BUFS = DT == DT_BF16 ? 3 : 2, KBYTES = KT * XaTile<DT, DK>::ROWB,
+                       VBYTES = KT * XaTile<DT, 32 * W>::ROWB, QBYTES = OUT ? KBYTES : 0, BYTES = KBYTES + VBYTES + QBYTES;
+};
+
+// W waves, 32 columns of values each. OUT: outputs, from the segment's start state; else what the segment adds.
+// CAREFUL: for a segment with values that are not finite. The weight 0 that such a value has for the queries before it would
+// make them NaN, so the product gets a 0 in its place, and the outputs from its token on are NaN.
+template <int DT, int DK, int W, bool OUT, bool CAREFUL>
+__device__ __forceinline__ void la_chunks(const LinP& p, const unsigned n, const unsigned h, const unsigned seg,
+                                          unsigned char (*tiles)[LaChunk<DT, DK, W, OUT>::BYTES]) {
   using TK = XaTile<DT, DK>;
   using TV = XaTile<DT, 32 * W>;
-  constexpr int KT = la_kt<DT, DK>, QT = KT / 32, DB = DK / 32, QN = xa_qn<DT, DK>, ES = TK::ES;
-  constexpr int KBYTES = KT * TK::ROWB, VBYTES = KT * TV::ROWB;
-  __shared__ __align__(16) unsigned char tiles[2][KBYTES + VBYTES];
+  using L = LaChunk<DT, DK, W, OUT>;
+  constexpr int KT = L::KT, QT = KT / 32, DB = DK / 32, QN = xa_qn<DT, DK>, ES = TK::ES;
+  constexpr int KBYTES = L::KBYTES, VBYTES = L::VBYTES, QBYTES = L::QBYTES, BUFS = L::BUFS, AHEAD = BUFS - 1;
   const int tid = threadIdx.x, lane0 = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int col = lane0 & 31, hl = lane0 >> 5;
-  // neighbouring heads of a segment, which share lines of rows, on one XCD
-  const unsigned total = (unsigned)(p.nk * p.nseg), span = (total + 7) >> 3, id = (blockIdx.x & 7) * span + (blockIdx.x >> 3);
-  if ((blockIdx.x >> 3) >= span || id >= total) return;
-  const unsigned rest = id / (unsigned)p.kv_heads, h = id - rest * (unsigned)p.kv_heads;
-  const unsigned n = rest / (unsigned)p.nseg, seg = rest - n * (unsigned)p.nseg;
   const int64_t nk = (int64_t)n * p.kv_heads + h;
   // padded places: token = place - pad
   const int64_t t0 = seg * p.seg, t1 = t0 + p.seg < p.l + p.pad ? t0 + p.seg : p.l + p.pad;
@@ -244,30 +250,22 @@ __global__ void __launch_bounds__(64 * W, 2) la_chunk_kernel(const LinP p) {
 
   const unsigned char* kp = (const unsigned char*)p.k + (n * p.kbs + (int64_t)h * p.dk) * ES;
   const unsigned char* vp = (const unsigned char*)p.v + (n * p.vbs + (int64_t)h * p.dv) * ES;
-  const LaCopy<DT, DK, KT, W> copy_k(p.ldk, wave, lane0);
+  const LaCopy<DT, DK, KT, W> copy_k(p.ldk, wave, lane0), copy_q(p.ldq, wave, lane0);
   const LaCopy<DT, 32 * W, KT, W> copy_v(p.ldv, wave, lane0);
-  auto fill = [&](int c, int buf) __attribute__((always_inline)) {
+  const unsigned char* qp0 = (const unsigned char*)p.q + (n * p.qbs + (int64_t)h * p.rep * p.dk) * ES;
+  auto fill = [&](int c) __attribute__((always_inline)) {
     const int64_t at = t0 + (int64_t)c * KT - p.pad;  // token of the chunk's first place, negative in the padding
     const int pad = at < 0 ? (int)-at : 0;
-    copy_k(kp + at * p.ldk * ES, p.dk, pad, tiles[buf], wave, lane0);
-    copy_v(vp + at * p.ldv * ES, p.dv, pad, tiles[buf] + KBYTES, wave, lane0);
+    unsigned char* to = tiles[c % BUFS];
+    copy_k(kp + at * p.ldk * ES, p.dk, pad, to, wave, lane0);
+    copy_v(vp + at * p.ldv * ES, p.dv, pad, to + KBYTES, wave, lane0);
+    if constexpr (OUT) copy_q(qp0 + at * p.ldq * ES, p.dk, pad, to + KBYTES + VBYTES, wave, lane0);
   };
-  u32x4 qf[OUT ? QT : 1][QN];  // of the next chunk from where this one's outputs are done
-  auto load_q = [&](int c, int r) __attribute__((always_inline)) {
+  // what a wave issues at least for a chunk: with as many operations in flight, the chunk before has landed
+  constexpr int COPIES = KBYTES / 1024 / W + VBYTES / 1024 / W + QBYTES / 1024 / W;
 #pragma unroll
-    for (int t = 0; t < QT; ++t) {
-      const int64_t place = t0 + (int64_t)c * KT + 32 * t + col - p.pad;
-      const unsigned char* qp = (const unsigned char*)p.q + (n * p.qbs + (place < 0 ? 0 : place) * p.ldq + (int64_t)(h * p.rep + r) * p.dk) * ES;
-#pragma unroll
-      for (int i = 0; i < QN; ++i) {
-        const int at = (2 * i + hl) * (16 / ES);
-        qf[t][i] = *reinterpret_cast<const u32x4*>(qp + (at < p.dk ? at : 0) * ES);
-        if (p.dk < DK && at >= p.dk) qf[t][i] = u32x4{0, 0, 0, 0};
-      }
-    }
-  };
-  fill(0, 0);
-  if constexpr (OUT) load_q(0, 0);
+  for (int c = 0; c < AHEAD; ++c)
+    if (c < nchunk) fill(c);
 #pragma unroll 1
   for (int c = 0; c < nchunk; ++c) {
     // LDS and output offsets are worked out for each chunk instead of kept over the loop, where they spill
@@ -276,10 +274,12 @@ __global__ void __launch_bounds__(64 * W, 2) la_chunk_kernel(const LinP p) {
     const int col = lane & 31, hl = lane >> 5;
     const int64_t first = t0 + (int64_t)c * KT - p.pad;
     const int pad = first < 0 ? (int)-first : 0;
-    __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0): this wave's copies have landed
-    barrier_keep_vm();                   // everybody's have, and the chunk before has been read
-    const unsigned char *kt = tiles[c & 1], *vt = tiles[c & 1] + KBYTES;
-    if (c + 1 < nchunk) fill(c + 1, (c & 1) ^ 1);
+    // this wave's copies of the chunk have landed, the next one's may be on their way
+    if (AHEAD == 2 && c + 1 < nchunk) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(COPIES) : "memory");
+    else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    barrier_keep_vm();  // everybody's have, and the chunk before has been read
+    const unsigned char *kt = tiles[c % BUFS], *vt = kt + KBYTES, *qt = vt + VBYTES;
+    if (BUFS == 2 && c + 1 < nchunk) fill(c + 1);
     bf16x8 vf[DT == DT_BF16 ? KT / 16 : 1];
     float vx[DT == DT_BF16 ? 1 : 16];
     if constexpr (DT == DT_BF16) {
@@ -290,10 +290,47 @@ __global__ void __launch_bounds__(64 * W, 2) la_chunk_kernel(const LinP p) {
       for (int j = 0; j < 16; ++j)
         vx[j] = *reinterpret_cast<const float*>(vt + TV::at_k(8 * (j >> 2) + 4 * hl + (j & 3), 8 * wave + (col >> 2)) + (col & 3) * 4);
     }
+    int bad = KT;  // the first token whose value in this lane's column is not finite
+    if constexpr (CAREFUL) {
+      if constexpr (DT == DT_BF16) {
+#pragma unroll
+        for (int ks = KT / 16 - 1; ks >= 0; --ks)
+#pragma unroll
+          for (int e = 7; e >= 0; --e)
+            if (!(fabsf((float)vf[ks][e]) < INFINITY)) {
+              bad = 16 * ks + 8 * (e >> 2) + 4 * hl + (e & 3);
+              vf[ks][e] = (bf16_t)0.f;
+            }
+      } else {
+#pragma unroll
+        for (int j = 15; j >= 0; --j)
+          if (!(fabsf(vx[j]) < INFINITY)) {
+            bad = 8 * (j >> 2) + 4 * hl + (j & 3);
+            vx[j] = 0.f;
+          }
+      }
+      const int other = __shfl_xor(bad, 32);
+      bad = other < bad ? other : bad;
+    }
     if constexpr (OUT) {
 #pragma unroll 1
       for (int r = 0; r < p.rep; ++r) {
-        if (r) load_q(c, r);
+        u32x4 qf[QT][QN];
+#pragma unroll
+        for (int t = 0; t < QT; ++t) {
+          const int64_t token = first + 32 * t + col;
+          const unsigned char* qp = qp0 + ((token < 0 ? 0 : token) * p.ldq + (int64_t)r * p.dk) * ES;
+#pragma unroll
+          for (int i = 0; i < QN; ++i) {
+            if (r == 0) {
+              qf[t][i] = *reinterpret_cast<const u32x4*>(qt + TK::at_k(32 * t + col, 2 * i + hl));
+            } else {
+              const int at = (2 * i + hl) * (16 / ES);
+              qf[t][i] = *reinterpret_cast<const u32x4*>(qp + (at < p.dk ? at : 0) * ES);
+              if (p.dk < DK && at >= p.dk) qf[t][i] = u32x4{0, 0, 0, 0};
+            }
+          }
+        }
         f32x16 o[QT];
 #pragma unroll
         for (int t = 0; t < QT; ++t)
@@ -371,6 +408,15 @@ __global__ void __launch_bounds__(64 * W, 2) la_chunk_kernel(const LinP p) {
               for (int j = 0; j < 16; ++j) o[t] = __builtin_amdgcn_mfma_f32_32x32x2f32(vx[j], w[j], o[t], 0, 0, 0);
             }
           }
+        if constexpr (CAREFUL) {
+#pragma unroll
+          for (int j = 0; j < 16; ++j) {
+            const int from = __shfl(bad, 8 * (j >> 2) + 4 * hl + (j & 3));
+#pragma unroll
+            for (int t = 0; t < QT; ++t)
+              if (32 * t + col >= from) o[t][j] = NAN;
+          }
+        }
 #pragma unroll
         for (int t = 0; t < QT; ++t) {
           const bool live = 32 * t + col >= pad;
@@ -398,7 +444,6 @@ __global__ void __launch_bounds__(64 * W, 2) la_chunk_kernel(const LinP p) {
         }
       }
       if (c + 1 == nchunk) break;  // no output needs the state behind the last chunk
-      load_q(c + 1, 0);
     }
     __builtin_amdgcn_sched_barrier(0);
     // the state behind this chunk
@@ -437,61 +482,117 @@ __global__ void __launch_bounds__(64 * W, 2) la_chunk_kernel(const LinP p) {
         }
       }
     }
+    if (CAREFUL && bad < KT) {
+#pragma unroll
+      for (int b = 0; b < DB; ++b)
+#pragma unroll
+        for (int j = 0; j < 16; ++j) s[b][j] = NAN;
+    }
+    // behind the outputs' stores, which the wait above would else wait for too
+    if (AHEAD == 2 && c + 2 < nchunk) fill(c + 2);
   }
   if constexpr (!OUT) {
 #pragma unroll
     for (int b = 0; b < DB; ++b)
 #pragma unroll
       for (int j = 0; j < 16; ++j) part[(b * 16 + j) * 64] = s[b][j];
+    // a value that is not finite leaves no row of its column finite
+    const bool careful = __any(!(fabsf(s[0][0]) < INFINITY));
+    if (lane0 == 0) p.careful[(nk * p.nseg + seg) * W + wave] = careful;
   }
 }
 
-// In place of what each segment adds the state that it starts with; the state behind the last. A thread per element, in the
-// accumulators' order; the next CB segments' loads in flight
-template <int CB>
+template <int DT, int DK, int W, bool OUT>
+__global__ void __launch_bounds__(64 * W, 2) la_chunk_kernel(const LinP p) {
+  using L = LaChunk<DT, DK, W, OUT>;
+  __shared__ __align__(16) unsigned char tiles[L::BUFS][L::BYTES];
+  // neighbouring heads of a segment, which share lines of rows, on one XCD
+  const unsigned total = (unsigned)(p.nk * p.nseg), span = (total + 7) >> 3, id = (blockIdx.x & 7) * span + (blockIdx.x >> 3);
+  if ((blockIdx.x >> 3) >= span || id >= total) return;
+  const unsigned rest = id / (unsigned)p.kv_heads, h = id - rest * (unsigned)p.kv_heads;
+  const unsigned n = rest / (unsigned)p.nseg, seg = rest - n * (unsigned)p.nseg;
+  if constexpr (OUT) {
+    int careful = 0;
+#pragma unroll
+    for (int w = 0; w < W; ++w) careful |= p.careful[(((int64_t)n * p.kv_heads + h) * p.nseg + seg) * W + w];
+    if (__builtin_amdgcn_readfirstlane(careful)) {
+      la_chunks<DT, DK, W, true, true>(p, n, h, seg, tiles);
+      return;
+    }
+  }
+  la_chunks<DT, DK, W, OUT, false>(p, n, h, seg, tiles);
+}
+
+// In place of what each segment adds the state that it starts with; the state behind the last. A workgroup takes 32 elements
+// (in the accumulators' order) and 8 x LA_GROUP segments at a time: a thread has LA_GROUP of them of one element in registers,
+// and the groups are chained through LDS (57600 tokens in 128 segments, 8 heads of 64 x 64: 15.0 us with a thread per element
+// and chain, the next 8 segments in flight)
+constexpr int LA_GROUP = 16, LA_GROUPS = LA_T / 32;
+
 __global__ void __launch_bounds__(LA_T) la_carry_kernel(const LinP p, int waves, int db) {
-  const int per = waves * db * 16 * 64;  // elements of a state, padded
-  const int64_t i = (int64_t)blockIdx.x * LA_T + threadIdx.x;
-  if (i >= p.nk * per) return;
-  const int64_t nk = i / per;
-  const int e = (int)(i - nk * per), lane = e & 63, reg = (e >> 6) % (db * 16), wave = e / (db * 16 * 64), j = reg & 15;
+  __shared__ float sums[LA_GROUPS][32];
+  __shared__ Factor facts[LA_GROUPS + 3];  // of the groups; of the first segment, one between, the last
+  const unsigned per = waves * db * 16 * 64;  // elements of a state, padded
+  const int tid = threadIdx.x, grp = tid >> 5;
+  const unsigned nk = blockIdx.x / (per / 32), e = (blockIdx.x - nk * (per / 32)) * 32 + (tid & 31), h = nk % (unsigned)p.kv_heads;
+  const int lane = e & 63, reg = (e >> 6) % (unsigned)(db * 16), wave = e / (unsigned)(db * 16 * 64), j = reg & 15;
   const int r = 32 * (reg >> 4) + 8 * (j >> 2) + 4 * (lane >> 5) + (j & 3), c = 32 * wave + (lane & 31);
   const bool in = r < p.dk && c < p.dv;
-  const int64_t at = nk * p.dk * p.dv + (int64_t)r * p.dv + c;
-  const int h = (int)(nk % p.kv_heads);
-  const Factor first = la_factor(p, h, p.seg - p.pad < p.l ? p.seg - p.pad : p.l), f = la_factor(p, h, p.seg),
-               last = la_factor(p, h, p.l + p.pad - (p.nseg - 1) * p.seg);
-  float* part = p.part + nk * p.nseg * per + e;
+  const int64_t at = (int64_t)nk * p.dk * p.dv + (int64_t)r * p.dv + c;
+  auto token = [&](int64_t s) __attribute__((always_inline)) {  // before segment s
+    const int64_t t = (s < p.nseg ? s : p.nseg) * p.seg - p.pad;
+    return t < 0 ? 0 : t < p.l ? t : p.l;
+  };
+  float* part = p.part + (int64_t)nk * p.nseg * per + e;
   float s = p.s_in && in ? p.s_in[at] : 0.f;
-  float add[2][CB];
-  auto load = [&](int buf, int64_t s0) __attribute__((always_inline)) {
+#pragma unroll 1
+  for (int64_t r0 = 0; r0 < p.nseg; r0 += LA_GROUP * LA_GROUPS) {
+    const int64_t s0 = r0 + grp * LA_GROUP;
+    const int mine = (int)(p.nseg - s0 < 0 ? 0 : p.nseg - s0 < LA_GROUP ? p.nseg - s0 : LA_GROUP);
+    float add[LA_GROUP];
 #pragma unroll
-    for (int k = 0; k < CB; ++k) add[buf][k] = part[(s0 + k < p.nseg ? s0 + k : p.nseg - 1) * per];
-  };
-  auto run = [&](int buf, int64_t s0) __attribute__((always_inline)) {
-#pragma unroll
-    for (int k = 0; k < CB; ++k) {
-      if (s0 + k >= p.nseg) break;
-      part[(s0 + k) * per] = s;
-      const Factor& by = s0 + k == 0 ? first : s0 + k == p.nseg - 1 ? last : f;
-      s = la_scaled(s, by, add[buf][k]);
+    for (int k = 0; k < LA_GROUP; ++k) add[k] = part[(s0 + k < p.nseg ? s0 + k : p.nseg - 1) * per];
+    __syncthreads();  // the groups before have been read
+    if (tid < LA_GROUPS + 3) {
+      const int64_t a = tid < LA_GROUPS ? r0 + tid * LA_GROUP : tid == LA_GROUPS ? 0 : tid == LA_GROUPS + 1 ? 1 : p.nseg - 1;
+      const int64_t b = tid < LA_GROUPS ? a + LA_GROUP : a + 1;
+      facts[tid] = la_factor(p, h, tid == LA_GROUPS + 1 ? p.seg : token(b) - token(a));
     }
-  };
-  load(0, 0);
-  for (int64_t s0 = 0; s0 < p.nseg; s0 += 2 * CB) {
-    load(1, s0 + CB);
-    run(0, s0);
-    load(0, s0 + 2 * CB);
-    run(1, s0 + CB);
+    __syncthreads();
+    // the first and the last segment's may differ from the others'
+    const float fh = facts[LA_GROUPS + 1].hi, fl = facts[LA_GROUPS + 1].lo;
+    const float h0 = s0 == 0 ? facts[LA_GROUPS].hi : fh, l0 = s0 == 0 ? facts[LA_GROUPS].lo : fl;
+    const int end = p.nseg - 1 - s0 < LA_GROUP && p.nseg - 1 > 0 ? (int)(p.nseg - 1 - s0) : -1;
+    const float h1 = facts[LA_GROUPS + 2].hi, l1 = facts[LA_GROUPS + 2].lo;
+    auto step = [&](float v, int k) __attribute__((always_inline)) {
+      const float hi = k == end ? h1 : k == 0 ? h0 : fh, lo = k == end ? l1 : k == 0 ? l0 : fl;
+      return fmaf(v, hi, fmaf(v, lo, add[k]));
+    };
+    float v = 0.f;
+#pragma unroll
+    for (int k = 0; k < LA_GROUP; ++k) v = k < mine ? step(v, k) : v;
+    sums[grp][tid & 31] = v;
+    __syncthreads();
+#pragma unroll
+    for (int g = 0; g < LA_GROUPS; ++g) {
+      if (g == grp) v = s;  // what this group starts with
+      s = fmaf(s, facts[g].hi, fmaf(s, facts[g].lo, sums[g][tid & 31]));
+    }
+#pragma unroll
+    for (int k = 0; k < LA_GROUP; ++k)
+      if (k < mine) {
+        part[(s0 + k) * per] = v;
+        v = step(v, k);
+      }
   }
-  if (in) p.s_out[at] = s;
+  if (grp == 0 && in) p.s_out[at] = s;
 }
 
 struct LaPlan {
   bool chunks;
   int64_t seg, nseg, pad;
   int waves, slice;  // of values: waves of 32 columns; columns of a step workgroup
-  size_t part;
+  size_t part, flags;  // bytes of scratch
 };
 
 LaPlan la_plan(int32_t dt, int64_t n, int64_t l, int64_t kv_heads, int64_t dk, int64_t dv) {
@@ -502,7 +603,7 @@ LaPlan la_plan(int32_t dt, int64_t n, int64_t l, int64_t kv_heads, int64_t dk, i
     while (g.slice > 32 && nk * cdiv(dv, g.slice) < 2 * device_cus()) g.slice /= 2;
     return g;
   }
-  const int64_t kt = dt == DT_BF16 && dk <= 64 ? 64 : 32, chunks = cdiv(l, kt);
+  const int64_t kt = dt == DT_BF16 && dk <= 32 ? 64 : 32, chunks = cdiv(l, kt);
   g.chunks = true;
   g.waves = (int)cdiv(dv, 32);
   g.pad = chunks * kt - l;
@@ -510,6 +611,7 @@ LaPlan la_plan(int32_t dt, int64_t n, int64_t l, int64_t kv_heads, int64_t dk, i
   g.seg = cdiv(chunks, std::max<int64_t>(std::min(want, cdiv(chunks, 2)), 1)) * kt;
   g.nseg = cdiv(chunks * kt, g.seg);
   g.part = (size_t)(nk * g.nseg) * g.waves * cdiv(dk, 32) * 4096;
+  g.flags = (size_t)(nk * g.nseg) * g.waves * 4;
   return g;
 }
 
@@ -522,7 +624,7 @@ void la_launch(const LinP& k, hipStream_t st) {
   const dim3 grid((unsigned)(8 * cdiv(k.nk * k.nseg, 8)));
   constexpr int DB = DK / 32;
   hipLaunchKernelGGL((la_chunk_kernel<DT, DK, W, false>), grid, dim3(64 * W), 0, st, k);
-  hipLaunchKernelGGL((la_carry_kernel<8>), dim3((unsigned)cdiv(k.nk * W * DB * 1024, LA_T)), dim3(LA_T), 0, st, k, W, DB);
+  hipLaunchKernelGGL(la_carry_kernel, dim3((unsigned)(k.nk * W * DB * 32)), dim3(LA_T), 0, st, k, W, DB);
   hipLaunchKernelGGL((la_chunk_kernel<DT, DK, W, true>), grid, dim3(64 * W), 0, st, k);
 }
 
@@ -567,7 +669,8 @@ extern "C" size_t clarus_hip_linear_attention_workspace(int32_t dtype, int64_t n
   if (n <= 0 || l <= 0 || heads <= 0 || kv_heads <= 0 || heads % kv_heads || dk <= 0 || dk > 128 || dv <= 0 || dv > 128 ||
       !la_fits(n, l, heads, kv_heads))
     return 0;
-  return la_plan(dtype, n, l, kv_heads, dk, dv).part;
+  const LaPlan g = la_plan(dtype, n, l, kv_heads, dk, dv);
+  return g.part + g.flags;
 }
 
 extern "C" int clarus_hip_linear_attention(const ClarusLinearArgs* a, void* scratch, size_t scratch_bytes, void* stream) {
@@ -588,17 +691,18 @@ extern "C" int clarus_hip_linear_attention(const ClarusLinearArgs* a, void* scra
                  "linear_attention: 16-byte aligned rows");
   CLARUS_REQUIRE(a->ldq >= 0 && a->ldk >= 0 && a->ldv >= 0 && a->q_bstride >= 0 && a->k_bstride >= 0 && a->v_bstride >= 0,
                  "linear_attention: strides");
-  CLARUS_REQUIRE(a->ldk < (1 << 24) && a->ldv < (1 << 24), "linear_attention: rows of k and v less than 2^24 elements apart");
+  CLARUS_REQUIRE(a->ldq < (1 << 24) && a->ldk < (1 << 24) && a->ldv < (1 << 24), "linear_attention: rows less than 2^24 elements apart");
   CLARUS_REQUIRE(aligned(a->state_in, 16) && aligned(a->state_out, 16) && aligned(a->log_decay, 4), "linear_attention: aligned states");
   CLARUS_REQUIRE(la_fits(a->n, a->l, a->heads, a->kv_heads), "linear_attention: too large");
   const LaPlan g = la_plan(a->dtype, a->n, a->l, a->kv_heads, a->dk, a->dv);
-  CLARUS_REQUIRE(!g.chunks || (a->n * a->kv_heads * g.nseg < (1 << 23) && a->n * a->kv_heads * g.waves * cdiv(a->dk, 32) * 4 < (1 << 23)),
+  CLARUS_REQUIRE(!g.chunks || (a->n * a->kv_heads * g.nseg < (1 << 23) && a->n * a->kv_heads * g.waves * cdiv(a->dk, 32) < (1 << 18)),
                  "linear_attention: too large");
-  CLARUS_REQUIRE(g.part == 0 || (scratch && aligned(scratch, 16) && scratch_bytes >= g.part),
-                 "linear_attention: scratch %zu < %zu bytes", scratch_bytes, g.part);
+  CLARUS_REQUIRE(g.part == 0 || (scratch && aligned(scratch, 16) && scratch_bytes >= g.part + g.flags),
+                 "linear_attention: scratch %zu < %zu bytes", scratch_bytes, g.part + g.flags);
   LinP k{};
   k.q = a->q; k.k = a->k; k.v = a->v; k.out = a->out;
   k.s_in = a->state_in; k.s_out = a->state_out; k.decay = a->log_decay; k.part = (float*)scratch;
+  k.careful = g.part ? (int*)((char*)scratch + g.part) : nullptr;
   k.qbs = a->q_bstride; k.ldq = a->ldq; k.kbs = a->k_bstride; k.ldk = a->ldk; k.vbs = a->v_bstride; k.ldv = a->ldv;
   k.l = a->l; k.nk = a->n * a->kv_heads; k.nseg = g.nseg; k.seg = g.seg; k.pad = g.pad;
   k.rep = (int)(a->heads / a->kv_heads); k.kv_heads = (int)a->kv_heads; k.dk = (int)a->dk; k.dv = (int)a->dv;

@@ -1221,8 +1221,8 @@ class HipOps(Backend):
         log_decay [kv_heads], at most 0; scale 1 / sqrt(dk) by default. state [N, kv_heads, dk, dv] fp32: S before the first
         token (None: zeros), so that a sequence can go on where an earlier call ended, piece by piece or token by
         token. Returns (out [N, ..., heads * dv], the state behind the last token); state_out: a tensor to write the
-        state to, which may be `state` itself. fp32 states and sums; with bf16, products q . k within 64 tokens are rounded
-        to bf16."""
+        state to, which may be `state` itself. fp32 states and sums; with bf16, products q . k within 32 or 64 tokens are rounded
+        to bf16. A value that is not finite leaves the outputs before it as they are."""
         kv_heads = heads if kv_heads is None else kv_heads
         if not (isinstance(heads, int) and isinstance(kv_heads, int)):  # before the plans, whose keys 4.0 and 4 share
             raise Unsupported(f"linear_attention: heads and kv_heads integers, got {heads!r} {kv_heads!r}")
@@ -1274,10 +1274,12 @@ class HipOps(Backend):
         if n * l == 0:
             return odt, shape, sshape, None, 0
         at, es = [_rows(t) for t in (q, k, v)], q.element_size()
-        if None in at or any(s * es % 16 for t in at for s in t[1:]) or max(at[1][1], at[2][1]) >= 1 << 24:
-            raise Unsupported("linear_attention: unit channel stride, one row stride (k and v: below 2^24), 16-byte aligned rows")
+        if None in at or any(s * es % 16 for t in at for s in t[1:]) or max(t[1] for t in at) >= 1 << 24:
+            raise Unsupported("linear_attention: unit channel stride, one row stride below 2^24, 16-byte aligned rows")
         if n * kv_heads >= 1 << 20 or heads >= 1 << 20 or l >= 1 << 31:
             raise Unsupported("linear_attention: fewer than 2^20 (image, kv head) pairs and 2^31 tokens")
+        if l > 16 and n * kv_heads * -(-dk // 32) * -(-dv // 32) >= 1 << 18:
+            raise Unsupported("linear_attention: of more than 16 tokens, fewer than 2^18 32 x 32 pieces of states")
         args = _lib.LinearArgs(n=n, l=l, heads=heads, kv_heads=kv_heads, dk=dk, dv=dv, q_bstride=at[0][2], ldq=at[0][1],
                                k_bstride=at[1][2], ldk=at[1][1], v_bstride=at[2][2], ldv=at[2][1], dtype=_lib.dtype_code(q.dtype),
                                o_dtype=_lib.dtype_code(odt), scale=held)

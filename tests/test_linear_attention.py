@@ -98,6 +98,7 @@ def test_refusals():
         ((q.clone().requires_grad_(), k, k, g, 4, 2), {}), ((q, k, k, g.clone().requires_grad_(), 4, 2), {}),
         ((q, k, k, g, 4, 2), {"state": s.clone().requires_grad_()}),
         ((z(1, 1, 64).expand(1 << 20, 1, 64), z(1, 1, 32).expand(1 << 20, 1, 32), z(1, 1, 32).expand(1 << 20, 1, 32), g, 4, 2), {}),
+        ((z(1, 17, 128).expand(1 << 14, 17, 128), *[z(1, 17, 128).expand(1 << 14, 17, 128)] * 2, z(1), 1), {}),
         ((q, z(2 * 5 * (1 << 24)).as_strided((2, 5, 32), (0, 1 << 24, 1)), k, g, 4, 2), {}),
     ]
     for i, (args, kw) in enumerate(cases):
@@ -130,7 +131,7 @@ def test_c_entry_refuses_before_launch():
     for kw in (dict(q=None), dict(k=None), dict(v=None), dict(out=None), dict(log_decay=None), dict(state_out=None), dict(n=0), dict(l=0),
                dict(heads=0), dict(kv_heads=0), dict(kv_heads=3), dict(dk=0), dict(dk=12), dict(dk=136), dict(dv=4), dict(dv=136),
                dict(dtype=2), dict(o_dtype=-1), dict(scale=math.nan), dict(scale=math.inf), dict(q=(1 << 20) + 8), dict(ldq=130),
-               dict(ldk=-64), dict(v_bstride=2), dict(ldk=1 << 24), dict(ldv=1 << 24), dict(state_in=8), dict(state_out=8), dict(log_decay=2),
+               dict(ldk=-64), dict(v_bstride=2), dict(ldq=1 << 24), dict(ldk=1 << 24), dict(ldv=1 << 24), dict(n=1 << 18, kv_heads=1), dict(state_in=8), dict(state_out=8), dict(log_decay=2),
                dict(n=1 << 19), dict(n=1 << 62), dict(n=1 << 60, kv_heads=16, heads=16), dict(heads=1 << 62), dict(l=1 << 31),
                dict(scratch=None), dict(size=16), dict(scratch=8)):
         assert call(**kw) == _lib.EINVAL, kw
@@ -246,6 +247,30 @@ def test_what_is_not_finite_stays_behind(dt, hips, gpu_device):
     got, last = hips[dt].linear_attention(q, kb, v, g, heads, state=s)
     assert torch.equal(got[..., :d], want[..., :d]) and torch.equal(got[:, :90], want[:, :90]) and torch.equal(last[:, 0], wlast[:, 0])
     assert not torch.isfinite(got[0, 90:, d:]).any()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("d", [32, 64, 104, 128])
+def test_a_value_that_is_not_finite_stays_behind_its_token(d, dt, hips, gpu_device):
+    """No output before it sees it, also in the chunk that holds it; from it on that column's are not finite."""
+    heads, kv_heads, l = 4, 2, 333
+    q, k, v, s = inputs(1, l, heads, kv_heads, d, d, dt, gpu_device)
+    g = torch.tensor([-1 / 16, 0.0], device=gpu_device)
+    want, wlast = hips[dt].linear_attention(q, k, v, g, heads, kv_heads, state=s)
+    for token, column, value in ((0, 3, math.nan), (200, d - 1, math.inf), (331, 17, -math.inf), (332, 0, math.nan), (301, d + 5, math.inf)):
+        vb = v.clone()
+        vb[0, token, column] = value
+        got, last = hips[dt].linear_attention(q, k, vb, g, heads, kv_heads, state=s)
+        h, c = divmod(column, d)
+        hit = torch.zeros(l, heads, d, dtype=torch.bool, device=gpu_device)
+        hit[token:, 2 * h:2 * h + 2, c] = True
+        assert torch.equal(torch.isfinite(got).view(l, heads, d), ~hit), (token, column, value)
+        assert torch.equal(got.view(l, heads, d)[~hit], want.view(l, heads, d)[~hit]), (token, column, value)
+        other = torch.ones(kv_heads, d, dtype=torch.bool, device=gpu_device)
+        other[h, c] = False
+        assert torch.equal(torch.isfinite(last[0]), other[:, None].expand(kv_heads, d, d)), (token, column, value)
+        assert torch.equal(last[0].transpose(1, 2)[other], wlast[0].transpose(1, 2)[other])
 
 
 @pytest.mark.gpu
