@@ -5,7 +5,7 @@
 //
 //   sp_means_kernel   the means of blocks of keys, or of groups of queries
 //   sp_pick_kernel    up to 1024 blocks: scores and choice, as bits, 64 blocks a word
-//   sp_score_kernel   more blocks: scores of a slab of rows (image, head, group), 64 bits
+//   sp_score_kernel   more blocks: scores of a slab of rows, 64 bits
 //   sp_choose_kernel  a row's choice from them
 //   sp_kernel         the attention: 32 rows per wave as in cross_attention.hip (a row is a query and one of the heads that
 //                     share a kv head); a workgroup takes the blocks that any of its rows has chosen, one after another
@@ -32,8 +32,9 @@ struct SparseP {
   const void* asks;       // rows of queries, or of their groups' means (fp32)
   int64_t abs, lda;
   double* score;          // of a slab, [row][nb]
-  int64_t nw, nb, groups, first;  // first: the slab's first row (image, head, group)
-  int64_t slab;           // rows of this slab
+  int64_t nw, nb, groups, first;  // first: the slab's first tile of rows
+  int64_t tiles;          // tiles of an image and kv head
+  int tile;               // rows of one
   int block, group, top, heads, ask_dt;
 };
 
@@ -78,51 +79,53 @@ __global__ void __launch_bounds__(SP_T) sp_means_kernel(const unsigned char* x, 
 }
 
 // ---------------------------------------------------------------- scores
+// The rows (group, head) of an image and kv head share its means. They are taken in tiles of at most SP_TILE, and rows of
+// a tile times 64 blocks are a workgroup's; waves without a row leave the products to the others. (8 images' token of 16 heads
+// and 4 kv heads of 128 against 2049 blocks: 1400 us with tiles of the heads in order, each with means of its own, 41-56 now)
 __global__ void __launch_bounds__(SP_T) sp_score_kernel(const SparseP p) {
   constexpr int KC = 32;  // columns at a time
   __shared__ float sa[SP_TILE][KC + 1], sm[SP_TILE][KC + 1];
   const int tid = threadIdx.x, tx = tid & 15, ty = tid >> 4, d = p.x.d;
-  const int64_t row0 = (int64_t)blockIdx.x * SP_TILE, b0 = (int64_t)blockIdx.y * SP_TILE;
+  const int64_t tile = p.first + blockIdx.x, nk = tile / p.tiles, row0 = (tile - nk * p.tiles) * p.tile, b0 = (int64_t)blockIdx.y * SP_TILE;
+  const int64_t n = nk / p.x.kv_heads, kvh = nk - n * p.x.kv_heads, rows = p.groups * p.x.rep;
+  const int all = (int)(rows - row0 < p.tile ? rows - row0 : p.tile);
   double acc[4][4];
 #pragma unroll
   for (int i = 0; i < 4; ++i)
 #pragma unroll
     for (int j = 0; j < 4; ++j) acc[i][j] = 0.0;
-  // rows of one workgroup may be of several heads, each with means of its own: one head after another
-  const int64_t all = p.slab - row0 < SP_TILE ? p.slab - row0 : SP_TILE;
-  for (int64_t i0 = 0; i0 < all;) {
-    const int64_t nh = (p.first + row0 + i0) / p.groups, g0 = p.first + row0 + i0 - nh * p.groups;
-    const int64_t i1 = std::min(all, i0 + p.groups - g0);
-    const int64_t n = nh / p.heads, h = nh - n * p.heads;
-    const float* mp = p.means + (n * p.nb * p.x.kv_heads + h / p.x.rep) * d;
-    for (int c0 = 0; c0 < d; c0 += KC) {
-      __syncthreads();
-      for (int i = tid; i < SP_TILE * KC; i += SP_T) {
-        const int r = i / KC, c = i - r * KC;
-        const bool mine = r >= i0 && r < i1 && c0 + c < d;
-        sa[r][c] = mine ? load1(p.asks, p.ask_dt, n * p.abs + (g0 + r - i0) * p.lda + h * d + c0 + c) : 0.f;
-        sm[r][c] = b0 + r < p.nb && c0 + c < d ? mp[(b0 + r) * p.x.kv_heads * d + c0 + c] : 0.f;
+  const float* mp = p.means + (n * p.nb * p.x.kv_heads + kvh) * d;
+  for (int c0 = 0; c0 < d; c0 += KC) {
+    __syncthreads();
+#pragma unroll
+    for (int j = 0; j < SP_TILE * KC / SP_T; ++j) {
+      const int r = (tid + j * SP_T) / KC, c = tid % KC;
+      if (r < all) {
+        const unsigned g = (unsigned)(row0 + r) / (unsigned)p.x.rep;  // rows < 2^31
+        const int64_t h = kvh * p.x.rep + row0 + r - (int64_t)g * p.x.rep;
+        sa[r][c] = c0 + c < d ? load1(p.asks, p.ask_dt, n * p.abs + g * p.lda + h * d + c0 + c) : 0.f;
       }
-      __syncthreads();
-#pragma unroll 4
-      for (int c = 0; c < KC; ++c) {
-        double a[4], m[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) a[i] = sa[ty + 16 * i][c], m[i] = sm[tx + 16 * i][c];
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-          if (ty + 16 * i >= i0 && ty + 16 * i < i1)
-#pragma unroll
-            for (int j = 0; j < 4; ++j) acc[i][j] = fma(a[i], m[j], acc[i][j]);
-      }
+      sm[r][c] = b0 + r < p.nb && c0 + c < d ? mp[(b0 + r) * p.x.kv_heads * d + c0 + c] : 0.f;
     }
-    i0 = i1;
+    __syncthreads();
+#pragma unroll 4
+    for (int c = 0; c < KC; ++c) {
+      double a[4], m[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) a[i] = sa[ty + 16 * i][c], m[i] = sm[tx + 16 * i][c];
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (ty + 16 * i < all)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) acc[i][j] = fma(a[i], m[j], acc[i][j]);
+    }
   }
 #pragma unroll
   for (int i = 0; i < 4; ++i)
 #pragma unroll
     for (int j = 0; j < 4; ++j)
-      if (ty + 16 * i < all && b0 + tx + 16 * j < p.nb) p.score[(row0 + ty + 16 * i) * p.nb + b0 + tx + 16 * j] = acc[i][j];
+      if (ty + 16 * i < all && b0 + tx + 16 * j < p.nb)
+        p.score[((int64_t)blockIdx.x * p.tile + ty + 16 * i) * p.nb + b0 + tx + 16 * j] = acc[i][j];
 }
 
 // order of scores as whole numbers; 0: none (NaN, -inf)
@@ -132,48 +135,87 @@ __device__ __forceinline__ uint64_t sp_key(double v) {
   return u >> 63 ? ~u : u | 1ull << 63;
 }
 
-// a workgroup per row: the top-th largest score found byte by byte from the highest, then the bits
+// A workgroup per row. The largest threshold that leaves `top` scores is halved towards by counts, and found as soon as one
+// leaves just `top`. K: scores that a thread holds in registers (0: more, read again for each count). 32768 rows of 2048 blocks:
+// 55 us; byte by byte from the highest with counters in LDS 417, and a token's 16 rows of 4097 blocks 106 instead of 15
+template <int K>
 __global__ void __launch_bounds__(SP_T) sp_choose_kernel(const SparseP p) {
-  __shared__ int hist[256], at[2], ties[SP_T / 64];
+  constexpr int W = SP_T / 64;
+  __shared__ int part[2][W];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int64_t tile = p.first + blockIdx.x / p.tile, nk = tile / p.tiles;
+  const int64_t row = (tile - nk * p.tiles) * p.tile + blockIdx.x % p.tile;
+  if (row >= p.groups * p.x.rep) return;
+  const int64_t n = nk / p.x.kv_heads, g = row / p.x.rep, h = (nk - n * p.x.kv_heads) * p.x.rep + row - g * p.x.rep;
   const double* s = p.score + (int64_t)blockIdx.x * p.nb;
-  uint64_t* to = p.chosen + (p.first + blockIdx.x) * p.nw;
-  uint64_t prefix = 0;
-  int left = p.top;  // of the top ones, those whose higher bytes are `prefix`
-  for (int shift = 56; shift >= 0; shift -= 8) {
-    __syncthreads();
-    hist[tid] = 0;
-    __syncthreads();
-    for (int64_t b = tid; b < p.nb; b += SP_T) {
-      const uint64_t k = sp_key(s[b]);
-      if (shift == 56 || k >> (shift + 8) == prefix) atomicAdd(&hist[k >> shift & 255], 1);
+  uint64_t* to = p.chosen + ((n * p.heads + h) * p.groups + g) * p.nw;
+  uint64_t key[K ? K : 1];
+  if constexpr (K != 0) {
+#pragma unroll
+    for (int i = 0; i < K; ++i) {
+      const int64_t b = i * SP_T + tid;
+      key[i] = sp_key(s[b < p.nb ? b : p.nb - 1]);
+      if (b >= p.nb) key[i] = 0;
     }
-    __syncthreads();
-    if (tid == 0) {
-      int i = 255, seen = 0;
-      while (i > 0 && seen + hist[i] < left) seen += hist[i--];
-      at[0] = i;
-      at[1] = left - seen;
-    }
-    __syncthreads();
-    prefix = prefix << 8 | (uint64_t)at[0];
-    left = at[1];
   }
-  // every score above prefix, and the first `left` equal to it
-  int before = 0;
-  for (int64_t b0 = 0; b0 < p.nb; b0 += SP_T) {
-    const int64_t b = b0 + tid;
-    const uint64_t k = b < p.nb ? sp_key(s[b]) : 0;
-    const uint64_t same = __ballot(k == prefix && k != 0);
+  int turn = 0;
+  auto total = [&](int mine) __attribute__((always_inline)) {  // of the waves
+    if (lane == 0) part[turn][wave] = mine;
     __syncthreads();
-    if (lane == 0) ties[wave] = __popcll(same);
-    __syncthreads();
-    int rank = before;
-    for (int w = 0; w < wave; ++w) rank += ties[w];
-    for (int w = 0; w < SP_T / 64; ++w) before += ties[w];
-    rank += __popcll(same & ((1ull << lane) - 1));
-    const uint64_t word = __ballot(k > prefix || (k == prefix && k != 0 && rank < left));
-    if (lane == 0 && b0 / 64 + wave < p.nw) to[b0 / 64 + wave] = word;
+    int c = 0;
+#pragma unroll
+    for (int w = 0; w < W; ++w) c += part[turn][w];
+    turn ^= 1;  // written again only behind the next barrier but one
+    return c;
+  };
+  auto count = [&](uint64_t t) __attribute__((always_inline)) {  // keys from t on
+    int c = 0;
+    if constexpr (K != 0) {
+#pragma unroll
+      for (int i = 0; i < K; ++i) c += __popcll(__ballot(key[i] >= t));
+    } else {
+      for (int64_t b = tid; b < p.nw * 64; b += SP_T) c += __popcll(__ballot(b < p.nb && sp_key(s[b < p.nb ? b : 0]) >= t));
+    }
+    return total(c);
+  };
+  // count(lo) >= top > count(hi), unless fewer have a score
+  uint64_t lo = 1, hi = 0xffffffffffffffffull;
+  int above = 0;  // count(hi)
+  bool just = count(lo) <= p.top;
+  while (!just && hi - lo > 1) {
+    const uint64_t mid = lo + (hi - lo) / 2;
+    const int c = count(mid);
+    if (c >= p.top) lo = mid;
+    else hi = mid, above = c;
+    just = c == p.top;
+  }
+  // the keys from lo on; or those above, and of the ones equal to lo the first
+  int left = p.top - above;
+  auto word = [&](uint64_t k, int64_t at) __attribute__((always_inline)) {
+    uint64_t w;
+    if (just) {
+      w = __ballot(k >= lo);
+    } else {
+      const uint64_t same = __ballot(k == lo);
+      int before = 0, sum = 0;
+      if (lane == 0) part[turn][wave] = __popcll(same);
+      __syncthreads();
+#pragma unroll
+      for (int i = 0; i < W; ++i) {
+        if (i < wave) before += part[turn][i];
+        sum += part[turn][i];
+      }
+      turn ^= 1;
+      w = __ballot(k > lo || (k == lo && before + (int)__popcll(same & ((1ull << lane) - 1)) < left));
+      left -= sum;
+    }
+    if (lane == 0 && at < p.nw) to[at] = w;
+  };
+  if constexpr (K != 0) {
+#pragma unroll
+    for (int i = 0; i < K; ++i) word(key[i], i * W + wave);
+  } else {
+    for (int64_t b0 = 0; b0 < p.nb; b0 += SP_T) word(b0 + tid < p.nb ? sp_key(s[b0 + tid]) : 0, b0 / 64 + wave);
   }
 }
 
@@ -666,8 +708,9 @@ int sp_pad(int64_t d) { return d <= 32 ? 32 : d <= 64 ? 64 : d <= 96 ? 96 : 128;
 int sp_waves(int32_t dt, int64_t rows, int64_t alike) { return rows <= 32 ? 1 : alike >= 128 ? 4 : dt == DT_BF16 ? 2 : 1; }
 
 struct SpPlan {
-  int64_t nb, nw, groups, nblk, slab;  // slab: rows of scores at a time
-  int splits, waves;
+  int64_t nb, nw, groups, nblk;
+  int64_t slab, tiles;  // tiles of rows whose scores are held at a time; of an image and kv head
+  int splits, waves, tile;  // tile: rows of one
   int pick_tiles, pick_waves;  // of 32 blocks per wave of sp_pick_kernel; 0: sp_score_kernel and sp_choose_kernel
   size_t means, asks, chosen, score, part;  // workspace bytes, each a multiple of 16
   size_t total() const { return means + asks + chosen + score + part; }
@@ -691,8 +734,10 @@ SpPlan sp_plan(int32_t dt, int64_t n, int64_t lq, int64_t lk, int64_t heads, int
     g.pick_waves = 1;
     while (g.pick_tiles * g.pick_waves < tiles) g.pick_waves *= 2;
   } else {
-    g.slab = std::min(asks, std::min<int64_t>(cdiv(SP_SLAB / 8, g.nb * SP_TILE), 1 << 16) * SP_TILE);
-    g.score = (size_t)cdiv(g.slab * g.nb, 2) * 16;
+    g.tile = (int)std::min<int64_t>(SP_TILE, g.groups * (heads / kv_heads));
+    g.tiles = cdiv(g.groups * (heads / kv_heads), g.tile);
+    g.slab = std::min(nk * g.tiles, std::min<int64_t>(cdiv(SP_SLAB / 8, g.nb * g.tile), 1 << 16));
+    g.score = (size_t)cdiv(g.slab * g.tile * g.nb, 2) * 16;
   }
   g.waves = sp_waves(dt, rows, group * (heads / kv_heads));
   g.nblk = cdiv(rows, 32 * g.waves);
@@ -853,15 +898,19 @@ extern "C" int clarus_hip_sparse_attention(const ClarusSparseArgs* a, void* scra
   k.chosen = a->chosen ? a->chosen : chosen;
   k.score = (double*)take(g.score);
   x.part = (float*)take(g.part);
-  const int64_t rows = a->n * a->heads * g.groups;
   if (g.pick_tiles) {
     if (a->d <= 64) sp_pick<64>(k, g, st);
     else sp_pick<128>(k, g, st);
   }
-  for (k.first = 0; !g.pick_tiles && k.first < rows; k.first += g.slab) {
-    k.slab = std::min(g.slab, rows - k.first);
-    hipLaunchKernelGGL(sp_score_kernel, dim3((unsigned)cdiv(k.slab, SP_TILE), (unsigned)cdiv(g.nb, SP_TILE)), dim3(SP_T), 0, st, k);
-    hipLaunchKernelGGL(sp_choose_kernel, dim3((unsigned)k.slab), dim3(SP_T), 0, st, k);
+  k.tile = g.tile; k.tiles = g.tiles;
+  for (k.first = 0; !g.pick_tiles && k.first < x.nk * g.tiles; k.first += g.slab) {
+    const unsigned tiles = (unsigned)std::min(g.slab, x.nk * g.tiles - k.first);
+    hipLaunchKernelGGL(sp_score_kernel, dim3(tiles, (unsigned)cdiv(g.nb, SP_TILE)), dim3(SP_T), 0, st, k);
+    const dim3 rows(tiles * (unsigned)g.tile);
+    if (g.nb <= 8 * SP_T) hipLaunchKernelGGL(sp_choose_kernel<8>, rows, dim3(SP_T), 0, st, k);
+    else if (g.nb <= 16 * SP_T) hipLaunchKernelGGL(sp_choose_kernel<16>, rows, dim3(SP_T), 0, st, k);
+    else if (g.nb <= 32 * SP_T) hipLaunchKernelGGL(sp_choose_kernel<32>, rows, dim3(SP_T), 0, st, k);
+    else hipLaunchKernelGGL(sp_choose_kernel<0>, rows, dim3(SP_T), 0, st, k);
   }
   if (const int rc = check_launch("sparse_attention")) return rc;
   note_kernel("sp_kernel d=%d waves=%d splits=%d", sp_pad(a->d), g.waves, g.splits);

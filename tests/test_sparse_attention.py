@@ -241,6 +241,28 @@ def test_shapes(n, lq, lk, heads, kv_heads, d, top, block, group, dt, hips, gpu_
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("n,lq,nb,heads,kv_heads,group", [(1, 1, 1025, 4, 1, 1), (3, 1, 2100, 6, 2, 1), (1, 130, 4097, 2, 1, 2),
+                                                          (2, 3, 8200, 2, 2, 1), (1, 16000, 1100, 2, 1, 1)])
+def test_choices_of_many_blocks(n, lq, nb, heads, kv_heads, group, hips, gpu_device):
+    """Means kept by the caller, some of them copies, some NaN or infinite; the last shape's scores take two turns."""
+    g = torch.Generator().manual_seed(nb)
+    d, lk = 8, 64 * nb - 13
+    q = torch.randn(n, lq, heads * d, generator=g).to(gpu_device)
+    q[:, ::11] = 0
+    k, v = (torch.randn(n, lk, kv_heads * d, generator=g).to(torch.bfloat16).float().to(gpu_device) for _ in "kv")
+    means = hips[torch.float32].block_means(k)
+    means[:, 5::9] = means[:, 700:701]
+    means[:, 64:80] = math.nan
+    means[:, 130, 0] = -math.inf
+    for top in (1, 7, 1000, nb - 1, nb, 1 << 30):
+        want = choice64(q, means, heads, kv_heads, group, min(top, nb))
+        if lq > 1000 and top > 7:  # the attention over nearly all keys would take its time
+            continue
+        _, chosen = hips[torch.float32].sparse_attention(q, k, v, heads, top, kv_heads, group=group, means=means, return_blocks=True)
+        assert torch.equal(chosen, want), top
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("dt", [torch.bfloat16, torch.float32])
 def test_equal_scores_go_to_the_lowest_index(dt, hips, gpu_device):
     """Blocks that are copies of each other, queries of zeros, keys of zeros, scores of both signs of zero."""
