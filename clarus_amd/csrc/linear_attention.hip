@@ -19,6 +19,11 @@
 // (2^-24 of them left out) where a segment's sum for the state is made, in two (2^-16) where only outputs follow, S in two
 // as an operand, and the weights q . k within a chunk are rounded once to bf16 (2^-8 of each, of independent
 // signs: about as much as the output's own rounding). fp32: every product on fp32 MFMAs.
+//
+// What bounds it: a token, memory (64 states of 16 heads of 128 x 128: 28.7 us, 4.7 TB/s). Chunks: K and V read twice, and a
+// wave's chain from chunk to chunk; 57600 tokens, 8 heads of 64 x 64, bf16: 34.6 us for the segments' sums, 9.1 for the chain
+// of segments, 66 for the outputs (236 MB in all: 46 us at a large copy's rate); 2 x 5003 of 48 x 96, 8 heads on 4, fp32: 14.2,
+// 9.9 and 50.8, of which the fp32 MFMAs alone are some 31 where two of the 1272 waves share a SIMD.
 #include <algorithm>
 #include <math.h>
 
@@ -523,18 +528,21 @@ __global__ void __launch_bounds__(64 * W, 2) la_chunk_kernel(const LinP p) {
   la_chunks<DT, DK, W, OUT, false>(p, n, h, seg, tiles);
 }
 
-// In place of what each segment adds the state that it starts with; the state behind the last. A workgroup takes 32 elements
-// (in the accumulators' order) and 8 x LA_GROUP segments at a time: a thread has LA_GROUP of them of one element in registers,
-// and the groups are chained through LDS (57600 tokens in 128 segments, 8 heads of 64 x 64: 15.0 us with a thread per element
-// and chain, the next 8 segments in flight)
-constexpr int LA_GROUP = 16, LA_GROUPS = LA_T / 32;
+// In place of what each segment adds the state that it starts with; the state behind the last. A workgroup takes LA_T / G elements
+// (in the accumulators' order) and G x N segments at a time: a thread has N of them of one element in registers,
+// and the G groups are chained through LDS (57600 tokens in 120 segments, 8 heads of 64 x 64: 9.1 us with G = 8, 15.0 with a
+// thread per element and chain, the next 8 segments in flight). As few as there are segments for (1024 states of
+// 128 x 128, one segment: 88 us with G = N = 1, 235 with N = 16, 1542 with G = 8 too)
+constexpr int LA_GROUP = 16, LA_MOST = 8;
 
+template <int G, int N>
 __global__ void __launch_bounds__(LA_T) la_carry_kernel(const LinP p, int waves, int db) {
-  __shared__ float sums[LA_GROUPS][32];
-  __shared__ Factor facts[LA_GROUPS + 3];  // of the groups; of the first segment, one between, the last
+  constexpr int E = LA_T / G;
+  __shared__ float sums[G][E];
+  __shared__ Factor facts[G + 3];  // of the groups; of the first segment, one between, the last
   const unsigned per = waves * db * 16 * 64;  // elements of a state, padded
-  const int tid = threadIdx.x, grp = tid >> 5;
-  const unsigned nk = blockIdx.x / (per / 32), e = (blockIdx.x - nk * (per / 32)) * 32 + (tid & 31), h = nk % (unsigned)p.kv_heads;
+  const int tid = threadIdx.x, grp = tid / E;
+  const unsigned nk = blockIdx.x / (per / E), e = (blockIdx.x - nk * (per / E)) * E + tid % E, h = nk % (unsigned)p.kv_heads;
   const int lane = e & 63, reg = (e >> 6) % (unsigned)(db * 16), wave = e / (unsigned)(db * 16 * 64), j = reg & 15;
   const int r = 32 * (reg >> 4) + 8 * (j >> 2) + 4 * (lane >> 5) + (j & 3), c = 32 * wave + (lane & 31);
   const bool in = r < p.dk && c < p.dv;
@@ -546,40 +554,40 @@ __global__ void __launch_bounds__(LA_T) la_carry_kernel(const LinP p, int waves,
   float* part = p.part + (int64_t)nk * p.nseg * per + e;
   float s = p.s_in && in ? p.s_in[at] : 0.f;
 #pragma unroll 1
-  for (int64_t r0 = 0; r0 < p.nseg; r0 += LA_GROUP * LA_GROUPS) {
-    const int64_t s0 = r0 + grp * LA_GROUP;
-    const int mine = (int)(p.nseg - s0 < 0 ? 0 : p.nseg - s0 < LA_GROUP ? p.nseg - s0 : LA_GROUP);
-    float add[LA_GROUP];
+  for (int64_t r0 = 0; r0 < p.nseg; r0 += N * G) {
+    const int64_t s0 = r0 + grp * N;
+    const int mine = (int)(p.nseg - s0 < 0 ? 0 : p.nseg - s0 < N ? p.nseg - s0 : N);
+    float add[N];
 #pragma unroll
-    for (int k = 0; k < LA_GROUP; ++k) add[k] = part[(s0 + k < p.nseg ? s0 + k : p.nseg - 1) * per];
+    for (int k = 0; k < N; ++k) add[k] = part[(s0 + k < p.nseg ? s0 + k : p.nseg - 1) * per];
     __syncthreads();  // the groups before have been read
-    if (tid < LA_GROUPS + 3) {
-      const int64_t a = tid < LA_GROUPS ? r0 + tid * LA_GROUP : tid == LA_GROUPS ? 0 : tid == LA_GROUPS + 1 ? 1 : p.nseg - 1;
-      const int64_t b = tid < LA_GROUPS ? a + LA_GROUP : a + 1;
-      facts[tid] = la_factor(p, h, tid == LA_GROUPS + 1 ? p.seg : token(b) - token(a));
+    if (tid < G + 3) {
+      const int64_t a = tid < G ? r0 + tid * N : tid == G ? 0 : tid == G + 1 ? 1 : p.nseg - 1;
+      const int64_t b = tid < G ? a + N : a + 1;
+      facts[tid] = la_factor(p, h, tid == G + 1 ? p.seg : token(b) - token(a));
     }
     __syncthreads();
     // the first and the last segment's may differ from the others'
-    const float fh = facts[LA_GROUPS + 1].hi, fl = facts[LA_GROUPS + 1].lo;
-    const float h0 = s0 == 0 ? facts[LA_GROUPS].hi : fh, l0 = s0 == 0 ? facts[LA_GROUPS].lo : fl;
-    const int end = p.nseg - 1 - s0 < LA_GROUP && p.nseg - 1 > 0 ? (int)(p.nseg - 1 - s0) : -1;
-    const float h1 = facts[LA_GROUPS + 2].hi, l1 = facts[LA_GROUPS + 2].lo;
+    const float fh = facts[G + 1].hi, fl = facts[G + 1].lo;
+    const float h0 = s0 == 0 ? facts[G].hi : fh, l0 = s0 == 0 ? facts[G].lo : fl;
+    const int end = p.nseg - 1 - s0 < N && p.nseg - 1 > 0 ? (int)(p.nseg - 1 - s0) : -1;
+    const float h1 = facts[G + 2].hi, l1 = facts[G + 2].lo;
     auto step = [&](float v, int k) __attribute__((always_inline)) {
       const float hi = k == end ? h1 : k == 0 ? h0 : fh, lo = k == end ? l1 : k == 0 ? l0 : fl;
       return fmaf(v, hi, fmaf(v, lo, add[k]));
     };
     float v = 0.f;
 #pragma unroll
-    for (int k = 0; k < LA_GROUP; ++k) v = k < mine ? step(v, k) : v;
-    sums[grp][tid & 31] = v;
+    for (int k = 0; k < N; ++k) v = k < mine ? step(v, k) : v;
+    sums[grp][tid % E] = v;
     __syncthreads();
 #pragma unroll
-    for (int g = 0; g < LA_GROUPS; ++g) {
+    for (int g = 0; g < G; ++g) {
       if (g == grp) v = s;  // what this group starts with
-      s = fmaf(s, facts[g].hi, fmaf(s, facts[g].lo, sums[g][tid & 31]));
+      s = fmaf(s, facts[g].hi, fmaf(s, facts[g].lo, sums[g][tid % E]));
     }
 #pragma unroll
-    for (int k = 0; k < LA_GROUP; ++k)
+    for (int k = 0; k < N; ++k)
       if (k < mine) {
         part[(s0 + k) * per] = v;
         v = step(v, k);
@@ -595,10 +603,20 @@ struct LaPlan {
   size_t part, flags;  // bytes of scratch
 };
 
-LaPlan la_plan(int32_t dt, int64_t n, int64_t l, int64_t kv_heads, int64_t dk, int64_t dv) {
+// Token by token a step of the state and one of each head's output, in chunks three launches, whatever the length up to a
+// chunk. us token by token / in chunks, bf16: 8 states of 64 x 64 8.7 / 15 (4 tokens), 14 / 15 (8), 25 / 15 (16); 32 with 4
+// heads each 20 / 19 (4), 38 / 19 (8), 256 39 / 24 (8); 32 in fp32 14 / 20 (8), 24 / 19 (16). Where moving the states is
+// most of the time: 1024 of 128 x 128 60 / 138 (8), 96 / 141 (16), 170 / 143 (32). States that are too many for a grid of
+// pieces stay with the first.
+bool la_by_token(int64_t nk, int64_t l, int64_t rep, int64_t dk, int64_t dv) {
+  if (nk * cdiv(dv, 32) * cdiv(dk, 32) >= 1 << 18) return true;
+  return l * (1 + rep) <= (nk * dk * dv >= 1 << 22 ? 40 : 20);
+}
+
+LaPlan la_plan(int32_t dt, int64_t n, int64_t l, int64_t heads, int64_t kv_heads, int64_t dk, int64_t dv) {
   LaPlan g{};
   const int64_t nk = n * kv_heads;
-  if (l <= 16) {
+  if (la_by_token(nk, l, heads / kv_heads, dk, dv)) {
     g.slice = dv <= 32 ? 32 : dv <= 64 ? 64 : 128;
     while (g.slice > 32 && nk * cdiv(dv, g.slice) < 2 * device_cus()) g.slice /= 2;
     return g;
@@ -607,7 +625,8 @@ LaPlan la_plan(int32_t dt, int64_t n, int64_t l, int64_t kv_heads, int64_t dk, i
   g.chunks = true;
   g.waves = (int)cdiv(dv, 32);
   g.pad = chunks * kt - l;
-  const int64_t want = cdiv(8LL * device_cus(), nk * g.waves);  // segments for two waves per SIMD
+  // as many segments as run at once, two waves per SIMD: the slowest of two rounds would be the time
+  const int64_t want = device_cus() * (8 / g.waves) / nk;
   g.seg = cdiv(chunks, std::max<int64_t>(std::min(want, cdiv(chunks, 2)), 1)) * kt;
   g.nseg = cdiv(chunks * kt, g.seg);
   g.part = (size_t)(nk * g.nseg) * g.waves * cdiv(dk, 32) * 4096;
@@ -624,7 +643,15 @@ void la_launch(const LinP& k, hipStream_t st) {
   const dim3 grid((unsigned)(8 * cdiv(k.nk * k.nseg, 8)));
   constexpr int DB = DK / 32;
   hipLaunchKernelGGL((la_chunk_kernel<DT, DK, W, false>), grid, dim3(64 * W), 0, st, k);
-  hipLaunchKernelGGL(la_carry_kernel, dim3((unsigned)(k.nk * W * DB * 32)), dim3(LA_T), 0, st, k, W, DB);
+  const unsigned states = (unsigned)(k.nk * W * DB * 4);  // in pieces of LA_T elements
+#define CLARUS_CARRY(G, N) hipLaunchKernelGGL((la_carry_kernel<G, N>), dim3(G * states), dim3(LA_T), 0, st, k, W, DB)
+  if (k.nseg == 1) CLARUS_CARRY(1, 1);
+  else if (k.nseg <= 4) CLARUS_CARRY(1, 4);
+  else if (k.nseg <= LA_GROUP) CLARUS_CARRY(1, LA_GROUP);
+  else if (k.nseg <= 2 * LA_GROUP) CLARUS_CARRY(2, LA_GROUP);
+  else if (k.nseg <= 4 * LA_GROUP) CLARUS_CARRY(4, LA_GROUP);
+  else CLARUS_CARRY(LA_MOST, LA_GROUP);
+#undef CLARUS_CARRY
   hipLaunchKernelGGL((la_chunk_kernel<DT, DK, W, true>), grid, dim3(64 * W), 0, st, k);
 }
 
@@ -669,7 +696,7 @@ extern "C" size_t clarus_hip_linear_attention_workspace(int32_t dtype, int64_t n
   if (n <= 0 || l <= 0 || heads <= 0 || kv_heads <= 0 || heads % kv_heads || dk <= 0 || dk > 128 || dv <= 0 || dv > 128 ||
       !la_fits(n, l, heads, kv_heads))
     return 0;
-  const LaPlan g = la_plan(dtype, n, l, kv_heads, dk, dv);
+  const LaPlan g = la_plan(dtype, n, l, heads, kv_heads, dk, dv);
   return g.part + g.flags;
 }
 
@@ -694,9 +721,7 @@ extern "C" int clarus_hip_linear_attention(const ClarusLinearArgs* a, void* scra
   CLARUS_REQUIRE(a->ldq < (1 << 24) && a->ldk < (1 << 24) && a->ldv < (1 << 24), "linear_attention: rows less than 2^24 elements apart");
   CLARUS_REQUIRE(aligned(a->state_in, 16) && aligned(a->state_out, 16) && aligned(a->log_decay, 4), "linear_attention: aligned states");
   CLARUS_REQUIRE(la_fits(a->n, a->l, a->heads, a->kv_heads), "linear_attention: too large");
-  const LaPlan g = la_plan(a->dtype, a->n, a->l, a->kv_heads, a->dk, a->dv);
-  CLARUS_REQUIRE(!g.chunks || (a->n * a->kv_heads * g.nseg < (1 << 23) && a->n * a->kv_heads * g.waves * cdiv(a->dk, 32) < (1 << 18)),
-                 "linear_attention: too large");
+  const LaPlan g = la_plan(a->dtype, a->n, a->l, a->heads, a->kv_heads, a->dk, a->dv);
   CLARUS_REQUIRE(g.part == 0 || (scratch && aligned(scratch, 16) && scratch_bytes >= g.part + g.flags),
                  "linear_attention: scratch %zu < %zu bytes", scratch_bytes, g.part + g.flags);
   LinP k{};

@@ -6,7 +6,8 @@
 // row (one head's V pairs, or V columns that stay), go over the tokens, four in flight. The turns pos * turn[j] and
 // their fraction are held in 64 bits (a position of a million is a million radians of the fastest pair, of which fp32
 // keeps one digit behind the point); the fraction is below 1/2 and goes through sincospi in 32.
-// What bounds it: memory, each element read and written once.
+// What bounds it: memory, each element read and written once. 57600 tokens of 1024 columns in bf16 55.9 us (4.2 TB/s; 45.8 at
+// the rate of a large copy), 36450 of 432 in fp32 28.3 (24.5); below some 1000 tokens the launch.
 #include <algorithm>
 
 #include "capi.hpp"

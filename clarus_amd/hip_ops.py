@@ -1278,8 +1278,6 @@ class HipOps(Backend):
             raise Unsupported("linear_attention: unit channel stride, one row stride below 2^24, 16-byte aligned rows")
         if n * kv_heads >= 1 << 20 or heads >= 1 << 20 or l >= 1 << 31:
             raise Unsupported("linear_attention: fewer than 2^20 (image, kv head) pairs and 2^31 tokens")
-        if l > 16 and n * kv_heads * -(-dk // 32) * -(-dv // 32) >= 1 << 18:
-            raise Unsupported("linear_attention: of more than 16 tokens, fewer than 2^18 32 x 32 pieces of states")
         args = _lib.LinearArgs(n=n, l=l, heads=heads, kv_heads=kv_heads, dk=dk, dv=dv, q_bstride=at[0][2], ldq=at[0][1],
                                k_bstride=at[1][2], ldk=at[1][1], v_bstride=at[2][2], ldv=at[2][1], dtype=_lib.dtype_code(q.dtype),
                                o_dtype=_lib.dtype_code(odt), scale=held)

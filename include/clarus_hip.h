@@ -584,8 +584,7 @@ int clarus_hip_add_norm(const ClarusAddNormArgs* args, void* stream);
  * rows, slices of wider rows, less than 2^24 elements apart; dk, dv multiples of 8, at most 128); out [n, l, heads * dv] contiguous. state_in
  * [n, kv_heads, dk, dv] fp32 or NULL for zeros; state_out the same, may be state_in itself; nothing else overlaps. log_decay
  * fp32 [kv_heads], at most 0 (0 keeps all, -inf nothing but the token). States, sums and factors in fp32; with bf16 the
- * products q . k of tokens up to 64 apart are rounded once to bf16. n * kv_heads < 2^20, l < 2^31; with l > 16 fewer than 2^18
- * 32 x 32 pieces of states. scratch holds clarus_hip_linear_attention_workspace(...) bytes (may be 0), 16-byte aligned. Deterministic. No counterpart in the reference
+ * products q . k of tokens up to 64 apart are rounded once to bf16. n * kv_heads < 2^20, l < 2^31. scratch holds clarus_hip_linear_attention_workspace(...) bytes (may be 0), 16-byte aligned. Deterministic. No counterpart in the reference
  * (its recurrence is selective_scan's).
  */
 typedef struct ClarusLinearArgs {

@@ -98,7 +98,6 @@ def test_refusals():
         ((q.clone().requires_grad_(), k, k, g, 4, 2), {}), ((q, k, k, g.clone().requires_grad_(), 4, 2), {}),
         ((q, k, k, g, 4, 2), {"state": s.clone().requires_grad_()}),
         ((z(1, 1, 64).expand(1 << 20, 1, 64), z(1, 1, 32).expand(1 << 20, 1, 32), z(1, 1, 32).expand(1 << 20, 1, 32), g, 4, 2), {}),
-        ((z(1, 17, 128).expand(1 << 14, 17, 128), *[z(1, 17, 128).expand(1 << 14, 17, 128)] * 2, z(1), 1), {}),
         ((q, z(2 * 5 * (1 << 24)).as_strided((2, 5, 32), (0, 1 << 24, 1)), k, g, 4, 2), {}),
     ]
     for i, (args, kw) in enumerate(cases):
@@ -131,7 +130,7 @@ def test_c_entry_refuses_before_launch():
     for kw in (dict(q=None), dict(k=None), dict(v=None), dict(out=None), dict(log_decay=None), dict(state_out=None), dict(n=0), dict(l=0),
                dict(heads=0), dict(kv_heads=0), dict(kv_heads=3), dict(dk=0), dict(dk=12), dict(dk=136), dict(dv=4), dict(dv=136),
                dict(dtype=2), dict(o_dtype=-1), dict(scale=math.nan), dict(scale=math.inf), dict(q=(1 << 20) + 8), dict(ldq=130),
-               dict(ldk=-64), dict(v_bstride=2), dict(ldq=1 << 24), dict(ldk=1 << 24), dict(ldv=1 << 24), dict(n=1 << 18, kv_heads=1), dict(state_in=8), dict(state_out=8), dict(log_decay=2),
+               dict(ldk=-64), dict(v_bstride=2), dict(ldq=1 << 24), dict(ldk=1 << 24), dict(ldv=1 << 24), dict(state_in=8), dict(state_out=8), dict(log_decay=2),
                dict(n=1 << 19), dict(n=1 << 62), dict(n=1 << 60, kv_heads=16, heads=16), dict(heads=1 << 62), dict(l=1 << 31),
                dict(scratch=None), dict(size=16), dict(scratch=8)):
         assert call(**kw) == _lib.EINVAL, kw
@@ -157,7 +156,8 @@ def hips(gpu_device):
 SHAPES = [(1, 1, 1, 1, 8, 8), (64, 1, 16, 8, 128, 128), (3, 2, 4, 4, 64, 64), (1, 5, 4, 2, 48, 96), (2, 16, 8, 2, 128, 40), (1, 17, 2, 2, 32, 32),
           (2, 31, 1, 1, 64, 8), (1, 32, 3, 3, 96, 64), (1, 33, 4, 4, 128, 128), (2, 63, 6, 2, 64, 64), (1, 64, 2, 1, 40, 72), (3, 65, 2, 2, 64, 96),
           (1, 127, 8, 8, 16, 128), (1, 128, 2, 2, 128, 32), (2, 129, 2, 2, 24, 24), (1, 300, 8, 8, 64, 64), (2, 501, 4, 1, 80, 112),
-          (1, 1537, 3, 3, 64, 64), (1, 2200, 1, 1, 128, 128), (5, 70, 8, 8, 56, 120)]
+          (1, 1537, 3, 3, 64, 64), (1, 2200, 1, 1, 128, 128), (5, 70, 8, 8, 56, 120), (9, 11, 2, 2, 32, 32), (64, 20, 16, 8, 128, 64), (128, 21, 8, 8, 128, 128),
+          (8200, 40, 8, 4, 24, 8), (34, 600, 8, 8, 32, 64), (1 << 16, 24, 4, 4, 8, 8)]
 
 
 @pytest.mark.gpu
