@@ -23,7 +23,7 @@
 // What bounds it: a token, memory (64 states of 16 heads of 128 x 128: 28.7 us, 4.7 TB/s). Chunks: K and V read twice, and a
 // wave's chain from chunk to chunk; 57600 tokens, 8 heads of 64 x 64, bf16: 34.6 us for the segments' sums, 9.1 for the chain
 // of segments, 66 for the outputs (236 MB in all: 46 us at a large copy's rate); 2 x 5003 of 48 x 96, 8 heads on 4, fp32: 14.2,
-// 9.9 and 50.8, of which the fp32 MFMAs alone are some 31 where two of the 1272 waves share a SIMD.
+// 6.8 and 50.8, of which the fp32 MFMAs alone are some 31 where two of the 1272 waves share a SIMD.
 #include <algorithm>
 #include <math.h>
 

@@ -11,8 +11,10 @@ Ops served: linear, down, up, intro, ending, conv3x3, channel_attention, linear_
 patch_filter, linear_patch_filter, patch_corr, ln_mul_linear (the GEMM family), plus dwconv
 (depthwise 3x3 + gates) and boxmean (the other ops of the NAFNet forward), selective_scan
 (EVSSM's state-space scan), attention_apply (MDTA attn . V), linear_ln_linear (a residual
-GEMM and the LayerNorm GEMM on its output), group_norm (with its activation) and cross_attention
-(positions over an encoder's states).
+GEMM and the LayerNorm GEMM on its output), group_norm (with its activation), cross_attention
+(positions over an encoder's states), and what a block over tokens runs between its linears: add_norm
+(residual, gate and norms), rotary (positions with several axes), linear_attention (with decay, chunks
+or single tokens), block_means and sparse_attention (over the blocks of keys that a score selects).
 
 Capture safety: kernels launch on torch's current stream, scratch comes from torch's
 allocator, weight re-layouts are computed once through `Backend.cached` (in the eager warm-up
