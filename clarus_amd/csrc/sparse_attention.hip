@@ -812,6 +812,8 @@ void sp_means(const void* x, int dt, int64_t xbs, int64_t ldx, const void* mask,
   const int64_t nb = cdiv(rows, size), oct = c / 8;
   int rg = 1;
   while (rg < 32 && rg < size && oct * rg * 2 <= SP_T) rg *= 2;
+  // few blocks: fewer columns and more rows at a time (one group of 14400 rows of 512: 95 us, 1180 with all columns at once)
+  while (rg < 64 && rg * 4 <= size && n * nb * cdiv(oct, SP_T / rg) < 2 * device_cus()) rg *= 2;
   const dim3 grid((unsigned)(n * nb), (unsigned)cdiv(oct, SP_T / rg));
   if (dt == DT_BF16)
     hipLaunchKernelGGL(sp_means_kernel<DT_BF16>, grid, dim3(SP_T), 0, st, (const unsigned char*)x, xbs, ldx, (const unsigned char*)mask, mbs, out,

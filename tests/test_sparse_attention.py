@@ -222,7 +222,7 @@ SHAPES = [  # n, lq, lk, heads, kv_heads, d, top, block, group
     (1, 1, 1, 1, 1, 8, 1, 64, 1), (2, 1, 300, 4, 4, 32, 2, 64, 1), (8, 1, 3001, 16, 4, 128, 5, 64, 1), (1, 5, 9000, 8, 2, 64, 7, 128, 1),
     (1, 300, 300, 2, 2, 64, 2, 64, 1), (2, 257, 700, 8, 2, 80, 3, 64, 64), (1, 130, 64, 3, 1, 64, 4, 64, 16), (1, 1000, 1000, 4, 4, 48, 4, 64, 100),
     (3, 97, 640, 1, 1, 112, 3, 128, 8), (1, 2000, 2500, 2, 2, 64, 6, 64, 256), (2, 33, 129, 6, 2, 24, 1, 64, 7), (1, 64, 4200, 4, 1, 96, 40, 64, 2),
-    (1, 300, 130, 1, 1, 16, 9, 64, 1000), (4, 3, 31, 32, 1, 128, 1, 64, 1), (1, 700, 5000, 2, 1, 40, 8, 256, 1), (1, 40, 70000, 2, 2, 32, 12, 64, 4)]
+    (1, 300, 130, 1, 1, 16, 9, 64, 1000), (4, 3, 31, 32, 1, 128, 1, 64, 1), (1, 700, 5000, 2, 1, 40, 8, 256, 1), (1, 40, 70000, 2, 2, 32, 12, 64, 4), (1, 3001, 3001, 2, 2, 64, 3, 1024, 5000)]
 
 
 @pytest.mark.gpu
