@@ -12,7 +12,7 @@
 //                     through LDS, and a wave those of its own rows; a row that has not chosen a block weighs it by 0
 //   xa_join_kernel    joins the parts of blocks split over workgroups, where rows are few
 //
-// What bounds it: 14400 queries of 8 heads of 64, each with 16 of 225 blocks, 373 us: in sp_kernel, where a wave's 32 rows
+// What bounds it: 14400 queries of 8 heads of 64, each with 16 of 225 blocks, 370 us: in sp_kernel, where a wave's 32 rows
 // have chosen 72 blocks between them and walk them all (under rocprof 292), and in sp_pick_kernel, the steps of the search beside fp32
 // MFMAs (109). 57600, 64 choosing together: 290, of which sp_kernel's softmax steps 242 (500 TFLOP/s). A token of 8
 // images over 30001 keys: 79, the latency of three launches and of the chain of blocks in each workgroup.
