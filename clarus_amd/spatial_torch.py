@@ -96,7 +96,9 @@ class TorchSpatialOps(Backend):
         in fp32 (False, True or "rms"), vectors [C] or [N, C]."""
         n, c = x.shape[0], x.shape[-1]
         affine = (gate, post_weight, post_bias, weight, bias)
-        if x.dim() < 2 or any(k not in (False, True, "rms") for k in (post, ln)) or (y is not None and y.shape != x.shape):
+        # a flag that only equals True (1, numpy's) would go past the test of the norm below
+        if (x.dim() < 2 or any(not isinstance(k, (bool, str)) or k not in (False, True, "rms") for k in (post, ln))
+                or (y is not None and y.shape != x.shape)):
             raise Unsupported(f"add_norm: x [N, ..., C], y of its shape, post and ln False, True or 'rms', got {post!r} {ln!r}")
         if any(t is not None and (tuple(t.shape) not in ((c,), (n, c)) or not t.is_floating_point()) for t in affine):
             raise Unsupported("add_norm: gate, weights and biases [C] or [N, C]")

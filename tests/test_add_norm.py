@@ -161,6 +161,20 @@ def test_plain_forms(post, ln):
         assert abs(got - want) <= 1e-4 * (abs(want) + 30), i
 
 
+def test_the_torch_form_refuses_flags_that_only_equal_true():
+    """What HipOps.add_norm hands on: 1, 1.0 and numpy's truth values are neither LayerNorm nor RMS (1 == True, but 1 is no True)."""
+    import numpy as np
+    from clarus_amd.spatial_torch import TorchSpatialOps
+    ops, h = TorchSpatialOps(torch.float32, torch.device("cpu")), cpu_hip()
+    x = rand(2, 5, 64)
+    for bad in (1, 0, 1.0, 0.0, np.True_, np.False_, None, "layer", torch.tensor(True)):
+        for kw in ({"ln": bad}, {"post": bad}):
+            for form in (h, ops):
+                with pytest.raises(Unsupported):
+                    form.add_norm(x, x, **kw)
+                    pytest.fail(f"{form.name} accepted {kw}")
+
+
 # ------------------------------------------------------------------ GPU
 @pytest.fixture(scope="module")
 def hips(gpu_device):
