@@ -228,11 +228,12 @@ __global__ void __launch_bounds__(SP_T) sp_choose_kernel(const SparseP p) {
 // A workgroup: W waves, 32 rows (groups and the heads that share a kv head) of one (image, kv head). A wave holds the scores of
 // NT tiles of 32 blocks in registers, from fp32 MFMAs (S^T = means asks^T: a lane holds a row's scores of 16 blocks of
 // each tile, its partner in lane ^ 32 the other 16). They are off by at most e = 2 (d + 8) 2^-24 |ask| |mean| (Cauchy-Schwarz over
-// the terms). A row's threshold is searched between its least and largest score, by counts; where the least score
+// the terms; the norms with what their squares may lose below 2^-126, SP_LOST, and products that small below 1e-35 in all). A row's threshold is searched between its least and largest score, by counts; where the least score
 // chosen and the largest left out are more than 2 e apart, 64 bits would choose the same. Where they are not, the blocks
 // within 2 e of the threshold are scored again in 64 bits by a wave, up to 64 of them; a row with more of them (equal blocks,
 // an ask of zeros), or with a norm that is not finite, is done by the whole workgroup, every block's rank counted.
 constexpr int SP_PICK = 1024;  // blocks, at most
+constexpr float SP_LOST = 0x1p-118f;  // of a sum of up to 128 squares, should each lose 2^-126
 
 template <int D, int NT, int W>
 __global__ void __launch_bounds__(64 * W, W > 8 ? 4 : 2) sp_pick_kernel(const SparseP p, unsigned row_tiles) {
@@ -357,7 +358,7 @@ __global__ void __launch_bounds__(64 * W, W > 8 ? 4 : 2) sp_pick_kernel(const Sp
     for (int w = 1; w < W; ++w) mm = fmaxf(mm, wide[w]);
   }
   valid = all_sum(hl == 0 ? valid : 0);
-  const float e = 2.f * (float)(d + 8) * 0x1p-24f * 1.01f * sqrtf(qq) * sqrtf(mm) + 1e-35f;
+  const float e = 2.f * (float)(d + 8) * 0x1p-24f * 1.01f * sqrtf(qq + SP_LOST) * sqrtf(mm + SP_LOST) + 1e-35f;
   const bool wild = !(qq < INFINITY && mm < INFINITY);  // products may leave fp32
   bool done = wild || valid <= p.top, exact = false;
   float thr = -3.402823466e38f;  // every block with a score

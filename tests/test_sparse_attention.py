@@ -298,6 +298,28 @@ def test_scores_that_fp32_does_not_tell_apart(hips, gpu_device):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("q_size,m_size", [(0, -80), (-80, 0), (-50, -50), (-120, 0), (0, -110), (-100, 60), (60, 60), (64, 0), (0, 70)])
+@pytest.mark.parametrize("nb", [50, 200])
+def test_choices_whatever_the_size_of_queries_and_means(nb, q_size, m_size, hips, gpu_device):
+    """The same near ties at sizes whose squares leave fp32: a power of two changes no choice of 64 bits."""
+    heads, d, lq = 1, 64, 120
+    g = torch.Generator().manual_seed(4)
+    base = torch.randn(1, 1, d, generator=g)
+    means = (base + 2.0 ** -20 * torch.randint(-3, 4, (1, nb, d), generator=g) * base.abs()).to(gpu_device)
+    q = torch.randn(1, lq, d, generator=g).to(gpu_device)
+    q = q - (q @ means[:, 0, :, None]) / (means[:, 0] ** 2).sum() * means[:, :1]
+    q[:, ::7] = torch.randn(1, 18, d, generator=g).to(gpu_device)  # and some that leave no doubt
+    # small sizes keep all digits: nothing below 2^-126
+    q = torch.where(q.abs() < 2.0 ** -4, torch.zeros_like(q), q) * 2.0 ** q_size
+    means = torch.where(means.abs() < 2.0 ** -4, torch.zeros_like(means), means) * 2.0 ** m_size
+    k = torch.randn(1, nb * 64, d, generator=g).to(gpu_device)
+    for top in (1, 9, nb - 3):
+        want = choice64(q, means, heads, heads, 1, top)
+        _, chosen = hips[torch.float32].sparse_attention(q, k, k, heads, top, means=means, scale=0.1 * 2.0 ** -max(q_size, 0), return_blocks=True)
+        assert torch.equal(chosen, want), f"{top}: {(chosen != want).any(-1).sum().item()} choices of {lq} differ"
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("dt", [torch.bfloat16, torch.float32])
 @pytest.mark.parametrize("lq,lk,group", [(70, 350, 1), (3, 3001, 1), (200, 900, 64)])
 def test_masked_keys_may_hold_anything(lq, lk, group, dt, hips, gpu_device):
