@@ -14,6 +14,7 @@ typedef __attribute__((ext_vector_type(4))) short s16x4;
 
 constexpr int XA_T = 256;    // threads of a join or bits workgroup
 constexpr float XA_FLOOR = -3e38f;  // running maximum before any key: exp2(-inf - XA_FLOOR) = 0, no inf - inf
+constexpr float XA_MOST = 3.402823466e38f;  // the largest finite fp32
 constexpr float XA_SLACK = 8.f;     // a running maximum may lag the scores' by this (log2)
 constexpr float XA_FAR = 8388608.f;  // 2^23: up to this size a running maximum is within a quarter of the product it rounds
 
@@ -187,9 +188,21 @@ __device__ __forceinline__ void xa_tile(const unsigned char* ks, const unsigned 
 #pragma unroll
   for (int b = 0; b < NB; ++b)
 #pragma unroll
-    for (int j = 0; j < 16; ++j) mx = fmaxf(mx, s[b][j]);
-  if (MASK == MASK_ROWS && !live) mx = -INFINITY;
-  if (__any(mx * c > m + XA_SLACK)) {
+    for (int j = 0; j < 16; ++j) mx = MASK == MASK_ROWS ? __builtin_elementwise_maximum(mx, s[b][j]) : fmaxf(mx, s[b][j]);
+  // of a row that is not live -inf as maximum makes every finite score a weight of 0; one that is not finite (the maximum
+  // of MASK_ROWS passes NaN on) is put to 0 first. 14400 queries that choose each for themselves: 385 us with this, 386
+  // without, 403 with a test of the weights behind the exponentials, which the products then wait for
+  const float limit = MASK == MASK_ROWS && !live ? XA_MOST : m + XA_SLACK;
+  if (MASK == MASK_ROWS ? __any(!(mx * c <= limit)) : __any(mx * c > m + XA_SLACK)) {
+    if (MASK == MASK_ROWS && !live) {
+      if (!(mx * c <= limit)) {
+#pragma unroll
+        for (int b = 0; b < NB; ++b)
+#pragma unroll
+          for (int j = 0; j < 16; ++j) s[b][j] = 0.f;
+      }
+      mx = -INFINITY;
+    }
     mx = max32(mx);
     const float mn = fmaxf(m, mx * c);
     const float alpha = __builtin_amdgcn_exp2f(m - mn);

@@ -680,7 +680,7 @@ __global__ void __launch_bounds__(64 * W, DT == DT_BF16 && D <= 64 ? 4 : 2) sp_k
         byte = key_byte(t);
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // this wave's copies have landed
         barrier_keep_vm();                   // everybody's have
-        if (__any(live)) xa_tile<DT, D, C, MASK_ROWS, KB, DT == DT_BF16 && C == 64>(tile, tile + T::BYTES, qf, o, m, l, far, p.c, bits, bits == T::ALL, false, live);
+        if (__any(live)) xa_tile<DT, D, C, MASK_ROWS, KB, DT == DT_BF16 && (C == 64 || (D == 64 && W == 4))>(tile, tile + T::BYTES, qf, o, m, l, far, p.c, bits, bits == T::ALL, false, live);
       }
     }
   }

@@ -623,8 +623,8 @@ int clarus_hip_block_means(const void* k, int32_t dtype, int64_t k_bstride, int6
  *   out[n, i, h] = sum_j p_j v[n, j, g'],  p = softmax_j(scale q[n, i, h] . k[n, j, g']),  g' = h / (heads / kv_heads)
  * over the kept keys j of the blocks chosen for i's group; 0 where there are none. q, k, v, out, scale, types, sizes and
  * arithmetic as clarus_hip_cross_attention's; mask NULL or bytes at mask + n * mask_bstride + j (0 masked: such a key
- * counts for nothing, whatever k and v hold; of the kept ones k and v have to be finite: a block that a query's neighbours have
- * chosen weighs 0 for it). means: those of k's blocks, kept by the caller while the keys stay, or NULL.
+ * counts for nothing, whatever k and v hold; of the kept ones v has to be finite: a block that a query's neighbours have
+ * chosen weighs 0 for it, which makes NaN of a v that is not). means: those of k's blocks, kept by the caller while the keys stay, or NULL.
  * chosen: NULL or [n, heads, groups, ceil(blocks / 64)] words that receive the choice, block b in bit b % 64 of word b / 64.
  * block a multiple of 64 below 2^20, n * blocks < 2^23 and fewer than 2^21 blocks, n * groups < 2^23 where group > 1,
  * n * heads * groups < 2^26. scratch holds clarus_hip_sparse_attention_workspace(...) bytes, 16-byte aligned.

@@ -351,6 +351,44 @@ def test_scores_that_are_not_finite(dt, hips, gpu_device):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("dt", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("lq", [40, 1003, 20000])
+def test_a_row_takes_nothing_from_blocks_that_only_others_have_chosen(lq, dt, hips, gpu_device):
+    """Queries that are not finite have no block and are 0, whatever their neighbours chose; a product that leaves fp32 in a block
+    that only the neighbours chose changes nothing."""
+    heads, d, nb, dev = 2, 32, 10, gpu_device
+    q, k, v = inputs(1, lq, nb * 64, heads, heads, d, dt, dev, seed=lq)
+    masks = (None, torch.rand(1, nb * 64, generator=torch.Generator().manual_seed(1)).to(dev) < 0.8)
+
+    def compare(q, k, mask, what):
+        got, chosen = hips[dt].sparse_attention(q, k, v, heads, 2, mask=mask, return_blocks=True, out_dtype=torch.float32)
+        want = choice64(q, means64(k, 64, mask), heads, heads, 1, 2)
+        assert torch.equal(chosen, want), what
+        ref, pv, big = attend64(torch.where(q.isnan(), torch.zeros_like(q), q), k, v, heads, heads, want, 64, 1, mask)
+        tol = (2 * (d + 8) * U * big + 2 * (nb * 64 + 16) * U + (2.0 ** -8 if dt == torch.bfloat16 else 0)) * pv + U * ref.abs()
+        assert torch.isfinite(got).all(), f"{what}: {(~torch.isfinite(got)).any(-1).sum().item()} rows of {lq} are not finite"
+        assert ((got.double() - ref).abs() <= tol).all(), what
+        return got, chosen
+    for mask in masks:
+        bad = q.clone()
+        bad[0, 5::17, :d] = math.nan
+        bad[0, 7::29, d + 3] = math.nan
+        got, chosen = compare(bad, k, mask, "queries")
+        assert not got[0, 5::17, :d].any() and not chosen[0, 0, 5::17].any() and not got[0, 7::29, d:].any()
+    # queries of 2^100 meet keys of +-2^30 (mean 0) in a block that the others choose
+    q, k = (q / 16).view(1, lq, heads, d), k.clone().view(1, nb, 64, heads, d)
+    q[..., 0], q[..., 1], k[..., 0], k[..., 1] = 0, 6, 0, 0
+    q[:, ::4, :, 0], q[:, ::4, :, 1], k[:, 3, :, :, 0], k[:, 7, :, :, 1] = 2.0 ** 100, -6, 2.0 ** -96, 5
+    k[:, 7, ::2, :, 0], k[:, 7, 1::2, :, 0] = 2.0 ** 30, -2.0 ** 30
+    q, k = q.view(1, lq, -1), k.view(1, nb * 64, -1)
+    mask = torch.ones(1, nb * 64, dtype=torch.bool, device=dev)
+    mask[0, 130:140] = mask[0, 450:452] = False  # also two keys of that block, one of each sign
+    for m in (None, mask):
+        _, chosen = compare(q, k, m, "products")
+        assert chosen[0, :, ::4, 3].all() and not chosen[0, :, ::4, 7].any() and chosen[0, :, 1::4, 7].all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt", [torch.bfloat16, torch.float32])
 def test_layouts(dt, hips, gpu_device):
     g = torch.Generator().manual_seed(2)
     hip, heads, d = hips[dt], 2, 32
