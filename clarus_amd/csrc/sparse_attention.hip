@@ -559,7 +559,7 @@ __global__ void __launch_bounds__(64 * W, DT == DT_BF16 && D <= 64 ? 4 : 2) sp_k
   using T = XaTile<DT, D>;
   constexpr int KT = T::KT, KB = KT / 32, DB = D / 32;
   const CrossP& p = sp.x;
-  const int tpb = sp.block / KT, lk = (int)p.lk;  // tiles of a block, keys
+  const int tpb = sp.block / KT, lk = (int)p.lk, tiles = (int)((p.lk + KT - 1) / KT);  // tiles of a block; keys and tiles in all
   __shared__ __align__(16) unsigned char tile[2 * T::BYTES];
   __shared__ uint64_t wants[W][SP_WORDS];
   __shared__ unsigned short list[SP_WORDS * 64];  // blocks of the words at hand that a row of the workgroup has chosen
@@ -653,7 +653,7 @@ __global__ void __launch_bounds__(64 * W, DT == DT_BF16 && D <= 64 ? 4 : 2) sp_k
       auto pop = [&](int& i) __attribute__((always_inline)) {  // the next tile and its place in the list, -1 past the last
         if (++sub < tpb) {
           const int t = ((int)w0 * 64 + __builtin_amdgcn_readlane(blk, e)) * tpb + sub;
-          if (t * KT < lk) return t;
+          if (t < tiles) return t;  // the last block's may end past 2^31
         }
         if (e + 1 >= cn) {
           sub = tpb;
@@ -664,7 +664,7 @@ __global__ void __launch_bounds__(64 * W, DT == DT_BF16 && D <= 64 ? 4 : 2) sp_k
         return ((int)w0 * 64 + __builtin_amdgcn_readlane(blk, e)) * tpb;
       };
       auto key_byte = [&](int t) __attribute__((always_inline)) {  // this lane's key of a tile counts
-        const bool in = lane < KT && lane < lk - t * KT && t >= 0;
+        const bool in = t >= 0 && lane < KT && lane < lk - t * KT;
         if constexpr (MASK == MASK_KEYS) return in ? (int)mkey[t * KT + lane] : 0;
         return (int)in;
       };

@@ -420,6 +420,23 @@ def test_offsets_past_32_bits(hips, gpu_device):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dt", [torch.bfloat16, torch.float32])
+def test_the_longest_keys(dt, hips, gpu_device):
+    """2^31 - 1 keys (rows of stride 0: all the same), the last block of which ends past 2^31."""
+    lk, block, d = (1 << 31) - 1, (1 << 20) - 64, 8
+    q, k, v = (torch.randn(1, 1, d, generator=torch.Generator().manual_seed(i)).to(dt).to(gpu_device) for i in range(3))
+    means = torch.zeros(1, -(-lk // block), d, device=gpu_device)
+    means[:, -1] = q[:, 0]
+    mask = torch.zeros(1, lk, dtype=torch.bool, device=gpu_device)
+    mask[0, -3000:] = True
+    for m in (None, mask):
+        got, chosen = hips[dt].sparse_attention(q, k.expand(1, lk, d), v.expand(1, lk, d), 1, 1, block=block, means=means, mask=m, return_blocks=True)
+        assert chosen[0, 0, 0].nonzero().flatten().tolist() == [means.shape[1] - 1]
+        # equal weights of equal values: what their sums of up to 2^17 terms round
+        assert ((got.double() - v.double()).abs() <= (2.0 ** 17 * 2 * U + (2.0 ** -7 if dt == torch.bfloat16 else 0)) * v.double().abs()).all()
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("lq,lk,group", [(400, 700, 1), (2, 3001, 1), (400, 700, 32)])
 def test_repeatable_streams_and_graph(lq, lk, group, hips, gpu_device):
     hip = hips[torch.bfloat16]
