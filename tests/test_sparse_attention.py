@@ -45,6 +45,20 @@ def choice64(q, means, heads, kv_heads, group, top):
     return torch.zeros_like(score, dtype=torch.bool).scatter_(-1, order, True) & (score > -math.inf)
 
 
+def choice_of_copies(q, means, heads, top):
+    """choice64 of a head for each kv head and groups of one, every block's products added in the same order: a large matrix product
+    adds in an order that differs from tile to tile, so that copies of a block differ in their last bit."""
+    d = q.shape[-1] // heads
+    out = []
+    for h in range(heads):
+        a, m = q[..., h * d:(h + 1) * d].double(), means[..., h * d:(h + 1) * d].double()
+        score = torch.cat([(t[:, :, None] * m[:, None]).sum(-1) for t in a.split(256, 1)], 1)
+        score = torch.where(score > -math.inf, score, torch.full_like(score, -math.inf))
+        order = score.sort(dim=-1, descending=True, stable=True)[1][..., :top]
+        out.append(torch.zeros_like(score, dtype=torch.bool).scatter_(-1, order, True) & (score > -math.inf))
+    return torch.stack(out, 1)
+
+
 def attend64(q, k, v, heads, kv_heads, chosen, block, group, mask=None, scale=None):
     """(o, p @ |v|, A), float64, over the chosen blocks' kept keys."""
     n, lq, c = q.shape
@@ -238,6 +252,52 @@ def test_shapes(n, lq, lk, heads, kv_heads, d, top, block, group, dt, hips, gpu_
             assert not got[-1].any() and not chosen[-1].any()
         means = hips[dt].block_means(k, block, mask)
         check(hips[dt], q, k, v, heads, top, kv_heads, block, group, mask, means, out_dtype=torch.float32, what="kept means")
+
+
+# Enough rows that every CU has a workgroup without splitting the blocks (more than 256 of rows): 2, 4 and 1 waves, the finished
+# rows stored by the kernel itself
+UNSPLIT = [  # n, lq, lk, heads, kv_heads, d, top, block, group
+    (2, 1201, 4470, 8, 8, 32, 9, 64, 1), (2, 1201, 4470, 8, 8, 64, 20, 64, 64), (2, 2101, 4470, 8, 8, 48, 40, 64, 256),
+    (40, 3, 2500, 8, 8, 104, 12, 64, 1), (1, 2301, 70390, 8, 8, 16, 40, 64, 1), (1, 4203, 9000, 4, 4, 72, 17, 128, 1),
+    (3, 1003, 4100, 12, 4, 64, 5, 64, 100), (2, 1077, 3000, 8, 8, 128, 33, 64, 7), (1, 5001, 5001, 8, 8, 64, 50, 64, 300)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("n,lq,lk,heads,kv_heads,d,top,block,group", UNSPLIT)
+def test_rows_that_fill_the_gpu(n, lq, lk, heads, kv_heads, d, top, block, group, dt, hips, gpu_device):
+    q, k, v = inputs(n, lq, lk, heads, kv_heads, d, dt, gpu_device, seed=lq + lk)
+    for mask in (None, make_mask(n, lk, gpu_device)):
+        print(f"[sparse] {n} {lq} {lk} {heads} {kv_heads} {d} {top} {block} {group} {dt} {mask is not None}", flush=True)
+        got, _ = check(hips[dt], q, k, v, heads, top, kv_heads, block, group, mask, what=str(mask is not None))
+        print(f"[sparse] {_lib.last_kernel()}", flush=True)
+        assert _lib.last_kernel().endswith("splits=1")
+        assert mask is None or n == 1 or not got[-1].any()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("d,nb", [(16, 70), (16, 300), (64, 1000), (72, 70), (72, 130), (128, 300), (128, 1000)])
+def test_choices_of_many_rows(d, nb, dt, hips, gpu_device):
+    """528 tiles of 32 rows, for which a wave holds the scores of 256 blocks (heads past 64: 128). Means kept by the caller: copies of
+    each other, NaN, infinite, and some that differ in their last bits, a head each; queries of zeros."""
+    g = torch.Generator().manual_seed(nb + d)
+    heads, lq, lk = 4, 4200, 64 * nb - 13
+    q = torch.randn(1, lq, heads * d, generator=g).to(dt)
+    means = torch.randn(1, nb, heads, d, generator=g)
+    means[:, 5::9, 0] = means[:, 6:7, 0]
+    means[:, 3::17, 1] = math.nan
+    means[:, 11, 2, 5], means[:, nb - 2, 2, 0] = math.inf, -math.inf
+    base = means[:, :1, 3].clone()
+    means[:, :, 3] = base + 2.0 ** -22 * torch.randint(-3, 4, (1, nb, d), generator=g) * base.abs()
+    q[:, ::50] = 0
+    q, means = q.to(gpu_device), means.reshape(1, nb, -1).to(gpu_device)
+    k = torch.randn(1, lk, heads * d, generator=g).to(dt).to(gpu_device)
+    for top in (1, 16, nb - 1):
+        print(f"[sparse] choices {d} {nb} {dt} {top}", flush=True)
+        want = choice_of_copies(q, means, heads, top)
+        _, chosen = hips[dt].sparse_attention(q, k, k, heads, top, means=means, return_blocks=True)
+        assert torch.equal(chosen, want), f"{top}: {(chosen != want).any(-1).sum().item()} choices differ"
 
 
 @pytest.mark.gpu
