@@ -176,6 +176,56 @@ def test_shapes(n, l, heads, kv_heads, dk, dv, dt, hips, gpu_device):
             check(got, q, k, v, g, heads, kv_heads, state, what=f"{odt}")
 
 
+def in_pieces64(q, k, v, log_decay, heads, kv_heads, state, size=1000, before=63):
+    """plain64 of a long sequence, a piece at a time from the state of the piece before (and the size of it)."""
+    zero = torch.zeros(q.shape[0], kv_heads, q.shape[-1] // heads, v.shape[-1] // kv_heads, dtype=torch.float64, device=q.device)
+    s, a = (zero, zero) if state is None else (state.double(), state.double().abs())
+    outs = []
+    for i in range(0, q.shape[1], size):
+        at = slice(i, i + size)
+        out, _, _, s, _ = plain64(q[:, at], k[:, at], v[:, at], log_decay, heads, kv_heads, s)
+        big, _, _, a, _ = plain64(q[:, at].abs(), k[:, at].abs(), v[:, at].abs(), log_decay, heads, kv_heads, a)
+        m = min(i, before)  # the tokens within 64 of the piece's first ones
+        wide = slice(i - m, i + size)
+        near = plain64(q[:, wide], k[:, wide], v[:, wide], log_decay, heads, kv_heads)[2][:, m:]
+        outs.append((out, big, near))
+    return [torch.cat(t, 1) for t in zip(*outs)] + [s, a]
+
+
+def test_pieces_are_the_whole():
+    q, k, v, s = inputs(2, 301, 4, 2, 16, 24, torch.float32, "cpu")
+    for state in (None, s):
+        for a, b in zip(in_pieces64(q, k, v, decays(2, "cpu"), 4, 2, state, 90), plain64(q, k, v, decays(2, "cpu"), 4, 2, state)):
+            assert (a - b).abs().max() <= 1e-12 * b.abs().max()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("n,l,heads,kv_heads,dk,dv,segments", [(1, 5003, 4, 4, 40, 40, 79), (1, 20011, 4, 4, 40, 40, 209), (1, 20011, 1, 1, 64, 96, 313),
+                                                               (2, 6031, 8, 4, 48, 32, 95), (1, 40013, 2, 1, 128, 24, 626)])
+def test_many_segments(n, l, heads, kv_heads, dk, dv, segments, dt, hips, gpu_device):
+    """More segments than 64, which groups of threads chain together, and more than 128, which they take in several rounds; none a
+    multiple of 128, and lengths that are padded in front."""
+    q, k, v, s = inputs(n, l, heads, kv_heads, dk, dv, dt, gpu_device, seed=l)
+    g = torch.tensor([0.0, -1e-4, -1 / 64, -0.5])[:kv_heads].to(gpu_device)
+    for state in (None, s):
+        out, last = hips[dt].linear_attention(q, k, v, g, heads, kv_heads, state, out_dtype=torch.float32)
+        torch.cuda.synchronize()
+        print(f"[la] {l} {dt} {_lib.last_kernel()}", flush=True)
+        assert f"segments={segments} " in _lib.last_kernel()
+        ref, big, near, rlast, slast = in_pieces64(q, k, v, g, heads, kv_heads, state)
+        m = (l / 4 + dk + 150) * U
+        tol = m * big + (2.0 ** -8 * near + 2.0 ** -14 * big if dt == torch.bfloat16 else 0) + U * ref.abs()
+        for name, t, r, e in (("out", out, ref, tol), ("state", last, rlast, m * slast)):
+            off = (t.double() - r).abs()
+            assert (off <= e).all(), f"{name}: max|d| {off.max().item():.3e}, {(off - e).max().item():.3e} past the tolerance"
+        again = hips[dt].linear_attention(q, k, v, g, heads, kv_heads, state, out_dtype=torch.float32)
+        assert torch.equal(again[0], out) and torch.equal(again[1], last)
+    held = s.clone()
+    over, same = hips[dt].linear_attention(q, k, v, g, heads, kv_heads, held, state_out=held, out_dtype=torch.float32)
+    assert same is held and torch.equal(held, last) and torch.equal(over, out)
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize("dt", [torch.bfloat16, torch.float32])
 def test_in_pieces(dt, hips, gpu_device):
