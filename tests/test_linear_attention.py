@@ -260,6 +260,27 @@ def test_a_state_does_not_drift(hips, gpu_device):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("dt", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("n,d,l", [(2100, 8, 20000), (520, 128, 10000)])
+def test_a_segment_does_not_drift(n, d, l, dt, hips, gpu_device):
+    """States only scaled, chunk after chunk of one segment: the last token's outputs against exp in 64 bits. Each chunk rounds a
+    state, up or down as its value decides, so the mean over n d states (16 800 or more, 625 roundings of 0.29 steps each) is off by 0.6 u
+    at 5 deviations; its factor must not round to the same side again and again. Left are a step of the factors together,
+    2 u |x| a chunk of the exponent x and, with bf16, the state's two parts (2^-17, as random: 2 u at 5 deviations)."""
+    z = torch.zeros(1, l, d, dtype=dt, device=gpu_device)
+    q = z.clone()
+    q[:, -1, 0] = 1
+    state = torch.linspace(1, 2, n * d * d, device=gpu_device).reshape(n, 1, d, d).contiguous()
+    for time in (45000, 30000, 7000):
+        g = torch.tensor([-1.0 / time], device=gpu_device)
+        out, _ = hips[dt].linear_attention(q.expand(n, l, d), z.expand(n, l, d), z.expand(n, l, d), g, 1, state=state, scale=1.0, out_dtype=torch.float32)
+        assert "segments=1 " in _lib.last_kernel()
+        want = state[:, 0, 0].double() * torch.exp(l * g.double())
+        off = ((out[:, -1].double() - want) / want).mean().abs().item()
+        assert off <= (4 + 2 * l / time) * U, f"{time}: {off / U:.1f} u"
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt", [torch.bfloat16, torch.float32])
 @pytest.mark.parametrize("l", [3, 54])
 def test_layouts(l, dt, hips, gpu_device):
     """Slices of wider rows, NHWC rows, images shared by stride 0, one token of [N, C], decays of another type."""
