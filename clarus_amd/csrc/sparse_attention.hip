@@ -141,7 +141,7 @@ __device__ __forceinline__ uint64_t sp_key(double v) {
 }
 
 // A workgroup per row. The largest threshold that leaves `top` scores is halved towards by counts, and found as soon as one
-// leaves just `top`. K: scores that a thread holds in registers (0: more, read again for each count). 32768 rows of 2048 blocks:
+// leaves just `top`. K: scores that a thread holds in registers (0: more, read again for each count). 8192 rows of 2048 blocks:
 // 55 us; byte by byte from the highest with counters in LDS 417, and a token's 16 rows of 4097 blocks 106 instead of 15
 template <int K>
 __global__ void __launch_bounds__(SP_T) sp_choose_kernel(const SparseP p) {
@@ -232,6 +232,7 @@ __global__ void __launch_bounds__(SP_T) sp_choose_kernel(const SparseP p) {
 // chosen and the largest left out are more than 2 e apart, 64 bits would choose the same. Where they are not, the blocks
 // within 2 e of the threshold are scored again in 64 bits by a wave, up to 64 of them; a row with more of them (equal blocks,
 // an ask of zeros), or with a norm that is not finite, is done by the whole workgroup, every block's rank counted.
+// Eight tiles of a wave and the ask do not fit its 256 VGPRs: 14 to 18 are spilled (14400 queries of 8 heads of 64, 225 blocks: 108 us)
 constexpr int SP_PICK = 1024;  // blocks, at most
 constexpr float SP_LOST = 0x1p-118f;  // of a sum of up to 128 squares, should each lose 2^-126
 
