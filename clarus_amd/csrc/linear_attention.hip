@@ -24,8 +24,9 @@
 // What bounds it: a token, memory (64 states of 16 heads of 128 x 128: 28.7 us, 4.7 TB/s). Chunks: K and V read twice, and a
 // wave's chain from chunk to chunk; 57600 tokens, 8 heads of 64 x 64, bf16: 34.6 us for the segments' sums, 9.1 for the chain
 // of segments, 66 for the outputs (236 MB in all: 46 us at a large copy's rate); 2 x 5003 of 48 x 96, 8 heads on 4, fp32: 14.6,
-// 6.7 and 51.3, of which the fp32 MFMAs alone are some 31 where two of the 1272 waves share a SIMD. Keys of 128 in bf16: 28800 tokens, 8 heads of 128 x 128:
-// 44, 16 and 156, where the output pass spills 112 to 121 of its VGPRs (fp32 keys of 96: 53 to 55; other forms 11 at most).
+// 6.7 and 51.3, of which the fp32 MFMAs alone are some 31 where two of the 1272 waves share a SIMD. Keys of
+// 128 in bf16: 28800 tokens, 8 heads of 128 x 128: 44, 16 and 156, where the output pass spills 112 to 121 of its
+// VGPRs (fp32 keys of 96: 53 to 55; other forms 11 at most).
 #include <algorithm>
 #include <math.h>
 

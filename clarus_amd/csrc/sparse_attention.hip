@@ -228,9 +228,10 @@ __global__ void __launch_bounds__(SP_T) sp_choose_kernel(const SparseP p) {
 // A workgroup: W waves, 32 rows (groups and the heads that share a kv head) of one (image, kv head). A wave holds the scores of
 // NT tiles of 32 blocks in registers, from fp32 MFMAs (S^T = means asks^T: a lane holds a row's scores of 16 blocks of
 // each tile, its partner in lane ^ 32 the other 16). They are off by at most e = 2 (d + 8) 2^-24 |ask| |mean| (Cauchy-Schwarz over
-// the terms; the norms with what their squares may lose below 2^-126, SP_LOST, and products that small below 1e-35 in all). A row's threshold is searched between its least and largest score, by counts; where the least score
-// chosen and the largest left out are more than 2 e apart, 64 bits would choose the same. Where they are not, the blocks
-// within 2 e of the threshold are scored again in 64 bits by a wave, up to 64 of them; a row with more of them (equal blocks,
+// the terms; the norms with what their squares may lose below 2^-126, SP_LOST, and products that small below 1e-35 in all).
+// A row's threshold is searched between its least and largest score, by counts; where the least score chosen and the
+// largest left out are more than 2 e apart, 64 bits would choose the same. Where they are not, the blocks within 2 e of the
+// threshold are scored again in 64 bits by a wave, up to 64 of them; a row with more of them (equal blocks,
 // an ask of zeros), or with a norm that is not finite, is done by the whole workgroup, every block's rank counted.
 // Eight tiles of a wave and the ask do not fit its 256 VGPRs: 14 to 18 are spilled (14400 queries of 8 heads of 64, 225 blocks: 108 us)
 constexpr int SP_PICK = 1024;  // blocks, at most
@@ -681,7 +682,8 @@ __global__ void __launch_bounds__(64 * W, DT == DT_BF16 && D <= 64 ? 4 : 2) sp_k
         byte = key_byte(t);
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // this wave's copies have landed
         barrier_keep_vm();                   // everybody's have
-        if (__any(live)) xa_tile<DT, D, C, MASK_ROWS, KB, DT == DT_BF16 && (C == 64 || (D == 64 && W == 4))>(tile, tile + T::BYTES, qf, o, m, l, far, p.c, bits, bits == T::ALL, false, live);
+        constexpr bool ANEW = DT == DT_BF16 && (C == 64 || (D == 64 && W == 4));  // the forms that else spill
+        if (__any(live)) xa_tile<DT, D, C, MASK_ROWS, KB, ANEW>(tile, tile + T::BYTES, qf, o, m, l, far, p.c, bits, bits == T::ALL, false, live);
       }
     }
   }

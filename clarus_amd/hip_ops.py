@@ -1144,8 +1144,8 @@ class HipOps(Backend):
         queries q [N, ..., heads * d] into groups of `group`. A head's group attends the kept keys of the `top` blocks whose
         mean key has the largest product with the group's mean query (means rounded to fp32, products in 64 bits; of equal
         ones the lowest index). mask: bool [N, Lk], a masked key counts for nothing whatever k and v hold (kept
-        values have to be finite); a block without a kept key, or with a score of NaN, is not chosen. means: block_means(k, block, mask), kept while the keys stay (None: made in the
-        call). 0 for a query without a block. Returns a contiguous tensor of q's shape; with return_blocks also the choice,
+        values have to be finite); a block without a kept key, or with a score of NaN, is not chosen. means: block_means(k,
+        block, mask), kept while the keys stay (None: made in the call). 0 for a query without a block. Returns a contiguous tensor of q's shape; with return_blocks also the choice,
         bool [N, heads, groups, blocks]."""
         kv_heads = heads if kv_heads is None else kv_heads
         if not all(isinstance(i, int) for i in (heads, kv_heads, top, block, group)):  # before the plans, whose keys 4.0 and 4 share
